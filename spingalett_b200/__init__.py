@@ -31,6 +31,7 @@ def lib():
         handle = C.CDLL(LIB_PATH)
         abi.bind_reference_abi(handle)
         abi.bind_extensions(handle)
+        abi.bind_operators(handle)
         _lib = handle
     return _lib
 

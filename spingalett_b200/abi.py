@@ -18,6 +18,9 @@ LOG_DEBUG, LOG_INFO, LOG_WARNING, LOG_ERROR, LOG_NONE = range(5)
 MATH_FAST, MATH_EXACT, MATH_AUTO = 0, 1, 2
 OK, ERR_ALLOC, ERR_INVALID, ERR_DEVICE = 0, 1, 2, 3
 
+TYPE_F16, TYPE_BF16, TYPE_F32 = range(3)               # SPGK_T_*
+MX4_BLOCK, SAMPLE_MAX_WIDTH = 32, 262144
+
 PRECISION_NAMES = {"fp32": 0, "fp16": 1, "bf16": 2, "int8": 3, "int4": 4, "int2": 5}
 
 f32p = C.POINTER(C.c_float)
@@ -80,6 +83,11 @@ class KLayer(C.Structure):
     """spgk_layer of include/spingalett_b200_kernels.h"""
     _fields_ = [("w", C.c_void_p), ("bias", C.c_void_p), ("w_scale", C.c_float), ("in_", C.c_uint32),
                 ("out", C.c_uint32), ("precision", C.c_int32), ("act", C.c_int32), ("bias_absmax", C.c_float)]
+
+
+class Mx4(C.Structure):
+    """spgk_mx4 of include/spingalett_b200_kernels.h: a matrix of microscaled 4-bit numbers"""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_uint32), ("cols", C.c_uint32), ("pitch", C.c_uint32)]
 
 
 # the 21 exported functions of the reference ABI (Spingalett.h:202-238)
@@ -191,4 +199,22 @@ def bind_extensions(lib):
     lib.spingalett_profile.restype = None
     lib.spingalett_profile_read.argtypes = [NetP, C.POINTER(C.c_double), C.POINTER(C.c_uint64)]
     lib.spingalett_profile_read.restype = None
+    return lib
+
+
+def bind_operators(lib):
+    """The kernel-level operators on device pointers (microscaled 4-bit numbers, draws from logits); 0 or a negative SPGK_E_* code."""
+    vp, u32, mx4 = C.c_void_p, C.c_uint32, C.POINTER(Mx4)
+    lib.spgk_error_string.argtypes = []
+    lib.spgk_error_string.restype = C.c_char_p
+    lib.spgk_mx4_pitch.argtypes = [u32]
+    lib.spgk_mx4_pitch.restype = u32
+    lib.spgk_mx4_scales_bytes.argtypes = [u32, u32]
+    lib.spgk_mx4_scales_bytes.restype = C.c_size_t
+    lib.spgk_mx4_scale_index.argtypes = [u32, u32, u32]
+    lib.spgk_mx4_scale_index.restype = C.c_size_t
+    lib.spgk_mx4_quantize.argtypes = [vp, C.c_int, u32, mx4, vp]
+    lib.spgk_mx4_dequantize.argtypes = [mx4, vp, C.c_int, u32, vp]
+    lib.spgk_layer_mx4.argtypes = [mx4, vp, C.c_int, mx4, vp, C.c_int, u32, mx4, vp, vp]
+    lib.spgk_sample_rows.argtypes = [vp, C.c_int, u32, u32, u32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     return lib

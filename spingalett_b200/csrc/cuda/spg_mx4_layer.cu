@@ -1,0 +1,376 @@
+// spg_mx4_layer.cu -- a dense layer on two microscaled 4-bit operands.
+//
+//   y[n][j] = act(bias[j] + sum_b 2^(Ew[j,b] + Ex[n,b]) * sum_{k in block b} w[j][k] x[n][k])
+//
+// tcgen05.mma kind::mxf4 multiplies E2M1 elements and their E8M0 scales as they lie in memory: nothing is unpacked.  The weights are the
+// 128-row side of a tile, rows of the batch its columns (16 to 256), so a batch of one costs no more products than one of sixteen, and a lane of
+// the epilogue has one output unit: its bias is a register, and 32 lanes hold a whole block of the next layer's input.
+// A k-block is 256 elements: rows of 128 bytes, 128-byte swizzle, four products of 64; its scales are two tiles of 512 bytes a side,
+// which tcgen05.cp copies to tensor memory in front of the products (both are issued by one thread and run in order).
+// Where there are few tiles, up to eight CTAs of a cluster share one, each with its part of the k-blocks, and add their sums in rank order.
+//
+// Every wait on an mbarrier is bounded; a CTA that gave up records a code in `status`, and its cluster leaves the tile's outputs alone.
+#include "spg_mx4.cuh"
+#include "spg_tc.cuh"
+#include <cstdio>
+#include <mutex>
+
+namespace {
+
+using namespace spgtc;
+
+constexpr uint32_t TM = 128;                  // output units of a tile
+constexpr uint32_t KB = 256;                  // elements of a k-block
+constexpr uint32_t W_BYTES = TM * 128;        // codes of a tile's weights
+constexpr uint32_t SF_TILE = 512;             // scales of 128 rows x 4 blocks
+constexpr uint32_t SF_BYTES = 2 * SF_TILE;    // of 128 rows in a k-block
+constexpr uint32_t THREADS = 192;             // warp 0: copies, warp 1: products, warps 2 to 5: outputs
+constexpr uint32_t MAX_STAGES = 8;
+constexpr uint32_t MAX_SPLIT = 8;
+constexpr uint32_t HEAD = 1024;
+
+struct LayerParams {
+    uint32_t N, out, cols, kblocks, kt;       // rows, units, inputs; k-blocks; scale tiles of a row
+    uint32_t split, stages;
+    const uint8_t *w_scales, *x_scales;
+    const float *bias;
+    int act;
+    void *y; int type; uint32_t ldy;
+    uint8_t *next_codes, *next_scales; uint32_t next_pitch, next_kt;
+    int32_t *status;
+};
+
+// kind::mxf4, E2M1 on both sides, UE8M0 scales, M = 128
+__host__ __device__ constexpr uint32_t idesc_mx4(uint32_t n) { return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24); }
+
+__device__ __forceinline__ void umma_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// 512 bytes (32 rows of 16) -> four columns of tensor memory, once for each quarter of the lanes
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc)
+{
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// no swizzle, groups of eight rows of 16 bytes 128 bytes apart
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr)
+{
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(128u >> 4) << 16 | (uint64_t)(128u >> 4) << 32 | (uint64_t)1u << 46;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr)
+{
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+template <typename T> __device__ __forceinline__ void put(void *y, uint64_t at, float v);
+template <> __device__ __forceinline__ void put<float>(void *y, uint64_t at, float v) { reinterpret_cast<float *>(y)[at] = v; }
+template <> __device__ __forceinline__ void put<__half>(void *y, uint64_t at, float v) { reinterpret_cast<__half *>(y)[at] = __float2half_rn(v); }
+template <> __device__ __forceinline__ void put<__nv_bfloat16>(void *y, uint64_t at, float v) { reinterpret_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v); }
+
+// Eight rows' values of this lane's unit, the warp's 32 units being one block of the next layer's input: scales, codes, stores.
+// A lane's eight codes are eight nibbles of a word, one a row; three exchanges among eight lanes turn that into eight nibbles of one row.
+__device__ __forceinline__ void put_next(const LayerParams &p, const float (&v)[8], uint32_t n0, uint32_t j0, uint32_t lane)
+{
+    float q[8];
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t byte = spgmx4::scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v[i]) & 0x7fffffffu));
+        q[i] = byte == 255u ? 0.0f : v[i] * spgmx4::inverse_scale(byte);
+        if (lane == (uint32_t)i) mine = byte;
+    }
+    uint32_t w = spgmx4::encode8(q);
+#pragma unroll
+    for (int s = 4, bits = 16; s; s >>= 1, bits >>= 1) {
+        const uint32_t low = bits == 16 ? 0x0000ffffu : (bits == 8 ? 0x00ff00ffu : 0x0f0f0f0fu);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, w, s);
+        w = (lane & s) ? ((w & ~low) | ((other >> bits) & low)) : ((w & low) | ((other & low) << bits));
+    }
+    const uint32_t n = n0 + lane % 8u, j = j0 + lane / 8u * 8u;
+    if (n < p.N && j0 < (p.out + 31u) / 32u * 32u) *reinterpret_cast<uint32_t *>(p.next_codes + (uint64_t)n * p.next_pitch + j / 2u) = w;
+    if (lane < 8u && n0 + lane < p.N) {
+        const uint32_t row = n0 + lane;
+        p.next_scales[((uint64_t)(row / 128u) * p.next_kt + j0 / 128u) * SF_TILE + spgmx4::scale_in_tile(row) + j0 % 128u / 32u] = (uint8_t)mine;
+    }
+}
+
+// columns c0 .. c0 + 8 of the tile (rows n0 ... of the batch) for this lane's unit
+__device__ __forceinline__ void finish8(const LayerParams &p, float (&v)[8], uint32_t n0, uint32_t j0, uint32_t lane, float bias)
+{
+    const uint32_t j = j0 + lane;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = j < p.out ? spg_activate(v[i] + bias, p.act) : 0.0f;
+    if (p.y && j < p.out) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (n0 + i >= p.N) break;
+            const uint64_t at = (uint64_t)(n0 + i) * p.ldy + j;
+            if (p.type == SPGK_T_F32) put<float>(p.y, at, v[i]);
+            else if (p.type == SPGK_T_F16) put<__half>(p.y, at, v[i]);
+            else put<__nv_bfloat16>(p.y, at, v[i]);
+        }
+    }
+    if (p.next_codes) put_next(p, v, n0, j0, lane);
+}
+
+template <uint32_t NT> struct Tile {
+    static constexpr uint32_t X_BYTES = NT * 128;
+    static constexpr uint32_t SFX_TILES = (NT + 127) / 128;
+    static constexpr uint32_t STAGE = (W_BYTES + X_BYTES + SF_BYTES + SFX_TILES * SF_BYTES + 1023) / 1024 * 1024;
+    static constexpr uint32_t SFX_COLS = NT < 128 ? 4 : NT / 32;              // columns of the rows' scales for four blocks
+    static constexpr uint32_t SFW = NT < 32 ? 16 : NT;                         // tensor memory: sums, weights' scales, rows' scales
+    static constexpr uint32_t SFX = SFW + 8;
+    static constexpr uint32_t USED = SFX + 2 * SFX_COLS;
+    static constexpr uint32_t COLS = USED <= 32 ? 32 : USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+};
+
+template <uint32_t NT>
+__global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LayerParams p)
+{
+    using L = Tile<NT>;
+    extern __shared__ uint8_t raw[];
+    uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t head = smem_u32(base), ring = head + HEAD;
+    const uint32_t full = head, empty = head + 8 * MAX_STAGES, done = empty + 8 * MAX_STAGES, slot = done + 8, aborted = slot + 4;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head));
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+    const uint32_t rank = blockIdx.x % p.split, j_tile = blockIdx.x / p.split, n0 = blockIdx.y * NT;
+    // this CTA's k-blocks
+    const uint32_t lo = (uint32_t)((uint64_t)p.kblocks * rank / p.split), hi = (uint32_t)((uint64_t)p.kblocks * (rank + 1) / p.split);
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc(slot, L::COLS);
+    if (warp == 0 && elect_one()) { prefetch_map(&map_w); prefetch_map(&map_x); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
+    spg_grid_wait();
+    volatile int never = 0;
+
+    if (warp == 0) {
+        const uint32_t sfx_tiles = min(L::SFX_TILES, (p.N + 127u) / 128u - n0 / 128u);      // (the last tile of rows may have fewer)
+        uint32_t last = 0;
+        for (uint32_t kb = lo, s = 0, phase = 1; kb < hi; kb++) {
+            mbar_wait_uniform(empty + 8 * s, phase, aborted, p.status, 1);
+            if (*abort_flag) break;
+            const uint32_t at = ring + s * L::STAGE, sf = min(2u, p.kt - 2 * kb) * SF_TILE;
+            if (elect_one()) {
+                mbar_expect_tx(full + 8 * s, W_BYTES + L::X_BYTES + sf * (1 + sfx_tiles));
+                tma_load_2d(at, &map_w, full + 8 * s, (int)(kb * 128u), (int)(j_tile * TM));
+                tma_load_2d(at + W_BYTES, &map_x, full + 8 * s, (int)(kb * 128u), (int)n0);
+                bulk_load(at + W_BYTES + L::X_BYTES, p.w_scales + ((uint64_t)j_tile * p.kt + 2 * kb) * SF_TILE, sf, full + 8 * s);
+                for (uint32_t t = 0; t < sfx_tiles; t++)
+                    bulk_load(at + W_BYTES + L::X_BYTES + SF_BYTES * (1 + t), p.x_scales + ((uint64_t)(n0 / 128u + t) * p.kt + 2 * kb) * SF_TILE, sf, full + 8 * s);
+            }
+            __syncwarp();
+            last = kb + 1 - lo;
+            if (++s == p.stages) { s = 0; phase ^= 1u; }
+        }
+        if (*abort_flag)                         // the copies under way end before this CTA does
+            for (uint32_t i = last > p.stages ? last - p.stages : 0; i < last; i++) mbar_wait(full + 8 * (i % p.stages), i / p.stages & 1u, &never, p.status, 4);
+    } else if (warp == 1) {
+        const uint32_t idesc = idesc_mx4(NT);
+        for (uint32_t kb = lo, s = 0, phase = 0; kb < hi; kb++) {
+            mbar_wait_uniform(full + 8 * s, phase, aborted, p.status, 2);
+            if (*abort_flag) break;
+            tc_fence_after();
+            const uint32_t at = ring + s * L::STAGE, steps = min(4u, (p.cols - kb * KB + 63u) / 64u);
+            if (elect_one()) {
+                const uint32_t sfw = at + W_BYTES + L::X_BYTES, sfx = sfw + SF_BYTES;
+                for (uint32_t i = 0; i < (steps + 1) / 2; i++) {
+                    copy_scales(tmem + L::SFW + 4 * i, scale_desc(sfw + i * SF_TILE));
+#pragma unroll
+                    for (uint32_t t = 0; t < L::SFX_TILES; t++)
+                        copy_scales(tmem + L::SFX + L::SFX_COLS * i + 4 * t, scale_desc(sfx + t * SF_BYTES + i * SF_TILE));
+                }
+                const uint64_t a = smem_desc_sw128(at), b = smem_desc_sw128(at + W_BYTES);
+                for (uint32_t i = 0; i < steps; i++) {
+                    const uint32_t id = (i & 1u) * 2u;          // which two of a tile's four scales
+                    umma_mx4(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, tmem + L::SFW + 4 * (i / 2), tmem + L::SFX + L::SFX_COLS * (i / 2), kb > lo || i > 0);
+                }
+                umma_commit(empty + 8 * s);
+            }
+            __syncwarp();
+            if (++s == p.stages) { s = 0; phase ^= 1u; }
+        }
+        if (elect_one()) umma_commit(done);
+        __syncwarp();
+    } else {
+        const uint32_t quad = warp % 4u, j0 = j_tile * TM + quad * 32u, j = j0 + lane;
+        const float bias = p.bias && j < p.out ? __ldg(p.bias + j) : 0.0f;
+        const bool ok = mbar_wait(done, 0, abort_flag, p.status, 3);
+        if (!ok) mbar_wait(done, 0, &never, p.status, 5);        // the products under way end before tensor memory is given back
+        tc_fence_after();
+        const uint32_t lanes = tmem + (quad * 32u << 16);
+        if (p.split == 1) {
+            if (ok && !*abort_flag) {
+                for (uint32_t c = 0; c < NT && n0 + c < p.N; c += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(lanes + c, r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int h = 0; h < 16; h += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[h + i]);
+                        finish8(p, v, n0 + c + h, j0, lane, bias);
+                    }
+                }
+            }
+        } else {
+            // this CTA's sums, [column][unit], into its own shared memory (no copy or product is under way any more)
+            for (uint32_t c = 0; c < NT; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(lanes + c, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; i++) *reinterpret_cast<uint32_t *>(base + HEAD + ((c + i) * TM + quad * 32u + lane) * 4u) = r[i];
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (p.split > 1) {
+        cluster_sync();
+        if (warp >= 2) {
+            const uint32_t quad = warp % 4u, j0 = j_tile * TM + quad * 32u, j = j0 + lane;
+            const float bias = p.bias && j < p.out ? __ldg(p.bias + j) : 0.0f;
+            bool ok = true;
+            for (uint32_t r = 0; r < p.split; r++) ok = ok && ld_cluster_u32(mapa(aborted, r)) == 0;
+            if (ok) {
+                for (uint32_t c = rank * 8u; c < NT && n0 + c < p.N; c += p.split * 8u) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = 0.0f;
+                    for (uint32_t r = 0; r < p.split; r++) {
+                        const uint32_t from = mapa(ring + (c * TM + quad * 32u + lane) * 4u, r);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[i] += ld_cluster_f32(from + i * TM * 4u);
+                    }
+                    finish8(p, v, n0 + c, j0, lane, bias);
+                }
+            }
+        }
+        cluster_sync();
+    }
+    if (warp == 1) { tc_fence_after(); tmem_free(tmem, L::COLS); }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// boxes of 256 elements x box_rows rows of a matrix' codes
+int codes_map(CUtensorMap *map, const spgk_mx4 *m, uint32_t box_rows)
+{
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(f);
+    });
+    if (!fn) { spgk_set_error("cuTensorMapEncodeTiled", "driver entry point not available"); return SPGK_E_CUDA; }
+    const cuuint64_t dims[2] = { spgk_mx4_pitch(m->cols), m->rows }, strides[1] = { m->pitch };
+    const cuuint32_t box[2] = { 128, box_rows }, steps[2] = { 1, 1 };
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, m->codes, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        char msg[64];
+        snprintf(msg, sizeof msg, "CUresult %d", (int)r);
+        spgk_set_error("cuTensorMapEncodeTiled (4-bit codes)", msg);
+        return SPGK_E_CUDA;
+    }
+    return SPGK_OK;
+}
+
+template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
+{
+    using L = Tile<NT>;
+    static SpgOncePerDevice once;
+    int rc = once.run(dev, [&]() -> int {
+        SPGK_CUDA(cudaFuncSetAttribute(spg_mx4_layer_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dp.smem_optin));
+        return SPGK_OK;
+    });
+    if (rc) return rc;
+    CUtensorMap map_w, map_x;
+    if ((rc = codes_map(&map_w, W, TM)) || (rc = codes_map(&map_x, X, NT))) return rc;
+    const uint32_t j_tiles = (p.out + TM - 1) / TM, n_tiles = (p.N + NT - 1) / NT;
+    const uint64_t tiles = (uint64_t)j_tiles * n_tiles;
+    p.split = 1;
+    if (NT <= 128) while (p.split < MAX_SPLIT && tiles * p.split * 2 <= (uint32_t)dp.sm_count && p.kblocks >= p.split * 4) p.split *= 2;
+    const uint32_t most = (uint32_t)(dp.smem_optin - HEAD - 1024) / L::STAGE, mine = (p.kblocks + p.split - 1) / p.split;
+    p.stages = mine < most ? mine : most;
+    if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+    uint32_t bytes = p.stages * L::STAGE;
+    if (p.split > 1 && bytes < NT * TM * 4u) bytes = NT * TM * 4u;
+    if (n_tiles > 65535u) { spgk_set_error("spgk_layer_mx4", "more than 65535 tiles of rows"); return SPGK_E_ARG; }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(j_tiles * p.split, n_tiles); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = HEAD + 1024 + bytes; cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    SPGK_CUDA(cudaLaunchKernelEx(&cfg, spg_mx4_layer_kernel<NT>, map_w, map_x, p));
+    return spgk_check_launch("spg_mx4_layer_kernel");
+}
+
+}  // namespace
+
+extern "C" int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, const spgk_mx4 *X, void *y, int type, uint32_t ldy,
+                              const spgk_mx4 *next, int32_t *status, void *stream)
+{
+    int rc;
+    if ((rc = spg_mx4_check("spgk_layer_mx4 (weights)", W)) || (rc = spg_mx4_check("spgk_layer_mx4 (inputs)", X))) return rc;
+    if (next && (rc = spg_mx4_check("spgk_layer_mx4 (next)", next))) return rc;
+    const char *why = nullptr;
+    if (W->rows == 0 || W->cols != X->cols) why = "weights and inputs do not belong together";
+    else if (act < SPG_ACT_SIGMOID || act > SPG_ACT_NONE) why = "unknown activation";
+    else if (!y && !next) why = "no output";
+    else if (y && type != SPGK_T_F16 && type != SPGK_T_BF16 && type != SPGK_T_F32) why = "unknown type";
+    else if (y && (uintptr_t)y % (type == SPGK_T_F32 ? 4u : 2u)) why = "output not aligned to its type";
+    else if (y && X->rows > 1 && ldy < W->rows) why = "rows of the output overlap";
+    else if (next && (next->rows != X->rows || next->cols != W->rows)) why = "the next operand has other rows or columns";
+    else if (next && act == SPG_ACT_SOFTMAX) why = "a softmax is left to spgk_softmax_rows";
+    else if (!status) why = "no status word";
+    else if ((uintptr_t)bias % 4u) why = "bias not aligned";
+    if (why) { spgk_set_error("spgk_layer_mx4", why); return SPGK_E_ARG; }
+    if (X->rows == 0) return SPGK_OK;
+    SpgDeviceProps dp;
+    int dev = 0;
+    if ((rc = spg_device_props(&dp))) return rc;
+    SPGK_CUDA(cudaGetDevice(&dev));
+    LayerParams p{};
+    p.N = X->rows; p.out = W->rows; p.cols = W->cols;
+    p.kblocks = (W->cols + KB - 1) / KB; p.kt = spgmx4::tiles4(W->cols);
+    p.w_scales = (const uint8_t *)W->scales; p.x_scales = (const uint8_t *)X->scales;
+    p.bias = bias; p.act = act; p.y = y; p.type = type; p.ldy = ldy; p.status = status;
+    if (next) { p.next_codes = (uint8_t *)next->codes; p.next_scales = (uint8_t *)next->scales; p.next_pitch = next->pitch; p.next_kt = spgmx4::tiles4(next->cols); }
+    cudaStream_t st = (cudaStream_t)stream;
+    if (p.N <= 16) return launch<16>(W, X, p, dp, dev, st);
+    if (p.N <= 32) return launch<32>(W, X, p, dp, dev, st);
+    if (p.N <= 64) return launch<64>(W, X, p, dp, dev, st);
+    if (p.N <= 512) return launch<128>(W, X, p, dp, dev, st);
+    return launch<256>(W, X, p, dp, dev, st);
+}
