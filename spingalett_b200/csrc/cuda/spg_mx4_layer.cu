@@ -274,12 +274,210 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
     if (warp == 1) { tc_fence_after(); tmem_free(tmem, L::COLS); }
 }
 
+// ---- pairs of CTAs, many rows -------------------------------------------------------------------------------------------------
+// 256 units x 256 rows of the batch a tile on a cluster of two (cta_group::2): each CTA holds 128 units' weights and half of the rows, so a k-block costs it
+// 35 KB for 512 cycles of products; a CTA alone would need 51. Persistent: the copies run ahead over the tile's end, and the sixteen
+// epilogue warps take all 256 columns of sums to registers at once (64 a thread), so the next tile's products wait for that alone (there
+// is no room in tensor memory for a second accumulator of 256 columns beside the scales).
+constexpr uint32_t PN = 256;                                   // rows of the batch a tile
+constexpr uint32_t P_EPI = 16, P_THREADS = 64 + 32 * P_EPI;
+constexpr uint32_t P_COLS = PN / (P_EPI / 4);                   // columns of an epilogue warp
+constexpr uint32_t P_CODES = W_BYTES + PN / 2 * 128;           // a CTA's codes of a k-block
+constexpr uint32_t P_STAGE = P_CODES + SF_BYTES + 2 * SF_BYTES;
+constexpr uint32_t P_STAGES = 6;
+constexpr uint32_t P_SFW = PN, P_SFX = PN + 8;                 // columns of tensor memory
+constexpr uint32_t P_SMEM = 1024 + HEAD + P_STAGES * P_STAGE;
+
+__device__ __forceinline__ void umma_mx4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// in both CTAs, each from its own shared memory to its own tensor memory
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc)
+{
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
+          "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr) : "memory");
+}
+
+// the activation of a thread's values, chosen outside the loops over them
+template <typename F> __device__ __forceinline__ void each(float (&v)[P_COLS], F f)
+{
+#pragma unroll
+    for (int i = 0; i < (int)P_COLS; i++) v[i] = f(v[i]);
+}
+__device__ __forceinline__ void activate_all(float (&v)[P_COLS], int act)
+{
+    switch (act) {
+        case SPG_ACT_RELU:    each(v, [](float x) { return spg_activate(x, SPG_ACT_RELU); }); break;
+        case SPG_ACT_LEAKY:   each(v, [](float x) { return spg_activate(x, SPG_ACT_LEAKY); }); break;
+        case SPG_ACT_SIGMOID: each(v, [](float x) { return spg_activate(x, SPG_ACT_SIGMOID); }); break;
+        case SPG_ACT_TANH:    each(v, [](float x) { return spg_activate(x, SPG_ACT_TANH); }); break;
+        case SPG_ACT_FOO52:   each(v, [](float x) { return spg_activate(x, SPG_ACT_FOO52); }); break;
+        default: break;
+    }
+}
+template <typename T> __device__ __forceinline__ void put_all(const LayerParams &p, const float (&v)[P_COLS], uint32_t n0, uint32_t j)
+{
+    T *y = reinterpret_cast<T *>(p.y) + (uint64_t)n0 * p.ldy + j;
+    const uint32_t rows = p.N - n0;
+#pragma unroll
+    for (int i = 0; i < (int)P_COLS; i++) if ((uint32_t)i < rows) put<T>(y, (uint64_t)i * p.ldy, v[i]);
+}
+
+// tile t of a walk over bands of eight tiles of units, the units fastest inside a band
+__device__ __forceinline__ void pair_tile(uint32_t t, uint32_t j_tiles, uint32_t n_tiles, uint32_t &j, uint32_t &n)
+{
+    const uint32_t band = 8u * n_tiles, g = t / band, r = t % band, here = min(8u, j_tiles - g * 8u);
+    j = g * 8u + r % here; n = r / here;
+}
+
+__global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                                    const __grid_constant__ CUtensorMap map_sw, const __grid_constant__ CUtensorMap map_sx,
+                                                                    const LayerParams p, uint32_t j_tiles, uint32_t n_tiles)
+{
+    extern __shared__ uint8_t raw[];
+    uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t head = smem_u32(base), ring = head + HEAD;
+    const uint32_t full = head, empty = full + 8 * P_STAGES, sums_full = empty + 8 * P_STAGES, sums_free = sums_full + 8, slot = sums_free + 8, aborted = slot + 4;
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head));
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = cluster_rank(), pairs = gridDim.x / 2u, pair = blockIdx.x / 2u, tiles = j_tiles * n_tiles;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < P_STAGES; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        mbar_init(sums_full, 1);
+        mbar_init(sums_free, 2 * P_EPI);
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc_pair(slot, 512);
+    if (warp == 0 && elect_one()) { prefetch_map(&map_w); prefetch_map(&map_x); prefetch_map(&map_sw); prefetch_map(&map_sx); }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
+    spg_grid_wait();
+    volatile int never = 0;
+
+    if (warp == 0) {
+        const uint32_t leader = mapa(full, 0);
+        uint32_t s = 0, phase = 1, issued = 0;
+        for (uint32_t t = pair; t < tiles && !*abort_flag; t += pairs) {
+            uint32_t j, n;
+            pair_tile(t, j_tiles, n_tiles, j, n);
+            for (uint32_t kb = 0; kb < p.kblocks; kb++) {
+                mbar_wait_uniform_cluster(empty + 8 * s, phase, aborted, p.status, 1);
+                if (*abort_flag) break;
+                const uint32_t at = ring + s * P_STAGE, bar = leader + 8 * s;
+                if (elect_one()) {
+                    if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * P_STAGE);
+                    tma_load_2d_pair(at, &map_w, bar, (int)(kb * 128u), (int)(j * 256u + rank * 128u));
+                    tma_load_2d_pair(at + W_BYTES, &map_x, bar, (int)(kb * 128u), (int)(n * PN + rank * (PN / 2)));
+                    tma_load_2d_pair(at + P_CODES, &map_sw, bar, (int)(kb * 256u), (int)(j * 2u + rank));
+                    tma_load_2d_pair(at + P_CODES + SF_BYTES, &map_sx, bar, (int)(kb * 256u), (int)(n * (PN / 128)));
+                }
+                __syncwarp();
+                issued++;
+                if (++s == P_STAGES) { s = 0; phase ^= 1u; }
+            }
+        }
+        if (*abort_flag && rank == 0)            // the copies under way end before the pair does
+            for (uint32_t i = issued > P_STAGES ? issued - P_STAGES : 0; i < issued; i++) mbar_wait(full + 8 * (i % P_STAGES), i / P_STAGES & 1u, &never, p.status, 4, 1u << 12);
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const uint32_t idesc = (idesc_mx4(PN) & ~(31u << 24)) | ((256u >> 4) << 24);
+            uint32_t s = 0, phase = 0, turn = 1;
+            for (uint32_t t = pair; t < tiles; t += pairs) {
+                mbar_wait_uniform_cluster(sums_free, turn, aborted, p.status, 6);
+                turn ^= 1u;
+                tc_fence_after();
+                for (uint32_t kb = 0; kb < p.kblocks; kb++) {
+                    mbar_wait_uniform_cluster(full + 8 * s, phase, aborted, p.status, 2);
+                    if (*abort_flag) break;
+                    tc_fence_after();
+                    const uint32_t at = ring + s * P_STAGE, steps = min(4u, (p.cols - kb * KB + 63u) / 64u);
+                    if (elect_one()) {
+                        const uint32_t sf = at + P_CODES;
+                        for (uint32_t i = 0; i < (steps + 1) / 2; i++) {
+                            copy_scales_pair(tmem + P_SFW + 4 * i, scale_desc(sf + i * SF_TILE));
+                            copy_scales_pair(tmem + P_SFX + 8 * i, scale_desc(sf + SF_BYTES + i * SF_TILE));
+                            copy_scales_pair(tmem + P_SFX + 8 * i + 4, scale_desc(sf + 2 * SF_BYTES + i * SF_TILE));
+                        }
+                        const uint64_t a = smem_desc_sw128(at), b = smem_desc_sw128(at + W_BYTES);
+                        for (uint32_t i = 0; i < steps; i++) {
+                            const uint32_t id = (i & 1u) * 2u;
+                            umma_mx4_pair(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, tmem + P_SFW + 4 * (i / 2), tmem + P_SFX + 8 * (i / 2), kb | i);
+                        }
+                        umma_commit_pair(empty + 8 * s);
+                    }
+                    __syncwarp();
+                    if (++s == P_STAGES) { s = 0; phase ^= 1u; }
+                }
+                if (elect_one()) umma_commit_pair(sums_full);
+                __syncwarp();
+                if (*abort_flag) break;
+            }
+        }
+    } else {
+        const uint32_t quad = warp % 4u, part = (warp - 2u) / 4u, free_at = mapa(sums_free, 0);
+        uint32_t turn = 0;
+        for (uint32_t t = pair; t < tiles; t += pairs) {
+            uint32_t jt, nt;
+            pair_tile(t, j_tiles, n_tiles, jt, nt);
+            const uint32_t j0 = jt * 256u + rank * 128u + quad * 32u, j = j0 + lane, n0 = nt * PN + part * P_COLS;
+            const float bias = p.bias && j < p.out ? __ldg(p.bias + j) : 0.0f;
+            if (!mbar_wait(sums_full, turn, abort_flag, p.status, 3)) { mbar_wait(sums_full, turn, &never, p.status, 5, 1u << 12); break; }
+            turn ^= 1u;
+            tc_fence_after();
+            float v[P_COLS];
+            const uint32_t from = tmem + (quad * 32u << 16) + part * P_COLS;
+#pragma unroll
+            for (int i = 0; i < (int)P_COLS; i += 32) tmem_ld32(from + i, v + i);
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(free_at);
+            if (n0 >= p.N || j0 >= p.out) continue;
+            each(v, [bias](float x) { return x + bias; });
+            activate_all(v, p.act);
+            if (p.y && j < p.out) {
+                if (p.type == SPGK_T_F32) put_all<float>(p, v, n0, j);
+                else if (p.type == SPGK_T_F16) put_all<__half>(p, v, n0, j);
+                else put_all<__nv_bfloat16>(p, v, n0, j);
+            }
+            if (p.next_codes) {
+#pragma unroll
+                for (int i = 0; i < (int)P_COLS; i += 8) {
+                    float q[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) q[k] = j < p.out ? v[i + k] : 0.0f;
+                    if (n0 + i < p.N) put_next(p, q, n0 + i, j0, lane);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) { tc_fence_after(); tmem_free_pair(tmem, 512); }
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// boxes of 256 elements x box_rows rows of a matrix' codes
-int codes_map(CUtensorMap *map, const spgk_mx4 *m, uint32_t box_rows)
+EncodeTiledFn encode_fn()
 {
     static EncodeTiledFn fn = nullptr;
     static std::once_flag once;
@@ -289,18 +487,35 @@ int codes_map(CUtensorMap *map, const spgk_mx4 *m, uint32_t box_rows)
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
             fn = reinterpret_cast<EncodeTiledFn>(f);
     });
+    return fn;
+}
+
+int encode(CUtensorMap *map, CUtensorMapDataType type, void *at, uint64_t width, uint64_t rows, uint64_t pitch, uint32_t box_width, uint32_t box_rows, CUtensorMapSwizzle swizzle)
+{
+    EncodeTiledFn fn = encode_fn();
     if (!fn) { spgk_set_error("cuTensorMapEncodeTiled", "driver entry point not available"); return SPGK_E_CUDA; }
-    const cuuint64_t dims[2] = { spgk_mx4_pitch(m->cols), m->rows }, strides[1] = { m->pitch };
-    const cuuint32_t box[2] = { 128, box_rows }, steps[2] = { 1, 1 };
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, m->codes, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint64_t dims[2] = { width, rows }, strides[1] = { pitch };
+    const cuuint32_t box[2] = { box_width, box_rows }, steps[2] = { 1, 1 };
+    const CUresult r = fn(map, type, 2, at, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         char msg[64];
         snprintf(msg, sizeof msg, "CUresult %d", (int)r);
-        spgk_set_error("cuTensorMapEncodeTiled (4-bit codes)", msg);
+        spgk_set_error("cuTensorMapEncodeTiled (4-bit operand)", msg);
         return SPGK_E_CUDA;
     }
     return SPGK_OK;
+}
+// boxes of 256 elements x box_rows rows of a matrix' codes
+int codes_map(CUtensorMap *map, const spgk_mx4 *m, uint32_t box_rows)
+{
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, m->codes, spgk_mx4_pitch(m->cols), m->rows, m->pitch, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// boxes of two scale tiles (of 256 elements a row) x box_tiles tiles of 128 rows
+int scales_map(CUtensorMap *map, const spgk_mx4 *m, uint32_t box_tiles)
+{
+    const uint64_t kt = spgmx4::tiles4(m->cols);
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, m->scales, kt * 128, ((uint64_t)m->rows + 127) / 128, kt * SF_TILE, 256, box_tiles, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
@@ -334,6 +549,32 @@ template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerPar
     cfg.attrs = attr; cfg.numAttrs = 2;
     SPGK_CUDA(cudaLaunchKernelEx(&cfg, spg_mx4_layer_kernel<NT>, map_w, map_x, p));
     return spgk_check_launch("spg_mx4_layer_kernel");
+}
+
+int launch_pairs(const spgk_mx4 *W, const spgk_mx4 *X, const LayerParams &p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
+{
+    static SpgOncePerDevice once;
+    int rc = once.run(dev, [&]() -> int {
+        SPGK_CUDA(cudaFuncSetAttribute(spg_mx4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P_SMEM));
+        return SPGK_OK;
+    });
+    if (rc) return rc;
+    CUtensorMap map_w, map_x, map_sw, map_sx;
+    if ((rc = codes_map(&map_w, W, TM)) || (rc = codes_map(&map_x, X, PN / 2)) || (rc = scales_map(&map_sw, W, 1)) || (rc = scales_map(&map_sx, X, PN / 128))) return rc;
+    const uint32_t j_tiles = (p.out + 255) / 256, n_tiles = (p.N + PN - 1) / PN;
+    const uint64_t tiles = (uint64_t)j_tiles * n_tiles;
+    if (tiles > 0x3fffffffu) { spgk_set_error("spgk_layer_mx4", "too many tiles"); return SPGK_E_ARG; }
+    const uint32_t pairs = tiles < (uint32_t)dp.sm_count / 2 ? (uint32_t)tiles : (uint32_t)dp.sm_count / 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(pairs * 2); cfg.blockDim = dim3(P_THREADS); cfg.dynamicSmemBytes = P_SMEM; cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    SPGK_CUDA(cudaLaunchKernelEx(&cfg, spg_mx4_pair_kernel, map_w, map_x, map_sw, map_sx, p, j_tiles, n_tiles));
+    return spgk_check_launch("spg_mx4_pair_kernel");
 }
 
 }  // namespace
@@ -372,5 +613,5 @@ extern "C" int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, con
     if (p.N <= 32) return launch<32>(W, X, p, dp, dev, st);
     if (p.N <= 64) return launch<64>(W, X, p, dp, dev, st);
     if (p.N <= 512) return launch<128>(W, X, p, dp, dev, st);
-    return launch<256>(W, X, p, dp, dev, st);
+    return launch_pairs(W, X, p, dp, dev, st);
 }
