@@ -76,30 +76,53 @@ struct Weights {
         if (isinf(top) || l == -INFINITY) return 0;
         return __double2ull_rn(exp(((double)l - m) * inv_t) * (double)(1ull << ONE_BITS));
     }
-    __device__ __forceinline__ uint64_t operator()(float l) const
+    // m * 2^((k >> 10) - 30), with m in [2^30, 2^31)
+    __device__ __forceinline__ uint32_t mantissa(float l, int &k) const
     {
-        if (!fast) return exact(l);
         l = fmaxf(l, floor);
         const float kf = fmaf(l, c_steps, MAGIC);
         const float y = rest(l, kf) - y_top;
-        const int k = __float_as_int(kf) - k_top;            // <= 0
+        k = __float_as_int(kf) - k_top;                      // <= 0
         const uint32_t t = table[k & (int)(STEPS - 1)];
         const float p = y * fmaf(y, 0.24022650695910072f, 0.69314718055994531f);
-        const uint32_t w = t + (uint32_t)__float2int_rn(__uint2float_rn(t) * p);      // [2^30, 2^31)
+        return t + (uint32_t)__float2int_rn(__uint2float_rn(t) * p);
+    }
+    __device__ __forceinline__ uint64_t quick(float l) const
+    {
+        int k;
+        const uint32_t w = mantissa(l, k);
         const int up = (k >> 10) + (ONE_BITS - 30);
         return (uint64_t)(w >> min(max(-up, 0), 31)) * (uint64_t)(1u << max(up, 0));
+    }
+    // Bins of a sixteenth of an octave (-k = 0, 1 .. 64, 65 .. 128 and so on: sixteen of them share k >> 10), the last for all that is lighter; in a bin all
+    // weights are mantissas times the same power of two (in the last one they are counted as they are)
+    __device__ __forceinline__ uint32_t bin(float l) const
+    {
+        const int k = __float_as_int(fmaf(fmaxf(l, floor), c_steps, MAGIC)) - k_top;
+        return min(BINS - 1, (uint32_t)(63 - k) >> 6);
+    }
+    __device__ __forceinline__ uint64_t operator()(float l) const { return fast ? quick(l) : exact(l); }
+    // body(weight) with the one or the other: loops over many logits have no choice inside
+    template <typename F> __device__ __forceinline__ void with(F body) const
+    {
+        if (fast) body([this](float l) { return quick(l); });
+        else body([this](float l) { return exact(l); });
     }
 };
 
 struct Item { float l; uint32_t index; uint64_t w; };
+constexpr uint32_t PIECES = 64;               // of a CTA's slice, in the order of the vocabulary, four a warp
 
 struct alignas(16) Shared {
     uint64_t mass[BINS];
-    uint32_t count[BINS];
-    union { uint32_t list[LIST]; Item few[FEW]; };
+    uint32_t count[BINS], count_low[BINS];
+    union { struct { uint32_t list[LIST]; uint16_t piece[LIST]; }; Item few[FEW]; };
     uint32_t table[STEPS];
+    uint64_t piece_sum[PIECES]; uint32_t piece_equal[PIECES];
+    float dense[WARPS][128];
+    uint32_t left;
     uint64_t out[2][4];                        // what this CTA tells the others, by turns
-    uint64_t warp_a[WARPS], warp_b[WARPS];
+    uint64_t warp[2][WARPS];
     uint32_t listed;
     uint32_t found_bin, found_last; uint64_t found_above; uint32_t found_count;
 };
@@ -119,8 +142,21 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr)
 
 struct Row {
     Shared &s;
-    const float *logits;
-    uint32_t n, split, rank, turn;             // logits of this CTA; CTAs of the row
+    const float4 *packs;                       // this CTA's logits by fours, -infinity in front of the first and behind the last
+    uint32_t count, per_piece;                 // fours, and fours of a piece (a multiple of 32)
+    uint32_t split, rank, turn, place;         // CTAs of the row
+    uint64_t told;
+
+    template <typename F> __device__ __forceinline__ void each(F f) const        // (four at a time, so that their chains of instructions overlap)
+    {
+        for (uint32_t i = threadIdx.x; i < count; i += THREADS) { const float4 v = packs[i]; f(v.x); f(v.y); f(v.z); f(v.w); }
+    }
+    // the fours of piece q of this warp
+    template <typename F> __device__ __forceinline__ void each_of_piece(uint32_t q, F f) const
+    {
+        const uint32_t a = (threadIdx.x / 32 * (PIECES / WARPS) + q) * per_piece, b = min(count, a + per_piece);
+        for (uint32_t i = a + threadIdx.x % 32; i < b; i += 32) { const float4 v = packs[i]; f(v.x); f(v.y); f(v.z); f(v.w); }
+    }
 
     __device__ __forceinline__ void sync() { if (split > 1) spgtc::cluster_sync(); else __syncthreads(); }
     __device__ __forceinline__ uint64_t sum_warp(uint64_t v)
@@ -129,54 +165,55 @@ struct Row {
         for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
     }
-    // over the CTA, to all threads
+    // Over the CTA, to all threads.  The warps' results lie in one of two places by turns: who writes to one again has passed the barrier behind the other.
+    __device__ __forceinline__ uint64_t *warps(uint64_t v, bool mine)
+    {
+        place ^= 1;
+        if (mine) s.warp[place][threadIdx.x / 32] = v;
+        __syncthreads();
+        return s.warp[place];
+    }
     __device__ __forceinline__ uint64_t sum_cta(uint64_t v)
     {
-        v = sum_warp(v);
-        __syncthreads();
-        if (threadIdx.x % 32 == 0) s.warp_a[threadIdx.x / 32] = v;
-        __syncthreads();
+        const uint64_t *w = warps(sum_warp(v), threadIdx.x % 32 == 0);
         uint64_t r = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < WARPS; i++) r += s.warp_a[i];
+        for (uint32_t i = 0; i < WARPS; i++) r += w[i];
         return r;
     }
     __device__ __forceinline__ uint32_t max_cta(uint32_t v)
     {
-        v = __reduce_max_sync(0xffffffffu, v);
-        __syncthreads();
-        if (threadIdx.x % 32 == 0) s.warp_a[threadIdx.x / 32] = v;
-        __syncthreads();
-        uint32_t r = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < WARPS; i++) r = max(r, (uint32_t)s.warp_a[i]);
-        return r;
+        const uint64_t *w = warps(__reduce_max_sync(0xffffffffu, v), threadIdx.x % 32 == 0);
+        return __reduce_max_sync(0xffffffffu, (uint32_t)w[threadIdx.x % WARPS]);
     }
-    __device__ __forceinline__ uint64_t scan_cta(uint64_t v)                     // sum over the threads up to this one
+    // sum over the threads up to this one, and over all
+    __device__ __forceinline__ uint64_t scan_cta(uint64_t v, uint64_t &total)
     {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t u = __shfl_up_sync(0xffffffffu, v, o);
             if (threadIdx.x % 32 >= (uint32_t)o) v += u;
         }
-        __syncthreads();
-        if (threadIdx.x % 32 == 31) s.warp_b[threadIdx.x / 32] = v;
-        __syncthreads();
-        for (uint32_t i = 0; i < threadIdx.x / 32; i++) v += s.warp_b[i];
+        const uint64_t *w = warps(v, threadIdx.x % 32 == 31);
+        total = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < WARPS; i++) { const uint64_t x = w[i]; if (i < threadIdx.x / 32) v += x; total += x; }
         return v;
     }
-    // up to four values of every CTA (the same in all its threads) to every CTA
+    // Up to four values of every CTA (the same in all its threads) to every CTA: a lane fetches one of them, heard() asks it (whole warps)
     __device__ __forceinline__ void tell(uint64_t a, uint64_t b = 0, uint64_t c = 0, uint64_t d = 0)
     {
         turn ^= 1;
         if (threadIdx.x == 0) { s.out[turn][0] = a; s.out[turn][1] = b; s.out[turn][2] = c; s.out[turn][3] = d; }
         sync();
+        const uint32_t from = threadIdx.x % 32 / 4;
+        told = from < split ? ld_cluster_u64(mapa(smem_u32(&s.out[turn][threadIdx.x % 4]), from)) : 0;
     }
-    __device__ __forceinline__ uint64_t heard(uint32_t from, int which) { return ld_cluster_u64(mapa(smem_u32(&s.out[turn][which]), from)); }
+    __device__ __forceinline__ uint64_t heard(uint32_t from, int which) { return __shfl_sync(0xffffffffu, told, from * 4 + which); }
 
     // [lo, hi] to the smallest and largest key in question, of which every CTA has told its own beside how many it has listed; where all are listed,
     // the border is found bit by bit: every thread takes its part of all CTAs' lists
-    template <bool MASS> __device__ void search(const Weights &w, uint32_t &lo, uint32_t &hi, uint32_t many, uint64_t goal, uint64_t &above)
+    template <typename F> __device__ void search(F weight, uint32_t &lo, uint32_t &hi, uint32_t many, uint64_t goal, uint64_t &above)
     {
         lo = 0xffffffffu; hi = 0;
         for (uint32_t r = 0; r < split; r++) { lo = min(lo, (uint32_t)heard(r, 0)); hi = max(hi, (uint32_t)heard(r, 1)); }
@@ -195,84 +232,36 @@ struct Row {
             at += c;
         }
 #pragma unroll
-        for (uint32_t i = 0; i < LIST / THREADS; i++) if (i * THREADS + threadIdx.x < at) weigh[i] = MASS ? w(of_key(mine[i])) : 1;
-        // v = the largest key with amount(>= v) reaching the goal
-        uint32_t bit = 1u << (31 - __clz((int)(hi ^ lo))), v = lo & ~(2u * bit - 1u);
-        for (; bit; bit >>= 1) {
-            const uint32_t trial = v | bit;
-            if (trial > hi) continue;
-            uint64_t a = 0;
+        for (uint32_t i = 0; i < LIST / THREADS; i++) if (i * THREADS + threadIdx.x < at) weigh[i] = weight(of_key(mine[i]));
+        // digit by digit: a bin is 2^shift keys, counted from hi down
+        uint32_t shift = 32 - __clz((int)(hi - lo));
+        shift = shift > 9 ? shift - 9 : 0;
+        for (;;) {
+            __syncthreads();
+            s.mass[threadIdx.x] = 0;
+            __syncthreads();
 #pragma unroll
-            for (uint32_t i = 0; i < LIST / THREADS; i++) if (mine[i] >= trial) a += weigh[i];
-            if (above + sum_cta(a) >= goal) v = trial;
+            for (uint32_t i = 0; i < LIST / THREADS; i++)
+                if (weigh[i] && mine[i] <= hi && mine[i] >= lo) atomicAdd((unsigned long long *)&s.mass[(hi - mine[i]) >> shift], (unsigned long long)weigh[i]);
+            __syncthreads();
+            uint64_t sum;
+            const uint64_t amount = s.mass[threadIdx.x], upto = scan_cta(amount, sum);
+            const uint64_t reach = min(goal, above + sum);
+            if (above + upto - amount < reach && above + upto >= reach && amount) { s.found_bin = threadIdx.x; s.found_above = above + upto - amount; }
+            __syncthreads();
+            above = s.found_above;
+            hi -= s.found_bin << shift;
+            if (shift == 0) break;
+            lo = max(lo, hi - ((1u << shift) - 1));
+            shift = shift > 9 ? shift - 9 : 0;
         }
-        uint64_t a = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < LIST / THREADS; i++) if (mine[i] > v) a += weigh[i];
-        above += sum_cta(a);
-        lo = hi = v;
+        lo = hi;
     }
 
     // The largest key v above `cut` with (amount of keys above v) < goal <= (amount of keys from v on), amounts being counts or weights;
     // goal >= 1 and no more than the amount of all keys above cut.  [lo, hi]: the smallest and the largest key in question.  above: the amount above v.
-    // MASS: `total` the weight of `have` logits at most above cut, share = goal / total
-    template <bool MASS> __device__ uint32_t select(const Weights &w, uint32_t lo, uint32_t hi, uint64_t goal, uint64_t total, uint32_t have, double share, uint64_t &above)
+    template <bool MASS> __device__ uint32_t select(const Weights &w, uint32_t lo, uint32_t hi, uint64_t goal, uint64_t &above, bool first = true)
     {
-        above = 0;
-        bool first = true;
-        if (MASS && w.fast && lo < hi) {
-            // Weights in 32 bits, a unit being 2^-30 of the total; a bin's amount is off by a unit and `off` of itself a logit at most.  Logits whose weights
-            // come to less than (1 - share) / 2 of the total, all of them together, are left aside.
-            const double cd = (double)w.c, one = (double)(1ull << ONE_BITS), light = 0.5 * fmax(1.0 - share, 0.0) * (double)total / (double)have / one;
-            const float least = light > 0.0 ? fmaxf(of_key(lo), (float)(w.m + log(light) / w.inv_t)) : of_key(lo), top = of_key(hi), per = (float)BINS / (top - least);
-            if (share < 1.0 - 1e-7 && per > 0.0f && per < INFINITY) {
-                first = false;
-                const float bias = (float)(30.0 - w.m * cd - log2((double)total / one));
-                const double off = (fabs(w.m) * cd + 130.0) * 0x1p-21 + 0x1p-20, goal_units = (double)goal / (double)total * 0x1p30;
-                const auto bin = [&](float l) { return min(BINS - 1, (uint32_t)((top - l) * per)); };
-                s.count[threadIdx.x] = 0;
-                if (threadIdx.x == 0) s.listed = 0;
-                __syncthreads();
-                for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-                    const float l = logits[i];
-                    if (l >= least && l <= top) {
-                        float e;
-                        asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(fmaf(l, w.c, bias)));
-                        atomicAdd(&s.count[bin(l)], (uint32_t)e);
-                    }
-                }
-                sync();
-                uint32_t amount = 0;
-                for (uint32_t r = 0; r < split; r++) amount += ld_cluster_u32(mapa(smem_u32(&s.count[threadIdx.x]), r));
-                const uint64_t upto = scan_cta(amount);
-                if (threadIdx.x == 0) { s.found_bin = BINS - 1; s.found_last = BINS - 1; }
-                __syncthreads();
-                if (((double)upto + (double)have) >= goal_units * (1.0 - off)) atomicMin(&s.found_bin, threadIdx.x);
-                if ((double)upto >= goal_units * (1.0 + off)) atomicMin(&s.found_last, threadIdx.x);
-                sync();
-                const uint32_t b0 = s.found_bin, b1 = s.found_last;
-                uint64_t over = 0;
-                uint32_t small = 0xffffffffu, large = 0, many = 0;
-                for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-                    const float l = logits[i];
-                    if (!(l >= least && l <= top)) continue;
-                    const uint32_t b = bin(l);
-                    if (b > b1) continue;
-                    if (b < b0) over += w(l);
-                    else {
-                        const uint32_t k = key_of(l), at = atomicAdd(&s.listed, 1u);
-                        small = min(small, k); large = max(large, k);
-                        if (at < LIST) s.list[at] = k;
-                    }
-                }
-                over = sum_cta(over);
-                small = ~max_cta(~small); large = max_cta(large);
-                tell(small, large, s.listed, over);
-                for (uint32_t r = 0; r < split; r++) { many += (uint32_t)heard(r, 2); above += heard(r, 3); }
-                search<MASS>(w, lo, hi, many, goal, above);
-                sync();
-            }
-        }
         for (; lo < hi; first = false) {
             const float top = of_key(hi), bottom = of_key(lo), per = first ? (float)BINS / (top - bottom) : 0.0f;
             const bool even = per > 0.0f && per < INFINITY;                      // bins of equal width in the logits, else in the keys
@@ -284,40 +273,157 @@ struct Row {
             s.count[threadIdx.x] = 0; s.mass[threadIdx.x] = 0;
             if (threadIdx.x == 0) s.listed = 0;
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-                const float l = logits[i];
-                if (!(l >= bottom && l <= top)) continue;
+            each([&](float l) {
+                if (!(l >= bottom && l <= top)) return;
                 const uint32_t b = bin(l);
                 atomicAdd(&s.count[b], 1u);
                 if (MASS) atomicAdd((unsigned long long *)&s.mass[b], (unsigned long long)w(l));
-            }
+            });
             sync();
             // the bin in which the goal is reached: a thread a bin
             uint64_t amount = 0; uint32_t count = 0;
-            for (uint32_t r = 0; r < split; r++) {
+#pragma unroll
+            for (uint32_t r = 0; r < MAX_SPLIT; r++) {
+                if (r >= split) continue;
                 const uint32_t c = ld_cluster_u32(mapa(smem_u32(&s.count[threadIdx.x]), r));
                 count += c;
                 amount += MASS ? ld_cluster_u64(mapa(smem_u32(&s.mass[threadIdx.x]), r)) : c;
             }
-            const uint64_t upto = scan_cta(amount);
-            if (above + upto - amount < goal && above + upto >= goal && amount) { s.found_bin = threadIdx.x; s.found_above = above + upto - amount; s.found_count = count; }
+            uint64_t sum;
+            const uint64_t upto = scan_cta(amount, sum);
+            const uint64_t reach = min(goal, above + sum);
+            if (above + upto - amount < reach && above + upto >= reach && amount) { s.found_bin = threadIdx.x; s.found_above = above + upto - amount; s.found_count = count; }
             sync();                                                              // (the others have read this CTA's bins)
             const uint32_t b = s.found_bin, many = s.found_count;
             above = s.found_above;
             uint32_t small = 0xffffffffu, large = 0;
-            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-                const float l = logits[i];
-                if (!(l >= bottom && l <= top) || bin(l) != b) continue;
+            each([&](float l) {
+                if (!(l >= bottom && l <= top) || bin(l) != b) return;
                 const uint32_t k = key_of(l);
                 small = min(small, k); large = max(large, k);
                 if (many <= LIST) s.list[atomicAdd(&s.listed, 1u)] = k;
-            }
+            });
             small = ~max_cta(~small); large = max_cta(large);
             tell(small, large, s.listed);
-            search<MASS>(w, lo, hi, many, goal, above);
+            search([&](float l) -> uint64_t { return MASS ? w(l) : 1; }, lo, hi, many, goal, above);
             sync();                                                              // (lists and bins are free again)
         }
         return lo;
+    }
+
+    // Cuts what is left -- the logits above `cut` and `ties` equal to it -- after the shortest beginning with `share` of its weight.  Two passes: the bins' weights
+    // (sums of mantissas in two halves of 32 bits), then a list of the border's bin and, a piece at a time, the sums of what is above it.
+    // Returns whether the pieces have the sums of what is above the new cut and the numbers of logits equal to it.
+    __device__ bool mass_cut(const Weights &w, float share, uint32_t &cut, uint32_t &ties)
+    {
+        const float over = of_key(cut);
+        s.count[threadIdx.x] = 0; s.count_low[threadIdx.x] = 0;
+        if (threadIdx.x == 0) s.listed = 0;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+            const float4 v = packs[i];
+            const float l[4] = { v.x, v.y, v.z, v.w };
+            uint32_t m[4], at[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                int k;
+                m[j] = w.mantissa(l[j], k);
+                at[j] = min(BINS - 1, (uint32_t)(63 - k) >> 6);
+                if (at[j] == BINS - 1) m[j] >>= min(-(k >> 10) - (ONE_BITS - 30), 31);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) if (l[j] > over) { atomicAdd(&s.count_low[at[j]], m[j] & 0xffffu); atomicAdd(&s.count[at[j]], m[j] >> 16); }
+        }
+        sync();
+        uint64_t low = 0, high = 0;
+#pragma unroll
+        for (uint32_t r = 0; r < MAX_SPLIT; r++) {
+            if (r >= split) continue;
+            low += ld_cluster_u32(mapa(smem_u32(&s.count_low[threadIdx.x]), r));
+            high += ld_cluster_u32(mapa(smem_u32(&s.count[threadIdx.x]), r));
+        }
+        const auto up_of = [](uint32_t bin) -> int { return bin == BINS - 1 ? 0 : ONE_BITS - 30 - (int)((bin + 15) >> 4); };
+        const int up = up_of(threadIdx.x);
+        uint64_t amount = (high << 16) + low, total;
+        amount = up >= 0 ? amount << up : amount >> -up;
+        const uint64_t upto = scan_cta(amount, total), one_tie = ties ? w.quick(over) : 0;
+        const double want = ceil((double)share * (double)(total + ties * one_tie));
+        const uint64_t goal = want >= 1.0 ? (uint64_t)want : 1;
+        if (upto - amount < goal && upto >= goal) { s.found_bin = threadIdx.x; s.found_above = upto - amount; }
+        sync();                                                                  // (the others have read this CTA's bins)
+        if (total < goal) {
+            ties = (uint32_t)min((uint64_t)ties, (goal - total + one_tie - 1) / max(one_tie, (uint64_t)1));
+            return false;
+        }
+        const uint32_t border = s.found_bin;
+        const int border_up = up_of(border);
+        // the goal in the units of the border's bin
+        uint64_t rest = goal - s.found_above;
+        rest = border_up >= 0 ? (rest + ((1ull << border_up) - 1)) >> border_up : rest << -border_up;
+        // few of a piece's logits are so large: 128 at a time, the warp puts them side by side first
+        const float bottom = border == BINS - 1 ? -INFINITY : w.top - (float)(border * 64 + 2) / (w.c * (float)STEPS) - 1e-6f * fabsf(w.top);
+        float *const dense = s.dense[threadIdx.x / 32];
+        const uint32_t lane = threadIdx.x % 32;
+        uint32_t small = 0xffffffffu, large = 0, many = 0, sure = 0;
+        for (uint32_t q = 0; q < PIECES / WARPS; q++) {
+            const uint32_t piece = threadIdx.x / 32 * (PIECES / WARPS) + q, a = piece * per_piece, b = min(this->count, a + per_piece);
+            uint64_t sum = 0;
+            for (uint32_t i0 = a; i0 < b; i0 += 32) {
+                const float4 v = i0 + lane < b ? packs[i0 + lane] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                const float l[4] = { v.x, v.y, v.z, v.w };
+                uint32_t held = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const bool in = l[j] > over && l[j] >= bottom;
+                    const uint32_t set = __ballot_sync(0xffffffffu, in);
+                    if (in) dense[held + __popc(set & ((1u << lane) - 1))] = l[j];
+                    held += __popc(set);
+                }
+                __syncwarp();
+                for (uint32_t i = lane; i < held; i += 32) {
+                    const float x = dense[i];
+                    const uint32_t at_bin = w.bin(x);
+                    if (at_bin < border) { sum += w.quick(x); sure++; }
+                    else if (at_bin == border) {
+                        const uint32_t k = key_of(x), at = atomicAdd(&s.listed, 1u);
+                        small = min(small, k); large = max(large, k);
+                        if (at < LIST) { s.list[at] = k; s.piece[at] = (uint16_t)piece; }
+                    }
+                }
+                __syncwarp();
+            }
+            sum = sum_warp(sum);
+            if (lane == 0) { s.piece_sum[piece] = sum; s.piece_equal[piece] = 0; }
+        }
+        if (threadIdx.x == 0) s.left = 0;
+        small = ~max_cta(~small); large = max_cta(large);
+        sure = __reduce_add_sync(0xffffffffu, sure);
+        if (lane == 0) atomicAdd(&s.left, sure);
+        tell(small, large, s.listed);
+        for (uint32_t r = 0; r < split; r++) many += (uint32_t)heard(r, 2);
+        uint64_t above = 0;
+        const auto weight = [&](float l) -> uint64_t { int k; return border == BINS - 1 ? w.quick(l) : w.mantissa(l, k); };
+        uint32_t lo, hi;
+        search(weight, lo, hi, many, rest, above);
+        const bool listed = many <= LIST;
+        if (lo < hi) {                                                           // too many for the list
+            above = s.found_above;
+            sync();
+            lo = select<true>(w, lo, hi, goal, above, false);
+            const uint64_t one = w(of_key(lo));
+            cut = lo; ties = (uint32_t)((goal > above ? goal - above + one - 1 : one) / one);
+            return false;
+        }
+        const uint64_t one = weight(of_key(lo));
+        cut = lo; ties = (uint32_t)((rest - above + one - 1) / one);
+        if (listed)
+            for (uint32_t i = threadIdx.x; i < s.listed; i += THREADS) {
+                const uint32_t k = s.list[i], piece = s.piece[i];
+                if (k > lo) { atomicAdd((unsigned long long *)&s.piece_sum[piece], (unsigned long long)w.quick(of_key(k))); atomicAdd(&s.left, 1u); }
+                else if (k == lo) atomicAdd(&s.piece_equal[piece], 1u);
+            }
+        sync();
+        return listed;
     }
 };
 
@@ -337,13 +443,24 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
     const uint32_t row = blockIdx.x / p.split, rank = blockIdx.x % p.split, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t from = min(p.width, rank * p.slice), n = min(p.width - from, p.slice);
     for (uint32_t i = threadIdx.x; i < STEPS; i += THREADS) s.table[i] = __double2uint_rn(exp2((double)i / STEPS) * (double)(1u << 30));
+    spg_grid_trigger();
     spg_grid_wait();
+
+    const float t = p.temperature ? p.temperature[row] : 1.0f;
+    const bool greedy = !(t > 0.0f);
+    const int32_t k = p.top_k ? p.top_k[row] : 0;
+    const float pp = p.top_p ? p.top_p[row] : 1.0f, mp = p.min_p ? p.min_p[row] : 0.0f, number = p.u[row];
 
     // The row, its largest and smallest logits and how many there are: 16 bytes a load between the ends that do not lie on 16 bytes
     const T *x = reinterpret_cast<const T *>(p.logits) + (uint64_t)row * p.ld + from;
     constexpr uint32_t PER = 16 / sizeof(T);
     const uint32_t off = (uint32_t)((uintptr_t)x % 16u / sizeof(T)), first = min(n, (PER - off) % PER), packs = (n - first) / PER;
-    logits += (4u - first % 4u) % 4u;                                            // packs lie on 16 bytes here too
+    const uint32_t lead = (4u - first % 4u) % 4u;                                // packs lie on 16 bytes here too
+    if (threadIdx.x < 8) {                                                       // what makes the first and the last four whole
+        if (threadIdx.x < lead) logits[threadIdx.x] = -INFINITY;
+        else if (threadIdx.x >= 4 && threadIdx.x - 4 < (4u - (lead + n) % 4u) % 4u) logits[lead + n + threadIdx.x - 4] = -INFINITY;
+    }
+    float *const row_logits = logits + lead;
     float mine = -INFINITY, least = INFINITY;
     uint32_t have = 0;
     const auto take = [&](float l) -> float {
@@ -357,13 +474,14 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
         *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(x + first) + i);
 #pragma unroll
         for (uint32_t j = 0; j < PER; j += 4)
-            *reinterpret_cast<float4 *>(logits + first + i * PER + j) = make_float4(take(to_f32(v[j])), take(to_f32(v[j + 1])), take(to_f32(v[j + 2])), take(to_f32(v[j + 3])));
+            *reinterpret_cast<float4 *>(row_logits + first + i * PER + j) = make_float4(take(to_f32(v[j])), take(to_f32(v[j + 1])), take(to_f32(v[j + 2])), take(to_f32(v[j + 3])));
     }
     if (threadIdx.x < 2 * PER) {                                                 // the ends
         const uint32_t i = threadIdx.x < PER ? threadIdx.x : first + packs * PER + threadIdx.x - PER;
-        if (i < (threadIdx.x < PER ? first : n)) logits[i] = take(to_f32(x[i]));
+        if (i < (threadIdx.x < PER ? first : n)) row_logits[i] = take(to_f32(x[i]));
     }
-    Row R{ s, logits, n, p.split, rank, 0 };
+    const uint32_t fours = (lead + n + 3u) / 4u;
+    Row R{ s, reinterpret_cast<const float4 *>(logits), fours, ((fours + PIECES - 1) / PIECES + 31u) / 32u * 32u, p.split, rank, 0, 0, 0 };
     uint32_t top = R.max_cta(key_of(mine)), low = ~R.max_cta(~key_of(least));
     have = (uint32_t)R.sum_cta(have);
     R.tell(top, low, have);
@@ -371,33 +489,40 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
     for (uint32_t r = 0; r < p.split; r++) { top = max(top, (uint32_t)R.heard(r, 0)); low = min(low, (uint32_t)R.heard(r, 1)); all += (uint32_t)R.heard(r, 2); }
     const float largest = of_key(top);
 
-    const float t = p.temperature ? p.temperature[row] : 1.0f;
-    const bool greedy = !(t > 0.0f);
-    const int32_t k = p.top_k ? p.top_k[row] : 0;
-    const float pp = p.top_p ? p.top_p[row] : 1.0f, mp = p.min_p ? p.min_p[row] : 0.0f;
     const double log_min_p = mp > 0.0f ? log((double)mp) : -INFINITY;
-    const double u = p.u[row] > 0.0f ? (double)p.u[row] : 0.0;
+    const double u = number > 0.0f ? (double)number : 0.0;
     Weights w;
     w.set(largest, greedy ? 1.0f : t, s.table);
 
     if (all && !greedy && k >= 1 && (uint32_t)k < all && (uint32_t)k <= FEW / 2) {
-        // the k / split largest threads' largest of every CTA: at least k logits of the row are no smaller than the least of them
-        const uint32_t want = ((uint32_t)k + p.split - 1) / p.split, key = key_of(mine);
-        uint32_t bound = 0;
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-            const uint32_t c = (uint32_t)__syncthreads_count(key >= (bound | bit));
-            if (c >= want) bound |= bit;
-            if (c == want) break;
-        }
-        if (threadIdx.x == 0) s.listed = 0;
-        R.tell(bound);
+        // At least k logits of the row are no smaller than the least of the CTAs' (k / split)-th largest of their threads' largest; a bin's lower end will do
+        const uint32_t want = ((uint32_t)k + p.split - 1) / p.split;
+        s.count[threadIdx.x] = 0;
+        if (threadIdx.x == 0) { s.listed = 0; s.found_bin = BINS; }
+        const bool some = mine > -INFINITY;
+        const float best = of_key(R.max_cta(key_of(mine))), worst = of_key(~R.max_cta(some ? ~key_of(mine) : 0)), width = (best - worst) * (1.0f / BINS);
+        const bool even = width > 0.0f && width < INFINITY;                      // (else they are all equal: no bound)
+        if (even && some) atomicAdd(&s.count[min(BINS - 1, (uint32_t)((best - mine) / width))], 1u);
+        __syncthreads();
+        uint64_t threads;
+        const uint32_t c = s.count[threadIdx.x], upto = (uint32_t)R.scan_cta(c, threads);
+        if (even && upto >= want && upto - c < want) s.found_bin = threadIdx.x;
+        __syncthreads();
+        const float end = best - ((float)s.found_bin + 1.001f) * width - 1e-6f * (fabsf(best) + fabsf(worst));
+        R.tell(key_of(s.found_bin < BINS && end > -FLT_MAX ? end : -FLT_MAX));
+        uint32_t bound = 0xffffffffu;
         for (uint32_t r = 0; r < p.split; r++) bound = min(bound, (uint32_t)R.heard(r, 0));
-        const float at_least = bound > key_of(-INFINITY) ? of_key(bound) : -FLT_MAX;
-        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-            const float l = logits[i];
-            if (l >= at_least) {
-                const uint32_t at = atomicAdd(&s.listed, 1u);
-                if (at < FEW) { s.few[at].l = l; s.few[at].index = from + i; }
+        const float at_least = of_key(bound);
+        for (uint32_t i = threadIdx.x; i < fours; i += THREADS) {
+            const float4 v = R.packs[i];
+            if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= at_least) {
+                const float l[4] = { v.x, v.y, v.z, v.w };
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++)
+                    if (l[j] >= at_least) {
+                        const uint32_t at = atomicAdd(&s.listed, 1u);
+                        if (at < FEW) { s.few[at].l = l[j]; s.few[at].index = from + 4 * i + j - lead; }
+                    }
             }
         }
         __syncthreads();
@@ -419,13 +544,17 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
                 }
                 __syncthreads();
                 if (threadIdx.x < many) s.few[threadIdx.x] = me;
+                if (threadIdx.x >= many && threadIdx.x < (many + 7) / 8 * 8) s.few[threadIdx.x] = me;       // (nothing, behind the last)
                 __syncthreads();
                 uint32_t place = 0;
                 uint64_t before = 0;
                 if (warp * 32 < many)
-                    for (uint32_t i = 0; i < many; i++) {
-                        const Item o = s.few[i];
-                        if (o.l > me.l || (o.l == me.l && o.index < me.index)) { place++; before += o.w; }
+                    for (uint32_t i = 0; i < many; i += 8) {
+                        Item o[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) o[j] = s.few[i + j];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) if (o[j].l > me.l || (o[j].l == me.l && o[j].index < me.index)) { place++; before += o[j].w; }
                     }
                 bool keep = threadIdx.x < many && place < (uint32_t)k;
                 if (pp < 1.0f) {
@@ -441,9 +570,13 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
                 const uint64_t goal = goal_d >= (double)(total - 1) ? total - 1 : (uint64_t)goal_d;
                 uint64_t upto = 0;
                 if (warp * 32 < many)
-                    for (uint32_t i = 0; i < many; i++) {
-                        const Item o = s.few[i];
-                        if (o.index <= me.index) upto += o.w;
+                    for (uint32_t i = 0; i < many; i += 8) {
+                        uint32_t index[8];
+                        uint64_t weigh[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) { index[j] = s.few[i + j].index; weigh[j] = s.few[i + j].w; }
+#pragma unroll
+                        for (int j = 0; j < 8; j++) if (index[j] <= me.index) upto += weigh[j];
                     }
                 if (me.w && upto > goal && upto - me.w <= goal) {
                     p.tokens[row] = (int32_t)me.index;
@@ -458,22 +591,22 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
 
     // what is left: logits above `cut`, and the first `ties` equal to it
     uint32_t cut = key_of(-INFINITY), ties = 0;
+    bool summed = false;
     if (all && greedy) { cut = top; ties = 1; }
     if (all && !greedy) {
         if (k >= 1 && (uint32_t)k < all) {
-            uint64_t above;
-            cut = R.select<false>(w, low, top, (uint64_t)k, 0, 0, 0.0, above);
+            uint64_t above = 0;
+            cut = R.select<false>(w, low, top, (uint64_t)k, above);
             ties = (uint32_t)(k - above);
         }
-        if (pp < 1.0f) {
+        if (pp < 1.0f && w.fast) summed = R.mass_cut(w, pp, cut, ties);
+        else if (pp < 1.0f) {
             uint64_t sum = 0;
-            uint32_t nearest = 0xffffffffu;
             const float over = of_key(cut);
-            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-                const float l = logits[i];
-                if (l > over) { sum += w(l); nearest = min(nearest, key_of(l)); }
-            }
-            sum = R.sum_cta(sum); nearest = ~R.max_cta(~nearest);
+            float close = INFINITY;
+            R.each([&](float l) { if (l > over) { sum += w.exact(l); close = fminf(close, l); } });
+            sum = R.sum_cta(sum);
+            uint32_t nearest = ~R.max_cta(~key_of(close));
             R.tell(sum, nearest);
             sum = 0; nearest = 0xffffffffu;
             for (uint32_t r = 0; r < p.split; r++) { sum += R.heard(r, 0); nearest = min(nearest, (uint32_t)R.heard(r, 1)); }
@@ -482,14 +615,14 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
             const uint64_t goal = want >= 1.0 ? (uint64_t)want : 1;
             if (sum < goal) ties = (uint32_t)min((uint64_t)ties, (goal - sum + each - 1) / max(each, (uint64_t)1));
             else {
-                uint64_t above;
-                cut = R.select<true>(w, nearest, top, goal, sum, all, (double)goal / (double)sum, above);
+                uint64_t above = 0;
+                cut = R.select<true>(w, nearest, top, goal, above);
                 const uint64_t one = w(of_key(cut));
                 ties = (uint32_t)((goal - above + one - 1) / one);
             }
         }
         if (mp > 0.0f) {
-            if (mp > 1.0f) { cut = top; ties = 1; }
+            if (mp > 1.0f) { cut = top; ties = 1; summed = false; }
             else {
                 // the smallest key whose weight is at least mp, by halving: from a guess on both sides where that brackets it
                 uint32_t a = key_of(-INFINITY), b = top;                         // a: too light, b: heavy enough
@@ -502,98 +635,104 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
                     const uint32_t mid = a + (b - a) / 2;
                     if (heavy(w, of_key(mid), log_min_p)) b = mid; else a = mid;
                 }
-                if (b - 1 >= cut) { cut = b - 1; ties = 0; }
+                if (b - 1 >= cut) { cut = b - 1; ties = 0; summed = false; }
             }
         }
     }
 
-    // Sums of what is left, for every warp's part of the slice (parts lie in the order of the vocabulary) and its quarters
-    constexpr uint32_t PIECES = 4;
+    // Sums of what is left and numbers of logits equal to the cut, for every piece
     const float over = of_key(cut);
-    const uint32_t piece = ((n + WARPS - 1) / WARPS + PIECES * 32 - 1) / (PIECES * 32) * 32, begin = min(n, warp * piece * PIECES), end = min(n, begin + piece * PIECES);
-    uint32_t equal = 0, left = 0;
-    uint64_t sums[PIECES];
-    uint32_t equals[PIECES];
-#pragma unroll
-    for (uint32_t q = 0; q < PIECES; q++) {
-        const uint32_t a = min(end, begin + q * piece), b = min(end, a + piece);
-        uint64_t sum = 0;
-        uint32_t same = 0;
-        for (uint32_t i = a + lane; i < b; i += 32) {
-            const float l = logits[i];
-            if (l > over) { sum += w(l); left++; }
-            same += ties && l == over;
-        }
-        sums[q] = R.sum_warp(sum);
-        equals[q] = __reduce_add_sync(0xffffffffu, same);
-        equal += equals[q];
-    }
-    left = __reduce_add_sync(0xffffffffu, left);
-    uint32_t equal_before = 0;
-    if (ties) {                                                                  // (the same in all threads of the cluster)
+    if (!summed) {
         __syncthreads();
-        if (lane == 0) s.warp_b[warp] = equal;
+        if (threadIdx.x == 0) s.left = 0;
         __syncthreads();
-        uint32_t equal_cta = 0;
-        for (uint32_t i = 0; i < WARPS; i++) { if (i < warp) equal_before += (uint32_t)s.warp_b[i]; equal_cta += (uint32_t)s.warp_b[i]; }
-        R.tell(equal_cta);
-        for (uint32_t r = 0; r < rank; r++) equal_before += (uint32_t)R.heard(r, 0);
+        uint32_t left = 0;
+        w.with([&](auto weight) {
+            for (uint32_t q = 0; q < PIECES / WARPS; q++) {
+                uint64_t sum = 0;
+                uint32_t same = 0;
+                R.each_of_piece(q, [&](float l) {
+                    const uint64_t one = weight(l);
+                    if (l > over) { sum += one; left++; }
+                    same += l == over;
+                });
+                sum = R.sum_warp(sum);
+                same = __reduce_add_sync(0xffffffffu, same);
+                if (lane == 0) { s.piece_sum[warp * (PIECES / WARPS) + q] = sum; s.piece_equal[warp * (PIECES / WARPS) + q] = same; }
+            }
+        });
+        left = __reduce_add_sync(0xffffffffu, left);
+        if (lane == 0) atomicAdd(&s.left, left);
     }
+    __syncthreads();
+    // the ties that are left are the first in the order of the vocabulary
     const uint64_t each = ties ? w(over) : 0;
-    uint64_t sum = 0;
-    uint32_t seen = equal_before;
-#pragma unroll
-    for (uint32_t q = 0; q < PIECES; q++) {
-        const uint32_t here = ties > seen ? min(equals[q], ties - seen) : 0;
-        seen += equals[q];
-        left += here;
-        sums[q] += here * each;
-        sum += sums[q];
+    const uint32_t equal = ties && threadIdx.x < PIECES ? s.piece_equal[threadIdx.x] : 0;
+    uint32_t equal_before = 0, taken = 0;
+    if (ties) {                                                                  // (the same in all threads of the cluster)
+        uint64_t here;
+        const uint32_t upto = (uint32_t)R.scan_cta(equal, here);
+        R.tell(here);
+        equal_before = upto - equal;
+        for (uint32_t r = 0; r < rank; r++) equal_before += (uint32_t)R.heard(r, 0);
+        taken = ties > equal_before ? min(equal, ties - equal_before) : 0;
     }
-    __syncthreads();
-    if (lane == 0) { s.warp_a[warp] = sum; s.warp_b[warp] = left; }
-    __syncthreads();
-    uint64_t before = 0, cta = 0, left_cta = 0;
-    for (uint32_t i = 0; i < WARPS; i++) { if (i < warp) before += s.warp_a[i]; cta += s.warp_a[i]; left_cta += s.warp_b[i]; }
-    R.tell(cta, left_cta);
-    uint64_t total = 0, left_all = 0;
-    for (uint32_t r = 0; r < p.split; r++) { if (r < rank) before += R.heard(r, 0); total += R.heard(r, 0); left_all += R.heard(r, 1); }
+    uint64_t cta;
+    const uint64_t amount = (threadIdx.x < PIECES ? s.piece_sum[threadIdx.x] : 0) + taken * each, upto = R.scan_cta(amount, cta);
+    const uint32_t left = s.left + (ties ? (uint32_t)R.sum_cta(taken) : 0);
+    R.tell(cta, left);
+    uint64_t before = 0, total = 0, left_all = 0;
+    for (uint32_t r = 0; r < p.split; r++) { const uint64_t c = R.heard(r, 0); if (r < rank) before += c; total += c; left_all += R.heard(r, 1); }
 
     if (total == 0) {
         if (rank == 0 && threadIdx.x == 0) { p.tokens[row] = -1; if (p.probs) p.probs[row] = 0.0f; if (p.kept) p.kept[row] = 0; }
     } else {
         const double goal_d = u * (double)total;
         const uint64_t goal = goal_d >= (double)(total - 1) ? total - 1 : (uint64_t)goal_d;
-        if (before <= goal && goal < before + sum) {                             // in this warp's part: in which quarter, and where
-            uint64_t run = before;
-            uint32_t a = begin;
-            seen = equal_before;
+        if (before <= goal && goal < before + cta) {                             // in this CTA: in which piece, and where
+            if (before + upto - amount <= goal && goal < before + upto) { s.found_bin = threadIdx.x; s.found_above = before + upto - amount; s.found_count = equal_before; }
+            __syncthreads();
+            if (warp == 0) {
+                uint64_t run = s.found_above;
+                uint32_t seen = s.found_count;
+                const uint32_t a = s.found_bin * R.per_piece, b = min(fours, a + R.per_piece);
+                for (uint32_t i0 = a; i0 < b; i0 += 32) {
+                    const uint32_t i = i0 + lane;
+                    const float4 four = i < b ? R.packs[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    const float l[4] = { four.x, four.y, four.z, four.w };
+                    uint64_t one[4], mine4 = 0;
+                    uint32_t same = 0;
 #pragma unroll
-            for (uint32_t q = 0; q + 1 < PIECES; q++)
-                if (a == min(end, begin + q * piece) && run + sums[q] <= goal) { run += sums[q]; seen += equals[q]; a = min(end, begin + (q + 1) * piece); }
-            for (uint32_t i0 = a; i0 < end; i0 += 32) {
-                const uint32_t i = i0 + lane;
-                const float l = i < end ? logits[i] : -INFINITY;
-                const uint32_t same = __ballot_sync(0xffffffffu, ties && l == over);
-                const bool tie = ties && l == over && seen + __popc(same & ((1u << lane) - 1)) < ties;
-                const uint64_t one = l > over ? w(l) : (tie ? each : 0);
-                uint64_t upto = one;
+                    for (int j = 0; j < 4; j++) same += ties && l[j] == over;
+                    uint32_t tie = same;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= (uint32_t)o) upto += v;
-                }
-                const uint32_t past = __ballot_sync(0xffffffffu, run + upto > goal);
-                if (past) {
-                    if (lane == (uint32_t)__ffs((int)past) - 1) {
-                        p.tokens[row] = (int32_t)(from + i);
-                        if (p.probs) p.probs[row] = (float)((double)one / (double)total);
-                        if (p.kept) p.kept[row] = (int32_t)left_all;
+                    for (int o = 1; o < 32; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, tie, o); if (lane >= (uint32_t)o) tie += v; }
+                    const uint32_t ties_here = __shfl_sync(0xffffffffu, tie, 31);
+                    tie += seen - same;                                          // equal logits in front of this lane's
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        one[j] = l[j] > over ? w(l[j]) : (ties && l[j] == over && tie++ < ties ? each : 0);
+                        mine4 += one[j];
                     }
-                    break;
+                    uint64_t past = mine4;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) { const uint64_t v = __shfl_up_sync(0xffffffffu, past, o); if (lane >= (uint32_t)o) past += v; }
+                    const uint32_t over_goal = __ballot_sync(0xffffffffu, run + past > goal);
+                    if (over_goal) {
+                        if (lane == (uint32_t)__ffs((int)over_goal) - 1) {
+                            uint64_t sum = run + past - mine4;
+                            int j = 0;
+                            uint64_t w1 = one[0];
+                            if (sum + w1 <= goal) { sum += w1; j = 1; w1 = one[1]; if (sum + w1 <= goal) { sum += w1; j = 2; w1 = one[2]; if (sum + w1 <= goal) { j = 3; w1 = one[3]; } } }
+                            p.tokens[row] = (int32_t)(from + 4 * i + j - lead);
+                            if (p.probs) p.probs[row] = (float)((double)w1 / (double)total);
+                            if (p.kept) p.kept[row] = (int32_t)left_all;
+                        }
+                        break;
+                    }
+                    run += __shfl_sync(0xffffffffu, past, 31);
+                    seen += ties_here;
                 }
-                run += __shfl_sync(0xffffffffu, upto, 31);
-                seen += __popc(same);
             }
         }
     }
@@ -613,7 +752,7 @@ template <typename T> int launch(SampleParams p, const SpgDeviceProps &dp, int d
     p.slice = ((p.width + p.split - 1) / p.split + 7u) / 8u * 8u;
     if ((uint64_t)p.N * p.split > 0x7fffffffu) { spgk_set_error("spgk_sample_rows", "too many rows"); return SPGK_E_ARG; }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.N * p.split); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = sizeof(Shared) + (size_t)p.slice * 4 + 16; cfg.stream = stream;
+    cfg.gridDim = dim3(p.N * p.split); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = sizeof(Shared) + (size_t)p.slice * 4 + 32; cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = p.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
