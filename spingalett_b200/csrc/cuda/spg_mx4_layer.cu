@@ -28,6 +28,7 @@ constexpr uint32_t THREADS = 192;             // warp 0: copies, warp 1: product
 constexpr uint32_t MAX_STAGES = 8;
 constexpr uint32_t MAX_SPLIT = 8;
 constexpr uint32_t HEAD = 1024;
+constexpr uint32_t ROOM_FOR_TWO = 112 * 1024;     // shared memory of a CTA that leaves room for one of the next launch
 
 struct LayerParams {
     uint32_t N, out, cols, kblocks, kt;       // rows, units, inputs; k-blocks; scale tiles of a row
@@ -61,11 +62,9 @@ __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr)
 {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(128u >> 4) << 16 | (uint64_t)(128u >> 4) << 32 | (uint64_t)1u << 46;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
+__device__ __forceinline__ void ld_cluster_4(uint32_t addr, float *v)
 {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr)
 {
@@ -106,33 +105,67 @@ __device__ __forceinline__ void put_next(const LayerParams &p, const float (&v)[
     }
 }
 
-// columns c0 .. c0 + 8 of the tile (rows n0 ... of the batch) for this lane's unit
-__device__ __forceinline__ void finish8(const LayerParams &p, float (&v)[8], uint32_t n0, uint32_t j0, uint32_t lane, float bias)
+// C rows' sums of this lane's unit to outputs.  What is chosen -- activation, type -- is chosen outside the loops over them: an epilogue runs a few times a
+// CTA and its instructions come from L2 as it runs (chosen inside, 128 columns took 36 000 cycles).
+template <int C, typename F> __device__ __forceinline__ void each(float (&v)[C], F f)
+{
+#pragma unroll
+    for (int i = 0; i < C; i++) v[i] = f(v[i]);
+}
+template <int C> __device__ __forceinline__ void activate(float (&v)[C], int act)
+{
+    switch (act) {
+        case SPG_ACT_RELU:    each(v, [](float x) { return spg_activate(x, SPG_ACT_RELU); }); break;
+        case SPG_ACT_LEAKY:   each(v, [](float x) { return spg_activate(x, SPG_ACT_LEAKY); }); break;
+        case SPG_ACT_SIGMOID: each(v, [](float x) { return spg_activate(x, SPG_ACT_SIGMOID); }); break;
+        case SPG_ACT_TANH:    each(v, [](float x) { return spg_activate(x, SPG_ACT_TANH); }); break;
+        case SPG_ACT_FOO52:   each(v, [](float x) { return spg_activate(x, SPG_ACT_FOO52); }); break;
+        default: break;
+    }
+}
+template <typename T, int C> __device__ __forceinline__ void put_rows(const LayerParams &p, const float (&v)[C], uint32_t n0, uint32_t j)
+{
+    T *y = reinterpret_cast<T *>(p.y) + (uint64_t)n0 * p.ldy + j;
+    const uint32_t rows = p.N - n0;
+#pragma unroll
+    for (int i = 0; i < C; i++) if ((uint32_t)i < rows) put<T>(y, (uint64_t)i * p.ldy, v[i]);
+}
+template <int C> __device__ __forceinline__ void finish(const LayerParams &p, float (&v)[C], uint32_t n0, uint32_t j0, uint32_t lane, float bias)
 {
     const uint32_t j = j0 + lane;
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = j < p.out ? spg_activate(v[i] + bias, p.act) : 0.0f;
+    each(v, [bias](float x) { return x + bias; });
+    activate(v, p.act);
     if (p.y && j < p.out) {
+        if (p.type == SPGK_T_F32) put_rows<float>(p, v, n0, j);
+        else if (p.type == SPGK_T_F16) put_rows<__half>(p, v, n0, j);
+        else put_rows<__nv_bfloat16>(p, v, n0, j);
+    }
+    if (p.next_codes) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (n0 + i >= p.N) break;
-            const uint64_t at = (uint64_t)(n0 + i) * p.ldy + j;
-            if (p.type == SPGK_T_F32) put<float>(p.y, at, v[i]);
-            else if (p.type == SPGK_T_F16) put<__half>(p.y, at, v[i]);
-            else put<__nv_bfloat16>(p.y, at, v[i]);
+        for (int i = 0; i < C; i += 8) {
+            float q[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) q[k] = j < p.out ? v[i + k] : 0.0f;
+            if (n0 + i < p.N) put_next(p, q, n0 + i, j0, lane);
         }
     }
-    if (p.next_codes) put_next(p, v, n0, j0, lane);
+}
+
+__device__ __forceinline__ void prefetch_l2(const CUtensorMap *map, int c0, int c1)
+{
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
 }
 
 template <uint32_t NT> struct Tile {
     static constexpr uint32_t X_BYTES = NT * 128;
     static constexpr uint32_t SFX_TILES = (NT + 127) / 128;
+    static constexpr uint32_t PART = NT + 4;                                   // floats from a unit's sums to the next one's, where CTAs share a tile
     static constexpr uint32_t STAGE = (W_BYTES + X_BYTES + SF_BYTES + SFX_TILES * SF_BYTES + 1023) / 1024 * 1024;
     static constexpr uint32_t SFX_COLS = NT < 128 ? 4 : NT / 32;              // columns of the rows' scales for four blocks
     static constexpr uint32_t SFW = NT < 32 ? 16 : NT;                         // tensor memory: sums, weights' scales, rows' scales
-    static constexpr uint32_t SFX = SFW + 8;
-    static constexpr uint32_t USED = SFX + 2 * SFX_COLS;
+    static constexpr uint32_t SFX = 8;                                         // (behind the weights' scales)
+    static constexpr uint32_t SF_COLS = 8 + 2 * SFX_COLS;                      // of a k-block, twice: copied while the products of the one before run
+    static constexpr uint32_t USED = SFW + 2 * SF_COLS;
     static constexpr uint32_t COLS = USED <= 32 ? 32 : USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
 };
 
@@ -161,7 +194,12 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
+    spg_grid_trigger();
+    // the first weights to L2 while the kernel in front still runs (whoever writes them: L2 is where writes meet)
+    if (warp == 0 && elect_one())
+        for (uint32_t kb = lo; kb < hi && kb < lo + p.stages; kb++) prefetch_l2(&map_w, (int)(kb * 128u), (int)(j_tile * TM));
+    __syncwarp();
     spg_grid_wait();
     volatile int never = 0;
 
@@ -192,19 +230,19 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
             mbar_wait_uniform(full + 8 * s, phase, aborted, p.status, 2);
             if (*abort_flag) break;
             tc_fence_after();
-            const uint32_t at = ring + s * L::STAGE, steps = min(4u, (p.cols - kb * KB + 63u) / 64u);
+            const uint32_t at = ring + s * L::STAGE, steps = min(4u, (p.cols - kb * KB + 63u) / 64u), sf = tmem + L::SFW + ((kb - lo) & 1u) * L::SF_COLS;
             if (elect_one()) {
                 const uint32_t sfw = at + W_BYTES + L::X_BYTES, sfx = sfw + SF_BYTES;
                 for (uint32_t i = 0; i < (steps + 1) / 2; i++) {
-                    copy_scales(tmem + L::SFW + 4 * i, scale_desc(sfw + i * SF_TILE));
+                    copy_scales(sf + 4 * i, scale_desc(sfw + i * SF_TILE));
 #pragma unroll
                     for (uint32_t t = 0; t < L::SFX_TILES; t++)
-                        copy_scales(tmem + L::SFX + L::SFX_COLS * i + 4 * t, scale_desc(sfx + t * SF_BYTES + i * SF_TILE));
+                        copy_scales(sf + L::SFX + L::SFX_COLS * i + 4 * t, scale_desc(sfx + t * SF_BYTES + i * SF_TILE));
                 }
                 const uint64_t a = smem_desc_sw128(at), b = smem_desc_sw128(at + W_BYTES);
                 for (uint32_t i = 0; i < steps; i++) {
                     const uint32_t id = (i & 1u) * 2u;          // which two of a tile's four scales
-                    umma_mx4(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, tmem + L::SFW + 4 * (i / 2), tmem + L::SFX + L::SFX_COLS * (i / 2), kb > lo || i > 0);
+                    umma_mx4(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, sf + 4 * (i / 2), sf + L::SFX + L::SFX_COLS * (i / 2), kb > lo || i > 0);
                 }
                 umma_commit(empty + 8 * s);
             }
@@ -224,25 +262,23 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
             if (ok && !*abort_flag) {
                 for (uint32_t c = 0; c < NT && n0 + c < p.N; c += 16) {
                     uint32_t r[16];
+                    float v[16];
                     tmem_ld16(lanes + c, r);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int h = 0; h < 16; h += 8) {
-                        float v[8];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[h + i]);
-                        finish8(p, v, n0 + c + h, j0, lane, bias);
-                    }
+                    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+                    finish(p, v, n0 + c, j0, lane, bias);
                 }
             }
         } else {
-            // this CTA's sums, [column][unit], into its own shared memory (no copy or product is under way any more)
-            for (uint32_t c = 0; c < NT; c += 16) {
+            // this CTA's sums, [unit][column], into its own shared memory (no copy or product is under way any more)
+            for (uint32_t c = 0; c < NT && n0 + c < p.N; c += 16) {
                 uint32_t r[16];
                 tmem_ld16(lanes + c, r);
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 16; i++) *reinterpret_cast<uint32_t *>(base + HEAD + ((c + i) * TM + quad * 32u + lane) * 4u) = r[i];
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<uint4 *>(base + HEAD + ((quad * 32u + lane) * L::PART + c + i) * 4u) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
             }
         }
         tc_fence_before();
@@ -257,15 +293,22 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
             for (uint32_t r = 0; r < p.split; r++) ok = ok && ld_cluster_u32(mapa(aborted, r)) == 0;
             if (ok) {
                 for (uint32_t c = rank * 8u; c < NT && n0 + c < p.N; c += p.split * 8u) {
-                    float v[8];
+                    float part[MAX_SPLIT][8], v[8];                              // all on their way before the first is needed
+                    const uint32_t at = ring + ((quad * 32u + lane) * L::PART + c) * 4u;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = 0.0f;
-                    for (uint32_t r = 0; r < p.split; r++) {
-                        const uint32_t from = mapa(ring + (c * TM + quad * 32u + lane) * 4u, r);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] += ld_cluster_f32(from + i * TM * 4u);
+                    for (uint32_t r = 0; r < MAX_SPLIT; r++) {
+                        each(part[r], [](float) { return 0.0f; });
+                        if (r < p.split) ld_cluster_4(mapa(at, r), part[r]);
+                        if (r < p.split && n0 + c + 4 < p.N) ld_cluster_4(mapa(at, r) + 16, part[r] + 4);
                     }
-                    finish8(p, v, n0 + c, j0, lane, bias);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] = part[0][i];
+#pragma unroll
+                    for (uint32_t r = 1; r < MAX_SPLIT; r++) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[i] += part[r][i];
+                    }
+                    finish(p, v, n0 + c, j0, lane, bias);
                 }
             }
         }
@@ -285,7 +328,7 @@ constexpr uint32_t P_COLS = PN / (P_EPI / 4);                   // columns of an
 constexpr uint32_t P_CODES = W_BYTES + PN / 2 * 128;           // a CTA's codes of a k-block
 constexpr uint32_t P_STAGE = P_CODES + SF_BYTES + 2 * SF_BYTES;
 constexpr uint32_t P_STAGES = 6;
-constexpr uint32_t P_SFW = PN, P_SFX = PN + 8;                 // columns of tensor memory
+constexpr uint32_t P_SF = PN, P_SFX = 8, P_SF_COLS = 24;        // columns of tensor memory: scales behind the sums, twice; those of the rows behind the weights'
 constexpr uint32_t P_SMEM = 1024 + HEAD + P_STAGES * P_STAGE;
 
 __device__ __forceinline__ void umma_mx4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate)
@@ -309,31 +352,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v)
           "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
           "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
         : "r"(taddr) : "memory");
-}
-
-// the activation of a thread's values, chosen outside the loops over them
-template <typename F> __device__ __forceinline__ void each(float (&v)[P_COLS], F f)
-{
-#pragma unroll
-    for (int i = 0; i < (int)P_COLS; i++) v[i] = f(v[i]);
-}
-__device__ __forceinline__ void activate_all(float (&v)[P_COLS], int act)
-{
-    switch (act) {
-        case SPG_ACT_RELU:    each(v, [](float x) { return spg_activate(x, SPG_ACT_RELU); }); break;
-        case SPG_ACT_LEAKY:   each(v, [](float x) { return spg_activate(x, SPG_ACT_LEAKY); }); break;
-        case SPG_ACT_SIGMOID: each(v, [](float x) { return spg_activate(x, SPG_ACT_SIGMOID); }); break;
-        case SPG_ACT_TANH:    each(v, [](float x) { return spg_activate(x, SPG_ACT_TANH); }); break;
-        case SPG_ACT_FOO52:   each(v, [](float x) { return spg_activate(x, SPG_ACT_FOO52); }); break;
-        default: break;
-    }
-}
-template <typename T> __device__ __forceinline__ void put_all(const LayerParams &p, const float (&v)[P_COLS], uint32_t n0, uint32_t j)
-{
-    T *y = reinterpret_cast<T *>(p.y) + (uint64_t)n0 * p.ldy + j;
-    const uint32_t rows = p.N - n0;
-#pragma unroll
-    for (int i = 0; i < (int)P_COLS; i++) if ((uint32_t)i < rows) put<T>(y, (uint64_t)i * p.ldy, v[i]);
 }
 
 // tile t of a walk over bands of eight tiles of units, the units fastest inside a band
@@ -368,6 +386,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
+    spg_grid_trigger();
     spg_grid_wait();
     volatile int never = 0;
 
@@ -407,18 +426,18 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
                     mbar_wait_uniform_cluster(full + 8 * s, phase, aborted, p.status, 2);
                     if (*abort_flag) break;
                     tc_fence_after();
-                    const uint32_t at = ring + s * P_STAGE, steps = min(4u, (p.cols - kb * KB + 63u) / 64u);
+                    const uint32_t at = ring + s * P_STAGE, steps = min(4u, (p.cols - kb * KB + 63u) / 64u), to = tmem + P_SF + (kb & 1u) * P_SF_COLS;
                     if (elect_one()) {
                         const uint32_t sf = at + P_CODES;
                         for (uint32_t i = 0; i < (steps + 1) / 2; i++) {
-                            copy_scales_pair(tmem + P_SFW + 4 * i, scale_desc(sf + i * SF_TILE));
-                            copy_scales_pair(tmem + P_SFX + 8 * i, scale_desc(sf + SF_BYTES + i * SF_TILE));
-                            copy_scales_pair(tmem + P_SFX + 8 * i + 4, scale_desc(sf + 2 * SF_BYTES + i * SF_TILE));
+                            copy_scales_pair(to + 4 * i, scale_desc(sf + i * SF_TILE));
+                            copy_scales_pair(to + P_SFX + 8 * i, scale_desc(sf + SF_BYTES + i * SF_TILE));
+                            copy_scales_pair(to + P_SFX + 8 * i + 4, scale_desc(sf + 2 * SF_BYTES + i * SF_TILE));
                         }
                         const uint64_t a = smem_desc_sw128(at), b = smem_desc_sw128(at + W_BYTES);
                         for (uint32_t i = 0; i < steps; i++) {
                             const uint32_t id = (i & 1u) * 2u;
-                            umma_mx4_pair(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, tmem + P_SFW + 4 * (i / 2), tmem + P_SFX + 8 * (i / 2), kb | i);
+                            umma_mx4_pair(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, to + 4 * (i / 2), to + P_SFX + 8 * (i / 2), kb | i);
                         }
                         umma_commit_pair(empty + 8 * s);
                     }
@@ -450,22 +469,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(free_at);
             if (n0 >= p.N || j0 >= p.out) continue;
-            each(v, [bias](float x) { return x + bias; });
-            activate_all(v, p.act);
-            if (p.y && j < p.out) {
-                if (p.type == SPGK_T_F32) put_all<float>(p, v, n0, j);
-                else if (p.type == SPGK_T_F16) put_all<__half>(p, v, n0, j);
-                else put_all<__nv_bfloat16>(p, v, n0, j);
-            }
-            if (p.next_codes) {
-#pragma unroll
-                for (int i = 0; i < (int)P_COLS; i += 8) {
-                    float q[8];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) q[k] = j < p.out ? v[i + k] : 0.0f;
-                    if (n0 + i < p.N) put_next(p, q, n0 + i, j0, lane);
-                }
-            }
+            finish(p, v, n0, j0, lane, bias);
         }
     }
     __syncthreads();
@@ -533,11 +537,12 @@ template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerPar
     const uint64_t tiles = (uint64_t)j_tiles * n_tiles;
     p.split = 1;
     if (NT <= 128) while (p.split < MAX_SPLIT && tiles * p.split * 2 <= (uint32_t)dp.sm_count && p.kblocks >= p.split * 4) p.split *= 2;
-    const uint32_t most = (uint32_t)(dp.smem_optin - HEAD - 1024) / L::STAGE, mine = (p.kblocks + p.split - 1) / p.split;
+    const uint32_t room = NT <= 64 ? ROOM_FOR_TWO : (uint32_t)dp.smem_optin;
+    const uint32_t most = (room - HEAD - 1024) / L::STAGE, mine = (p.kblocks + p.split - 1) / p.split;
     p.stages = mine < most ? mine : most;
     if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
     uint32_t bytes = p.stages * L::STAGE;
-    if (p.split > 1 && bytes < NT * TM * 4u) bytes = NT * TM * 4u;
+    if (p.split > 1 && bytes < L::PART * TM * 4u) bytes = L::PART * TM * 4u;
     if (n_tiles > 65535u) { spgk_set_error("spgk_layer_mx4", "more than 65535 tiles of rows"); return SPGK_E_ARG; }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(j_tiles * p.split, n_tiles); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = HEAD + 1024 + bytes; cfg.stream = stream;
