@@ -228,21 +228,31 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         const uint32_t idesc = idesc_mx4(NT);
         for (uint32_t kb = lo, s = 0, phase = 0; kb < hi; kb++) {
             mbar_wait_uniform(full + 8 * s, phase, aborted, p.status, 2);
-            if (*abort_flag) break;
             tc_fence_after();
-            const uint32_t at = ring + s * L::STAGE, steps = min(4u, (p.cols - kb * KB + 63u) / 64u), sf = tmem + L::SFW + ((kb - lo) & 1u) * L::SF_COLS;
+            const uint32_t at = ring + s * L::STAGE, sf = tmem + L::SFW + ((kb - lo) & 1u) * L::SF_COLS;
             if (elect_one()) {
+                // (written out: a whole k-block takes 800 cycles to issue from loops that end at run time)
                 const uint32_t sfw = at + W_BYTES + L::X_BYTES, sfx = sfw + SF_BYTES;
-                for (uint32_t i = 0; i < (steps + 1) / 2; i++) {
-                    copy_scales(sf + 4 * i, scale_desc(sfw + i * SF_TILE));
+                const uint64_t dw = scale_desc(sfw), dx = scale_desc(sfx), a = smem_desc_sw128(at), b = smem_desc_sw128(at + W_BYTES);
+                const auto scales = [&](uint32_t i) {
+                    copy_scales(sf + 4 * i, dw + i * (SF_TILE >> 4));
 #pragma unroll
-                    for (uint32_t t = 0; t < L::SFX_TILES; t++)
-                        copy_scales(sf + L::SFX + L::SFX_COLS * i + 4 * t, scale_desc(sfx + t * SF_BYTES + i * SF_TILE));
-                }
-                const uint64_t a = smem_desc_sw128(at), b = smem_desc_sw128(at + W_BYTES);
-                for (uint32_t i = 0; i < steps; i++) {
+                    for (uint32_t t = 0; t < L::SFX_TILES; t++) copy_scales(sf + L::SFX + L::SFX_COLS * i + 4 * t, dx + ((t * SF_BYTES + i * SF_TILE) >> 4));
+                };
+                const auto product = [&](uint32_t i, uint32_t more) {
                     const uint32_t id = (i & 1u) * 2u;          // which two of a tile's four scales
-                    umma_mx4(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, sf + 4 * (i / 2), sf + L::SFX + L::SFX_COLS * (i / 2), kb > lo || i > 0);
+                    umma_mx4(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, sf + 4 * (i / 2), sf + L::SFX + L::SFX_COLS * (i / 2), more);
+                };
+                if (kb * KB + KB - 64u < p.cols) {
+                    scales(0); scales(1);
+                    product(0, kb > lo); product(1, 1); product(2, 1); product(3, 1);
+                } else {
+                    const uint32_t steps = (p.cols - kb * KB + 63u) / 64u;
+                    scales(0);
+                    if (steps > 2) scales(1);
+                    product(0, kb > lo);
+                    if (steps > 1) product(1, 1);
+                    if (steps > 2) product(2, 1);
                 }
                 umma_commit(empty + 8 * s);
             }
@@ -424,20 +434,29 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
                 tc_fence_after();
                 for (uint32_t kb = 0; kb < p.kblocks; kb++) {
                     mbar_wait_uniform_cluster(full + 8 * s, phase, aborted, p.status, 2);
-                    if (*abort_flag) break;
                     tc_fence_after();
-                    const uint32_t at = ring + s * P_STAGE, steps = min(4u, (p.cols - kb * KB + 63u) / 64u), to = tmem + P_SF + (kb & 1u) * P_SF_COLS;
+                    const uint32_t at = ring + s * P_STAGE, to = tmem + P_SF + (kb & 1u) * P_SF_COLS;
                     if (elect_one()) {
-                        const uint32_t sf = at + P_CODES;
-                        for (uint32_t i = 0; i < (steps + 1) / 2; i++) {
-                            copy_scales_pair(to + 4 * i, scale_desc(sf + i * SF_TILE));
-                            copy_scales_pair(to + P_SFX + 8 * i, scale_desc(sf + SF_BYTES + i * SF_TILE));
-                            copy_scales_pair(to + P_SFX + 8 * i + 4, scale_desc(sf + 2 * SF_BYTES + i * SF_TILE));
-                        }
-                        const uint64_t a = smem_desc_sw128(at), b = smem_desc_sw128(at + W_BYTES);
-                        for (uint32_t i = 0; i < steps; i++) {
+                        const uint64_t sf = scale_desc(at + P_CODES), a = smem_desc_sw128(at), b = smem_desc_sw128(at + W_BYTES);
+                        const auto scales = [&](uint32_t i) {
+                            copy_scales_pair(to + 4 * i, sf + i * (SF_TILE >> 4));
+                            copy_scales_pair(to + P_SFX + 8 * i, sf + ((SF_BYTES + i * SF_TILE) >> 4));
+                            copy_scales_pair(to + P_SFX + 8 * i + 4, sf + ((2 * SF_BYTES + i * SF_TILE) >> 4));
+                        };
+                        const auto product = [&](uint32_t i, uint32_t more) {
                             const uint32_t id = (i & 1u) * 2u;
-                            umma_mx4_pair(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, to + 4 * (i / 2), to + P_SFX + 8 * (i / 2), kb | i);
+                            umma_mx4_pair(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, to + 4 * (i / 2), to + P_SFX + 8 * (i / 2), more);
+                        };
+                        if (kb * KB + KB - 64u < p.cols) {
+                            scales(0); scales(1);
+                            product(0, kb); product(1, 1); product(2, 1); product(3, 1);
+                        } else {
+                            const uint32_t steps = (p.cols - kb * KB + 63u) / 64u;
+                            scales(0);
+                            if (steps > 2) scales(1);
+                            product(0, kb);
+                            if (steps > 1) product(1, 1);
+                            if (steps > 2) product(2, 1);
                         }
                         umma_commit_pair(empty + 8 * s);
                     }
