@@ -24,7 +24,7 @@ constexpr uint32_t KB = 256;                  // elements of a k-block
 constexpr uint32_t W_BYTES = TM * 128;        // codes of a tile's weights
 constexpr uint32_t SF_TILE = 512;             // scales of 128 rows x 4 blocks
 constexpr uint32_t SF_BYTES = 2 * SF_TILE;    // of 128 rows in a k-block
-constexpr uint32_t THREADS = 192;             // warp 0: copies, warp 1: products, warps 2 to 5: outputs
+constexpr uint32_t EPI = 8, THREADS = 64 + 32 * EPI;   // warp 0: copies, warp 1: products, warps 2 to 9: outputs, two a quarter of the lanes
 constexpr uint32_t MAX_STAGES = 8;
 constexpr uint32_t MAX_SPLIT = 8;
 constexpr uint32_t HEAD = 1024;
@@ -73,14 +73,21 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr)
     return v;
 }
 
-template <typename T> __device__ __forceinline__ void put(void *y, uint64_t at, float v);
-template <> __device__ __forceinline__ void put<float>(void *y, uint64_t at, float v) { reinterpret_cast<float *>(y)[at] = v; }
-template <> __device__ __forceinline__ void put<__half>(void *y, uint64_t at, float v) { reinterpret_cast<__half *>(y)[at] = __float2half_rn(v); }
-template <> __device__ __forceinline__ void put<__nv_bfloat16>(void *y, uint64_t at, float v) { reinterpret_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v); }
+// (predicated: branches around the stores cost 80 cycles each)
+__device__ __forceinline__ void put(float *y, float v, uint32_t yes)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.f32 [%0], %1;\n\t}" ::"l"(y), "f"(v), "r"(yes) : "memory");
+}
+__device__ __forceinline__ void put16(void *y, uint16_t v, uint32_t yes)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.u16 [%0], %1;\n\t}" ::"l"(y), "h"(v), "r"(yes) : "memory");
+}
+__device__ __forceinline__ void put(__half *y, float v, uint32_t yes) { put16(y, __half_as_ushort(__float2half_rn(v)), yes); }
+__device__ __forceinline__ void put(__nv_bfloat16 *y, float v, uint32_t yes) { put16(y, __bfloat16_as_ushort(__float2bfloat16_rn(v)), yes); }
 
 // Eight rows' values of this lane's unit, the warp's 32 units being one block of the next layer's input: scales, codes, stores.
 // A lane's eight codes are eight nibbles of a word, one a row; three exchanges among eight lanes turn that into eight nibbles of one row.
-__device__ __forceinline__ void put_next(const LayerParams &p, const float (&v)[8], uint32_t n0, uint32_t j0, uint32_t lane)
+__device__ __forceinline__ void put_next(const LayerParams &p, const float (&v)[8], uint32_t n0, uint32_t rows, uint32_t j0, uint32_t lane)
 {
     float q[8];
     uint32_t mine = 0;
@@ -98,8 +105,8 @@ __device__ __forceinline__ void put_next(const LayerParams &p, const float (&v)[
         w = (lane & s) ? ((w & ~low) | ((other >> bits) & low)) : ((w & low) | ((other & low) << bits));
     }
     const uint32_t n = n0 + lane % 8u, j = j0 + lane / 8u * 8u;
-    if (n < p.N && j0 < (p.out + 31u) / 32u * 32u) *reinterpret_cast<uint32_t *>(p.next_codes + (uint64_t)n * p.next_pitch + j / 2u) = w;
-    if (lane < 8u && n0 + lane < p.N) {
+    if (lane % 8u < rows && j0 < (p.out + 31u) / 32u * 32u) *reinterpret_cast<uint32_t *>(p.next_codes + (uint64_t)n * p.next_pitch + j / 2u) = w;
+    if (lane < 8u && lane < rows) {
         const uint32_t row = n0 + lane;
         p.next_scales[((uint64_t)(row / 128u) * p.next_kt + j0 / 128u) * SF_TILE + spgmx4::scale_in_tile(row) + j0 % 128u / 32u] = (uint8_t)mine;
     }
@@ -123,22 +130,22 @@ template <int C> __device__ __forceinline__ void activate(float (&v)[C], int act
         default: break;
     }
 }
-template <typename T, int C> __device__ __forceinline__ void put_rows(const LayerParams &p, const float (&v)[C], uint32_t n0, uint32_t j)
+template <typename T, int C> __device__ __forceinline__ void put_rows(const LayerParams &p, const float (&v)[C], uint32_t n0, uint32_t rows, uint32_t j)
 {
     T *y = reinterpret_cast<T *>(p.y) + (uint64_t)n0 * p.ldy + j;
-    const uint32_t rows = p.N - n0;
 #pragma unroll
-    for (int i = 0; i < C; i++) if ((uint32_t)i < rows) put<T>(y, (uint64_t)i * p.ldy, v[i]);
+    for (int i = 0; i < C; i++, y += p.ldy) put(y, v[i], (uint32_t)i < rows && j < p.out);
 }
-template <int C> __device__ __forceinline__ void finish(const LayerParams &p, float (&v)[C], uint32_t n0, uint32_t j0, uint32_t lane, float bias)
+// (rows: how many of them there are; with none it only brings its instructions to the SM)
+template <int C> __device__ __forceinline__ void finish(const LayerParams &p, float (&v)[C], uint32_t n0, uint32_t rows, uint32_t j0, uint32_t lane, float bias)
 {
     const uint32_t j = j0 + lane;
     each(v, [bias](float x) { return x + bias; });
     activate(v, p.act);
-    if (p.y && j < p.out) {
-        if (p.type == SPGK_T_F32) put_rows<float>(p, v, n0, j);
-        else if (p.type == SPGK_T_F16) put_rows<__half>(p, v, n0, j);
-        else put_rows<__nv_bfloat16>(p, v, n0, j);
+    if (p.y) {
+        if (p.type == SPGK_T_F32) put_rows<float>(p, v, n0, rows, j);
+        else if (p.type == SPGK_T_F16) put_rows<__half>(p, v, n0, rows, j);
+        else put_rows<__nv_bfloat16>(p, v, n0, rows, j);
     }
     if (p.next_codes) {
 #pragma unroll
@@ -146,9 +153,14 @@ template <int C> __device__ __forceinline__ void finish(const LayerParams &p, fl
             float q[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) q[k] = j < p.out ? v[i + k] : 0.0f;
-            if (n0 + i < p.N) put_next(p, q, n0 + i, j0, lane);
+            put_next(p, q, n0 + i, rows > (uint32_t)i ? rows - i : 0, j0, lane);
         }
     }
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
 }
 
 __device__ __forceinline__ void prefetch_l2(const CUtensorMap *map, int c0, int c1)
@@ -200,7 +212,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
     if (warp == 0 && elect_one())
         for (uint32_t kb = lo; kb < hi && kb < lo + p.stages; kb++) prefetch_l2(&map_w, (int)(kb * 128u), (int)(j_tile * TM));
     __syncwarp();
-    spg_grid_wait();
+    if (warp < 2) spg_grid_wait();
     volatile int never = 0;
 
     if (warp == 0) {
@@ -262,48 +274,43 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         if (elect_one()) umma_commit(done);
         __syncwarp();
     } else {
-        const uint32_t quad = warp % 4u, j0 = j_tile * TM + quad * 32u, j = j0 + lane;
-        const float bias = p.bias && j < p.out ? __ldg(p.bias + j) : 0.0f;
-        const bool ok = mbar_wait(done, 0, abort_flag, p.status, 3);
-        if (!ok) mbar_wait(done, 0, &never, p.status, 5);        // the products under way end before tensor memory is given back
-        tc_fence_after();
+        const uint32_t quad = warp % 4u, half = (warp - 2u) / 4u, j0 = j_tile * TM + quad * 32u, j = j0 + lane;
         const uint32_t lanes = tmem + (quad * 32u << 16);
-        if (p.split == 1) {
-            if (ok && !*abort_flag) {
-                for (uint32_t c = 0; c < NT && n0 + c < p.N; c += 16) {
-                    uint32_t r[16];
-                    float v[16];
-                    tmem_ld16(lanes + c, r);
-                    tmem_ld_wait();
+        // Once without a row before the launch in front has ended: the outputs' instructions come from L2, some 1500 cycles that would follow the products
+        float bias = 0.0f;
+        bool ok = true;
+#pragma unroll 1
+        for (uint32_t dry = 1;; dry = 0) {
+            if (!dry) {
+                spg_grid_wait();
+                if (p.bias && j < p.out) bias = __ldg(p.bias + j);
+                ok = mbar_wait(done, 0, abort_flag, p.status, 3);
+                if (!ok) mbar_wait(done, 0, &never, p.status, 5);                // the products under way end before tensor memory is given back
+                tc_fence_after();
+                if (p.split > 1) {
+                    // this CTA's sums, [unit][column], into its own shared memory (no copy or product is under way any more)
+                    for (uint32_t c = half * 16u; c < NT && n0 + c < p.N; c += 32) {
+                        uint32_t r[16];
+                        tmem_ld16(lanes + c, r);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
-                    finish(p, v, n0 + c, j0, lane, bias);
+                        for (int i = 0; i < 16; i += 4)
+                            *reinterpret_cast<uint4 *>(base + HEAD + ((quad * 32u + lane) * L::PART + c + i) * 4u) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+                    }
+                    cluster_sync();
+                    for (uint32_t r = 0; r < p.split; r++) ok = ok && ld_cluster_u32(mapa(aborted, r)) == 0;
                 }
+                if (!ok) break;
             }
-        } else {
-            // this CTA's sums, [unit][column], into its own shared memory (no copy or product is under way any more)
-            for (uint32_t c = 0; c < NT && n0 + c < p.N; c += 16) {
-                uint32_t r[16];
-                tmem_ld16(lanes + c, r);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<uint4 *>(base + HEAD + ((quad * 32u + lane) * L::PART + c + i) * 4u) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
-            }
-        }
-        tc_fence_before();
-    }
-    __syncthreads();
-    if (p.split > 1) {
-        cluster_sync();
-        if (warp >= 2) {
-            const uint32_t quad = warp % 4u, j0 = j_tile * TM + quad * 32u, j = j0 + lane;
-            const float bias = p.bias && j < p.out ? __ldg(p.bias + j) : 0.0f;
-            bool ok = true;
-            for (uint32_t r = 0; r < p.split; r++) ok = ok && ld_cluster_u32(mapa(aborted, r)) == 0;
-            if (ok) {
-                for (uint32_t c = rank * 8u; c < NT && n0 + c < p.N; c += p.split * 8u) {
-                    float part[MAX_SPLIT][8], v[8];                              // all on their way before the first is needed
+            const uint32_t end = dry ? n0 + 1 : p.N;
+#pragma unroll 1
+            for (uint32_t c = dry ? 0 : (half * p.split + rank) * 8u; c < NT && n0 + c < end; c += p.split * 16u) {
+                float v[8];
+                if (p.split == 1 || dry) {
+                    if (!dry) { tmem_ld8(lanes + c, v); tmem_ld_wait(); }
+                    else each(v, [](float) { return 0.0f; });
+                } else {
+                    float part[MAX_SPLIT][8];                                    // all on their way before the first is needed
                     const uint32_t at = ring + ((quad * 32u + lane) * L::PART + c) * 4u;
 #pragma unroll
                     for (uint32_t r = 0; r < MAX_SPLIT; r++) {
@@ -318,12 +325,18 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
 #pragma unroll
                         for (int i = 0; i < 8; i++) v[i] += part[r][i];
                     }
-                    finish(p, v, n0 + c, j0, lane, bias);
                 }
+                finish(p, v, n0 + c, dry ? 0u : p.N - (n0 + c), j0, lane, bias);
             }
+            if (!dry) break;
         }
-        cluster_sync();
+        tc_fence_before();
     }
+    if (p.split > 1) {
+        if (warp < 2) cluster_sync();
+        cluster_sync();                                                          // (nobody leaves while its sums are read)
+    }
+    __syncthreads();
     if (warp == 1) { tc_fence_after(); tmem_free(tmem, L::COLS); }
 }
 
@@ -397,7 +410,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
     spg_grid_trigger();
-    spg_grid_wait();
+    if (warp < 2) spg_grid_wait();
     volatile int never = 0;
 
     if (warp == 0) {
@@ -470,25 +483,47 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
         }
     } else {
         const uint32_t quad = warp % 4u, part = (warp - 2u) / 4u, free_at = mapa(sums_free, 0);
-        uint32_t turn = 0;
-        for (uint32_t t = pair; t < tiles; t += pairs) {
+        uint32_t turn = 0, dry = 1;                                              // (dry: once without a row, as above)
+#pragma unroll 1
+        for (uint32_t t = pair; t < tiles;) {
             uint32_t jt, nt;
             pair_tile(t, j_tiles, n_tiles, jt, nt);
             const uint32_t j0 = jt * 256u + rank * 128u + quad * 32u, j = j0 + lane, n0 = nt * PN + part * P_COLS;
-            const float bias = p.bias && j < p.out ? __ldg(p.bias + j) : 0.0f;
-            if (!mbar_wait(sums_full, turn, abort_flag, p.status, 3)) { mbar_wait(sums_full, turn, &never, p.status, 5, 1u << 12); break; }
-            turn ^= 1u;
-            tc_fence_after();
-            float v[P_COLS];
+            const float bias = !dry && p.bias && j < p.out ? __ldg(p.bias + j) : 0.0f;
             const uint32_t from = tmem + (quad * 32u << 16) + part * P_COLS;
+            if (!dry) {
+                if (!mbar_wait(sums_full, turn, abort_flag, p.status, 3)) { mbar_wait(sums_full, turn, &never, p.status, 5, 1u << 12); break; }
+                turn ^= 1u;
+                tc_fence_after();
+            }
+            if (dry || t + pairs >= tiles) {
+                // the last: nobody waits for tensor memory, and a short loop is quicker than 64 columns written out that come from L2
+#pragma unroll 1
+                for (uint32_t c = 0; c < (dry ? 1u : P_COLS) && (dry || (n0 + c < p.N && j0 < p.out)); c += 16) {
+                    uint32_t r[16];
+                    float v[16];
+                    each(v, [](float) { return 0.0f; });
+                    if (!dry) {
+                        tmem_ld16(from + c, r);
+                        tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < (int)P_COLS; i += 32) tmem_ld32(from + i, v + i);
-            tmem_ld_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(free_at);
-            if (n0 >= p.N || j0 >= p.out) continue;
-            finish(p, v, n0, j0, lane, bias);
+                        for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+                    }
+                    finish(p, v, n0 + c, dry ? 0u : p.N - (n0 + c), j0, lane, bias);
+                }
+                tc_fence_before();
+                if (dry) { dry = 0; spg_grid_wait(); continue; }
+            } else {
+                float v[P_COLS];
+#pragma unroll
+                for (int i = 0; i < (int)P_COLS; i += 32) tmem_ld32(from + i, v + i);
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(free_at);
+                if (n0 < p.N && j0 < p.out) finish(p, v, n0, p.N - n0, j0, lane, bias);
+            }
+            t += pairs;
         }
     }
     __syncthreads();
@@ -541,6 +576,28 @@ int scales_map(CUtensorMap *map, const spgk_mx4 *m, uint32_t box_tiles)
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, m->scales, kt * 128, ((uint64_t)m->rows + 127) / 128, kt * SF_TILE, 256, box_tiles, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// How a product is arranged: CTAs that share a tile, and an estimate in cycles (of a chain of launches on a B200 at 1.9 GHz: k-blocks at what the MMA warp,
+// HBM or L2 needs for them; what a launch, sixteen columns of outputs, sums from other CTAs' memory take is from cycle counters).
+struct Plan { uint32_t split; uint64_t cycles; };
+Plan plan_single(const LayerParams &p, uint32_t nt, uint32_t sms)
+{
+    const uint64_t tiles = (uint64_t)((p.out + TM - 1) / TM) * ((p.N + nt - 1) / nt);
+    const uint32_t cols = p.N < nt ? p.N : nt;
+    Plan best = { 1, ~0ull };
+    for (uint32_t s = 1; s <= MAX_SPLIT && s <= p.kblocks; s *= 2) {
+        if (s > 1 && tiles * s > sms) break;
+        const uint64_t waves = (tiles * s + sms - 1) / sms, outputs = s == 1 ? (cols + 31) / 32 * 900 : 2500 + (cols + 16 * s - 1) / (16 * s) * 1800;
+        const uint64_t cycles = 3000 + waves * ((uint64_t)((p.kblocks + s - 1) / s) * 570 + outputs);
+        if (cycles < best.cycles) best = { s, cycles };
+    }
+    return best;
+}
+uint64_t pair_cycles(const LayerParams &p, uint32_t sms)
+{
+    const uint64_t tiles = (uint64_t)((p.out + 255) / 256) * ((p.N + PN - 1) / PN), waves = (tiles + sms / 2 - 1) / (sms / 2);
+    return 8000 + waves * ((uint64_t)p.kblocks * 512 + 600);
+}
+
 template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
 {
     using L = Tile<NT>;
@@ -553,9 +610,7 @@ template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerPar
     CUtensorMap map_w, map_x;
     if ((rc = codes_map(&map_w, W, TM)) || (rc = codes_map(&map_x, X, NT))) return rc;
     const uint32_t j_tiles = (p.out + TM - 1) / TM, n_tiles = (p.N + NT - 1) / NT;
-    const uint64_t tiles = (uint64_t)j_tiles * n_tiles;
-    p.split = 1;
-    if (NT <= 128) while (p.split < MAX_SPLIT && tiles * p.split * 2 <= (uint32_t)dp.sm_count && p.kblocks >= p.split * 4) p.split *= 2;
+    p.split = plan_single(p, NT, (uint32_t)dp.sm_count).split;
     const uint32_t room = NT <= 64 ? ROOM_FOR_TWO : (uint32_t)dp.smem_optin;
     const uint32_t most = (room - HEAD - 1024) / L::STAGE, mine = (p.kblocks + p.split - 1) / p.split;
     p.stages = mine < most ? mine : most;
@@ -636,6 +691,7 @@ extern "C" int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, con
     if (p.N <= 16) return launch<16>(W, X, p, dp, dev, st);
     if (p.N <= 32) return launch<32>(W, X, p, dp, dev, st);
     if (p.N <= 64) return launch<64>(W, X, p, dp, dev, st);
-    if (p.N <= 512) return launch<128>(W, X, p, dp, dev, st);
+    // (256 x 8192 x 8192: 14.7 us with single CTAs, 16 in pairs; 512 rows 28.9 and 16; 300 x 1000 x 512 6 and 9)
+    if (plan_single(p, 128, (uint32_t)dp.sm_count).cycles <= pair_cycles(p, (uint32_t)dp.sm_count)) return launch<128>(W, X, p, dp, dev, st);
     return launch_pairs(W, X, p, dp, dev, st);
 }
