@@ -62,9 +62,11 @@ __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr)
 {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(128u >> 4) << 16 | (uint64_t)(128u >> 4) << 32 | (uint64_t)1u << 46;
 }
-__device__ __forceinline__ void ld_cluster_4(uint32_t addr, float *v)
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
 {
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
 }
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr)
 {
@@ -171,7 +173,6 @@ __device__ __forceinline__ void prefetch_l2(const CUtensorMap *map, int c0, int 
 template <uint32_t NT> struct Tile {
     static constexpr uint32_t X_BYTES = NT * 128;
     static constexpr uint32_t SFX_TILES = (NT + 127) / 128;
-    static constexpr uint32_t PART = NT + 4;                                   // floats from a unit's sums to the next one's, where CTAs share a tile
     static constexpr uint32_t STAGE = (W_BYTES + X_BYTES + SF_BYTES + SFX_TILES * SF_BYTES + 1023) / 1024 * 1024;
     static constexpr uint32_t SFX_COLS = NT < 128 ? 4 : NT / 32;              // columns of the rows' scales for four blocks
     static constexpr uint32_t SFW = NT < 32 ? 16 : NT;                         // tensor memory: sums, weights' scales, rows' scales
@@ -288,14 +289,13 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
                 if (!ok) mbar_wait(done, 0, &never, p.status, 5);                // the products under way end before tensor memory is given back
                 tc_fence_after();
                 if (p.split > 1) {
-                    // this CTA's sums, [unit][column], into its own shared memory (no copy or product is under way any more)
+                    // this CTA's sums, [column][unit], into its own shared memory (no copy or product is under way any more)
                     for (uint32_t c = half * 16u; c < NT && n0 + c < p.N; c += 32) {
                         uint32_t r[16];
                         tmem_ld16(lanes + c, r);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4)
-                            *reinterpret_cast<uint4 *>(base + HEAD + ((quad * 32u + lane) * L::PART + c + i) * 4u) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+                        for (int i = 0; i < 16; i++) *reinterpret_cast<uint32_t *>(base + HEAD + ((c + i) * TM + quad * 32u + lane) * 4u) = r[i];
                     }
                     cluster_sync();
                     for (uint32_t r = 0; r < p.split; r++) ok = ok && ld_cluster_u32(mapa(aborted, r)) == 0;
@@ -311,12 +311,12 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
                     else each(v, [](float) { return 0.0f; });
                 } else {
                     float part[MAX_SPLIT][8];                                    // all on their way before the first is needed
-                    const uint32_t at = ring + ((quad * 32u + lane) * L::PART + c) * 4u;
+                    const uint32_t at = ring + (c * TM + quad * 32u + lane) * 4u, rows = p.N - (n0 + c);
 #pragma unroll
                     for (uint32_t r = 0; r < MAX_SPLIT; r++) {
-                        each(part[r], [](float) { return 0.0f; });
-                        if (r < p.split) ld_cluster_4(mapa(at, r), part[r]);
-                        if (r < p.split && n0 + c + 4 < p.N) ld_cluster_4(mapa(at, r) + 16, part[r] + 4);
+                        const uint32_t from = mapa(at, r < p.split ? r : 0);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) part[r][i] = r < p.split && (uint32_t)i < rows ? ld_cluster_f32(from + i * TM * 4u) : 0.0f;
                     }
 #pragma unroll
                     for (int i = 0; i < 8; i++) v[i] = part[0][i];
@@ -616,7 +616,7 @@ template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerPar
     p.stages = mine < most ? mine : most;
     if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
     uint32_t bytes = p.stages * L::STAGE;
-    if (p.split > 1 && bytes < L::PART * TM * 4u) bytes = L::PART * TM * 4u;
+    if (p.split > 1 && bytes < NT * TM * 4u) bytes = NT * TM * 4u;
     if (n_tiles > 65535u) { spgk_set_error("spgk_layer_mx4", "more than 65535 tiles of rows"); return SPGK_E_ARG; }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(j_tiles * p.split, n_tiles); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = HEAD + 1024 + bytes; cfg.stream = stream;
