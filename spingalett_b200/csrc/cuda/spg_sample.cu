@@ -115,11 +115,11 @@ constexpr uint32_t PIECES = 64;               // of a CTA's slice, in the order 
 
 struct alignas(16) Shared {
     uint64_t mass[BINS];
-    uint32_t count[BINS], count_low[BINS];
+    uint32_t count[BINS + 32], count_low[BINS + 32];
     union { struct { uint32_t list[LIST]; uint16_t piece[LIST]; }; Item few[FEW]; };
     uint32_t table[STEPS];
     uint64_t piece_sum[PIECES]; uint32_t piece_equal[PIECES];
-    float dense[WARPS][128];
+    float dense[WARPS][256];
     uint32_t left;
     uint64_t out[2][4];                        // what this CTA tells the others, by turns
     uint64_t warp[2][WARPS];
@@ -161,9 +161,9 @@ struct Row {
     __device__ __forceinline__ void sync() { if (split > 1) spgtc::cluster_sync(); else __syncthreads(); }
     __device__ __forceinline__ uint64_t sum_warp(uint64_t v)
     {
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        return v;
+        const uint32_t mask = (1u << 26) - 1;                                    // (three parts whose sums fit 32 bits)
+        const uint64_t a = __reduce_add_sync(0xffffffffu, (uint32_t)v & mask), b = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 26) & mask);
+        return a + (b << 26) + ((uint64_t)__reduce_add_sync(0xffffffffu, (uint32_t)(v >> 52)) << 52);
     }
     // Over the CTA, to all threads.  The warps' results lie in one of two places by turns: who writes to one again has passed the barrier behind the other.
     __device__ __forceinline__ uint64_t *warps(uint64_t v, bool mine)
@@ -317,10 +317,11 @@ struct Row {
     __device__ bool mass_cut(const Weights &w, float share, uint32_t &cut, uint32_t &ties)
     {
         const float over = of_key(cut);
+        const auto up_of = [](uint32_t bin) -> int { return bin == BINS - 1 ? 0 : ONE_BITS - 30 - (int)((bin + 15) >> 4); };
         s.count[threadIdx.x] = 0; s.count_low[threadIdx.x] = 0;
         if (threadIdx.x == 0) s.listed = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+        for (uint32_t i = threadIdx.x; i < this->count; i += THREADS) {
             const float4 v = packs[i];
             const float l[4] = { v.x, v.y, v.z, v.w };
             uint32_t m[4], at[4];
@@ -328,11 +329,12 @@ struct Row {
             for (int j = 0; j < 4; j++) {
                 int k;
                 m[j] = w.mantissa(l[j], k);
-                at[j] = min(BINS - 1, (uint32_t)(63 - k) >> 6);
-                if (at[j] == BINS - 1) m[j] >>= min(-(k >> 10) - (ONE_BITS - 30), 31);
+                const uint32_t bin = min(BINS - 1, (uint32_t)(63 - k) >> 6);
+                if (bin == BINS - 1) m[j] >>= min(-(k >> 10) - (ONE_BITS - 30), 31);
+                at[j] = l[j] > over ? bin : BINS + threadIdx.x % 32;             // (what is not left goes to a place of its lane: no branches)
             }
 #pragma unroll
-            for (int j = 0; j < 4; j++) if (l[j] > over) { atomicAdd(&s.count_low[at[j]], m[j] & 0xffffu); atomicAdd(&s.count[at[j]], m[j] >> 16); }
+            for (int j = 0; j < 4; j++) { atomicAdd(&s.count_low[at[j]], m[j] & 0xffffu); atomicAdd(&s.count[at[j]], m[j] >> 16); }
         }
         sync();
         uint64_t low = 0, high = 0;
@@ -342,7 +344,6 @@ struct Row {
             low += ld_cluster_u32(mapa(smem_u32(&s.count_low[threadIdx.x]), r));
             high += ld_cluster_u32(mapa(smem_u32(&s.count[threadIdx.x]), r));
         }
-        const auto up_of = [](uint32_t bin) -> int { return bin == BINS - 1 ? 0 : ONE_BITS - 30 - (int)((bin + 15) >> 4); };
         const int up = up_of(threadIdx.x);
         uint64_t amount = (high << 16) + low, total;
         amount = up >= 0 ? amount << up : amount >> -up;
@@ -360,7 +361,7 @@ struct Row {
         // the goal in the units of the border's bin
         uint64_t rest = goal - s.found_above;
         rest = border_up >= 0 ? (rest + ((1ull << border_up) - 1)) >> border_up : rest << -border_up;
-        // few of a piece's logits are so large: 128 at a time, the warp puts them side by side first
+        // few of a piece's logits are so large: 256 at a time, the warp puts them side by side first
         const float bottom = border == BINS - 1 ? -INFINITY : w.top - (float)(border * 64 + 2) / (w.c * (float)STEPS) - 1e-6f * fabsf(w.top);
         float *const dense = s.dense[threadIdx.x / 32];
         const uint32_t lane = threadIdx.x % 32;
@@ -368,12 +369,12 @@ struct Row {
         for (uint32_t q = 0; q < PIECES / WARPS; q++) {
             const uint32_t piece = threadIdx.x / 32 * (PIECES / WARPS) + q, a = piece * per_piece, b = min(this->count, a + per_piece);
             uint64_t sum = 0;
-            for (uint32_t i0 = a; i0 < b; i0 += 32) {
-                const float4 v = i0 + lane < b ? packs[i0 + lane] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                const float l[4] = { v.x, v.y, v.z, v.w };
+            for (uint32_t i0 = a; i0 < b; i0 += 64) {
+                const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), v = i0 + lane < b ? packs[i0 + lane] : none, v2 = i0 + 32 + lane < b ? packs[i0 + 32 + lane] : none;
+                const float l[8] = { v.x, v.y, v.z, v.w, v2.x, v2.y, v2.z, v2.w };
                 uint32_t held = 0;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+                for (int j = 0; j < 8; j++) {
                     const bool in = l[j] > over && l[j] >= bottom;
                     const uint32_t set = __ballot_sync(0xffffffffu, in);
                     if (in) dense[held + __popc(set & ((1u << lane) - 1))] = l[j];
