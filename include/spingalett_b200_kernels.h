@@ -582,8 +582,9 @@ SPGK_API int spgk_layer_gemm_tc_noalloc(const spgk_layer *L,
  *   codes : row r starts at codes + r * pitch; element c is in byte c / 2, an even one in the low nibble.  16-byte aligned; pitch is a
  *           multiple of 16 and at least spgk_mx4_pitch(cols).  The last block's elements beyond cols are zero.
  *   scales: tiles of 128 rows x 4 blocks of 512 bytes, a row tile's after one another, 16-byte aligned, spgk_mx4_scales_bytes(rows, cols) bytes;
- *           the scale of block b of row r is byte spgk_mx4_scale_index(cols, r, b).  Scales of rows and blocks beyond the matrix have to be below
- *           0xFF (spgk_mx4_quantize writes zeros there). */
+ *           the scale of block b of row r is byte spgk_mx4_scale_index(cols, r, b).  Scales of a row's blocks beyond cols (up to a multiple of four)
+ *           have to be below 0xFF: whatever writes a matrix here writes zeros there.
+ * Of these functions' operands none may overlap what they write. */
 #define SPGK_T_F32   2        /* with SPGK_T_F16 and SPGK_T_BF16: the type of rows below */
 #define SPGK_MX4_BLOCK 32u
 typedef struct {
@@ -597,15 +598,15 @@ SPGK_API size_t spgk_mx4_scales_bytes(uint32_t rows, uint32_t cols);
 SPGK_API size_t spgk_mx4_scale_index(uint32_t cols, uint32_t row, uint32_t block);
 /* dst = x (rows of ldx elements of `type`): a block's scale is 2^(floor(log2 max|x|) - 2), at least 2^-127; its elements are rounded to nearest
  * (ties to the even code) and stay at 6 where x / scale is beyond it.  A block with a NaN or an infinity becomes NaN.  Every byte of dst's matrix
- * is written: the codes of whole blocks and the scales of whole tiles. */
+ * is written: the codes of whole blocks and the scales of whole tiles, rows beyond the last included. */
 SPGK_API int spgk_mx4_quantize(const void *x, int type, uint32_t ldx, const spgk_mx4 *dst, void *stream);
 /* y (rows of ldy elements of `type`) = the values of src: exact in fp32 and bf16 (beyond their range infinite), rounded in fp16. */
 SPGK_API int spgk_mx4_dequantize(const spgk_mx4 *src, void *y, int type, uint32_t ldy, void *stream);
 /* A dense layer whose weights W (out x in) and inputs X (N x in) are both microscaled:
  *   y[n][j] = act(bias[j] + sum_k W[j][k] * X[n][k])        (bias: dev fp32 [out] or NULL)
- * with exact products and fp32 sums on the tensor cores.  y: rows of ldy elements of `type`, rounded once, or NULL; next: the same values quantised
- * as by spgk_mx4_quantize from fp32 (next->rows == X->rows, next->cols == W->rows), the operand of the layer behind, or NULL; one of the two at
- * least.  ACT_SOFTMAX is left to spgk_softmax_rows, and refused with `next`.
+ * with exact products and fp32 sums on the tensor cores (at most 2^27 inputs).  y: rows of ldy elements of `type`, rounded once, or NULL; next: the same values quantised
+ * as by spgk_mx4_quantize from fp32 (next->rows == X->rows, next->cols == W->rows; scales of rows beyond the last are left as they were), the operand of the
+ * layer behind, or NULL; one of the two at least.  ACT_SOFTMAX is left to spgk_softmax_rows, and refused with `next`.
  * status: dev int32, zero before the first call, as for spgk_layer_gemm_tc (read with spgk_gemm_tc_status).
  * Does forward()'s layer step, reference Network.c:218-247, on another number format. */
 SPGK_API int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, const spgk_mx4 *X, void *y, int type, uint32_t ldy,
@@ -624,7 +625,7 @@ SPGK_API int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, const
  * NaN or <= 0.  A temperature that is NaN or not above zero takes the first of the largest logits.  u: dev fp32 [N] in [0, 1).
  * tokens: dev int32 [N]; probs: dev fp32 [N], the token's share of what was left, or NULL; kept: dev int32 [N], how many logits were left, or NULL.
  * A row with nothing above -infinity: token -1, probability 0, kept 0.  Where the largest logit is +infinity its equals share the weight.
- * Weights are summed as whole multiples of 2^-44 of the largest, so no result hangs on the order of a sum. */
+ * A weight is good to 2^-30 of itself and taken as a whole multiple of 2^-44 of the largest, so no result hangs on the order of a sum. */
 #define SPGK_SAMPLE_MAX_WIDTH 262144u
 SPGK_API int spgk_sample_rows(const void *logits, int type, uint32_t ld, uint32_t N, uint32_t width, const float *temperature,
                               const int32_t *top_k, const float *top_p, const float *min_p, const float *u,

@@ -491,6 +491,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
             const uint32_t j0 = jt * 256u + rank * 128u + quad * 32u, j = j0 + lane, n0 = nt * PN + part * P_COLS;
             const float bias = !dry && p.bias && j < p.out ? __ldg(p.bias + j) : 0.0f;
             const uint32_t from = tmem + (quad * 32u << 16) + part * P_COLS;
+            const bool some = j0 < (p.next_codes ? (p.out + 127u) / 128u * 128u : p.out);       // (the next operand's scale tiles are written whole)
             if (!dry) {
                 if (!mbar_wait(sums_full, turn, abort_flag, p.status, 3)) { mbar_wait(sums_full, turn, &never, p.status, 5, 1u << 12); break; }
                 turn ^= 1u;
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
             if (dry || t + pairs >= tiles) {
                 // the last: nobody waits for tensor memory, and a short loop is quicker than 64 columns written out that come from L2
 #pragma unroll 1
-                for (uint32_t c = 0; c < (dry ? 1u : P_COLS) && (dry || (n0 + c < p.N && j0 < p.out)); c += 16) {
+                for (uint32_t c = 0; c < (dry ? 1u : P_COLS) && (dry || (n0 + c < p.N && some)); c += 16) {
                     uint32_t r[16];
                     float v[16];
                     each(v, [](float) { return 0.0f; });
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(free_at);
-                if (n0 < p.N && j0 < p.out) finish(p, v, n0, p.N - n0, j0, lane, bias);
+                if (n0 < p.N && some) finish(p, v, n0, p.N - n0, j0, lane, bias);
             }
             t += pairs;
         }
@@ -666,6 +667,7 @@ extern "C" int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, con
     if (next && (rc = spg_mx4_check("spgk_layer_mx4 (next)", next))) return rc;
     const char *why = nullptr;
     if (W->rows == 0 || W->cols != X->cols) why = "weights and inputs do not belong together";
+    else if (W->cols > (1u << 27)) why = "more than 2^27 inputs";             // (a tile's products end well before the waits for them give up)
     else if (act < SPG_ACT_SIGMOID || act > SPG_ACT_NONE) why = "unknown activation";
     else if (!y && !next) why = "no output";
     else if (y && type != SPGK_T_F16 && type != SPGK_T_BF16 && type != SPGK_T_F32) why = "unknown type";

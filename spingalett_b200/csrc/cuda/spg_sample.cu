@@ -486,8 +486,11 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
     uint32_t top = R.max_cta(key_of(mine)), low = ~R.max_cta(~key_of(least));
     have = (uint32_t)R.sum_cta(have);
     R.tell(top, low, have);
-    uint32_t all = 0;
-    for (uint32_t r = 0; r < p.split; r++) { top = max(top, (uint32_t)R.heard(r, 0)); low = min(low, (uint32_t)R.heard(r, 1)); all += (uint32_t)R.heard(r, 2); }
+    uint32_t all = 0, rich = 0;                                                  // (rich: CTAs of whose logits no more than half are masked)
+    for (uint32_t r = 0; r < p.split; r++) {
+        const uint32_t c = (uint32_t)R.heard(r, 2);
+        top = max(top, (uint32_t)R.heard(r, 0)); low = min(low, (uint32_t)R.heard(r, 1)); all += c; rich += c >= p.slice / 2;
+    }
     const float largest = of_key(top);
 
     const double log_min_p = mp > 0.0f ? log((double)mp) : -INFINITY;
@@ -495,9 +498,9 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
     Weights w;
     w.set(largest, greedy ? 1.0f : t, s.table);
 
-    if (all && !greedy && k >= 1 && (uint32_t)k < all && (uint32_t)k <= FEW / 2) {
-        // At least k logits of the row are no smaller than the least of the CTAs' (k / split)-th largest of their threads' largest; a bin's lower end will do
-        const uint32_t want = ((uint32_t)k + p.split - 1) / p.split;
+    if (rich && !greedy && k >= 1 && (uint32_t)k < all && (uint32_t)k <= FEW / 2) {
+        // At least k logits of the row are no smaller than the least of the rich CTAs' (k / rich)-th largest of their threads' largest; a bin's lower end will do
+        const uint32_t want = ((uint32_t)k + rich - 1) / rich;
         s.count[threadIdx.x] = 0;
         if (threadIdx.x == 0) { s.listed = 0; s.found_bin = BINS; }
         const bool some = mine > -INFINITY;
@@ -510,7 +513,7 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
         if (even && upto >= want && upto - c < want) s.found_bin = threadIdx.x;
         __syncthreads();
         const float end = best - ((float)s.found_bin + 1.001f) * width - 1e-6f * (fabsf(best) + fabsf(worst));
-        R.tell(key_of(s.found_bin < BINS && end > -FLT_MAX ? end : -FLT_MAX));
+        R.tell(have < p.slice / 2 ? 0xffffffffu : key_of(s.found_bin < BINS && end > -FLT_MAX ? end : -FLT_MAX));
         uint32_t bound = 0xffffffffu;
         for (uint32_t r = 0; r < p.split; r++) bound = min(bound, (uint32_t)R.heard(r, 0));
         const float at_least = of_key(bound);

@@ -29,7 +29,7 @@ class Packed:
         import torch
         self.rows, self.cols, self.pitch = rows, cols, -(-cols // 32) * 16 + more
         self.codes = torch.full((rows + 1, self.pitch), 0xA5, dtype=torch.uint8, device="cuda")
-        self.tiles = torch.full((-(-rows // 128) * -(-cols // 128) * 512 + 16,), 0xA5, dtype=torch.uint8, device="cuda")
+        self.tiles = torch.full((-(-rows // 128) * -(-cols // 128) * 512 + 16,), 0xFF, dtype=torch.uint8, device="cuda")
         if codes is not None:
             self.codes[:rows] = torch.from_numpy(codes).cuda()
             self.tiles[:-16] = torch.from_numpy(tiles).cuda()
@@ -90,7 +90,7 @@ def test_quantize_and_back(spg, lib, t, rows, cols, pad, off):
     assert np.array_equal(scale, want_scale)
     assert np.array_equal(code, want_code)
     codes, tiles = m.codes.cpu().numpy(), m.tiles.cpu().numpy()
-    assert (codes[rows] == 0xA5).all() and (tiles[-16:] == 0xA5).all() and (codes[:, -(-cols // 32) * 16:] == 0xA5).all()
+    assert (codes[rows] == 0xA5).all() and (tiles[-16:] == 0xFF).all() and (codes[:, -(-cols // 32) * 16:] == 0xA5).all()
     used = np.zeros(tiles.size - 16, bool)
     r, b = np.meshgrid(np.arange(rows), np.arange(scale.shape[1]), indexing="ij")
     used[plain.scale_place(cols, r, b)] = True
@@ -107,7 +107,7 @@ def test_quantize_and_back(spg, lib, t, rows, cols, pad, off):
 
 
 SHAPES = [(1, 1, 1), (1, 10, 1000), (2, 333, 777), (16, 128, 256), (17, 129, 31), (33, 300, 64), (65, 257, 1025), (128, 512, 784), (300, 1000, 512), (513, 130, 4100), (600, 64, 33),
-          (1, 128, 16384), (8, 200, 8192), (40, 96, 3001), (700, 1500, 320), (129, 1, 200), (257, 2, 40)]
+          (1, 128, 16384), (8, 200, 8192), (40, 96, 3001), (700, 1500, 320), (129, 1, 200), (257, 2, 40), (2500, 2700, 300), (4100, 1100, 70), (90, 33, 20000)]
 
 
 def _layer(spg, lib, rng, n, out, k, act, t, exact, bias=True):
@@ -169,7 +169,7 @@ def test_layer_output_as_the_next_operand(spg, lib, n, out, k):
     for m in (a, c):
         for mine, theirs in zip(m.host(), both.host()):
             assert np.array_equal(mine, theirs)
-        assert (m.codes[n].cpu().numpy() == 0xA5).all() and (m.tiles[-16:].cpu().numpy() == 0xA5).all()
+        assert (m.codes[n].cpu().numpy() == 0xA5).all() and (m.tiles[-16:].cpu().numpy() == 0xFF).all()
     # and it is an operand: the scales of blocks beyond the matrix are no NaN
     got2 = torch.empty((n, out), dtype=torch.float32, device="cuda")
     unit, uv = _random(spg, out, out, rng, True)

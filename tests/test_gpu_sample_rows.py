@@ -64,6 +64,24 @@ def test_draws(lib, n, width, cuts):
     _check(_draw(lib, x, t, k, p, m, u, kind), x, t, k, p, m, u)
 
 
+def test_a_vocabulary_masked_in_runs(lib):
+    """Whole stretches of a long row masked, as the unused end of a vocabulary is: some CTAs of the row have nothing, some a single logit."""
+    import torch
+    rng = np.random.default_rng(2)
+    n, width = 9, 60000
+    x = rng.standard_normal((n, width)).astype(np.float32)
+    for i in range(n):
+        x[i, width * (i + 1) // 10:] = -np.inf
+        x[i, -1 - i] = 0.25 * i
+        if i % 3 == 2:
+            x[i, :5000 * i] = -np.inf
+    xd = torch.from_numpy(x).cuda()
+    for k, p, m in ((50, None, None), (256, 0.9, None), (3, None, 0.1), (None, 0.6, None), (700, None, None)):
+        t, u = np.full(n, 0.9), rng.random(n).astype(np.float32)
+        a = [None if v is None else np.full(n, v) for v in (k, p, m)]
+        _check(_draw(lib, xd, t, *a, u), xd, t, *a, u)
+
+
 @pytest.mark.parametrize("width", [40, 3000, 70000])
 def test_masks_ties_and_odd_values(lib, width):
     """Rows without a logit, with one, with equal ones only, infinities, NaN, differences beyond the weights' range."""

@@ -71,6 +71,8 @@ def test_bad_layers_are_refused(spg, lib):
     assert call(x=other) == -2 and call(w=_matrix(spg, rows=0)) == -2
     assert call(act=7) == -2 and call(act=-1) == -2 and call(y=0) == -2 and call(kind=3) == -2 and call(y=SOME + 2) == -2 and call(y=SOME + 1, kind=0) == -2
     assert call(ldy=47) == -2 and call(status=0) == -2 and call(bias=SOME + 2) == -2
+    wide = _matrix(spg, cols=(1 << 27) + 32)
+    assert call(w=wide, x=wide, ldy=4) == -2
     assert call(nxt=wrong) == -2 and call(nxt=other) == -2 and call(nxt=nxt, act=5) == -2
     assert call(x=_matrix(spg, rows=0)) == 0
 
