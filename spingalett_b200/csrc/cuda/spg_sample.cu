@@ -37,12 +37,10 @@ struct SampleParams {
     int32_t *tokens; float *probs; int32_t *kept;
 };
 
-// a NaN like -infinity, -0 like 0
-__device__ __forceinline__ float logit_of(float l) { return l >= -INFINITY ? l + 0.0f : -INFINITY; }
-// integers in the order of the logits
+// Integers in the order of the logits, -0 like 0.  (A NaN has none: it is in none of the ranges that are asked for before a key is.)
 __device__ __forceinline__ uint32_t key_of(float l)
 {
-    const uint32_t b = __float_as_uint(l);
+    const uint32_t b = __float_as_uint(l + 0.0f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
@@ -57,7 +55,7 @@ struct Weights {
     const uint32_t *table;
 
     static constexpr float MAGIC = 12582912.0f;            // 1.5 * 2^23: the sum's low bits are a whole number
-    __device__ __forceinline__ float rest(float l, float kf) const { return fmaf(l, c_lo, fmaf(l, c, (kf - MAGIC) * (-1.0f / STEPS))); }
+    __device__ __forceinline__ float rest(float l, float kf) const { return fmaf(l, c_lo, fmaf(l, c, fmaf(kf, -1.0f / STEPS, MAGIC / STEPS))); }      // (-K / 1024 is exact)
     __device__ __forceinline__ void set(float largest, float t, const uint32_t *tab)
     {
         top = largest; m = largest; inv_t = 1.0 / (double)t; table = tab;
@@ -84,8 +82,9 @@ struct Weights {
         const float y = rest(l, kf) - y_top;
         k = __float_as_int(kf) - k_top;                      // <= 0
         const uint32_t t = table[k & (int)(STEPS - 1)];
-        const float p = y * fmaf(y, 0.24022650695910072f, 0.69314718055994531f);
-        return t + (uint32_t)__float2int_rn(__uint2float_rn(t) * p);
+        const float p = y * fmaf(y, 0.24022650695910072f * (1 << 30), 0.69314718055994531f * (1 << 30));
+        // t * p in whole numbers, without a conversion: t's upper bits are the fraction of a number from 1 to 2, and MAGIC rounds the product
+        return t + (uint32_t)(__float_as_int(fmaf(__uint_as_float((t >> 7) + 0x3f000000u), p, MAGIC)) - 0x4b400000);
     }
     __device__ __forceinline__ uint64_t quick(float l) const
     {
@@ -465,17 +464,38 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
     float mine = -INFINITY, least = INFINITY;
     uint32_t have = 0;
     const auto take = [&](float l) -> float {
-        l = logit_of(l);
-        if (l > -INFINITY) { mine = fmaxf(mine, l); least = fminf(least, l); have++; }
+        const bool some = l > -INFINITY;
+        mine = fmaxf(mine, l); least = fminf(least, some ? l : INFINITY); have += some;             // (of a NaN and a number both give the number)
         return l;
     };
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x; i < packs; i += THREADS) {
-        alignas(16) T v[PER];
-        *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(x + first) + i);
+    if (sizeof(T) == 4) {
+        // straight to shared memory, the whole slice on its way at once (through registers 132 SMs drew 4 TB/s); a thread looks at what it has asked for, by quarters
+        const uint32_t quarter = (packs + 4 * THREADS - 1) / (4 * THREADS) * THREADS;
 #pragma unroll
-        for (uint32_t j = 0; j < PER; j += 4)
-            *reinterpret_cast<float4 *>(row_logits + first + i * PER + j) = make_float4(take(to_f32(v[j])), take(to_f32(v[j + 1])), take(to_f32(v[j + 2])), take(to_f32(v[j + 3])));
+        for (uint32_t q = 0; q < 4; q++) {
+            for (uint32_t i = q * quarter + threadIdx.x; i < min(packs, (q + 1) * quarter); i += THREADS)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(row_logits + first) + 16 * i), "l"(reinterpret_cast<const uint4 *>(x + first) + i) : "memory");
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        const auto look = [&](uint32_t q) {
+            for (uint32_t i = q * quarter + threadIdx.x; i < min(packs, (q + 1) * quarter); i += THREADS) {
+                const float4 v = *reinterpret_cast<const float4 *>(row_logits + first + 4 * i);
+                take(v.x); take(v.y); take(v.z); take(v.w);
+            }
+        };
+        asm volatile("cp.async.wait_group 3;" ::: "memory"); look(0);
+        asm volatile("cp.async.wait_group 2;" ::: "memory"); look(1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory"); look(2);
+        asm volatile("cp.async.wait_group 0;" ::: "memory"); look(3);
+    } else {
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < packs; i += THREADS) {
+            alignas(16) T v[PER];
+            *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(x + first) + i);
+#pragma unroll
+            for (uint32_t j = 0; j < PER; j += 4)
+                *reinterpret_cast<float4 *>(row_logits + first + i * PER + j) = make_float4(take(to_f32(v[j])), take(to_f32(v[j + 1])), take(to_f32(v[j + 2])), take(to_f32(v[j + 3])));
+        }
     }
     if (threadIdx.x < 2 * PER) {                                                 // the ends
         const uint32_t i = threadIdx.x < PER ? threadIdx.x : first + packs * PER + threadIdx.x - PER;
