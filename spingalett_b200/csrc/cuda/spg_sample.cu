@@ -23,6 +23,7 @@ using spgtc::smem_u32; using spgtc::mapa; using spgtc::cluster_rank;
 
 constexpr uint32_t THREADS = 512, WARPS = THREADS / 32;
 constexpr uint32_t BINS = 512;
+constexpr uint32_t DENSE = 512;               // places that a warp puts side by side
 constexpr uint32_t LIST = 2048;               // logits of a range that are searched bit by bit
 constexpr uint32_t FEW = 512;                 // logits among which every thread counts what stands before its own
 constexpr uint32_t MAX_SPLIT = 8;
@@ -30,6 +31,17 @@ constexpr uint32_t SLICE = SPGK_SAMPLE_MAX_WIDTH / MAX_SPLIT;
 constexpr int ONE_BITS = 44;
 constexpr uint32_t STEPS = 1024;              // of the table of 2^(i / STEPS)
 static_assert(BINS == THREADS && LIST % THREADS == 0 && FEW <= THREADS && STEPS % THREADS == 0, "a thread a bin, a logit, two steps");
+
+// 2^(i / STEPS) in units of 2^-30 (repeated multiplication errs by less than 2^-42)
+struct Steps {
+    uint32_t v[STEPS];
+    constexpr Steps() : v()
+    {
+        double x = 1.0;
+        for (uint32_t i = 0; i < STEPS; i++, x *= 1.000677130693066356678727) v[i] = (uint32_t)(x * (double)(1u << 30) + 0.5);
+    }
+};
+__device__ const Steps g_steps;
 
 struct SampleParams {
     const void *logits; int type; uint32_t ld, N, width, split, slice;
@@ -110,7 +122,8 @@ struct Weights {
 };
 
 struct Item { float l; uint32_t index; uint64_t w; };
-constexpr uint32_t PIECES = 64;               // of a CTA's slice, in the order of the vocabulary, four a warp
+constexpr uint32_t PIECES = 64;               // of a CTA's slice, in the order of the vocabulary: four a warp, two a lane
+static_assert(PIECES == 64 && PIECES % WARPS == 0 && SLICE + 8 <= 65536, "two a lane; places in 16 bits");
 
 struct alignas(16) Shared {
     uint64_t mass[BINS];
@@ -118,7 +131,7 @@ struct alignas(16) Shared {
     union { struct { uint32_t list[LIST]; uint16_t piece[LIST]; }; Item few[FEW]; };
     uint32_t table[STEPS];
     uint64_t piece_sum[PIECES]; uint32_t piece_equal[PIECES];
-    float dense[WARPS][256];
+    uint16_t dense[WARPS][DENSE];
     uint32_t left;
     uint64_t out[2][4];                        // what this CTA tells the others, by turns
     uint64_t warp[2][WARPS];
@@ -360,40 +373,65 @@ struct Row {
         // the goal in the units of the border's bin
         uint64_t rest = goal - s.found_above;
         rest = border_up >= 0 ? (rest + ((1ull << border_up) - 1)) >> border_up : rest << -border_up;
-        // few of a piece's logits are so large: 256 at a time, the warp puts them side by side first
+        // Few of a piece's logits are so large.  A warp first puts the places of those of all its pieces side by side, then weighs them, a lane each: the
+        // way from a logit to its weight is long, and so it is gone a few times a warp.
         const float bottom = border == BINS - 1 ? -INFINITY : w.top - (float)(border * 64 + 2) / (w.c * (float)STEPS) - 1e-6f * fabsf(w.top);
-        float *const dense = s.dense[threadIdx.x / 32];
-        const uint32_t lane = threadIdx.x % 32;
-        uint32_t small = 0xffffffffu, large = 0, many = 0, sure = 0;
-        for (uint32_t q = 0; q < PIECES / WARPS; q++) {
-            const uint32_t piece = threadIdx.x / 32 * (PIECES / WARPS) + q, a = piece * per_piece, b = min(this->count, a + per_piece);
-            uint64_t sum = 0;
+        constexpr uint32_t MINE = PIECES / WARPS;
+        uint16_t *const dense = s.dense[threadIdx.x / 32];
+        const float *const logits = reinterpret_cast<const float *>(packs);
+        const uint32_t lane = threadIdx.x % 32, first_piece = threadIdx.x / 32 * MINE;
+        uint32_t small = 0xffffffffu, large = 0, many = 0, sure = 0, held = 0, ends[MINE];              // ends: of the pieces among the places
+        uint64_t sums[MINE];
+#pragma unroll
+        for (uint32_t q = 0; q < MINE; q++) { sums[q] = 0; ends[q] = 0xffffffffu; }
+        const auto weigh = [&]() {
+            __syncwarp();
+            for (uint32_t i = lane; i < held; i += 32) {
+                const float x = logits[dense[i]];
+                const uint32_t at_bin = w.bin(x);
+                const uint64_t one = w.quick(x);
+                uint32_t piece = 0;
+#pragma unroll
+                for (uint32_t q = 0; q + 1 < MINE; q++) piece += i >= ends[q];
+                if (at_bin < border) {
+                    sure++;
+#pragma unroll
+                    for (uint32_t q = 0; q < MINE; q++) sums[q] += piece == q ? one : 0;
+                } else if (at_bin == border) {
+                    const uint32_t k = key_of(x), at = atomicAdd(&s.listed, 1u);
+                    small = min(small, k); large = max(large, k);
+                    if (at < LIST) { s.list[at] = k; s.piece[at] = (uint16_t)(first_piece + piece); }
+                }
+            }
+            __syncwarp();
+            held = 0;
+        };
+#pragma unroll
+        for (uint32_t q = 0; q < MINE; q++) {
+            const uint32_t a = (first_piece + q) * per_piece, b = min(this->count, a + per_piece);
             for (uint32_t i0 = a; i0 < b; i0 += 64) {
+                if (held > DENSE - 256) {
+                    weigh();
+#pragma unroll
+                    for (uint32_t r = 0; r < q; r++) ends[r] = 0;
+                }
                 const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), v = i0 + lane < b ? packs[i0 + lane] : none, v2 = i0 + 32 + lane < b ? packs[i0 + 32 + lane] : none;
                 const float l[8] = { v.x, v.y, v.z, v.w, v2.x, v2.y, v2.z, v2.w };
-                uint32_t held = 0;
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
+                for (uint32_t j = 0; j < 8; j++) {
                     const bool in = l[j] > over && l[j] >= bottom;
                     const uint32_t set = __ballot_sync(0xffffffffu, in);
-                    if (in) dense[held + __popc(set & ((1u << lane) - 1))] = l[j];
+                    if (in) dense[held + __popc(set & ((1u << lane) - 1))] = (uint16_t)(4 * (i0 + j / 4 * 32 + lane) + j % 4);
                     held += __popc(set);
                 }
-                __syncwarp();
-                for (uint32_t i = lane; i < held; i += 32) {
-                    const float x = dense[i];
-                    const uint32_t at_bin = w.bin(x);
-                    if (at_bin < border) { sum += w.quick(x); sure++; }
-                    else if (at_bin == border) {
-                        const uint32_t k = key_of(x), at = atomicAdd(&s.listed, 1u);
-                        small = min(small, k); large = max(large, k);
-                        if (at < LIST) { s.list[at] = k; s.piece[at] = (uint16_t)piece; }
-                    }
-                }
-                __syncwarp();
             }
-            sum = sum_warp(sum);
-            if (lane == 0) { s.piece_sum[piece] = sum; s.piece_equal[piece] = 0; }
+            ends[q] = held;
+        }
+        weigh();
+#pragma unroll
+        for (uint32_t q = 0; q < MINE; q++) {
+            const uint64_t sum = sum_warp(sums[q]);
+            if (lane == 0) { s.piece_sum[first_piece + q] = sum; s.piece_equal[first_piece + q] = 0; }
         }
         if (threadIdx.x == 0) s.left = 0;
         small = ~max_cta(~small); large = max_cta(large);
@@ -442,7 +480,7 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
     float *logits = reinterpret_cast<float *>(raw + sizeof(Shared));
     const uint32_t row = blockIdx.x / p.split, rank = blockIdx.x % p.split, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t from = min(p.width, rank * p.slice), n = min(p.width - from, p.slice);
-    for (uint32_t i = threadIdx.x; i < STEPS; i += THREADS) s.table[i] = __double2uint_rn(exp2((double)i / STEPS) * (double)(1u << 30));
+    for (uint32_t i = threadIdx.x; i < STEPS; i += THREADS) s.table[i] = __ldg(&g_steps.v[i]);
     spg_grid_trigger();
     spg_grid_wait();
 
@@ -689,22 +727,26 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
         if (lane == 0) atomicAdd(&s.left, left);
     }
     __syncthreads();
-    // the ties that are left are the first in the order of the vocabulary
+    // The ties that are left are the first in the order of the vocabulary.  (Every warp the same, two pieces a lane: no barrier in between.)
     const uint64_t each = ties ? w(over) : 0;
-    const uint32_t equal = ties && threadIdx.x < PIECES ? s.piece_equal[threadIdx.x] : 0;
-    uint32_t equal_before = 0, taken = 0;
+    const uint32_t e0 = ties ? s.piece_equal[2 * lane] : 0, e1 = ties ? s.piece_equal[2 * lane + 1] : 0;
+    uint32_t before0 = 0, t0 = 0, t1 = 0;                                        // equal logits in front of this lane's pieces; ties of them
     if (ties) {                                                                  // (the same in all threads of the cluster)
-        uint64_t here;
-        const uint32_t upto = (uint32_t)R.scan_cta(equal, here);
-        R.tell(here);
-        equal_before = upto - equal;
-        for (uint32_t r = 0; r < rank; r++) equal_before += (uint32_t)R.heard(r, 0);
-        taken = ties > equal_before ? min(equal, ties - equal_before) : 0;
+        uint32_t upto = e0 + e1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += v; }
+        R.tell(__shfl_sync(0xffffffffu, upto, 31));
+        before0 = upto - e0 - e1;
+        for (uint32_t r = 0; r < rank; r++) before0 += (uint32_t)R.heard(r, 0);
+        t0 = ties > before0 ? min(e0, ties - before0) : 0;
+        t1 = ties > before0 + e0 ? min(e1, ties - before0 - e0) : 0;
     }
-    uint64_t cta;
-    const uint64_t amount = (threadIdx.x < PIECES ? s.piece_sum[threadIdx.x] : 0) + taken * each, upto = R.scan_cta(amount, cta);
-    const uint32_t left = s.left + (ties ? (uint32_t)R.sum_cta(taken) : 0);
-    R.tell(cta, left);
+    const uint64_t a0 = s.piece_sum[2 * lane] + t0 * each, a1 = s.piece_sum[2 * lane + 1] + t1 * each;
+    uint64_t upto = a0 + a1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const uint64_t v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += v; }
+    const uint64_t cta = __shfl_sync(0xffffffffu, upto, 31);
+    R.tell(cta, s.left + __reduce_add_sync(0xffffffffu, t0 + t1));
     uint64_t before = 0, total = 0, left_all = 0;
     for (uint32_t r = 0; r < p.split; r++) { const uint64_t c = R.heard(r, 0); if (r < rank) before += c; total += c; left_all += R.heard(r, 1); }
 
@@ -713,50 +755,50 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
     } else {
         const double goal_d = u * (double)total;
         const uint64_t goal = goal_d >= (double)(total - 1) ? total - 1 : (uint64_t)goal_d;
-        if (before <= goal && goal < before + cta) {                             // in this CTA: in which piece, and where
-            if (before + upto - amount <= goal && goal < before + upto) { s.found_bin = threadIdx.x; s.found_above = before + upto - amount; s.found_count = equal_before; }
-            __syncthreads();
-            if (warp == 0) {
-                uint64_t run = s.found_above;
-                uint32_t seen = s.found_count;
-                const uint32_t a = s.found_bin * R.per_piece, b = min(fours, a + R.per_piece);
-                for (uint32_t i0 = a; i0 < b; i0 += 32) {
-                    const uint32_t i = i0 + lane;
-                    const float4 four = i < b ? R.packs[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                    const float l[4] = { four.x, four.y, four.z, four.w };
-                    uint64_t one[4], mine4 = 0;
-                    uint32_t same = 0;
+        if (warp == 0 && before <= goal && goal < before + cta) {                // in this CTA: in which piece, and where
+            const uint32_t in = (uint32_t)__ffs((int)__ballot_sync(0xffffffffu, before + upto > goal)) - 1;
+            uint64_t run = before + __shfl_sync(0xffffffffu, upto - a0 - a1, in);
+            uint32_t seen = __shfl_sync(0xffffffffu, before0, in), piece = 2 * in;
+            const uint64_t first_sum = __shfl_sync(0xffffffffu, a0, in);
+            const uint32_t first_equal = __shfl_sync(0xffffffffu, e0, in);
+            if (run + first_sum <= goal) { run += first_sum; seen += first_equal; piece++; }
+            const uint32_t a = piece * R.per_piece, b = min(fours, a + R.per_piece);
+            for (uint32_t i0 = a; i0 < b; i0 += 32) {
+                const uint32_t i = i0 + lane;
+                const float4 four = i < b ? R.packs[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                const float l[4] = { four.x, four.y, four.z, four.w };
+                uint64_t one[4], mine4 = 0;
+                uint32_t same = 0;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) same += ties && l[j] == over;
-                    uint32_t tie = same;
+                for (int j = 0; j < 4; j++) same += ties && l[j] == over;
+                uint32_t tie = same;
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, tie, o); if (lane >= (uint32_t)o) tie += v; }
-                    const uint32_t ties_here = __shfl_sync(0xffffffffu, tie, 31);
-                    tie += seen - same;                                          // equal logits in front of this lane's
+                for (int o = 1; o < 32; o <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, tie, o); if (lane >= (uint32_t)o) tie += v; }
+                const uint32_t ties_here = __shfl_sync(0xffffffffu, tie, 31);
+                tie += seen - same;                                          // equal logits in front of this lane's
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        one[j] = l[j] > over ? w(l[j]) : (ties && l[j] == over && tie++ < ties ? each : 0);
-                        mine4 += one[j];
-                    }
-                    uint64_t past = mine4;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) { const uint64_t v = __shfl_up_sync(0xffffffffu, past, o); if (lane >= (uint32_t)o) past += v; }
-                    const uint32_t over_goal = __ballot_sync(0xffffffffu, run + past > goal);
-                    if (over_goal) {
-                        if (lane == (uint32_t)__ffs((int)over_goal) - 1) {
-                            uint64_t sum = run + past - mine4;
-                            int j = 0;
-                            uint64_t w1 = one[0];
-                            if (sum + w1 <= goal) { sum += w1; j = 1; w1 = one[1]; if (sum + w1 <= goal) { sum += w1; j = 2; w1 = one[2]; if (sum + w1 <= goal) { j = 3; w1 = one[3]; } } }
-                            p.tokens[row] = (int32_t)(from + 4 * i + j - lead);
-                            if (p.probs) p.probs[row] = (float)((double)w1 / (double)total);
-                            if (p.kept) p.kept[row] = (int32_t)left_all;
-                        }
-                        break;
-                    }
-                    run += __shfl_sync(0xffffffffu, past, 31);
-                    seen += ties_here;
+                for (int j = 0; j < 4; j++) {
+                    one[j] = l[j] > over ? w(l[j]) : (ties && l[j] == over && tie++ < ties ? each : 0);
+                    mine4 += one[j];
                 }
+                uint64_t past = mine4;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) { const uint64_t v = __shfl_up_sync(0xffffffffu, past, o); if (lane >= (uint32_t)o) past += v; }
+                const uint32_t over_goal = __ballot_sync(0xffffffffu, run + past > goal);
+                if (over_goal) {
+                    if (lane == (uint32_t)__ffs((int)over_goal) - 1) {
+                        uint64_t sum = run + past - mine4;
+                        int j = 0;
+                        uint64_t w1 = one[0];
+                        if (sum + w1 <= goal) { sum += w1; j = 1; w1 = one[1]; if (sum + w1 <= goal) { sum += w1; j = 2; w1 = one[2]; if (sum + w1 <= goal) { j = 3; w1 = one[3]; } } }
+                        p.tokens[row] = (int32_t)(from + 4 * i + j - lead);
+                        if (p.probs) p.probs[row] = (float)((double)w1 / (double)total);
+                        if (p.kept) p.kept[row] = (int32_t)left_all;
+                    }
+                    break;
+                }
+                run += __shfl_sync(0xffffffffu, past, 31);
+                seen += ties_here;
             }
         }
     }
