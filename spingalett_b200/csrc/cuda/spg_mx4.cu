@@ -5,6 +5,8 @@
 // All of it is exact but the last rounding: the exponent of the largest magnitude is a bit field, division by 2^E a multiplication.
 // Both directions are bound by bytes.  A block of threads has one tile of 128 rows x 128 columns, whose 512 bytes of scales leave or come at once; sixteen
 // lanes have a row of it, eight values a lane (16-byte loads of 16-bit values, two of fp32; four bytes of codes), four rows on their way at a time.
+// 16384 x 8192: to 4 bits 93 us of fp32 (6.5 TB/s), 65 of bf16 (5.2 TB/s; 64 % of the issue slots: eight values are some fifty instructions), back 115 us to
+// fp32 (5.3 TB/s, nearly all of it writes), 55 to bf16 (6.1).
 #include "spg_mx4.cuh"
 
 namespace {

@@ -9,6 +9,11 @@
 // which tcgen05.cp copies to tensor memory in front of the products (both are issued by one thread and run in order).
 // Where there are few tiles, up to eight CTAs of a cluster share one, each with its part of the k-blocks, and add their sums in rank order.
 //
+// More than some hundred rows go to pairs of CTAs (below); which, and how many CTAs share a tile, an estimate in cycles says.
+// What bounds it: one row x 8192 x 16384 14.4 us (4.9 TB/s; 570 cycles a k-block on 128 CTAs is HBM's rate, the rest start and end of a launch),
+// 64 x 16384 x 16384 30.7 us (4.8 TB/s), 1 x 784 x 512 3.1 us (a launch), 16384 x 8192 x 8192 365 us (6020 TFLOP/s, 500 cycles a k-block of 512 at the
+// tensor pipe's best; 430 us in a long run, under the power limit).
+//
 // Every wait on an mbarrier is bounded; a CTA that gave up records a code in `status`, and its cluster leaves the tile's outputs alone.
 #include "spg_mx4.cuh"
 #include "spg_tc.cuh"
