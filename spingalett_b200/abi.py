@@ -216,5 +216,6 @@ def bind_operators(lib):
     lib.spgk_mx4_quantize.argtypes = [vp, C.c_int, u32, mx4, vp]
     lib.spgk_mx4_dequantize.argtypes = [mx4, vp, C.c_int, u32, vp]
     lib.spgk_layer_mx4.argtypes = [mx4, vp, C.c_int, mx4, vp, C.c_int, u32, mx4, vp, vp]
+    lib.spgk_gemm_tc_status.argtypes = [vp, vp]
     lib.spgk_sample_rows.argtypes = [vp, C.c_int, u32, u32, u32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     return lib

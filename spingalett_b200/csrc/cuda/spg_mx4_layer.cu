@@ -175,6 +175,9 @@ __device__ __forceinline__ void prefetch_l2(const CUtensorMap *map, int c0, int 
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
 }
 
+// the warps that read sums from tensor memory, and the one that gives it back
+__device__ __forceinline__ void sums_taken() { asm volatile("bar.sync 1, %0;" ::"n"(32 * (EPI + 1)) : "memory"); }
+
 template <uint32_t NT> struct Tile {
     static constexpr uint32_t X_BYTES = NT * 128;
     static constexpr uint32_t SFX_TILES = (NT + 127) / 128;
@@ -279,6 +282,12 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         }
         if (elect_one()) umma_commit(done);
         __syncwarp();
+        if (p.split > 1) {
+            // Given back before this CTA waits for the others: one that has none on its SM, and so cannot finish, may hold up a cluster that holds some elsewhere
+            sums_taken();
+            tc_fence_after();
+            tmem_free(tmem, L::COLS);
+        }
     } else {
         const uint32_t quad = warp % 4u, half = (warp - 2u) / 4u, j0 = j_tile * TM + quad * 32u, j = j0 + lane;
         const uint32_t lanes = tmem + (quad * 32u << 16);
@@ -302,6 +311,8 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
 #pragma unroll
                         for (int i = 0; i < 16; i++) *reinterpret_cast<uint32_t *>(base + HEAD + ((c + i) * TM + quad * 32u + lane) * 4u) = r[i];
                     }
+                    tc_fence_before();
+                    sums_taken();
                     cluster_sync();
                     for (uint32_t r = 0; r < p.split; r++) ok = ok && ld_cluster_u32(mapa(aborted, r)) == 0;
                 }
@@ -342,7 +353,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         cluster_sync();                                                          // (nobody leaves while its sums are read)
     }
     __syncthreads();
-    if (warp == 1) { tc_fence_after(); tmem_free(tmem, L::COLS); }
+    if (warp == 1 && p.split == 1) { tc_fence_after(); tmem_free(tmem, L::COLS); }
 }
 
 // ---- pairs of CTAs, many rows -------------------------------------------------------------------------------------------------

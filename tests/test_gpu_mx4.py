@@ -180,6 +180,25 @@ def test_layer_output_as_the_next_operand(spg, lib, n, out, k):
     assert (np.abs(got2.double().cpu().numpy() - xv @ uv.T) <= steps * 65 * 2.0 ** -24 * (np.abs(xv) @ np.abs(uv).T) + 1e-30).all()
 
 
+@pytest.mark.parametrize("ws,xs", [(254, 0), (0, 254), (253, 3), (20, 240), (127, 127)])
+@pytest.mark.parametrize("n", [3, 100, 600])
+def test_scales_at_their_ends(spg, lib, ws, xs, n):
+    """Scales at the ends of their range whose products are near one: sums that need no rounding, and values in the range of fp32."""
+    import torch
+    rng = np.random.default_rng(ws + n)
+    out, k = 150, 160
+    half = 2.0 ** (ws + xs - 254)
+    mats = []
+    for rows, byte in ((out, ws), (n, xs)):
+        code = rng.integers(0, 16, (rows, k)).astype(np.uint8)
+        scale = np.full((rows, k // 32), byte, np.uint8)
+        mats.append((Packed(spg, rows, k, *plain.pack(code, scale, k)), plain.values(code, np.full_like(scale, 127), k)))
+    y = torch.empty((n, out), dtype=torch.float32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert lib.spgk_layer_mx4(mats[0][0].ref, None, 6, mats[1][0].ref, y.data_ptr(), 2, out, None, status.data_ptr(), None) == 0
+    assert np.array_equal(y.double().cpu().numpy(), mats[1][1] @ mats[0][1].T * half)
+
+
 @pytest.mark.parametrize("n,out,k", [(5, 140, 300), (140, 300, 300), (600, 140, 700)])
 def test_nan_blocks_stay_in_their_rows(spg, lib, n, out, k):
     import torch
