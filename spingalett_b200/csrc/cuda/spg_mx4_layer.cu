@@ -93,30 +93,31 @@ __device__ __forceinline__ void put(__half *y, float v, uint32_t yes) { put16(y,
 __device__ __forceinline__ void put(__nv_bfloat16 *y, float v, uint32_t yes) { put16(y, __bfloat16_as_ushort(__float2bfloat16_rn(v)), yes); }
 
 // Eight rows' values of this lane's unit, the warp's 32 units being one block of the next layer's input: scales, codes, stores.
-// A lane's eight codes are eight nibbles of a word, one a row; three exchanges among eight lanes turn that into eight nibbles of one row.
+// Lane i makes row i's scale for all.  A lane's eight codes are eight nibbles of a word, one a row; three exchanges among eight lanes turn that into
+// eight nibbles of one row.  (Instructions bound it: with every lane making every scale a tile of 256 x 256 took longer to put out than 4096 inputs to multiply.)
 __device__ __forceinline__ void put_next(const LayerParams &p, const float (&v)[8], uint32_t n0, uint32_t rows, uint32_t j0, uint32_t lane)
 {
-    float q[8];
-    uint32_t mine = 0;
+    uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const uint32_t byte = spgmx4::scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(v[i]) & 0x7fffffffu));
-        q[i] = byte == 255u ? 0.0f : v[i] * spgmx4::inverse_scale(byte);
-        if (lane == (uint32_t)i) mine = byte;
+        const uint32_t a = __reduce_max_sync(0xffffffffu, __float_as_uint(v[i]) & 0x7fffffffu);
+        if (lane % 8u == (uint32_t)i) most = a;
     }
-    uint32_t w = spgmx4::encode8(q);
+    const uint32_t mine = spgmx4::scale_byte(most);                              // row lane % 8
+    const float inv = spgmx4::inverse_scale(mine);
+    float q[8];
 #pragma unroll
-    for (int s = 4, bits = 16; s; s >>= 1, bits >>= 1) {
-        const uint32_t low = bits == 16 ? 0x0000ffffu : (bits == 8 ? 0x00ff00ffu : 0x0f0f0f0fu);
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, w, s);
-        w = (lane & s) ? ((w & ~low) | ((other >> bits) & low)) : ((w & low) | ((other & low) << bits));
-    }
+    for (int i = 0; i < 8; i++) q[i] = v[i] * __shfl_sync(0xffffffffu, inv, i);
+    uint32_t w = spgmx4::encode8(q);
+    w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 4), lane & 4u ? 0x3276 : 0x5410);
+    w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 2), lane & 2u ? 0x3715 : 0x6240);
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, w, 1);
+    w = lane & 1u ? ((w & 0xf0f0f0f0u) | ((other >> 4) & 0x0f0f0f0fu)) : ((w & 0x0f0f0f0fu) | ((other & 0x0f0f0f0fu) << 4));
+    if (mine == 255u) w = 0;                                                     // a NaN block
     const uint32_t n = n0 + lane % 8u, j = j0 + lane / 8u * 8u;
     if (lane % 8u < rows && j0 < (p.out + 31u) / 32u * 32u) *reinterpret_cast<uint32_t *>(p.next_codes + (uint64_t)n * p.next_pitch + j / 2u) = w;
-    if (lane < 8u && lane < rows) {
-        const uint32_t row = n0 + lane;
-        p.next_scales[((uint64_t)(row / 128u) * p.next_kt + j0 / 128u) * SF_TILE + spgmx4::scale_in_tile(row) + j0 % 128u / 32u] = (uint8_t)mine;
-    }
+    if (lane < 8u && lane < rows)
+        p.next_scales[((uint64_t)(n / 128u) * p.next_kt + j0 / 128u) * SF_TILE + spgmx4::scale_in_tile(n) + j0 % 128u / 32u] = (uint8_t)mine;
 }
 
 // C rows' sums of this lane's unit to outputs.  What is chosen -- activation, type -- is chosen outside the loops over them: an epilogue runs a few times a
