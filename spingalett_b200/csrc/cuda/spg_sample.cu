@@ -5,7 +5,8 @@
 //   weights that are left exceeds u times their total.
 //
 // All three cuts leave a beginning of the same order, so what is left is told by one logit and a number: the logits above it, and the first r of
-// those equal to it.  Nothing is sorted.  A row belongs to a cluster of up to eight CTAs and is read once, into shared memory.
+// those equal to it.  Nothing is sorted.  A row belongs to a cluster of up to eight CTAs and is read once, into shared memory; many long rows have a CTA each, which
+// reads its row from L2 pass by pass.
 //   - A small top_k: each thread has the largest of its logits, and the (k / CTAs)-th largest of those in a CTA bounds the k-th logit of the row from
 //     below; the few logits above the least of these bounds meet in one CTA, where every thread counts what stands before its own.
 //   - Otherwise a cut is found by a histogram over the range in question (counts for top-k, weights for top-p), a list of the bin in which the border
@@ -13,12 +14,13 @@
 // Sums of 131072 weights in 32 bits would put a number drawn close to a border on its wrong side in some rows of a hundred.  Here a weight is a
 // whole multiple of 2^-44 (the largest is 1) that is good to 2^-30 of itself: errors that are independent of one another, so a sum of n of them is good to
 // 2^-30 / sqrt(n), and sums in 64 bits that do not hang on an order.
-// What bounds it: 256 x 131072 of fp32 226 us with top_p, 122 without a cut, 104 with top_k 50 (HBM would take 21), 64 x 50001 of bf16 with all cuts 14, 1 x 1000 6.5.
-// A row's logits fill a CTA's shared memory, so sixteen warps have an SM, and the way through the barriers of a row (some 20 of its 50 thousand cycles with
-// top_p) and some hundred instructions a logit are what they wait for, not memory.  Slower: two CTAs with half the logits each on an SM (the same
-// rows at work), 1024 threads (what every warp does for itself), 64-bit atomics, additions to bins left out for light logits, rows fetched to L2 ahead.
+// What bounds it: 256 x 131072 of fp32 143 us with top_p, 90 without a cut, 66 with top_k 50 (HBM would take 21), 64 x 50001 of bf16 with all cuts 14, 1 x 1000 6.5.
+// With top_p some hundred instructions a logit, issued at two fifths of the rate (a row's way through its barriers is some 20 of 50 thousand cycles), bound it
+// and not memory.  Kept in shared memory, such rows fill it, so that sixteen warps have an SM (228 us).  Slower there: two CTAs with half the logits each on an SM (the
+// same rows at work), 1024 threads (what every warp does for itself), 64-bit atomics, additions to bins left out for light logits, rows fetched to L2 ahead.
 #include "spg_common.cuh"
 #include "spg_tc.cuh"
+#include <type_traits>
 
 namespace {
 
@@ -128,13 +130,14 @@ struct Item { float l; uint32_t index; uint64_t w; };
 constexpr uint32_t PIECES = 64;               // of a CTA's slice, in the order of the vocabulary: four a warp, two a lane
 static_assert(PIECES == 64 && PIECES % WARPS == 0 && SLICE + 8 <= 65536, "two a lane; places in 16 bits");
 
-struct alignas(16) Shared {
+// Place: what a warp puts side by side of a logit -- where it lies in shared memory, or itself
+template <typename Place> struct alignas(16) Shared {
     uint64_t mass[BINS];
     uint32_t count[BINS + 32], count_low[BINS + 32];
     union { struct { uint32_t list[LIST]; uint16_t piece[LIST]; }; Item few[FEW]; };
     uint32_t table[STEPS];
     uint64_t piece_sum[PIECES]; uint32_t piece_equal[PIECES];
-    uint16_t dense[WARPS][DENSE];
+    Place dense[WARPS][DENSE];
     uint32_t left;
     uint64_t out[2][4];                        // what this CTA tells the others, by turns
     uint64_t warp[2][WARPS];
@@ -155,24 +158,76 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr)
     return v;
 }
 
-struct Row {
-    Shared &s;
-    const float4 *packs;                       // this CTA's logits by fours, -infinity in front of the first and behind the last
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// This CTA's logits by fours, -infinity in front of the first and behind the last: from its shared memory, or as they lie in the row
+struct Kept {
+    using Place = uint16_t;
+    static constexpr uint32_t AT_ONCE = 1;     // fours of a thread on their way at a time
+    const float4 *fours;
+    __device__ __forceinline__ float4 operator()(uint32_t i) const { return fours[i]; }
+    __device__ __forceinline__ float at(Place place) const { return reinterpret_cast<const float *>(fours)[place]; }
+    __device__ __forceinline__ static Place place(uint32_t i, float) { return (Place)i; }
+};
+__device__ __forceinline__ float4 load4(const float *x) { return __ldg(reinterpret_cast<const float4 *>(x)); }
+template <typename T> __device__ __forceinline__ float4 load4(const T *x)
+{
+    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(x));
+    const T *t = reinterpret_cast<const T *>(&v);
+    return make_float4(to_f32(t[0]), to_f32(t[1]), to_f32(t[2]), to_f32(t[3]));
+}
+template <typename T> struct Streamed {
+    using Place = float;
+    static constexpr uint32_t AT_ONCE = 4;
+    const T *x;                                // four elements' alignment, `lead` of them in front of the row
+    uint32_t lead, end;
+    __device__ __forceinline__ float4 operator()(uint32_t i) const
+    {
+        const uint32_t e = 4 * i;
+        if (e >= lead && e + 4 <= end) return load4(x + e);
+        float v[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) v[j] = e + j >= lead && e + j < end ? to_f32(x[e + j]) : -INFINITY;
+        return make_float4(v[0], v[1], v[2], v[3]);
+    }
+    __device__ __forceinline__ float at(Place place) const { return place; }
+    __device__ __forceinline__ static Place place(uint32_t, float l) { return l; }
+};
+
+template <typename Source> struct Row {
+    Shared<typename Source::Place> &s;
+    Source fours;
     uint32_t count, per_piece;                 // fours, and fours of a piece (a multiple of 32)
     uint32_t split, rank, turn, place;         // CTAs of the row
     uint64_t told;
 
-    template <typename F> __device__ __forceinline__ void each(F f) const        // (four at a time, so that their chains of instructions overlap)
+    static constexpr uint32_t AT_ONCE = Source::AT_ONCE;
+
+    __device__ __forceinline__ static float4 nothing() { return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
+    // fours a, a + step, ... below b
+    template <typename F> __device__ __forceinline__ void each_four(uint32_t a, uint32_t b, uint32_t step, F f) const
     {
-        for (uint32_t i = threadIdx.x; i < count; i += THREADS) { const float4 v = packs[i]; f(v.x); f(v.y); f(v.z); f(v.w); }
+        for (uint32_t i = a; i < b; i += AT_ONCE * step) {
+            float4 v[AT_ONCE];
+#pragma unroll
+            for (uint32_t u = 0; u < AT_ONCE; u++) v[u] = u == 0 || i + u * step < b ? fours(i + u * step) : nothing();
+#pragma unroll
+            for (uint32_t u = 0; u < AT_ONCE; u++) f(v[u]);
+        }
     }
-    // the fours of piece q of this warp
+    // (four logits at a time, so that their chains of instructions overlap)
+    template <typename F> __device__ __forceinline__ void each(F f) const
+    {
+        each_four(threadIdx.x, count, THREADS, [&](const float4 &v) { f(v.x); f(v.y); f(v.z); f(v.w); });
+    }
+    // the logits of piece q of this warp
     template <typename F> __device__ __forceinline__ void each_of_piece(uint32_t q, F f) const
     {
         const uint32_t a = (threadIdx.x / 32 * (PIECES / WARPS) + q) * per_piece, b = min(count, a + per_piece);
-        for (uint32_t i = a + threadIdx.x % 32; i < b; i += 32) { const float4 v = packs[i]; f(v.x); f(v.y); f(v.z); f(v.w); }
+        each_four(a + threadIdx.x % 32, b, 32, [&](const float4 &v) { f(v.x); f(v.y); f(v.z); f(v.w); });
     }
-
     __device__ __forceinline__ void sync() { if (split > 1) spgtc::cluster_sync(); else __syncthreads(); }
     __device__ __forceinline__ uint64_t sum_warp(uint64_t v)
     {
@@ -336,8 +391,7 @@ struct Row {
         s.count[threadIdx.x] = 0; s.count_low[threadIdx.x] = 0;
         if (threadIdx.x == 0) s.listed = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < this->count; i += THREADS) {
-            const float4 v = packs[i];
+        each_four(threadIdx.x, this->count, THREADS, [&](const float4 &v) {
             const float l[4] = { v.x, v.y, v.z, v.w };
             uint32_t m[4], at[4];
 #pragma unroll
@@ -350,7 +404,7 @@ struct Row {
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) { atomicAdd(&s.count_low[at[j]], m[j] & 0xffffu); atomicAdd(&s.count[at[j]], m[j] >> 16); }
-        }
+        });
         sync();
         uint64_t low = 0, high = 0;
 #pragma unroll
@@ -380,8 +434,7 @@ struct Row {
         // way from a logit to its weight is long, and so it is gone a few times a warp.
         const float bottom = border == BINS - 1 ? -INFINITY : w.top - (float)(border * 64 + 2) / (w.c * (float)STEPS) - 1e-6f * fabsf(w.top);
         constexpr uint32_t MINE = PIECES / WARPS;
-        uint16_t *const dense = s.dense[threadIdx.x / 32];
-        const float *const logits = reinterpret_cast<const float *>(packs);
+        typename Source::Place *const dense = s.dense[threadIdx.x / 32];
         const uint32_t lane = threadIdx.x % 32, first_piece = threadIdx.x / 32 * MINE;
         uint32_t small = 0xffffffffu, large = 0, many = 0, sure = 0, held = 0, ends[MINE];              // ends: of the pieces among the places
         uint64_t sums[MINE];
@@ -390,7 +443,7 @@ struct Row {
         const auto weigh = [&]() {
             __syncwarp();
             for (uint32_t i = lane; i < held; i += 32) {
-                const float x = logits[dense[i]];
+                const float x = fours.at(dense[i]);
                 const uint32_t at_bin = w.bin(x);
                 const uint64_t one = w.quick(x);
                 uint32_t piece = 0;
@@ -418,13 +471,13 @@ struct Row {
 #pragma unroll
                     for (uint32_t r = 0; r < q; r++) ends[r] = 0;
                 }
-                const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), v = i0 + lane < b ? packs[i0 + lane] : none, v2 = i0 + 32 + lane < b ? packs[i0 + 32 + lane] : none;
+                const float4 v = i0 + lane < b ? fours(i0 + lane) : nothing(), v2 = i0 + 32 + lane < b ? fours(i0 + 32 + lane) : nothing();
                 const float l[8] = { v.x, v.y, v.z, v.w, v2.x, v2.y, v2.z, v2.w };
 #pragma unroll
                 for (uint32_t j = 0; j < 8; j++) {
                     const bool in = l[j] > over && l[j] >= bottom;
                     const uint32_t set = __ballot_sync(0xffffffffu, in);
-                    if (in) dense[held + __popc(set & ((1u << lane) - 1))] = (uint16_t)(4 * (i0 + j / 4 * 32 + lane) + j % 4);
+                    if (in) dense[held + __popc(set & ((1u << lane) - 1))] = Source::place(4 * (i0 + j / 4 * 32 + lane) + j % 4, l[j]);
                     held += __popc(set);
                 }
             }
@@ -471,16 +524,13 @@ struct Row {
 // whether l weighs min_p of the largest
 __device__ __forceinline__ bool heavy(const Weights &w, float l, double log_min_p) { return l == w.top || (!isinf(w.top) && ((double)l - w.m) * w.inv_t >= log_min_p); }
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-template <typename T>
-__global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams p)
+template <typename T, bool STREAM>
+__global__ void __launch_bounds__(THREADS, 2) spg_sample_kernel(const SampleParams p)
 {
     extern __shared__ __align__(16) uint8_t raw[];
-    Shared &s = *reinterpret_cast<Shared *>(raw);
-    float *logits = reinterpret_cast<float *>(raw + sizeof(Shared));
+    using Source = std::conditional_t<STREAM, Streamed<T>, Kept>;
+    Shared<typename Source::Place> &s = *reinterpret_cast<Shared<typename Source::Place> *>(raw);
+    float *logits = reinterpret_cast<float *>(raw + sizeof(s));
     const uint32_t row = blockIdx.x / p.split, rank = blockIdx.x % p.split, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t from = min(p.width, rank * p.slice), n = min(p.width - from, p.slice);
     for (uint32_t i = threadIdx.x; i < STEPS; i += THREADS) s.table[i] = __ldg(&g_steps.v[i]);
@@ -494,14 +544,6 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
 
     // The row, its largest and smallest logits and how many there are: 16 bytes a load between the ends that do not lie on 16 bytes
     const T *x = reinterpret_cast<const T *>(p.logits) + (uint64_t)row * p.ld + from;
-    constexpr uint32_t PER = 16 / sizeof(T);
-    const uint32_t off = (uint32_t)((uintptr_t)x % 16u / sizeof(T)), first = min(n, (PER - off) % PER), packs = (n - first) / PER;
-    const uint32_t lead = (4u - first % 4u) % 4u;                                // packs lie on 16 bytes here too
-    if (threadIdx.x < 8) {                                                       // what makes the first and the last four whole
-        if (threadIdx.x < lead) logits[threadIdx.x] = -INFINITY;
-        else if (threadIdx.x >= 4 && threadIdx.x - 4 < (4u - (lead + n) % 4u) % 4u) logits[lead + n + threadIdx.x - 4] = -INFINITY;
-    }
-    float *const row_logits = logits + lead;
     float mine = -INFINITY, least = INFINITY;
     uint32_t have = 0;
     const auto take = [&](float l) -> float {
@@ -509,41 +551,54 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
         mine = fmaxf(mine, l); least = fminf(least, some ? l : INFINITY); have += some;             // (of a NaN and a number both give the number)
         return l;
     };
-    if (sizeof(T) == 4) {
-        // straight to shared memory, the whole slice on its way at once (through registers 132 SMs drew 4 TB/s); a thread looks at what it has asked for, by quarters
-        const uint32_t quarter = (packs + 4 * THREADS - 1) / (4 * THREADS) * THREADS;
-#pragma unroll
-        for (uint32_t q = 0; q < 4; q++) {
-            for (uint32_t i = q * quarter + threadIdx.x; i < min(packs, (q + 1) * quarter); i += THREADS)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(row_logits + first) + 16 * i), "l"(reinterpret_cast<const uint4 *>(x + first) + i) : "memory");
-            asm volatile("cp.async.commit_group;" ::: "memory");
+    constexpr uint32_t PER = 16 / sizeof(T);
+    const uint32_t off = (uint32_t)((uintptr_t)x % 16u / sizeof(T)), first = min(n, (PER - off) % PER), packs = (n - first) / PER;
+    const uint32_t lead = STREAM ? off % 4u : (4u - first % 4u) % 4u, fours = (lead + n + 3u) / 4u;           // packs lie on 16 bytes here too
+    Source source;
+    if constexpr (STREAM) { source.x = x - lead; source.lead = lead; source.end = lead + n; }
+    else source.fours = reinterpret_cast<const float4 *>(logits);
+    Row<Source> R{ s, source, fours, ((fours + PIECES - 1) / PIECES + 31u) / 32u * 32u, p.split, rank, 0, 0, 0 };
+    if constexpr (STREAM) R.each([&](float l) { take(l); });
+    else {
+        if (threadIdx.x < 8) {                                                       // what makes the first and the last four whole
+            if (threadIdx.x < lead) logits[threadIdx.x] = -INFINITY;
+            else if (threadIdx.x >= 4 && threadIdx.x - 4 < (4u - (lead + n) % 4u) % 4u) logits[lead + n + threadIdx.x - 4] = -INFINITY;
         }
-        const auto look = [&](uint32_t q) {
-            for (uint32_t i = q * quarter + threadIdx.x; i < min(packs, (q + 1) * quarter); i += THREADS) {
-                const float4 v = *reinterpret_cast<const float4 *>(row_logits + first + 4 * i);
-                take(v.x); take(v.y); take(v.z); take(v.w);
+        float *const row_logits = logits + lead;
+        if (sizeof(T) == 4) {
+            // straight to shared memory, the whole slice on its way at once (through registers 132 SMs drew 4 TB/s); a thread looks at what it has asked for, by quarters
+            const uint32_t quarter = (packs + 4 * THREADS - 1) / (4 * THREADS) * THREADS;
+#pragma unroll
+            for (uint32_t q = 0; q < 4; q++) {
+                for (uint32_t i = q * quarter + threadIdx.x; i < min(packs, (q + 1) * quarter); i += THREADS)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(row_logits + first) + 16 * i), "l"(reinterpret_cast<const uint4 *>(x + first) + i) : "memory");
+                asm volatile("cp.async.commit_group;" ::: "memory");
             }
-        };
-        asm volatile("cp.async.wait_group 3;" ::: "memory"); look(0);
-        asm volatile("cp.async.wait_group 2;" ::: "memory"); look(1);
-        asm volatile("cp.async.wait_group 1;" ::: "memory"); look(2);
-        asm volatile("cp.async.wait_group 0;" ::: "memory"); look(3);
-    } else {
+            const auto look = [&](uint32_t q) {
+                for (uint32_t i = q * quarter + threadIdx.x; i < min(packs, (q + 1) * quarter); i += THREADS) {
+                    const float4 v = *reinterpret_cast<const float4 *>(row_logits + first + 4 * i);
+                    take(v.x); take(v.y); take(v.z); take(v.w);
+                }
+            };
+            asm volatile("cp.async.wait_group 3;" ::: "memory"); look(0);
+            asm volatile("cp.async.wait_group 2;" ::: "memory"); look(1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory"); look(2);
+            asm volatile("cp.async.wait_group 0;" ::: "memory"); look(3);
+        } else {
 #pragma unroll 4
-        for (uint32_t i = threadIdx.x; i < packs; i += THREADS) {
-            alignas(16) T v[PER];
-            *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(x + first) + i);
+            for (uint32_t i = threadIdx.x; i < packs; i += THREADS) {
+                alignas(16) T v[PER];
+                *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(x + first) + i);
 #pragma unroll
-            for (uint32_t j = 0; j < PER; j += 4)
-                *reinterpret_cast<float4 *>(row_logits + first + i * PER + j) = make_float4(take(to_f32(v[j])), take(to_f32(v[j + 1])), take(to_f32(v[j + 2])), take(to_f32(v[j + 3])));
+                for (uint32_t j = 0; j < PER; j += 4)
+                    *reinterpret_cast<float4 *>(row_logits + first + i * PER + j) = make_float4(take(to_f32(v[j])), take(to_f32(v[j + 1])), take(to_f32(v[j + 2])), take(to_f32(v[j + 3])));
+            }
+        }
+        if (threadIdx.x < 2 * PER) {                                                 // the ends
+            const uint32_t i = threadIdx.x < PER ? threadIdx.x : first + packs * PER + threadIdx.x - PER;
+            if (i < (threadIdx.x < PER ? first : n)) row_logits[i] = take(to_f32(x[i]));
         }
     }
-    if (threadIdx.x < 2 * PER) {                                                 // the ends
-        const uint32_t i = threadIdx.x < PER ? threadIdx.x : first + packs * PER + threadIdx.x - PER;
-        if (i < (threadIdx.x < PER ? first : n)) row_logits[i] = take(to_f32(x[i]));
-    }
-    const uint32_t fours = (lead + n + 3u) / 4u;
-    Row R{ s, reinterpret_cast<const float4 *>(logits), fours, ((fours + PIECES - 1) / PIECES + 31u) / 32u * 32u, p.split, rank, 0, 0, 0 };
     uint32_t top = R.max_cta(key_of(mine)), low = ~R.max_cta(~key_of(least));
     have = (uint32_t)R.sum_cta(have);
     R.tell(top, low, have);
@@ -579,7 +634,7 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
         for (uint32_t r = 0; r < p.split; r++) bound = min(bound, (uint32_t)R.heard(r, 0));
         const float at_least = of_key(bound);
         for (uint32_t i = threadIdx.x; i < fours; i += THREADS) {
-            const float4 v = R.packs[i];
+            const float4 v = R.fours(i);
             if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= at_least) {
                 const float l[4] = { v.x, v.y, v.z, v.w };
 #pragma unroll
@@ -661,7 +716,7 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
     if (all && !greedy) {
         if (k >= 1 && (uint32_t)k < all) {
             uint64_t above = 0;
-            cut = R.select<false>(w, low, top, (uint64_t)k, above);
+            cut = R.template select<false>(w, low, top, (uint64_t)k, above);
             ties = (uint32_t)(k - above);
         }
         if (pp < 1.0f && w.fast) summed = R.mass_cut(w, pp, cut, ties);
@@ -681,7 +736,7 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
             if (sum < goal) ties = (uint32_t)min((uint64_t)ties, (goal - sum + each - 1) / max(each, (uint64_t)1));
             else {
                 uint64_t above = 0;
-                cut = R.select<true>(w, nearest, top, goal, above);
+                cut = R.template select<true>(w, nearest, top, goal, above);
                 const uint64_t one = w(of_key(cut));
                 ties = (uint32_t)((goal - above + one - 1) / one);
             }
@@ -768,7 +823,7 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
             const uint32_t a = piece * R.per_piece, b = min(fours, a + R.per_piece);
             for (uint32_t i0 = a; i0 < b; i0 += 32) {
                 const uint32_t i = i0 + lane;
-                const float4 four = i < b ? R.packs[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                const float4 four = i < b ? R.fours(i) : R.nothing();
                 const float l[4] = { four.x, four.y, four.z, four.w };
                 uint64_t one[4], mine4 = 0;
                 uint32_t same = 0;
@@ -808,28 +863,38 @@ __global__ void __launch_bounds__(THREADS) spg_sample_kernel(const SampleParams 
     R.sync();                                                                    // (nobody leaves while its shared memory is read)
 }
 
-template <typename T> int launch(SampleParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
+template <typename T, bool STREAM> int launch(const SampleParams &p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
 {
     static SpgOncePerDevice once;
     const int rc = once.run(dev, [&]() -> int {
-        SPGK_CUDA(cudaFuncSetAttribute(spg_sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dp.smem_optin));
+        SPGK_CUDA(cudaFuncSetAttribute(spg_sample_kernel<T, STREAM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dp.smem_optin));
         return SPGK_OK;
     });
     if (rc) return rc;
-    p.split = 1;
-    while (p.split < MAX_SPLIT && (p.width > p.split * SLICE || (p.width > p.split * 2048u && (uint64_t)p.N * p.split * 2 <= (uint32_t)dp.sm_count * 2u))) p.split *= 2;
-    p.slice = ((p.width + p.split - 1) / p.split + 7u) / 8u * 8u;
-    if ((uint64_t)p.N * p.split > 0x7fffffffu) { spgk_set_error("spgk_sample_rows", "too many rows"); return SPGK_E_ARG; }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.N * p.split); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = sizeof(Shared) + (size_t)p.slice * 4 + 32; cfg.stream = stream;
+    cfg.gridDim = dim3(p.N * p.split); cfg.blockDim = dim3(THREADS); cfg.stream = stream;
+    cfg.dynamicSmemBytes = STREAM ? sizeof(Shared<float>) : sizeof(Shared<uint16_t>) + (size_t)p.slice * 4 + 32;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = p.split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    SPGK_CUDA(cudaLaunchKernelEx(&cfg, spg_sample_kernel<T>, p));
+    SPGK_CUDA(cudaLaunchKernelEx(&cfg, spg_sample_kernel<T, STREAM>, p));
     return spgk_check_launch("spg_sample_kernel");
+}
+
+template <typename T> int launch_rows(SampleParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
+{
+    // Rows that would fill an SM's shared memory, and enough of them: a CTA each, two an SM, which reads its row again from L2 for every pass instead of keeping it.
+    // us kept and streamed, with top_p: 256 x 131072 228 and 143, 148 x 131072 143 and 95, 148 x 60000 57 and 50, 512 x 32000 106 and 97; 96 x 131072 88 and 115,
+    // 512 x 16000 with top_k 21 and 23, 64 x 50001 14 and 17.
+    const bool streamed = p.width > SLICE / 2 && p.N >= (uint32_t)dp.sm_count * 7 / 8;
+    p.split = 1;
+    while (!streamed && p.split < MAX_SPLIT && (p.width > p.split * SLICE || (p.width > p.split * 2048u && (uint64_t)p.N * p.split * 2 <= (uint32_t)dp.sm_count * 2u))) p.split *= 2;
+    p.slice = ((p.width + p.split - 1) / p.split + 7u) / 8u * 8u;
+    if ((uint64_t)p.N * p.split > 0x7fffffffu) { spgk_set_error("spgk_sample_rows", "too many rows"); return SPGK_E_ARG; }
+    return streamed ? launch<T, true>(p, dp, dev, stream) : launch<T, false>(p, dp, dev, stream);
 }
 
 }  // namespace
@@ -853,7 +918,7 @@ extern "C" int spgk_sample_rows(const void *logits, int type, uint32_t ld, uint3
     if (rc) return rc;
     SPGK_CUDA(cudaGetDevice(&dev));
     SampleParams p{ logits, type, ld, N, width, 1, width, temperature, top_k, top_p, min_p, u, tokens, probs, kept };
-    if (type == SPGK_T_F32) return launch<float>(p, dp, dev, (cudaStream_t)stream);
-    if (type == SPGK_T_F16) return launch<__half>(p, dp, dev, (cudaStream_t)stream);
-    return launch<__nv_bfloat16>(p, dp, dev, (cudaStream_t)stream);
+    if (type == SPGK_T_F32) return launch_rows<float>(p, dp, dev, (cudaStream_t)stream);
+    if (type == SPGK_T_F16) return launch_rows<__half>(p, dp, dev, (cudaStream_t)stream);
+    return launch_rows<__nv_bfloat16>(p, dp, dev, (cudaStream_t)stream);
 }

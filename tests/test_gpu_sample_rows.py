@@ -176,3 +176,27 @@ def test_outputs_that_are_not_wanted_and_replay(lib):
         for i in range(6):
             assert tokens[i].item() == plain.sample_row(rows[i], 1.0, None, float(np.float32(0.9)), None, u[i].item())[0]
     del graph
+
+
+@pytest.mark.parametrize("cuts", ["none", "k", "p", "kpm", "K", "Kp"])
+@pytest.mark.parametrize("kind,pad", [(2, 0), (2, 3), (1, 0), (0, 5)])
+def test_many_long_rows(lib, cuts, kind, pad):
+    """Rows that are read pass by pass, at every alignment of their ends; the first of them masked, equal, or full of ties."""
+    import torch
+    rng = np.random.default_rng(len(cuts) + 7 * kind + pad)
+    n, width = 150, 16411
+    x = (rng.standard_normal((n, width + pad)) * 3).astype(np.float32)
+    x[0] = -np.inf
+    x[1] = 0.5
+    x[2] = np.round(x[2])
+    x[3, ::2] = np.nan
+    x[4, 5], x[4, width - 1] = np.inf, np.inf
+    x[5, 9000:] = -np.inf
+    x = torch.from_numpy(x).cuda().to({0: torch.float16, 1: torch.bfloat16, 2: torch.float32}[kind])[:, :width]
+    t = rng.uniform(0.4, 1.5, n)
+    t[6] = 0
+    k = rng.integers(300, 3000, n) if "K" in cuts else rng.integers(1, 250, n) if "k" in cuts else None
+    p = rng.uniform(0.05, 1.02, n) if "p" in cuts else None
+    m = rng.uniform(0.0, 0.2, n) if "m" in cuts else None
+    u = rng.random(n).astype(np.float32)
+    _check(_draw(lib, x, t, k, p, m, u, kind), x, t, k, p, m, u)
