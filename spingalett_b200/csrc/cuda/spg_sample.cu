@@ -8,7 +8,8 @@
 // those equal to it.  Nothing is sorted.  A row belongs to a cluster of up to eight CTAs and is read once, into shared memory; many long rows have a CTA each, which
 // reads its row from L2 pass by pass.
 //   - A small top_k: each thread has the largest of its logits, and the (k / CTAs)-th largest of those in a CTA bounds the k-th logit of the row from
-//     below; the few logits above the least of these bounds meet in one CTA, where every thread counts what stands before its own.
+//     below; the few logits above the least of these bounds meet in one CTA, where every thread counts what stands before its own.  So do the logits
+//     of a short row, or of one with nearly all of them masked.
 //   - Otherwise a cut is found by a histogram over the range in question (counts for top-k, weights for top-p), a list of the bin in which the border
 //     falls (or, where that is too long, another histogram over it), and a search in the list digit by digit.
 // Sums of 131072 weights in 32 bits would put a number drawn close to a border on its wrong side in some rows of a hundred.  Here a weight is a
@@ -31,6 +32,7 @@ constexpr uint32_t BINS = 512;
 constexpr uint32_t DENSE = 512;               // places that a warp puts side by side
 constexpr uint32_t LIST = 2048;               // logits of a range that are searched digit by digit
 constexpr uint32_t FEW = 512;                 // logits among which every thread counts what stands before its own
+constexpr uint32_t TINY = 128;                // rows with no more logits are all of them few (512 x 100 with top_p: 15.5 us, as long rows 25.0; without a cut 14.9 and 12.4)
 constexpr uint32_t MAX_SPLIT = 8;
 constexpr uint32_t SLICE = SPGK_SAMPLE_MAX_WIDTH / MAX_SPLIT;
 constexpr int ONE_BITS = 44;
@@ -614,25 +616,32 @@ __global__ void __launch_bounds__(THREADS, 2) spg_sample_kernel(const SamplePara
     Weights w;
     w.set(largest, greedy ? 1.0f : t, s.table);
 
-    if (rich && !greedy && k >= 1 && (uint32_t)k < all && (uint32_t)k <= FEW / 2) {
-        // At least k logits of the row are no smaller than the least of the rich CTAs' (k / rich)-th largest of their threads' largest; a bin's lower end will do
-        const uint32_t want = ((uint32_t)k + rich - 1) / rich;
-        s.count[threadIdx.x] = 0;
-        if (threadIdx.x == 0) { s.listed = 0; s.found_bin = BINS; }
-        const bool some = mine > -INFINITY;
-        const float best = of_key(R.max_cta(key_of(mine))), worst = of_key(~R.max_cta(some ? ~key_of(mine) : 0)), width = (best - worst) * (1.0f / BINS);
-        const bool even = width > 0.0f && width < INFINITY;                      // (else they are all equal: no bound)
-        if (even && some) atomicAdd(&s.count[min(BINS - 1, (uint32_t)((best - mine) / width))], 1u);
+    const uint32_t first_k = k >= 1 && (uint32_t)k < all ? (uint32_t)k : all;    // logits that top_k leaves
+    const bool cuts = first_k < all || pp < 1.0f || mp > 0.0f;
+    if (all && !greedy && ((cuts && all <= TINY) || (rich && first_k < all && first_k <= FEW / 2))) {
+        float at_least = -FLT_MAX;
+        if (all > TINY) {
+            // At least k logits of the row are no smaller than the least of the rich CTAs' (k / rich)-th largest of their threads' largest; a bin's lower end will do
+            const uint32_t want = (first_k + rich - 1) / rich;
+            s.count[threadIdx.x] = 0;
+            if (threadIdx.x == 0) s.found_bin = BINS;
+            const bool some = mine > -INFINITY;
+            const float best = of_key(R.max_cta(key_of(mine))), worst = of_key(~R.max_cta(some ? ~key_of(mine) : 0)), width = (best - worst) * (1.0f / BINS);
+            const bool even = width > 0.0f && width < INFINITY;                  // (else they are all equal: no bound)
+            if (even && some) atomicAdd(&s.count[min(BINS - 1, (uint32_t)((best - mine) / width))], 1u);
+            __syncthreads();
+            uint64_t threads;
+            const uint32_t c = s.count[threadIdx.x], upto = (uint32_t)R.scan_cta(c, threads);
+            if (even && upto >= want && upto - c < want) s.found_bin = threadIdx.x;
+            __syncthreads();
+            const float end = best - ((float)s.found_bin + 1.001f) * width - 1e-6f * (fabsf(best) + fabsf(worst));
+            R.tell(have < p.slice / 2 ? 0xffffffffu : key_of(s.found_bin < BINS && end > -FLT_MAX ? end : -FLT_MAX));
+            uint32_t bound = 0xffffffffu;
+            for (uint32_t r = 0; r < p.split; r++) bound = min(bound, (uint32_t)R.heard(r, 0));
+            at_least = of_key(bound);
+        }
+        if (threadIdx.x == 0) s.listed = 0;
         __syncthreads();
-        uint64_t threads;
-        const uint32_t c = s.count[threadIdx.x], upto = (uint32_t)R.scan_cta(c, threads);
-        if (even && upto >= want && upto - c < want) s.found_bin = threadIdx.x;
-        __syncthreads();
-        const float end = best - ((float)s.found_bin + 1.001f) * width - 1e-6f * (fabsf(best) + fabsf(worst));
-        R.tell(have < p.slice / 2 ? 0xffffffffu : key_of(s.found_bin < BINS && end > -FLT_MAX ? end : -FLT_MAX));
-        uint32_t bound = 0xffffffffu;
-        for (uint32_t r = 0; r < p.split; r++) bound = min(bound, (uint32_t)R.heard(r, 0));
-        const float at_least = of_key(bound);
         for (uint32_t i = threadIdx.x; i < fours; i += THREADS) {
             const float4 v = R.fours(i);
             if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= at_least) {
@@ -676,7 +685,7 @@ __global__ void __launch_bounds__(THREADS, 2) spg_sample_kernel(const SamplePara
 #pragma unroll
                         for (int j = 0; j < 8; j++) if (o[j].l > me.l || (o[j].l == me.l && o[j].index < me.index)) { place++; before += o[j].w; }
                     }
-                bool keep = threadIdx.x < many && place < (uint32_t)k;
+                bool keep = threadIdx.x < many && place < first_k;
                 if (pp < 1.0f) {
                     const double reach = ceil((double)pp * (double)R.sum_cta(keep ? me.w : 0));
                     keep = keep && before < (reach >= 1.0 ? (uint64_t)reach : 1);
@@ -714,10 +723,10 @@ __global__ void __launch_bounds__(THREADS, 2) spg_sample_kernel(const SamplePara
     bool summed = false;
     if (all && greedy) { cut = top; ties = 1; }
     if (all && !greedy) {
-        if (k >= 1 && (uint32_t)k < all) {
+        if (first_k < all) {
             uint64_t above = 0;
-            cut = R.template select<false>(w, low, top, (uint64_t)k, above);
-            ties = (uint32_t)(k - above);
+            cut = R.template select<false>(w, low, top, first_k, above);
+            ties = (uint32_t)(first_k - above);
         }
         if (pp < 1.0f && w.fast) summed = R.mass_cut(w, pp, cut, ties);
         else if (pp < 1.0f) {
