@@ -51,10 +51,11 @@ template <typename T> __device__ __forceinline__ uint32_t largest(const T (&t)[8
     return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&a)));
 }
 
+// (Plain loads, here and below: those through the read-only path may be moved in front of the wait for the launch that writes what they read.)
 // VEC: rows of x lie on 16 bytes.  AT_ONCE: rows of a group on their way at a time
 template <typename T, bool VEC, uint32_t AT_ONCE>
-__global__ void __launch_bounds__(THREADS) spg_mx4_quantize_kernel(const T *__restrict__ x, uint32_t ldx, uint8_t *__restrict__ codes, uint32_t pitch,
-                                                                  uint8_t *__restrict__ scales, uint32_t rows, uint32_t cols, uint32_t share)
+__global__ void __launch_bounds__(THREADS) spg_mx4_quantize_kernel(const T *x, uint32_t ldx, uint8_t *codes, uint32_t pitch,
+                                                                  uint8_t *scales, uint32_t rows, uint32_t cols, uint32_t share)
 {
     spg_grid_trigger();
     spg_grid_wait();
@@ -70,7 +71,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_quantize_kernel(const T *__re
             const T *src = x + (uint64_t)(row0 + r) * ldx + c0;
             if (VEC && r < p.end && c0 + 8u <= cols) {
 #pragma unroll
-                for (uint32_t i = 0; i < sizeof(T) / 2; i++) reinterpret_cast<uint4 *>(t[k])[i] = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
+                for (uint32_t i = 0; i < sizeof(T) / 2; i++) reinterpret_cast<uint4 *>(t[k])[i] = reinterpret_cast<const uint4 *>(src)[i];
             } else {
 #pragma unroll
                 for (uint32_t i = 0; i < 8; i++) t[k][i] = r < p.end && c0 + i < cols ? src[i] : from_f32<T>(0.0f);
@@ -99,8 +100,8 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_quantize_kernel(const T *__re
 }
 
 template <typename T, bool VEC, uint32_t AT_ONCE>
-__global__ void __launch_bounds__(THREADS) spg_mx4_dequantize_kernel(const uint8_t *__restrict__ codes, uint32_t pitch, const uint8_t *__restrict__ scales,
-                                                                    T *__restrict__ y, uint32_t ldy, uint32_t rows, uint32_t cols, uint32_t share)
+__global__ void __launch_bounds__(THREADS) spg_mx4_dequantize_kernel(const uint8_t *codes, uint32_t pitch, const uint8_t *scales,
+                                                                    T *y, uint32_t ldy, uint32_t rows, uint32_t cols, uint32_t share)
 {
     __shared__ float side[VEC ? 1 : THREADS / 32][2][128];       // values whose rows do not lie on 16 bytes leave side by side, one a lane
     spg_grid_trigger();
@@ -118,11 +119,11 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_dequantize_kernel(const uint8
             code[k] = word[k] = 0;
             if (r >= p.end) continue;
             const uint8_t *src = codes + (uint64_t)(row0 + r) * pitch;
-            word[k] = __ldg(words + scale_in_tile(r) / 4u);
+            word[k] = words[scale_in_tile(r) / 4u];
             if (HALVES) {
-                if (c0 < cols) code[k] = __ldg(reinterpret_cast<const uint16_t *>(src + c0 / 2u));
-                if (c1 < cols) code[k] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(src + c1 / 2u)) << 16;
-            } else if (c0 < cols) code[k] = __ldg(reinterpret_cast<const uint32_t *>(src + c0 / 2u));
+                if (c0 < cols) code[k] = *reinterpret_cast<const uint16_t *>(src + c0 / 2u);
+                if (c1 < cols) code[k] |= (uint32_t)*reinterpret_cast<const uint16_t *>(src + c1 / 2u) << 16;
+            } else if (c0 < cols) code[k] = *reinterpret_cast<const uint32_t *>(src + c0 / 2u);
         }
 #pragma unroll
         for (uint32_t k = 0; k < AT_ONCE; k++) {

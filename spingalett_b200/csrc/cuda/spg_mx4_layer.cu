@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         for (uint32_t dry = 1;; dry = 0) {
             if (!dry) {
                 spg_grid_wait();
-                if (p.bias && j < p.out) bias = __ldg(p.bias + j);
+                if (p.bias && j < p.out) bias = p.bias[j];
                 ok = mbar_wait(done, 0, abort_flag, p.status, 3);
                 if (!ok) mbar_wait(done, 0, &never, p.status, 5);                // the products under way end before tensor memory is given back
                 tc_fence_after();
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
             uint32_t jt, nt;
             pair_tile(t, j_tiles, n_tiles, jt, nt);
             const uint32_t j0 = jt * 256u + rank * 128u + quad * 32u, j = j0 + lane, n0 = nt * PN + part * P_COLS;
-            const float bias = !dry && p.bias && j < p.out ? __ldg(p.bias + j) : 0.0f;
+            const float bias = !dry && p.bias && j < p.out ? p.bias[j] : 0.0f;
             const uint32_t from = tmem + (quad * 32u << 16) + part * P_COLS;
             const bool some = j0 < (p.next_codes ? (p.out + 127u) / 128u * 128u : p.out);       // (the next operand's scale tiles are written whole)
             if (!dry) {

@@ -29,6 +29,7 @@ using spgtc::smem_u32; using spgtc::mapa; using spgtc::cluster_rank;
 
 constexpr uint32_t THREADS = 512, WARPS = THREADS / 32;
 constexpr uint32_t BINS = 512;
+constexpr uint32_t ONCE = 65536 / 4;          // fours whose mantissas' halves, all in one bin, come to less than 2^32
 constexpr uint32_t DENSE = 512;               // places that a warp puts side by side
 constexpr uint32_t LIST = 2048;               // logits of a range that are searched digit by digit
 constexpr uint32_t FEW = 512;                 // logits among which every thread counts what stands before its own
@@ -173,10 +174,11 @@ struct Kept {
     __device__ __forceinline__ float at(Place place) const { return reinterpret_cast<const float *>(fours)[place]; }
     __device__ __forceinline__ static Place place(uint32_t i, float) { return (Place)i; }
 };
-__device__ __forceinline__ float4 load4(const float *x) { return __ldg(reinterpret_cast<const float4 *>(x)); }
+// (plain loads: one through the read-only path may be moved in front of the wait for the launch that writes the logits)
+__device__ __forceinline__ float4 load4(const float *x) { return *reinterpret_cast<const float4 *>(x); }
 template <typename T> __device__ __forceinline__ float4 load4(const T *x)
 {
-    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(x));
+    const uint2 v = *reinterpret_cast<const uint2 *>(x);
     const T *t = reinterpret_cast<const T *>(&v);
     return make_float4(to_f32(t[0]), to_f32(t[1]), to_f32(t[2]), to_f32(t[3]));
 }
@@ -393,22 +395,30 @@ template <typename Source> struct Row {
         s.count[threadIdx.x] = 0; s.count_low[threadIdx.x] = 0;
         if (threadIdx.x == 0) s.listed = 0;
         __syncthreads();
-        each_four(threadIdx.x, this->count, THREADS, [&](const float4 &v) {
-            const float l[4] = { v.x, v.y, v.z, v.w };
-            uint32_t m[4], at[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                int k;
-                m[j] = w.mantissa(l[j], k);
-                const uint32_t bin = min(BINS - 1, (uint32_t)(63 - k) >> 6);
-                if (bin == BINS - 1) m[j] >>= min(-(k >> 10) - (ONE_BITS - 30), 31);
-                at[j] = l[j] > over ? bin : BINS + threadIdx.x % 32;             // (what is not left goes to a place of its lane: no branches)
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) { atomicAdd(&s.count_low[at[j]], m[j] & 0xffffu); atomicAdd(&s.count[at[j]], m[j] >> 16); }
-        });
-        sync();
         uint64_t low = 0, high = 0;
+        for (uint32_t from = 0; from < this->count; from += ONCE) {
+            each_four(from + threadIdx.x, min(this->count, from + ONCE), THREADS, [&](const float4 &v) {
+                const float l[4] = { v.x, v.y, v.z, v.w };
+                uint32_t m[4], at[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    int k;
+                    m[j] = w.mantissa(l[j], k);
+                    const uint32_t bin = min(BINS - 1, (uint32_t)(63 - k) >> 6);
+                    if (bin == BINS - 1) m[j] >>= min(-(k >> 10) - (ONE_BITS - 30), 31);
+                    at[j] = l[j] > over ? bin : BINS + threadIdx.x % 32;             // (what is not left goes to a place of its lane: no branches)
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) { atomicAdd(&s.count_low[at[j]], m[j] & 0xffffu); atomicAdd(&s.count[at[j]], m[j] >> 16); }
+            });
+            if (from + ONCE < this->count) {                                     // (a whole long row: what is there is taken out of the 32 bits)
+                __syncthreads();
+                low += s.count_low[threadIdx.x]; high += s.count[threadIdx.x];
+                s.count_low[threadIdx.x] = 0; s.count[threadIdx.x] = 0;
+                __syncthreads();
+            }
+        }
+        sync();
 #pragma unroll
         for (uint32_t r = 0; r < MAX_SPLIT; r++) {
             if (r >= split) continue;
@@ -590,7 +600,7 @@ __global__ void __launch_bounds__(THREADS, 2) spg_sample_kernel(const SamplePara
 #pragma unroll 4
             for (uint32_t i = threadIdx.x; i < packs; i += THREADS) {
                 alignas(16) T v[PER];
-                *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(x + first) + i);
+                *reinterpret_cast<uint4 *>(v) = reinterpret_cast<const uint4 *>(x + first)[i];
 #pragma unroll
                 for (uint32_t j = 0; j < PER; j += 4)
                     *reinterpret_cast<float4 *>(row_logits + first + i * PER + j) = make_float4(take(to_f32(v[j])), take(to_f32(v[j + 1])), take(to_f32(v[j + 2])), take(to_f32(v[j + 3])));

@@ -200,3 +200,24 @@ def test_many_long_rows(lib, cuts, kind, pad):
     m = rng.uniform(0.0, 0.2, n) if "m" in cuts else None
     u = rng.random(n).astype(np.float32)
     _check(_draw(lib, x, t, k, p, m, u, kind), x, t, k, p, m, u)
+
+
+@pytest.mark.parametrize("n", [2, 130])
+def test_rows_of_one_value_but_few(lib, n):
+    """More equal logits in one bin than sums of 32 bits would hold, below a few larger ones: kept in shared memory, and read pass by pass."""
+    import torch
+    rng = np.random.default_rng(n)
+    width = 200001
+    x = np.full((n, width), -0.3, np.float32)
+    x[:, 77], x[:, 150000] = 1.0, 0.25
+    x[0, 5] = 9.0
+    x[1, 1000:1100] = rng.standard_normal(100)
+    if n > 2:
+        x[2:, ::3] += rng.uniform(0, 0.01, (n - 2, 66667)).astype(np.float32)
+    xd = torch.from_numpy(x).cuda()
+    rows = np.unique(np.r_[0, 1, rng.integers(0, n, 10)])                        # (a plain sort of each)
+    for cuts in ((None, 0.5, None), (None, 0.99, None), (1000, 0.7, None), (None, None, None), (70000, None, None), (None, 0.3, 0.2)):
+        t, u = np.full(n, 0.7), rng.random(n).astype(np.float32)
+        a = [None if v is None else np.full(n, v) for v in cuts]
+        got = _draw(lib, xd, t, *a, u)
+        _check([g[rows] for g in got], xd[torch.from_numpy(rows).cuda()], t[rows], *[None if v is None else v[rows] for v in a], u[rows])
