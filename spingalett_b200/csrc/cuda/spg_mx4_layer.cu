@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
             if (++s == p.stages) { s = 0; phase ^= 1u; }
         }
         if (*abort_flag)                         // the copies under way end before this CTA does
-            for (uint32_t i = last > p.stages ? last - p.stages : 0; i < last; i++) mbar_wait(full + 8 * (i % p.stages), i / p.stages & 1u, &never, p.status, 4);
+            for (uint32_t i = last > p.stages ? last - p.stages : 0; i < last; i++) mbar_wait(full + 8 * (i % p.stages), i / p.stages & 1u, &never, p.status, 4, 1u << 12);
     } else if (warp == 1) {
         const uint32_t idesc = idesc_mx4(NT);
         for (uint32_t kb = lo, s = 0, phase = 0; kb < hi; kb++) {
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
                 spg_grid_wait();
                 if (p.bias && j < p.out) bias = p.bias[j];
                 ok = mbar_wait(done, 0, abort_flag, p.status, 3);
-                if (!ok) mbar_wait(done, 0, &never, p.status, 5);                // the products under way end before tensor memory is given back
+                if (!ok) mbar_wait(done, 0, &never, p.status, 5, 1u << 12);                // the products under way end before tensor memory is given back
                 tc_fence_after();
                 if (p.split > 1) {
                     // this CTA's sums, [column][unit], into its own shared memory (no copy or product is under way any more)
@@ -594,8 +594,10 @@ int scales_map(CUtensorMap *map, const spgk_mx4 *m, uint32_t box_tiles)
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, m->scales, kt * 128, ((uint64_t)m->rows + 127) / 128, kt * SF_TILE, 256, box_tiles, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-// How a product is arranged: CTAs that share a tile, and an estimate in cycles (of a chain of launches on a B200 at 1.9 GHz: k-blocks at what the MMA warp,
-// HBM or L2 needs for them; what a launch, sixteen columns of outputs, sums from other CTAs' memory take is from cycle counters).
+// How a product is arranged: CTAs that share a tile, and an estimate in cycles of a chain of launches on a B200 at 1.9 GHz.  Fitted to 280 products (1 to 3001 rows,
+// 512 to 16384 inputs, 128 to 8192 units): what it picks takes 0.4 % longer on average than the best of all arrangements, 19 % at most.  A k-block takes 440 cycles, and up to 590
+// where all SMs draw on HBM; eight CTAs that share a tile find room for 15 clusters at a time, four for 33
+// (twice that where two CTAs have room on an SM).
 struct Plan { uint32_t split; uint64_t cycles; };
 Plan plan_single(const LayerParams &p, uint32_t nt, uint32_t sms)
 {
@@ -603,9 +605,10 @@ Plan plan_single(const LayerParams &p, uint32_t nt, uint32_t sms)
     const uint32_t cols = p.N < nt ? p.N : nt;
     Plan best = { 1, ~0ull };
     for (uint32_t s = 1; s <= MAX_SPLIT && s <= p.kblocks; s *= 2) {
-        if (s > 1 && tiles * s > sms) break;
-        const uint64_t waves = (tiles * s + sms - 1) / sms, outputs = s == 1 ? (cols + 31) / 32 * 900 : 2500 + (cols + 16 * s - 1) / (16 * s) * 1800;
-        const uint64_t cycles = 3000 + waves * ((uint64_t)((p.kblocks + s - 1) / s) * 570 + outputs);
+        if (s > 1 && tiles > (s == 8 ? 15u : s == 4 ? 33u : 74u) * (nt <= 64 ? 2u : 1u) * sms / 148u) break;
+        const uint64_t waves = (tiles * s + sms - 1) / sms, block = 440 + (tiles * s < sms ? tiles * s : sms);
+        const uint64_t outputs = s == 1 ? (cols + 31) / 32 * 900 : 3000 + s * 250 + cols / s * 120;
+        const uint64_t cycles = 4500 + waves * ((uint64_t)((p.kblocks + s - 1) / s) * block + outputs);
         if (cycles < best.cycles) best = { s, cycles };
     }
     return best;
@@ -613,7 +616,7 @@ Plan plan_single(const LayerParams &p, uint32_t nt, uint32_t sms)
 uint64_t pair_cycles(const LayerParams &p, uint32_t sms)
 {
     const uint64_t tiles = (uint64_t)((p.out + 255) / 256) * ((p.N + PN - 1) / PN), waves = (tiles + sms / 2 - 1) / (sms / 2);
-    return 8000 + waves * ((uint64_t)p.kblocks * 512 + 600);
+    return 10000 + waves * ((uint64_t)p.kblocks * 530 + 600);
 }
 
 template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
@@ -710,7 +713,7 @@ extern "C" int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, con
     if (p.N <= 16) return launch<16>(W, X, p, dp, dev, st);
     if (p.N <= 32) return launch<32>(W, X, p, dp, dev, st);
     if (p.N <= 64) return launch<64>(W, X, p, dp, dev, st);
-    // (256 x 8192 x 8192: 14.7 us with single CTAs, 16 in pairs; 512 rows 28.9 and 16; 300 x 1000 x 512 6 and 9)
+    // (us with single CTAs and in pairs: 256 x 8192 x 8192 14.9 and 16.2, 512 rows 28.9 and 17.1, 300 x 1000 x 512 6.0 and 6.7, 130 x 8192 x 1000 10.0 and 14.0)
     if (plan_single(p, 128, (uint32_t)dp.sm_count).cycles <= pair_cycles(p, (uint32_t)dp.sm_count)) return launch<128>(W, X, p, dp, dev, st);
     return launch_pairs(W, X, p, dp, dev, st);
 }
