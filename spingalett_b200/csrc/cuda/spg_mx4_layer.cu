@@ -10,7 +10,7 @@
 // Where there are few tiles, up to eight CTAs of a cluster share one, each with its part of the k-blocks, and add their sums in rank order.
 //
 // More than some hundred rows go to pairs of CTAs (below); which, and how many CTAs share a tile, an estimate in cycles says.
-// What bounds it: one row x 8192 x 16384 14.4 us (4.9 TB/s; 570 cycles a k-block on 128 CTAs is HBM's rate, the rest start and end of a launch),
+// What bounds it: one row x 8192 x 16384 14.3 us (5.0 TB/s; 570 cycles a k-block on 128 CTAs is HBM's rate, the rest start and end of a launch),
 // 64 x 16384 x 16384 30.7 us (4.8 TB/s), 1 x 784 x 512 3.1 us (a launch), 16384 x 8192 x 8192 365 us (6020 TFLOP/s, 500 cycles a k-block of 512 at the
 // tensor pipe's best; 430 us in a long run, under the power limit).
 //
@@ -32,6 +32,7 @@ constexpr uint32_t SF_BYTES = 2 * SF_TILE;    // of 128 rows in a k-block
 constexpr uint32_t EPI = 8, THREADS = 64 + 32 * EPI;   // warp 0: copies, warp 1: products, warps 2 to 9: outputs, two a quarter of the lanes
 constexpr uint32_t MAX_STAGES = 8;
 constexpr uint32_t MAX_SPLIT = 8;
+constexpr uint32_t AHEAD = 2;
 constexpr uint32_t HEAD = 1024;
 constexpr uint32_t ROOM_FOR_TWO = 112 * 1024;     // shared memory of a CTA that leaves room for one of the next launch
 
@@ -181,14 +182,12 @@ __device__ __forceinline__ void sums_taken() { asm volatile("bar.sync 1, %0;" ::
 
 template <uint32_t NT> struct Tile {
     static constexpr uint32_t X_BYTES = NT * 128;
-    static constexpr uint32_t SFX_TILES = (NT + 127) / 128;
-    static constexpr uint32_t STAGE = (W_BYTES + X_BYTES + SF_BYTES + SFX_TILES * SF_BYTES + 1023) / 1024 * 1024;
-    static constexpr uint32_t SFX_COLS = NT < 128 ? 4 : NT / 32;              // columns of the rows' scales for four blocks
-    static constexpr uint32_t SFW = NT < 32 ? 16 : NT;                         // tensor memory: sums, weights' scales, rows' scales
+    static constexpr uint32_t STAGE = (W_BYTES + X_BYTES + 2 * SF_BYTES + 1023) / 1024 * 1024;
+    static constexpr uint32_t SFW = NT;                                        // tensor memory: sums, weights' scales, rows' scales
     static constexpr uint32_t SFX = 8;                                         // (behind the weights' scales)
-    static constexpr uint32_t SF_COLS = 8 + 2 * SFX_COLS;                      // of a k-block, twice: copied while the products of the one before run
+    static constexpr uint32_t SF_COLS = 16;                                    // of a k-block, twice: copied while the products of the one before run
     static constexpr uint32_t USED = SFW + 2 * SF_COLS;
-    static constexpr uint32_t COLS = USED <= 32 ? 32 : USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+    static constexpr uint32_t COLS = USED <= 64 ? 64 : USED <= 128 ? 128 : 256;
 };
 
 template <uint32_t NT>
@@ -218,27 +217,26 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
     spg_grid_trigger();
-    // the first weights to L2 while the kernel in front still runs (whoever writes them: L2 is where writes meet)
+    // The first weights to L2 while the kernel in front still runs (whoever writes them: L2 is where writes meet).  Two k-blocks: none cost two layers
+    // of 8 rows 0.1 us of 26.9, eight cost them 0.5 and a layer of one row 0.9 us of 15.1, as the copies behind the wait queue behind them.
     if (warp == 0 && elect_one())
-        for (uint32_t kb = lo; kb < hi && kb < lo + p.stages; kb++) prefetch_l2(&map_w, (int)(kb * 128u), (int)(j_tile * TM));
+        for (uint32_t kb = lo; kb < hi && kb < lo + AHEAD; kb++) prefetch_l2(&map_w, (int)(kb * 128u), (int)(j_tile * TM));
     __syncwarp();
     if (warp < 2) spg_grid_wait();
     volatile int never = 0;
 
     if (warp == 0) {
-        const uint32_t sfx_tiles = min(L::SFX_TILES, (p.N + 127u) / 128u - n0 / 128u);      // (the last tile of rows may have fewer)
         uint32_t last = 0;
         for (uint32_t kb = lo, s = 0, phase = 1; kb < hi; kb++) {
             mbar_wait_uniform(empty + 8 * s, phase, aborted, p.status, 1);
             if (*abort_flag) break;
             const uint32_t at = ring + s * L::STAGE, sf = min(2u, p.kt - 2 * kb) * SF_TILE;
             if (elect_one()) {
-                mbar_expect_tx(full + 8 * s, W_BYTES + L::X_BYTES + sf * (1 + sfx_tiles));
+                mbar_expect_tx(full + 8 * s, W_BYTES + L::X_BYTES + sf * 2);
                 tma_load_2d(at, &map_w, full + 8 * s, (int)(kb * 128u), (int)(j_tile * TM));
                 tma_load_2d(at + W_BYTES, &map_x, full + 8 * s, (int)(kb * 128u), (int)n0);
                 bulk_load(at + W_BYTES + L::X_BYTES, p.w_scales + ((uint64_t)j_tile * p.kt + 2 * kb) * SF_TILE, sf, full + 8 * s);
-                for (uint32_t t = 0; t < sfx_tiles; t++)
-                    bulk_load(at + W_BYTES + L::X_BYTES + SF_BYTES * (1 + t), p.x_scales + ((uint64_t)(n0 / 128u + t) * p.kt + 2 * kb) * SF_TILE, sf, full + 8 * s);
+                bulk_load(at + W_BYTES + L::X_BYTES + SF_BYTES, p.x_scales + ((uint64_t)(n0 / 128u) * p.kt + 2 * kb) * SF_TILE, sf, full + 8 * s);
             }
             __syncwarp();
             last = kb + 1 - lo;
@@ -258,12 +256,11 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
                 const uint64_t dw = scale_desc(sfw), dx = scale_desc(sfx), a = smem_desc_sw128(at), b = smem_desc_sw128(at + W_BYTES);
                 const auto scales = [&](uint32_t i) {
                     copy_scales(sf + 4 * i, dw + i * (SF_TILE >> 4));
-#pragma unroll
-                    for (uint32_t t = 0; t < L::SFX_TILES; t++) copy_scales(sf + L::SFX + L::SFX_COLS * i + 4 * t, dx + ((t * SF_BYTES + i * SF_TILE) >> 4));
+                    copy_scales(sf + L::SFX + 4 * i, dx + i * (SF_TILE >> 4));
                 };
                 const auto product = [&](uint32_t i, uint32_t more) {
                     const uint32_t id = (i & 1u) * 2u;          // which two of a tile's four scales
-                    umma_mx4(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, sf + 4 * (i / 2), sf + L::SFX + L::SFX_COLS * (i / 2), more);
+                    umma_mx4(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, sf + 4 * (i / 2), sf + L::SFX + 4 * (i / 2), more);
                 };
                 if (kb * KB + KB - 64u < p.cols) {
                     scales(0); scales(1);
