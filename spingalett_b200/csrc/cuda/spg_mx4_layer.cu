@@ -10,8 +10,8 @@
 // Where there are few tiles, up to eight CTAs of a cluster share one, each with its part of the k-blocks, and add their sums in rank order.
 //
 // More than some hundred rows go to pairs of CTAs (below); which, and how many CTAs share a tile, an estimate in cycles says.
-// What bounds it: one row x 8192 x 16384 14.3 us (5.0 TB/s; 570 cycles a k-block on 128 CTAs is HBM's rate, the rest start and end of a launch),
-// 64 x 16384 x 16384 30.7 us (4.8 TB/s), 1 x 784 x 512 3.1 us (a launch), 16384 x 8192 x 8192 365 us (6020 TFLOP/s, 500 cycles a k-block of 512 at the
+// What bounds it: one row x 8192 x 16384 12.8 us (5.6 TB/s; HBM, and start and end of a launch), 64 x 16384 x 16384 27.2 us (5.4 TB/s),
+// 1 x 784 x 512 3.1 us (a launch), 16384 x 8192 x 8192 365 us (6020 TFLOP/s, 500 cycles a k-block of 512 at the
 // tensor pipe's best; 430 us in a long run, under the power limit).
 //
 // Every wait on an mbarrier is bounded; a CTA that gave up records a code in `status`, and its cluster leaves the tile's outputs alone.
@@ -34,7 +34,10 @@ constexpr uint32_t MAX_STAGES = 8;
 constexpr uint32_t MAX_SPLIT = 8;
 constexpr uint32_t AHEAD = 2;
 constexpr uint32_t HEAD = 1024;
-constexpr uint32_t ROOM_FOR_TWO = 112 * 1024;     // shared memory of a CTA that leaves room for one of the next launch
+// Shared memory of a CTA: room for another one beside it where an SM has more than one to do (a wave's end under the next one's start), else a longer ring.
+// (us with 112 and 180 KB: 64 x 16384 x 16384 on 128 CTAs 31.0 and 28.0, 64 x 8192 x 16384 16.9 and 14.9, 64 x 4096 x 65536 on 512 31.4 and 41; 227 KB
+// leave the rest of an SM's memory too small a cache: one row x 8192 x 16384 14.2, 13.6 and, with 227, 14.4)
+constexpr uint32_t ROOM_FOR_TWO = 112 * 1024, ROOM_ALONE = 180 * 1024;
 
 struct LayerParams {
     uint32_t N, out, cols, kblocks, kt;       // rows, units, inputs; k-blocks; scale tiles of a row
@@ -50,18 +53,20 @@ struct LayerParams {
 // kind::mxf4, E2M1 on both sides, UE8M0 scales, M = 128
 __host__ __device__ constexpr uint32_t idesc_mx4(uint32_t n) { return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24); }
 
-__device__ __forceinline__ void umma_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate)
+// (predicated: a k-block's products and copies are one way without branches)
+__device__ __forceinline__ void umma_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate, uint32_t yes)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+        "setp.ne.b32 q, %7, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(yes) : "memory");
 }
 // 512 bytes (32 rows of 16) -> four columns of tensor memory, once for each quarter of the lanes
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc)
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc, uint32_t yes)
 {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(yes) : "memory");
 }
 // no swizzle, groups of eight rows of 16 bytes 128 bytes apart
 __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr)
@@ -227,58 +232,45 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
 
     if (warp == 0) {
         uint32_t last = 0;
-        for (uint32_t kb = lo, s = 0, phase = 1; kb < hi; kb++) {
-            mbar_wait_uniform(empty + 8 * s, phase, aborted, p.status, 1);
-            if (*abort_flag) break;
-            const uint32_t at = ring + s * L::STAGE, sf = min(2u, p.kt - 2 * kb) * SF_TILE;
-            if (elect_one()) {
+        if (elect_one())
+            for (uint32_t kb = lo, s = 0, phase = 1; kb < hi; kb++) {
+                if (!mbar_wait(empty + 8 * s, phase, abort_flag, p.status, 1)) break;
+                const uint32_t at = ring + s * L::STAGE, sf = min(2u, p.kt - 2 * kb) * SF_TILE;
                 mbar_expect_tx(full + 8 * s, W_BYTES + L::X_BYTES + sf * 2);
                 tma_load_2d(at, &map_w, full + 8 * s, (int)(kb * 128u), (int)(j_tile * TM));
                 tma_load_2d(at + W_BYTES, &map_x, full + 8 * s, (int)(kb * 128u), (int)n0);
                 bulk_load(at + W_BYTES + L::X_BYTES, p.w_scales + ((uint64_t)j_tile * p.kt + 2 * kb) * SF_TILE, sf, full + 8 * s);
                 bulk_load(at + W_BYTES + L::X_BYTES + SF_BYTES, p.x_scales + ((uint64_t)(n0 / 128u) * p.kt + 2 * kb) * SF_TILE, sf, full + 8 * s);
+                last = kb + 1 - lo;
+                if (++s == p.stages) { s = 0; phase ^= 1u; }
             }
-            __syncwarp();
-            last = kb + 1 - lo;
-            if (++s == p.stages) { s = 0; phase ^= 1u; }
-        }
+        last = __reduce_max_sync(0xffffffffu, last);
         if (*abort_flag)                         // the copies under way end before this CTA does
             for (uint32_t i = last > p.stages ? last - p.stages : 0; i < last; i++) mbar_wait(full + 8 * (i % p.stages), i / p.stages & 1u, &never, p.status, 4, 1u << 12);
     } else if (warp == 1) {
+        // (One lane runs the loop, and the last k-block has one commit, not two: 340 cycles a k-block.  With the lane chosen anew for each, a way of its own for
+        // a row's end and a second commit behind the loop it took 445, whatever the copies and products were, and a short layer 0.1 us more.)
         const uint32_t idesc = idesc_mx4(NT);
-        for (uint32_t kb = lo, s = 0, phase = 0; kb < hi; kb++) {
-            mbar_wait_uniform(full + 8 * s, phase, aborted, p.status, 2);
-            tc_fence_after();
-            const uint32_t at = ring + s * L::STAGE, sf = tmem + L::SFW + ((kb - lo) & 1u) * L::SF_COLS;
-            if (elect_one()) {
-                // (written out: a whole k-block takes 800 cycles to issue from loops that end at run time)
+        if (elect_one())
+            for (uint32_t kb = lo, s = 0, phase = 0; kb < hi; kb++) {
+                mbar_wait_uniform(full + 8 * s, phase, aborted, p.status, 2);
+                tc_fence_after();
+                const uint32_t at = ring + s * L::STAGE, sf = tmem + L::SFW + ((kb - lo) & 1u) * L::SF_COLS, left = p.cols - kb * KB;
                 const uint32_t sfw = at + W_BYTES + L::X_BYTES, sfx = sfw + SF_BYTES;
                 const uint64_t dw = scale_desc(sfw), dx = scale_desc(sfx), a = smem_desc_sw128(at), b = smem_desc_sw128(at + W_BYTES);
-                const auto scales = [&](uint32_t i) {
-                    copy_scales(sf + 4 * i, dw + i * (SF_TILE >> 4));
-                    copy_scales(sf + L::SFX + 4 * i, dx + i * (SF_TILE >> 4));
+                const auto scales = [&](uint32_t i, uint32_t yes) {
+                    copy_scales(sf + 4 * i, dw + i * (SF_TILE >> 4), yes);
+                    copy_scales(sf + L::SFX + 4 * i, dx + i * (SF_TILE >> 4), yes);
                 };
-                const auto product = [&](uint32_t i, uint32_t more) {
+                const auto product = [&](uint32_t i, uint32_t more, uint32_t yes) {
                     const uint32_t id = (i & 1u) * 2u;          // which two of a tile's four scales
-                    umma_mx4(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, sf + 4 * (i / 2), sf + L::SFX + 4 * (i / 2), more);
+                    umma_mx4(tmem, a + 2 * i, b + 2 * i, idesc | id << 4 | id << 29, sf + 4 * (i / 2), sf + L::SFX + 4 * (i / 2), more, yes);
                 };
-                if (kb * KB + KB - 64u < p.cols) {
-                    scales(0); scales(1);
-                    product(0, kb > lo); product(1, 1); product(2, 1); product(3, 1);
-                } else {
-                    const uint32_t steps = (p.cols - kb * KB + 63u) / 64u;
-                    scales(0);
-                    if (steps > 2) scales(1);
-                    product(0, kb > lo);
-                    if (steps > 1) product(1, 1);
-                    if (steps > 2) product(2, 1);
-                }
-                umma_commit(empty + 8 * s);
+                scales(0, 1); scales(1, left > 128);
+                product(0, kb > lo, 1); product(1, 1, left > 64); product(2, 1, left > 128); product(3, 1, left > 192);
+                umma_commit(kb + 1 < hi ? empty + 8 * s : done);
+                if (++s == p.stages) { s = 0; phase ^= 1u; }
             }
-            __syncwarp();
-            if (++s == p.stages) { s = 0; phase ^= 1u; }
-        }
-        if (elect_one()) umma_commit(done);
         __syncwarp();
         if (p.split > 1) {
             // Given back before this CTA waits for the others: one that has none on its SM, and so cannot finish, may hold up a cluster that holds some elsewhere
@@ -591,10 +583,11 @@ int scales_map(CUtensorMap *map, const spgk_mx4 *m, uint32_t box_tiles)
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, m->scales, kt * 128, ((uint64_t)m->rows + 127) / 128, kt * SF_TILE, 256, box_tiles, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-// How a product is arranged: CTAs that share a tile, and an estimate in cycles of a chain of launches on a B200 at 1.9 GHz.  Fitted to 280 products (1 to 3001 rows,
-// 512 to 16384 inputs, 128 to 8192 units): what it picks takes 0.4 % longer on average than the best of all arrangements, 19 % at most.  A k-block takes 440 cycles, and up to 590
-// where all SMs draw on HBM; eight CTAs that share a tile find room for 15 clusters at a time, four for 33
-// (twice that where two CTAs have room on an SM).
+// How a product is arranged: CTAs that share a tile, and an estimate in cycles of a chain of launches on a B200 at 1.9 GHz.  Fitted to 1377 products (1 to 1000 rows,
+// 256 to 16384 inputs, 128 to 16384 units): what it picks takes 0.2 % longer on average than the best of all arrangements, 20 % at most.  A k-block takes some 300 cycles, and 430
+// where all SMs draw on HBM.
+// clusters of this many CTAs that find room at a time, one CTA an SM
+uint32_t at_a_time(uint32_t split, uint32_t sms) { return (split == 8 ? 15u : split == 4 ? 33u : split == 2 ? 74u : 148u) * sms / 148u; }
 struct Plan { uint32_t split; uint64_t cycles; };
 Plan plan_single(const LayerParams &p, uint32_t nt, uint32_t sms)
 {
@@ -602,9 +595,9 @@ Plan plan_single(const LayerParams &p, uint32_t nt, uint32_t sms)
     const uint32_t cols = p.N < nt ? p.N : nt;
     Plan best = { 1, ~0ull };
     for (uint32_t s = 1; s <= MAX_SPLIT && s <= p.kblocks; s *= 2) {
-        if (s > 1 && tiles > (s == 8 ? 15u : s == 4 ? 33u : 74u) * (nt <= 64 ? 2u : 1u) * sms / 148u) break;
-        const uint64_t waves = (tiles * s + sms - 1) / sms, block = 440 + (tiles * s < sms ? tiles * s : sms);
-        const uint64_t outputs = s == 1 ? (cols + 31) / 32 * 900 : 3000 + s * 250 + cols / s * 120;
+        if (s > 1 && tiles > at_a_time(s, sms)) break;
+        const uint64_t waves = (tiles * s + sms - 1) / sms, block = 280 + (tiles * s < sms ? tiles * s : sms);
+        const uint64_t outputs = s == 1 ? (cols + 31) / 32 * 900 : 4500 + s * 450 + cols / s * 120;
         const uint64_t cycles = 4500 + waves * ((uint64_t)((p.kblocks + s - 1) / s) * block + outputs);
         if (cycles < best.cycles) best = { s, cycles };
     }
@@ -629,7 +622,7 @@ template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerPar
     if ((rc = codes_map(&map_w, W, TM)) || (rc = codes_map(&map_x, X, NT))) return rc;
     const uint32_t j_tiles = (p.out + TM - 1) / TM, n_tiles = (p.N + NT - 1) / NT;
     p.split = plan_single(p, NT, (uint32_t)dp.sm_count).split;
-    const uint32_t room = NT <= 64 ? ROOM_FOR_TWO : (uint32_t)dp.smem_optin;
+    const uint32_t room = NT > 64 ? (uint32_t)dp.smem_optin : (uint64_t)j_tiles * n_tiles > at_a_time(p.split, (uint32_t)dp.sm_count) ? ROOM_FOR_TWO : ROOM_ALONE;
     const uint32_t most = (room - HEAD - 1024) / L::STAGE, mine = (p.kblocks + p.split - 1) / p.split;
     p.stages = mine < most ? mine : most;
     if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
@@ -710,7 +703,7 @@ extern "C" int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, con
     if (p.N <= 16) return launch<16>(W, X, p, dp, dev, st);
     if (p.N <= 32) return launch<32>(W, X, p, dp, dev, st);
     if (p.N <= 64) return launch<64>(W, X, p, dp, dev, st);
-    // (us with single CTAs and in pairs: 256 x 8192 x 8192 14.9 and 16.2, 512 rows 28.9 and 17.1, 300 x 1000 x 512 6.0 and 6.7, 130 x 8192 x 1000 10.0 and 14.0)
+    // (us with single CTAs and in pairs: 256 x 8192 x 8192 13.6 and 16.0, 512 rows 25.4 and 16.8, 300 x 1024 x 512 5.9 and 6.8, 130 x 8192 x 1000 9.7 and 14.0)
     if (plan_single(p, 128, (uint32_t)dp.sm_count).cycles <= pair_cycles(p, (uint32_t)dp.sm_count)) return launch<128>(W, X, p, dp, dev, st);
     return launch_pairs(W, X, p, dp, dev, st);
 }
