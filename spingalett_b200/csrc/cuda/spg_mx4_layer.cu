@@ -7,11 +7,12 @@
 // the epilogue has one output unit: its bias is a register, and 32 lanes hold a whole block of the next layer's input.
 // A k-block is 256 elements: rows of 128 bytes, 128-byte swizzle, four products of 64; its scales are two tiles of 512 bytes a side,
 // which tcgen05.cp copies to tensor memory in front of the products (both are issued by one thread and run in order).
-// Where there are few tiles, up to eight CTAs of a cluster share one, each with its part of the k-blocks, and add their sums in rank order.
+// Where there are few tiles, up to eight CTAs of a cluster share one, each with its part of the k-blocks, and send one another their sums, which are added in
+// rank order.
 //
 // More than some hundred rows go to pairs of CTAs (below); which, and how many CTAs share a tile, an estimate in cycles says.
 // What bounds it: one row x 8192 x 16384 12.8 us (5.6 TB/s; HBM, and start and end of a launch), 64 x 16384 x 16384 27.2 us (5.4 TB/s),
-// 1 x 784 x 512 3.1 us (a launch), 16384 x 8192 x 8192 365 us (6020 TFLOP/s, 500 cycles a k-block of 512 at the
+// 1 x 16384 x 1000 4.8 us (eight CTAs a tile), 1 x 784 x 512 3.1 us (a launch), 16384 x 8192 x 8192 365 us (6020 TFLOP/s, 500 cycles a k-block of 512 at the
 // tensor pipe's best; 430 us in a long run, under the power limit).
 //
 // Every wait on an mbarrier is bounded; a CTA that gave up records a code in `status`, and its cluster leaves the tile's outputs alone.
@@ -33,6 +34,7 @@ constexpr uint32_t EPI = 8, THREADS = 64 + 32 * EPI;   // warp 0: copies, warp 1
 constexpr uint32_t MAX_STAGES = 8;
 constexpr uint32_t MAX_SPLIT = 8;
 constexpr uint32_t AHEAD = 2;
+constexpr uint32_t PART = 8 * TM * 4;             // a CTA's sums of eight rows
 constexpr uint32_t HEAD = 1024;
 // Shared memory of a CTA: room for another one beside it where an SM has more than one to do (a wave's end under the next one's start), else a longer ring.
 // (us with 112 and 180 KB: 64 x 16384 x 16384 on 128 CTAs 31.0 and 28.0, 64 x 8192 x 16384 16.9 and 14.9, 64 x 4096 x 65536 on 512 31.4 and 41; 227 KB
@@ -73,18 +75,13 @@ __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr)
 {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(128u >> 4) << 16 | (uint64_t)(128u >> 4) << 32 | (uint64_t)1u << 46;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr)
+__device__ __forceinline__ void st_cluster_if(uint32_t addr, float v, uint32_t yes)
 {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.shared::cluster.f32 [%0], %1;\n\t}" ::"r"(addr), "f"(v), "r"(yes) : "memory");
 }
-__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr)
-{
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // (predicated: branches around the stores cost 80 cycles each)
 __device__ __forceinline__ void put(float *y, float v, uint32_t yes)
@@ -195,16 +192,24 @@ template <uint32_t NT> struct Tile {
     static constexpr uint32_t COLS = USED <= 64 ? 64 : USED <= 128 ? 128 : 256;
 };
 
+// Where CTAs share a tile, chunks of eight of its rows go to them by turns, and each sends its sums of a chunk to the CTA that has it
+__host__ __device__ constexpr uint32_t chunks_of(uint32_t n, uint32_t nt) { return ((n < nt ? n : nt) + 7) / 8; }
+template <uint32_t NT> __host__ __device__ constexpr uint32_t parts_bytes(uint32_t n, uint32_t split)
+{
+    return split > 1 ? (chunks_of(n, NT) + split - 1) / split * split * PART : 0;
+}
+
 template <uint32_t NT>
 __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LayerParams p)
 {
     using L = Tile<NT>;
     extern __shared__ uint8_t raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-    const uint32_t head = smem_u32(base), ring = head + HEAD;
-    const uint32_t full = head, empty = head + 8 * MAX_STAGES, done = empty + 8 * MAX_STAGES, slot = done + 8, aborted = slot + 4;
+    const uint32_t head = smem_u32(base), parts = head + HEAD, ring = parts + parts_bytes<NT>(p.N, p.split);
+    const uint32_t full = head, empty = head + 8 * MAX_STAGES, done = empty + 8 * MAX_STAGES, slot = done + 8, aborted = slot + 4, told = aborted + 4;
     volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head));
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+    if (p.split > 1) cluster_arrive();                                           // (in front of the wait for tensor memory: see below)
     const uint32_t rank = blockIdx.x % p.split, j_tile = blockIdx.x / p.split, n0 = blockIdx.y * NT;
     // this CTA's k-blocks
     const uint32_t lo = (uint32_t)((uint64_t)p.kblocks * rank / p.split), hi = (uint32_t)((uint64_t)p.kblocks * (rank + 1) / p.split);
@@ -293,18 +298,26 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
                 if (!ok) mbar_wait(done, 0, &never, p.status, 5, 1u << 12);                // the products under way end before tensor memory is given back
                 tc_fence_after();
                 if (p.split > 1) {
-                    // this CTA's sums, [column][unit], into its own shared memory (no copy or product is under way any more)
-                    for (uint32_t c = half * 16u; c < NT && n0 + c < p.N; c += 32) {
-                        uint32_t r[16];
-                        tmem_ld16(lanes + c, r);
+                    // This CTA's sums to those that put them out, [chunk][CTA][row][unit].  (Sent before one barrier, not fetched behind it: reading the others' took 6800
+                    // cycles from the last product to the end, 2700 of them the instructions of 64 loads.)
+                    cluster_wait();                                              // all have begun
+                    const uint32_t chunks = chunks_of(p.N, NT);
+                    for (uint32_t c = half; c < chunks && n0 + 8 * c < p.N; c += 2) {
+                        float v[8];
+                        tmem_ld8(lanes + 8 * c, v);
                         tmem_ld_wait();
+                        const uint32_t to = mapa(parts + (c / p.split * p.split + rank) * PART + (quad * 32u + lane) * 4u, c % p.split), left = p.N - (n0 + 8 * c);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) *reinterpret_cast<uint32_t *>(base + HEAD + ((c + i) * TM + quad * 32u + lane) * 4u) = r[i];
+                        for (int i = 0; i < 8; i++) st_cluster_if(to + i * TM * 4u, v[i], (uint32_t)i < left);
                     }
+                    if (warp == 2 && lane < p.split) st_cluster_u32(mapa(told + 4 * rank, lane), *abort_flag != 0);
                     tc_fence_before();
+                    __syncwarp();
                     sums_taken();
-                    cluster_sync();
-                    for (uint32_t r = 0; r < p.split; r++) ok = ok && ld_cluster_u32(mapa(aborted, r)) == 0;
+                    cluster_arrive();
+                    cluster_wait();
+                    const volatile uint32_t *flags = reinterpret_cast<const volatile uint32_t *>(base + (told - head));
+                    ok = !__any_sync(0xffffffffu, !ok || (lane < p.split && flags[lane] != 0));
                 }
                 if (!ok) break;
             }
@@ -316,20 +329,12 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
                     if (!dry) { tmem_ld8(lanes + c, v); tmem_ld_wait(); }
                     else each(v, [](float) { return 0.0f; });
                 } else {
-                    float part[MAX_SPLIT][8];                                    // all on their way before the first is needed
-                    const uint32_t at = ring + (c * TM + quad * 32u + lane) * 4u, rows = p.N - (n0 + c);
+                    const float *part = reinterpret_cast<const float *>(base + HEAD) + (c / 8 / p.split * p.split) * (PART / 4) + quad * 32u + lane;
+                    each(v, [](float) { return 0.0f; });
+#pragma unroll 1
+                    for (uint32_t r = 0; r < p.split; r++, part += PART / 4) {   // in rank order
 #pragma unroll
-                    for (uint32_t r = 0; r < MAX_SPLIT; r++) {
-                        const uint32_t from = mapa(at, r < p.split ? r : 0);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) part[r][i] = r < p.split && (uint32_t)i < rows ? ld_cluster_f32(from + i * TM * 4u) : 0.0f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[i] = part[0][i];
-#pragma unroll
-                    for (uint32_t r = 1; r < MAX_SPLIT; r++) {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] += part[r][i];
+                        for (int i = 0; i < 8; i++) v[i] += part[i * TM];
                     }
                 }
                 finish(p, v, n0 + c, dry ? 0u : p.N - (n0 + c), j0, lane, bias);
@@ -338,10 +343,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         }
         tc_fence_before();
     }
-    if (p.split > 1) {
-        if (warp < 2) cluster_sync();
-        cluster_sync();                                                          // (nobody leaves while its sums are read)
-    }
+    if (p.split > 1 && warp < 2) { cluster_wait(); cluster_arrive(); cluster_wait(); }
     __syncthreads();
     if (warp == 1 && p.split == 1) { tc_fence_after(); tmem_free(tmem, L::COLS); }
 }
@@ -584,8 +586,8 @@ int scales_map(CUtensorMap *map, const spgk_mx4 *m, uint32_t box_tiles)
 }
 
 // How a product is arranged: CTAs that share a tile, and an estimate in cycles of a chain of launches on a B200 at 1.9 GHz.  Fitted to 1377 products (1 to 1000 rows,
-// 256 to 16384 inputs, 128 to 16384 units): what it picks takes 0.2 % longer on average than the best of all arrangements, 20 % at most.  A k-block takes some 300 cycles, and 430
-// where all SMs draw on HBM.
+// 256 to 16384 inputs, 128 to 16384 units): what it picks takes 0.7 % longer on average than the best of all arrangements, 17 % at most.  A k-block takes 310 cycles, and 580
+// where all SMs draw on HBM; clusters on more than half of the SMs leave the next launch's no room beside them.
 // clusters of this many CTAs that find room at a time, one CTA an SM
 uint32_t at_a_time(uint32_t split, uint32_t sms) { return (split == 8 ? 15u : split == 4 ? 33u : split == 2 ? 74u : 148u) * sms / 148u; }
 struct Plan { uint32_t split; uint64_t cycles; };
@@ -596,9 +598,9 @@ Plan plan_single(const LayerParams &p, uint32_t nt, uint32_t sms)
     Plan best = { 1, ~0ull };
     for (uint32_t s = 1; s <= MAX_SPLIT && s <= p.kblocks; s *= 2) {
         if (s > 1 && tiles > at_a_time(s, sms)) break;
-        const uint64_t waves = (tiles * s + sms - 1) / sms, block = 280 + (tiles * s < sms ? tiles * s : sms);
-        const uint64_t outputs = s == 1 ? (cols + 31) / 32 * 900 : 4500 + s * 450 + cols / s * 120;
-        const uint64_t cycles = 4500 + waves * ((uint64_t)((p.kblocks + s - 1) / s) * block + outputs);
+        const uint64_t ctas = tiles * s, waves = (ctas + sms - 1) / sms, block = 310 + (ctas < sms ? ctas : sms) * 9 / 5;
+        const uint64_t outputs = s == 1 ? (cols + 31) / 32 * 1700 : 2010 + s * 190 + cols / s * 70 + cols * 20;
+        const uint64_t cycles = 2660 + waves * ((uint64_t)((p.kblocks + s - 1) / s) * block + outputs) + (s > 1 && ctas * 2 > sms ? 1360 : 0);
         if (cycles < best.cycles) best = { s, cycles };
     }
     return best;
@@ -606,7 +608,7 @@ Plan plan_single(const LayerParams &p, uint32_t nt, uint32_t sms)
 uint64_t pair_cycles(const LayerParams &p, uint32_t sms)
 {
     const uint64_t tiles = (uint64_t)((p.out + 255) / 256) * ((p.N + PN - 1) / PN), waves = (tiles + sms / 2 - 1) / (sms / 2);
-    return 10000 + waves * ((uint64_t)p.kblocks * 530 + 600);
+    return 4650 + waves * ((uint64_t)p.kblocks * 580 + 4660);
 }
 
 template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
@@ -623,11 +625,10 @@ template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerPar
     const uint32_t j_tiles = (p.out + TM - 1) / TM, n_tiles = (p.N + NT - 1) / NT;
     p.split = plan_single(p, NT, (uint32_t)dp.sm_count).split;
     const uint32_t room = NT > 64 ? (uint32_t)dp.smem_optin : (uint64_t)j_tiles * n_tiles > at_a_time(p.split, (uint32_t)dp.sm_count) ? ROOM_FOR_TWO : ROOM_ALONE;
-    const uint32_t most = (room - HEAD - 1024) / L::STAGE, mine = (p.kblocks + p.split - 1) / p.split;
+    const uint32_t parts = parts_bytes<NT>(p.N, p.split), most = (room - HEAD - 1024 - parts) / L::STAGE, mine = (p.kblocks + p.split - 1) / p.split;
     p.stages = mine < most ? mine : most;
     if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-    uint32_t bytes = p.stages * L::STAGE;
-    if (p.split > 1 && bytes < NT * TM * 4u) bytes = NT * TM * 4u;
+    const uint32_t bytes = parts + p.stages * L::STAGE;
     if (n_tiles > 65535u) { spgk_set_error("spgk_layer_mx4", "more than 65535 tiles of rows"); return SPGK_E_ARG; }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(j_tiles * p.split, n_tiles); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = HEAD + 1024 + bytes; cfg.stream = stream;

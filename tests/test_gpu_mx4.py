@@ -107,7 +107,8 @@ def test_quantize_and_back(spg, lib, t, rows, cols, pad, off):
 
 
 SHAPES = [(1, 1, 1), (1, 10, 1000), (2, 333, 777), (16, 128, 256), (17, 129, 31), (33, 300, 64), (65, 257, 1025), (128, 512, 784), (300, 1000, 512), (513, 130, 4100), (600, 64, 33),
-          (1, 128, 16384), (8, 200, 8192), (40, 96, 3001), (700, 1500, 320), (129, 1, 200), (257, 2, 40), (2500, 2700, 300), (4100, 1100, 70), (90, 33, 20000)]
+          (1, 128, 16384), (8, 200, 8192), (40, 96, 3001), (700, 1500, 320), (129, 1, 200), (257, 2, 40), (2500, 2700, 300), (4100, 1100, 70), (90, 33, 20000),
+          (9, 900, 2048), (24, 130, 4096), (64, 1030, 4096), (100, 260, 2048), (128, 1100, 1024), (300, 390, 4096)]     # tiles that two to eight CTAs share
 
 
 def _layer(spg, lib, rng, n, out, k, act, t, exact, bias=True):
