@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
                 if (p.split > 1) {
                     // This CTA's sums to those that put them out, [chunk][CTA][row][unit].  (Sent before one barrier, not fetched behind it: reading the others' took 6800
                     // cycles from the last product to the end, 2700 of them the instructions of 64 loads.)
+                    __syncwarp();
                     cluster_wait();                                              // all have begun
                     const uint32_t chunks = chunks_of(p.N, NT);
                     for (uint32_t c = half; c < chunks && n0 + 8 * c < p.N; c += 2) {
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         }
         tc_fence_before();
     }
-    if (p.split > 1 && warp < 2) { cluster_wait(); cluster_arrive(); cluster_wait(); }
+    if (p.split > 1 && warp < 2) { __syncwarp(); cluster_wait(); cluster_arrive(); cluster_wait(); }
     __syncthreads();
     if (warp == 1 && p.split == 1) { tc_fence_after(); tmem_free(tmem, L::COLS); }
 }
