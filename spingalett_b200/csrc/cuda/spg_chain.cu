@@ -100,8 +100,8 @@ __device__ __forceinline__ void fence_async_global() { asm volatile("fence.proxy
 template <uint32_t EPI> __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI) : "memory"); }
 
 // (relaxed: who waits reads nothing that was written before; a release would wait for the outputs' stores, 1400 cycles)
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { __syncwarp(); asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Bounded wait on a barrier that the other CTAs of the cluster arrive on, whose writes to global memory are read afterwards
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int *abort_flag, int32_t *status, int code)

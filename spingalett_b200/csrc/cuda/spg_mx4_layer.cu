@@ -80,8 +80,8 @@ __device__ __forceinline__ void st_cluster_if(uint32_t addr, float v, uint32_t y
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.shared::cluster.f32 [%0], %1;\n\t}" ::"r"(addr), "f"(v), "r"(yes) : "memory");
 }
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { __syncwarp(); asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // (predicated: branches around the stores cost 80 cycles each)
 __device__ __forceinline__ void put(float *y, float v, uint32_t yes)
@@ -300,7 +300,6 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
                 if (p.split > 1) {
                     // This CTA's sums to those that put them out, [chunk][CTA][row][unit].  (Sent before one barrier, not fetched behind it: reading the others' took 6800
                     // cycles from the last product to the end, 2700 of them the instructions of 64 loads.)
-                    __syncwarp();
                     cluster_wait();                                              // all have begun
                     const uint32_t chunks = chunks_of(p.N, NT);
                     for (uint32_t c = half; c < chunks && n0 + 8 * c < p.N; c += 2) {
@@ -344,7 +343,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         }
         tc_fence_before();
     }
-    if (p.split > 1 && warp < 2) { __syncwarp(); cluster_wait(); cluster_arrive(); cluster_wait(); }
+    if (p.split > 1 && warp < 2) { cluster_wait(); cluster_arrive(); cluster_wait(); }
     __syncthreads();
     if (warp == 1 && p.split == 1) { tc_fence_after(); tmem_free(tmem, L::COLS); }
 }

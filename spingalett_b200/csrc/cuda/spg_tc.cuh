@@ -243,9 +243,10 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr)
 {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// all threads of both CTAs
+// all threads of the cluster's CTAs (.aligned: a warp's threads come to it together, which only __syncwarp brings about behind code that parts them)
 __device__ __forceinline__ void cluster_sync()
 {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
