@@ -15,8 +15,10 @@
 // 1 x 16384 x 1000 4.8 us (eight CTAs a tile), 1 x 784 x 512 3.1 us (a launch), 16384 x 8192 x 8192 365 us (6020 TFLOP/s, 500 cycles a k-block of 512 at the
 // tensor pipe's best; 430 us in a long run, under the power limit).
 //
-// Every wait on an mbarrier is bounded; a CTA that gave up records a code in `status`, and its cluster leaves the tile's outputs alone.
+// Every wait on an mbarrier is bounded.  One that gave up records a code in `status`; the sums of its tile are then never said to be complete, and all CTAs that
+// work on the tile leave its outputs alone.  Copies and products under way end, again waited for with a limit, before the memory that they write to is given back.
 #include "spg_mx4.cuh"
+#include "spg_gemm.cuh"
 #include "spg_tc.cuh"
 #include <cstdio>
 #include <mutex>
@@ -50,7 +52,70 @@ struct LayerParams {
     void *y; int type; uint32_t ldy;
     uint8_t *next_codes, *next_scales; uint32_t next_pitch, next_kt;
     int32_t *status;
+    uint32_t patience, limit;                 // (the check of the failure path) the first tile whose products give up, in clusters their first CTA's; attempts of a pair's waits for a k-block
 };
+constexpr uint32_t DRAIN = 1u << 12;          // attempts of a last wait
+
+__device__ __forceinline__ uint32_t ld_shared(uint32_t addr) { uint32_t v; asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory"); return v; }
+// The products' wait for a k-block, as mbar_wait_uniform.  Where it gives up, `to` and `end`, the barriers that are told of the products, become `nowhere`, others that nobody
+// waits for: the loop runs out with products of whatever lies there, but no place of the ring is given back to copies, and no sums are said to be complete.
+// (Found out behind the wait instead, by its result and a branch, that cost 15 cycles a k-block.)
+__device__ __forceinline__ void wait_or_nowhere(uint32_t bar, uint32_t parity, uint32_t aborted, int32_t *status, int code, uint32_t &to, uint32_t &end, uint32_t nowhere,
+                                                uint32_t limit = 1u << 16)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        ".reg .u32 n, a;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%2], %3;\n\t"
+        "@p bra SPG_MX4_DONE;\n\t"
+        "mov.u32 n, 0;\n\t"
+        "SPG_MX4_LOOP:\n\t"
+        "ld.volatile.shared.u32 a, [%4];\n\t"
+        "setp.ne.u32 q, a, 0;\n\t"
+        "@q bra SPG_MX4_NOWHERE;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%2], %3, %8;\n\t"
+        "@p bra SPG_MX4_DONE;\n\t"
+        "add.u32 n, n, 1;\n\t"
+        "setp.lt.u32 q, n, %7;\n\t"
+        "@q bra SPG_MX4_LOOP;\n\t"
+        "st.volatile.shared.u32 [%4], 1;\n\t"
+        "atom.global.cas.b32 a, [%5], 0, %6;\n\t"
+        "SPG_MX4_NOWHERE:\n\t"
+        "mov.u32 %0, %9;\n\t"
+        "mov.u32 %1, %9;\n\t"
+        "SPG_MX4_DONE:\n\t"
+        "}"
+        : "+r"(to), "+r"(end) : "r"(bar), "r"(parity), "r"(aborted), "l"(status), "r"(code), "r"(limit), "r"(SPG_WAIT_HINT_NS), "r"(nowhere) : "memory");
+}
+// (the check of the failure path: as if it had)
+__device__ __forceinline__ void give_up_if(uint32_t yes, uint32_t aborted, int32_t *status, int code, uint32_t &to, uint32_t &end, uint32_t nowhere)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .pred q;\n\t"
+        ".reg .u32 a;\n\t"
+        "setp.ne.u32 q, %2, 0;\n\t"
+        "@q st.volatile.shared.u32 [%3], 1;\n\t"
+        "@q atom.global.cas.b32 a, [%4], 0, %5;\n\t"
+        "@q mov.u32 %0, %6;\n\t"
+        "@q mov.u32 %1, %6;\n\t"
+        "}"
+        : "+r"(to), "+r"(end) : "r"(yes), "r"(aborted), "l"(status), "r"(code), "r"(nowhere) : "memory");
+}
+// After a wait for a k-block that gave up, by the warp of the products when they have ended: the copies under way end.  `begun`: where the k-blocks whose copies were begun
+// are told, and one, when there will be no more.  (A call, so that its instructions are not in the way of CTAs that need none of them.)
+__device__ __noinline__ void end_copies(uint32_t full, uint32_t stages, uint32_t begun, uint32_t late, int32_t *status)
+{
+    uint32_t count = 0;
+    for (uint32_t i = 0; i < DRAIN && count == 0; i++) {
+        __nanosleep(SPG_WAIT_HINT_NS);
+        count = __reduce_max_sync(0xffffffffu, ld_shared(begun));
+    }
+    if (count == 0) return;
+    count--;
+    for (uint32_t i = count > stages ? count - stages : 0; i < count; i++) mbar_wait_uniform(full + 8 * (i % stages), i / stages & 1u, late, status, 4, DRAIN);
+}
 
 // kind::mxf4, E2M1 on both sides, UE8M0 scales, M = 128
 __host__ __device__ constexpr uint32_t idesc_mx4(uint32_t n) { return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24); }
@@ -206,18 +271,21 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
     extern __shared__ uint8_t raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     const uint32_t head = smem_u32(base), parts = head + HEAD, ring = parts + parts_bytes<NT>(p.N, p.split);
-    const uint32_t full = head, empty = head + 8 * MAX_STAGES, done = empty + 8 * MAX_STAGES, slot = done + 8, aborted = slot + 4, told = aborted + 4;
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head));
+    const uint32_t full = head, empty = head + 8 * MAX_STAGES, nowhere = empty + 8 * MAX_STAGES, done = nowhere + 8 * MAX_STAGES, ended = done + 8, slot = ended + 8, aborted = slot + 4, late = aborted + 4, begun = late + 4, told = begun + 4;
+    // (aborted: a wait of this CTA gave up; late: one of the last waits did; begun: k-blocks whose copies were, and one; told: one of the cluster's CTAs does not have its sums)
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head)), *told_flag = reinterpret_cast<volatile int *>(base + (told - head));
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+    if (threadIdx.x == 0) *told_flag = 0;
     if (p.split > 1) cluster_arrive();                                           // (in front of the wait for tensor memory: see below)
     const uint32_t rank = blockIdx.x % p.split, j_tile = blockIdx.x / p.split, n0 = blockIdx.y * NT;
     // this CTA's k-blocks
     const uint32_t lo = (uint32_t)((uint64_t)p.kblocks * rank / p.split), hi = (uint32_t)((uint64_t)p.kblocks * (rank + 1) / p.split);
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (uint32_t s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); mbar_init(nowhere + 8 * s, 1); }
         mbar_init(done, 1);
-        *abort_flag = 0;
+        mbar_init(ended, 1);
+        for (uint32_t i = 0; i < 3; i++) abort_flag[i] = 0;
         mbar_fence_init();
     }
     if (warp == 1) tmem_alloc(slot, L::COLS);
@@ -233,12 +301,10 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         for (uint32_t kb = lo; kb < hi && kb < lo + AHEAD; kb++) prefetch_l2(&map_w, (int)(kb * 128u), (int)(j_tile * TM));
     __syncwarp();
     if (warp < 2) spg_grid_wait();
-    volatile int never = 0;
-
     if (warp == 0) {
-        uint32_t last = 0;
-        if (elect_one())
-            for (uint32_t kb = lo, s = 0, phase = 1; kb < hi; kb++) {
+        if (elect_one()) {
+            uint32_t kb = lo;
+            for (uint32_t s = 0, phase = 1; kb < hi; kb++) {
                 if (!mbar_wait(empty + 8 * s, phase, abort_flag, p.status, 1)) break;
                 const uint32_t at = ring + s * L::STAGE, sf = min(2u, p.kt - 2 * kb) * SF_TILE;
                 mbar_expect_tx(full + 8 * s, W_BYTES + L::X_BYTES + sf * 2);
@@ -246,19 +312,20 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
                 tma_load_2d(at + W_BYTES, &map_x, full + 8 * s, (int)(kb * 128u), (int)n0);
                 bulk_load(at + W_BYTES + L::X_BYTES, p.w_scales + ((uint64_t)j_tile * p.kt + 2 * kb) * SF_TILE, sf, full + 8 * s);
                 bulk_load(at + W_BYTES + L::X_BYTES + SF_BYTES, p.x_scales + ((uint64_t)(n0 / 128u) * p.kt + 2 * kb) * SF_TILE, sf, full + 8 * s);
-                last = kb + 1 - lo;
                 if (++s == p.stages) { s = 0; phase ^= 1u; }
             }
-        last = __reduce_max_sync(0xffffffffu, last);
-        if (*abort_flag)                         // the copies under way end before this CTA does
-            for (uint32_t i = last > p.stages ? last - p.stages : 0; i < last; i++) mbar_wait(full + 8 * (i % p.stages), i / p.stages & 1u, &never, p.status, 4, 1u << 12);
+            abort_flag[2] = (int)(kb - lo + 1);                                  // (begun)
+        }
+        __syncwarp();
     } else if (warp == 1) {
         // (One lane runs the loop, and the last k-block has one commit, not two: 340 cycles a k-block.  With the lane chosen anew for each, a way of its own for
         // a row's end and a second commit behind the loop it took 445, whatever the copies and products were, and a short layer 0.1 us more.)
         const uint32_t idesc = idesc_mx4(NT);
-        if (elect_one())
+        uint32_t to = empty, end = done;
+        if (elect_one()) {
+            give_up_if(p.patience == 0 && rank == 0, aborted, p.status, 2, to, end, nowhere);
             for (uint32_t kb = lo, s = 0, phase = 0; kb < hi; kb++) {
-                mbar_wait_uniform(full + 8 * s, phase, aborted, p.status, 2);
+                wait_or_nowhere(full + 8 * s, phase, aborted, p.status, 2, to, end, nowhere);
                 tc_fence_after();
                 const uint32_t at = ring + s * L::STAGE, sf = tmem + L::SFW + ((kb - lo) & 1u) * L::SF_COLS, left = p.cols - kb * KB;
                 const uint32_t sfw = at + W_BYTES + L::X_BYTES, sfx = sfw + SF_BYTES;
@@ -273,10 +340,16 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
                 };
                 scales(0, 1); scales(1, left > 128);
                 product(0, kb > lo, 1); product(1, 1, left > 64); product(2, 1, left > 128); product(3, 1, left > 192);
-                umma_commit(kb + 1 < hi ? empty + 8 * s : done);
+                umma_commit(kb + 1 < hi ? to + 8 * s : end);
                 if (++s == p.stages) { s = 0; phase ^= 1u; }
             }
+        }
         __syncwarp();
+        // The products end here, beside the outputs.  So have the copies then, each of which was waited for, but where a wait gave up
+        if (elect_one()) umma_commit(ended);
+        __syncwarp();
+        mbar_wait_uniform(ended, 0, late, p.status, 5);
+        if (__any_sync(0xffffffffu, end == nowhere)) end_copies(full, p.stages, begun, late, p.status);
         if (p.split > 1) {
             // Given back before this CTA waits for the others: one that has none on its SM, and so cannot finish, may hold up a cluster that holds some elsewhere
             sums_taken();
@@ -294,14 +367,13 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
             if (!dry) {
                 spg_grid_wait();
                 if (p.bias && j < p.out) bias = p.bias[j];
-                ok = mbar_wait(done, 0, abort_flag, p.status, 3);
-                if (!ok) mbar_wait(done, 0, &never, p.status, 5, 1u << 12);                // the products under way end before tensor memory is given back
+                ok = __all_sync(0xffffffffu, mbar_wait(done, 0, abort_flag, p.status, 3));           // (a warp goes one way)
                 tc_fence_after();
                 if (p.split > 1) {
                     // This CTA's sums to those that put them out, [chunk][CTA][row][unit].  (Sent before one barrier, not fetched behind it: reading the others' took 6800
                     // cycles from the last product to the end, 2700 of them the instructions of 64 loads.)
                     cluster_wait();                                              // all have begun
-                    const uint32_t chunks = chunks_of(p.N, NT);
+                    const uint32_t chunks = ok ? chunks_of(p.N, NT) : 0;
                     for (uint32_t c = half; c < chunks && n0 + 8 * c < p.N; c += 2) {
                         float v[8];
                         tmem_ld8(lanes + 8 * c, v);
@@ -310,14 +382,13 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
 #pragma unroll
                         for (int i = 0; i < 8; i++) st_cluster_if(to + i * TM * 4u, v[i], (uint32_t)i < left);
                     }
-                    if (warp == 2 && lane < p.split) st_cluster_u32(mapa(told + 4 * rank, lane), *abort_flag != 0);
+                    if (!ok && lane < p.split) st_cluster_u32(mapa(told, lane), 1);
                     tc_fence_before();
                     __syncwarp();
                     sums_taken();
                     cluster_arrive();
                     cluster_wait();
-                    const volatile uint32_t *flags = reinterpret_cast<const volatile uint32_t *>(base + (told - head));
-                    ok = !__any_sync(0xffffffffu, !ok || (lane < p.split && flags[lane] != 0));
+                    ok = !__any_sync(0xffffffffu, *told_flag);
                 }
                 if (!ok) break;
             }
@@ -344,6 +415,7 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         tc_fence_before();
     }
     if (p.split > 1 && warp < 2) { cluster_wait(); cluster_arrive(); cluster_wait(); }
+    __syncwarp();
     __syncthreads();
     if (warp == 1 && p.split == 1) { tc_fence_after(); tmem_free(tmem, L::COLS); }
 }
@@ -392,6 +464,41 @@ __device__ __forceinline__ void pair_tile(uint32_t t, uint32_t j_tiles, uint32_t
     j = g * 8u + r % here; n = r / here;
 }
 
+constexpr uint32_t P_ENDED = 24 * P_STAGES + 16, P_LATE = P_ENDED + 16, P_TOLD = P_LATE + 4;      // places in the head: the barrier of the last products, the flag of the last waits, k-blocks begun
+// one k-block's copies of a CTA (one lane; leader: the first CTA's barrier, which counts those of both)
+__device__ __forceinline__ void copy_pair(const CUtensorMap *w, const CUtensorMap *x, const CUtensorMap *sw, const CUtensorMap *sx, uint32_t at, uint32_t leader,
+                                          uint32_t rank, uint32_t kb, uint32_t j, uint32_t n)
+{
+    tma_load_2d_pair(at, w, leader, (int)(kb * 128u), (int)(j * 256u + rank * 128u));
+    tma_load_2d_pair(at + W_BYTES, x, leader, (int)(kb * 128u), (int)(n * PN + rank * (PN / 2)));
+    tma_load_2d_pair(at + P_CODES, sw, leader, (int)(kb * 256u), (int)(j * 2u + rank));
+    tma_load_2d_pair(at + P_CODES + SF_BYTES, sx, leader, (int)(kb * 256u), (int)(n * (PN / 128)));
+}
+// The same of a pair, by its first CTA, which first ends the waits of both.
+// Each k-block's are counted for both CTAs at once: where one of them began fewer, as many bytes are fetched here once more, or expected of the other alone.
+__device__ __noinline__ void end_pair(const CUtensorMap *w, const CUtensorMap *x, const CUtensorMap *sw, const CUtensorMap *sx, uint32_t head, uint32_t aborted, int32_t *status)
+{
+    atomicCAS(status, 0, 2);
+    for (uint32_t r = 0; r < 2; r++) st_cluster_u32(mapa(aborted, r), 1);
+    uint32_t mine = 0, other = 0;
+    for (uint32_t i = 0; i < DRAIN && (mine == 0 || other == 0); i++) {
+        __nanosleep(SPG_WAIT_HINT_NS);
+        mine = __reduce_max_sync(0xffffffffu, ld_shared(head + P_TOLD));
+        other = __reduce_max_sync(0xffffffffu, ld_shared(head + P_TOLD + 4));
+    }
+    if (mine == 0 || other == 0) return;
+    const uint32_t most = max(--mine, --other);
+    for (uint32_t i = min(mine, other); i < most; i++) {
+        const uint32_t s = i % P_STAGES, bar = head + 8 * s;
+        if (elect_one()) {
+            if (i >= mine) mbar_expect_tx(bar, P_STAGE);                         // (the other's)
+            else copy_pair(w, x, sw, sx, head + HEAD + s * P_STAGE, mapa(bar, 0), 0, 0, 0, 0);
+        }
+        __syncwarp();
+    }
+    for (uint32_t i = most > P_STAGES ? most - P_STAGES : 0; i < most; i++) mbar_wait_uniform_cluster(head + 8 * (i % P_STAGES), i / P_STAGES & 1u, head + P_LATE, status, 4, DRAIN);
+}
+
 __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                     const __grid_constant__ CUtensorMap map_sw, const __grid_constant__ CUtensorMap map_sx,
                                                                     const LayerParams p, uint32_t j_tiles, uint32_t n_tiles)
@@ -399,15 +506,16 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
     extern __shared__ uint8_t raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     const uint32_t head = smem_u32(base), ring = head + HEAD;
-    const uint32_t full = head, empty = full + 8 * P_STAGES, sums_full = empty + 8 * P_STAGES, sums_free = sums_full + 8, slot = sums_free + 8, aborted = slot + 4;
+    const uint32_t full = head, empty = full + 8 * P_STAGES, nowhere = empty + 8 * P_STAGES, sums_full = nowhere + 8 * P_STAGES, sums_free = sums_full + 8, ended = head + P_ENDED, slot = ended + 8, aborted = slot + 4, told = head + P_TOLD;
     volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head));
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = cluster_rank(), pairs = gridDim.x / 2u, pair = blockIdx.x / 2u, tiles = j_tiles * n_tiles;
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < P_STAGES; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (uint32_t s = 0; s < P_STAGES; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); mbar_init(nowhere + 8 * s, 1); }
         mbar_init(sums_full, 1);
         mbar_init(sums_free, 2 * P_EPI);
-        *abort_flag = 0;
+        mbar_init(ended, 1);
+        for (uint32_t i = 0; i < 4; i++) abort_flag[i] = 0;                      // (and the flag of the last waits, and what is told of k-blocks)
         mbar_fence_init();
     }
     if (warp == 1) tmem_alloc_pair(slot, 512);
@@ -419,42 +527,37 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
     spg_grid_trigger();
     if (warp < 2) spg_grid_wait();
-    volatile int never = 0;
 
     if (warp == 0) {
         const uint32_t leader = mapa(full, 0);
-        uint32_t s = 0, phase = 1, issued = 0;
+        uint32_t s = 0, phase = 1, begun = 0;
         for (uint32_t t = pair; t < tiles && !*abort_flag; t += pairs) {
             uint32_t j, n;
             pair_tile(t, j_tiles, n_tiles, j, n);
             for (uint32_t kb = 0; kb < p.kblocks; kb++) {
                 mbar_wait_uniform_cluster(empty + 8 * s, phase, aborted, p.status, 1);
                 if (*abort_flag) break;
-                const uint32_t at = ring + s * P_STAGE, bar = leader + 8 * s;
                 if (elect_one()) {
                     if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * P_STAGE);
-                    tma_load_2d_pair(at, &map_w, bar, (int)(kb * 128u), (int)(j * 256u + rank * 128u));
-                    tma_load_2d_pair(at + W_BYTES, &map_x, bar, (int)(kb * 128u), (int)(n * PN + rank * (PN / 2)));
-                    tma_load_2d_pair(at + P_CODES, &map_sw, bar, (int)(kb * 256u), (int)(j * 2u + rank));
-                    tma_load_2d_pair(at + P_CODES + SF_BYTES, &map_sx, bar, (int)(kb * 256u), (int)(n * (PN / 128)));
+                    copy_pair(&map_w, &map_x, &map_sw, &map_sx, ring + s * P_STAGE, leader + 8 * s, rank, kb, j, n);
                 }
                 __syncwarp();
-                issued++;
+                begun++;
                 if (++s == P_STAGES) { s = 0; phase ^= 1u; }
             }
         }
-        if (*abort_flag && rank == 0)            // the copies under way end before the pair does
-            for (uint32_t i = issued > P_STAGES ? issued - P_STAGES : 0; i < issued; i++) mbar_wait(full + 8 * (i % P_STAGES), i / P_STAGES & 1u, &never, p.status, 4, 1u << 12);
+        if (lane == 0) st_cluster_u32(mapa(told + 4 * rank, 0), begun + 1);       // (k-blocks whose copies were begun here, and one: see end_pair)
     } else if (warp == 1) {
         if (rank == 0) {
             const uint32_t idesc = (idesc_mx4(PN) & ~(31u << 24)) | ((256u >> 4) << 24);
-            uint32_t s = 0, phase = 0, turn = 1;
+            uint32_t s = 0, phase = 0, turn = 1, back = empty, end = sums_full;
             for (uint32_t t = pair; t < tiles; t += pairs) {
-                mbar_wait_uniform_cluster(sums_free, turn, aborted, p.status, 6);
+                if (t >= p.patience) back = end = nowhere;
+                wait_or_nowhere(sums_free, turn, aborted, p.status, 6, back, end, nowhere);
                 turn ^= 1u;
                 tc_fence_after();
                 for (uint32_t kb = 0; kb < p.kblocks; kb++) {
-                    mbar_wait_uniform_cluster(full + 8 * s, phase, aborted, p.status, 2);
+                    wait_or_nowhere(full + 8 * s, phase, aborted, p.status, 2, back, end, nowhere, p.limit);
                     tc_fence_after();
                     const uint32_t at = ring + s * P_STAGE, to = tmem + P_SF + (kb & 1u) * P_SF_COLS;
                     if (elect_one()) {
@@ -479,15 +582,21 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
                             if (steps > 1) product(1, 1);
                             if (steps > 2) product(2, 1);
                         }
-                        umma_commit_pair(empty + 8 * s);
+                        umma_commit_pair(back + 8 * s);
                     }
                     __syncwarp();
                     if (++s == P_STAGES) { s = 0; phase ^= 1u; }
                 }
-                if (elect_one()) umma_commit_pair(sums_full);
+                if (elect_one()) umma_commit_pair(end);
                 __syncwarp();
-                if (*abort_flag) break;
+                if (__any_sync(0xffffffffu, end == nowhere)) break;
             }
+            // The products end here, beside the last tile's outputs.  So have the copies then, each of which was waited for, but where a wait gave up
+            if (elect_one()) umma_commit_pair(ended);
+            __syncwarp();
+            mbar_wait_uniform(ended, 0, head + P_LATE, p.status, 5);
+            if (__any_sync(0xffffffffu, end == nowhere)) end_pair(&map_w, &map_x, &map_sw, &map_sx, head, aborted, p.status);
+            __syncwarp();
         }
     } else {
         const uint32_t quad = warp % 4u, part = (warp - 2u) / 4u, free_at = mapa(sums_free, 0);
@@ -501,7 +610,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
             const uint32_t from = tmem + (quad * 32u << 16) + part * P_COLS;
             const bool some = j0 < (p.next_codes ? (p.out + 127u) / 128u * 128u : p.out);       // (the next operand's scale tiles are written whole)
             if (!dry) {
-                if (!mbar_wait(sums_full, turn, abort_flag, p.status, 3)) { mbar_wait(sums_full, turn, &never, p.status, 5, 1u << 12); break; }
+                if (!__all_sync(0xffffffffu, mbar_wait(sums_full, turn, abort_flag, p.status, 3))) break;           // (a warp goes one way)
                 turn ^= 1u;
                 tc_fence_after();
             }
@@ -535,6 +644,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
             t += pairs;
         }
     }
+    __syncwarp();
     __syncthreads();
     cluster_sync();
     if (warp == 1) { tc_fence_after(); tmem_free_pair(tmem, 512); }
@@ -642,7 +752,7 @@ template <uint32_t NT> int launch(const spgk_mx4 *W, const spgk_mx4 *X, LayerPar
     return spgk_check_launch("spg_mx4_layer_kernel");
 }
 
-int launch_pairs(const spgk_mx4 *W, const spgk_mx4 *X, const LayerParams &p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
+int launch_pairs(const spgk_mx4 *W, const spgk_mx4 *X, LayerParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
 {
     static SpgOncePerDevice once;
     int rc = once.run(dev, [&]() -> int {
@@ -656,6 +766,7 @@ int launch_pairs(const spgk_mx4 *W, const spgk_mx4 *X, const LayerParams &p, con
     const uint64_t tiles = (uint64_t)j_tiles * n_tiles;
     if (tiles > 0x3fffffffu) { spgk_set_error("spgk_layer_mx4", "too many tiles"); return SPGK_E_ARG; }
     const uint32_t pairs = tiles < (uint32_t)dp.sm_count / 2 ? (uint32_t)tiles : (uint32_t)dp.sm_count / 2;
+    if (p.patience == 0) p.patience = (uint32_t)tiles - pairs;             // (each pair's last tile)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(pairs * 2); cfg.blockDim = dim3(P_THREADS); cfg.dynamicSmemBytes = P_SMEM; cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -698,7 +809,7 @@ extern "C" int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, con
     p.N = X->rows; p.out = W->rows; p.cols = W->cols;
     p.kblocks = (W->cols + KB - 1) / KB; p.kt = spgmx4::tiles4(W->cols);
     p.w_scales = (const uint8_t *)W->scales; p.x_scales = (const uint8_t *)X->scales;
-    p.bias = bias; p.act = act; p.y = y; p.type = type; p.ldy = ldy; p.status = status;
+    p.bias = bias; p.act = act; p.y = y; p.type = type; p.ldy = ldy; p.status = status; p.patience = spg_gemm_impatient() ? 0 : 0xffffffffu; p.limit = spg_gemm_impatient() ? 64 : 1u << 16;
     if (next) { p.next_codes = (uint8_t *)next->codes; p.next_scales = (uint8_t *)next->scales; p.next_pitch = next->pitch; p.next_kt = spgmx4::tiles4(next->cols); }
     cudaStream_t st = (cudaStream_t)stream;
     if (p.N <= 16) return launch<16>(W, X, p, dp, dev, st);
