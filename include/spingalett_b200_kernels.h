@@ -608,7 +608,8 @@ SPGK_API int spgk_mx4_dequantize(const spgk_mx4 *src, void *y, int type, uint32_
  * with exact products and fp32 sums on the tensor cores (at most 2^27 inputs).  y: rows of ldy elements of `type`, rounded once, or NULL; next: the same values quantised
  * as by spgk_mx4_quantize from fp32 (next->rows == X->rows, next->cols == W->rows; scales of rows beyond the last are left as they were), the operand of the
  * layer behind, or NULL; one of the two at least.  ACT_SOFTMAX is left to spgk_softmax_rows, and refused with `next`.
- * status: dev int32, zero before the first call, as for spgk_layer_gemm_tc (read with spgk_gemm_tc_status).
+ * status: dev int32, zero before the first call, as for spgk_layer_gemm_tc (read with spgk_gemm_tc_status). Where it says that a wait gave up, the
+ * outputs whose sums were not complete are as they were before the call.
  * Does forward()'s layer step, reference Network.c:218-247, on another number format. */
 SPGK_API int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, const spgk_mx4 *X, void *y, int type, uint32_t ldy,
                             const spgk_mx4 *next, int32_t *status, void *stream);

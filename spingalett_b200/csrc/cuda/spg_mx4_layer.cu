@@ -12,8 +12,8 @@
 //
 // More than some hundred rows go to pairs of CTAs (below); which, and how many CTAs share a tile, an estimate in cycles says.
 // What bounds it: one row x 8192 x 16384 12.8 us (5.6 TB/s; HBM, and start and end of a launch), 64 x 16384 x 16384 27.2 us (5.4 TB/s),
-// 1 x 16384 x 1000 4.8 us (eight CTAs a tile), 1 x 784 x 512 3.1 us (a launch), 16384 x 8192 x 8192 365 us (6020 TFLOP/s, 500 cycles a k-block of 512 at the
-// tensor pipe's best; 430 us in a long run, under the power limit).
+// 1 x 16384 x 1000 5.1 us (eight CTAs a tile), 1 x 784 x 512 3.1 us (a launch), 16384 x 8192 x 8192 366 us (6010 TFLOP/s, the tensor pipe; 430 us in a long run, under the
+// power limit).
 //
 // Every wait on an mbarrier is bounded.  One that gave up records a code in `status`; the sums of its tile are then never said to be complete, and all CTAs that
 // work on the tile leave its outputs alone.  Copies and products under way end, again waited for with a limit, before the memory that they write to is given back.

@@ -6,19 +6,22 @@
 //
 // All three cuts leave a beginning of the same order, so what is left is told by one logit and a number: the logits above it, and the first r of
 // those equal to it.  Nothing is sorted.  A row belongs to a cluster of up to eight CTAs and is read once, into shared memory; many long rows have a CTA each, which
-// reads its row from L2 pass by pass.
+// reads its row anew for every pass, from L2 as far as that holds what all of them read.
 //   - A small top_k: each thread has the largest of its logits, and the (k / CTAs)-th largest of those in a CTA bounds the k-th logit of the row from
 //     below; the few logits above the least of these bounds meet in one CTA, where every thread counts what stands before its own.  So do the logits
 //     of a short row, or of one with nearly all of them masked.
 //   - Otherwise a cut is found by a histogram over the range in question (counts for top-k, weights for top-p), a list of the bin in which the border
 //     falls (or, where that is too long, another histogram over it), and a search in the list digit by digit.
-// Sums of 131072 weights in 32 bits would put a number drawn close to a border on its wrong side in some rows of a hundred.  Here a weight is a
-// whole multiple of 2^-44 (the largest is 1) that is good to 2^-30 of itself: errors that are independent of one another, so a sum of n of them is good to
-// 2^-30 / sqrt(n), and sums in 64 bits that do not hang on an order.
-// What bounds it: 256 x 131072 of fp32 143 us with top_p, 90 without a cut, 66 with top_k 50 (HBM would take 21), 64 x 50001 of bf16 with all cuts 14, 1 x 1000 6.5.
-// With top_p some hundred instructions a logit, issued at two fifths of the rate (a row's way through its barriers is some 20 of 50 thousand cycles), bound it
-// and not memory.  Kept in shared memory, such rows fill it, so that sixteen warps have an SM (228 us).  Slower there: two CTAs with half the logits each on an SM (the
-// same rows at work), 1024 threads (what every warp does for itself), 64-bit atomics, additions to bins left out for light logits, rows fetched to L2 ahead.
+// Sums of 131072 weights in 32 bits would put a number drawn close to a border on its wrong side in some rows of a hundred.  Here a weight is good to 2^-30 of itself
+// and a whole multiple of 2^-44 (the largest is 1; what is below is cut off where the weight comes from the table, and rounded where it comes from exp()), so sums in 64 bits
+// do not hang on an order, and one of n weights is good to 2^-30 of itself and n * 2^-44.  A number closer than that to a border may still fall on its other side.
+// What bounds it: 256 x 131072 of fp32 142 us with top_p, 84 without a cut, 80 at temperature 0, 64 with top_k 50 (HBM would take 21), 64 x 50001 of bf16 with all cuts 14,
+// 1 x 1000 6.7; 512 x 131072 of bf16 with top_k 500 and top_p 430.
+// With top_p 83 instructions a logit, issued at 58 % of the rate with 26 warps an SM, bound it; and the bytes: the rows of one launch are more than L2 holds, so that of the 403 MB of its
+// three passes 330 come from HBM, which would take 50 us for them.  Kept in shared memory, such rows fill it, so that sixteen warps have an SM (228 us).  Slower there: two
+// CTAs with half the logits each on an SM (the same rows at work), 1024 threads (what every warp does for itself), 64-bit atomics, additions to bins left out for light logits, rows
+// fetched to L2 ahead.
+// Where |largest| * log2(e) / temperature is beyond 4000 every weight is an exp() in 64 bits: 256 x 131072 with top_p 440 us, without a cut 152.
 #include "spg_common.cuh"
 #include "spg_tc.cuh"
 #include <type_traits>
@@ -52,7 +55,7 @@ struct Steps {
 __device__ const Steps g_steps;
 
 struct SampleParams {
-    const void *logits; int type; uint32_t ld, N, width, split, slice;
+    const void *logits; uint32_t ld, N, width, split, slice;
     const float *temperature; const int32_t *top_k; const float *top_p, *min_p, *u;
     int32_t *tokens; float *probs; int32_t *kept;
 };
@@ -145,7 +148,7 @@ template <typename Place> struct alignas(16) Shared {
     uint64_t out[2][4];                        // what this CTA tells the others, by turns
     uint64_t warp[2][WARPS];
     uint32_t listed;
-    uint32_t found_bin, found_last; uint64_t found_above; uint32_t found_count;
+    uint32_t found_bin; uint64_t found_above; uint32_t found_count;
 };
 
 __device__ __forceinline__ uint64_t ld_cluster_u64(uint32_t addr)
@@ -905,7 +908,7 @@ template <typename T, bool STREAM> int launch(const SampleParams &p, const SpgDe
 
 template <typename T> int launch_rows(SampleParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
 {
-    // Rows that would fill an SM's shared memory, and enough of them: a CTA each, two an SM, which reads its row again from L2 for every pass instead of keeping it.
+    // Rows that would fill an SM's shared memory, and enough of them: a CTA each, two an SM, which reads its row again for every pass instead of keeping it.
     // us kept and streamed, with top_p: 256 x 131072 228 and 143, 148 x 131072 143 and 95, 148 x 60000 57 and 50, 512 x 32000 106 and 97; 96 x 131072 88 and 115,
     // 512 x 16000 with top_k 21 and 23, 64 x 50001 14 and 17.
     const bool streamed = p.width > SLICE / 2 && p.N >= (uint32_t)dp.sm_count * 7 / 8;
@@ -936,7 +939,7 @@ extern "C" int spgk_sample_rows(const void *logits, int type, uint32_t ld, uint3
     const int rc = spg_device_props(&dp);
     if (rc) return rc;
     SPGK_CUDA(cudaGetDevice(&dev));
-    SampleParams p{ logits, type, ld, N, width, 1, width, temperature, top_k, top_p, min_p, u, tokens, probs, kept };
+    SampleParams p{ logits, ld, N, width, 1, width, temperature, top_k, top_p, min_p, u, tokens, probs, kept };
     if (type == SPGK_T_F32) return launch_rows<float>(p, dp, dev, (cudaStream_t)stream);
     if (type == SPGK_T_F16) return launch_rows<__half>(p, dp, dev, (cudaStream_t)stream);
     return launch_rows<__nv_bfloat16>(p, dp, dev, (cudaStream_t)stream);
