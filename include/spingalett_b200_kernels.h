@@ -530,7 +530,8 @@ SPGK_API int spgk_nccl_abort(void *comm);
  *   status3[0] holds the wait's code, and the call returns SPGK_E_TIMEOUT exactly as a GEMM whose wait gave up does.
  * spgk_selftest_impatient: the calling thread's products of few tiles (spg_gemm_split.cu) take the wait for a finished tile as given
  *   up as soon as they come to it, with copies and products under way: outputs stay as they were and the status word says so. So do
- *   layers on microscaled operands (spgk_layer_mx4): all tiles, and where pairs of CTAs have several each, the last one of each.
+ *   layers on microscaled operands (spgk_layer_mx4): all tiles, and where pairs of CTAs have several each, the last one of each;
+ *   with `on` 2 instead pairs give up the wait for tensor memory whose sums are not taken yet.
  * spgk_selftest_timed_call: host only: a call that answers after answer_ms under the rendezvous timeout wrapper with a
  *   limit of timeout_ms: 0 or SPGK_E_TIMEOUT.
  * spgk_selftest_once_per_device: host only: the once-per-device bookkeeping of the launchers over `devices` fake indices and

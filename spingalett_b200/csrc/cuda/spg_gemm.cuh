@@ -31,4 +31,4 @@ int spg_gemm_split_try(const SpgGemmArgs &a, const SpgDeviceProps &dp, int dev, 
 uint32_t spg_gemm_steps(const spgk_layer *L, uint32_t N, uint32_t a_parts, uint32_t w_parts, bool softmax_fused, const SpgDeviceProps &dp, int dev);
 
 // spgk_selftest_impatient
-bool spg_gemm_impatient();
+int spg_gemm_impatient();

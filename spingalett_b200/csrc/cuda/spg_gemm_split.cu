@@ -32,7 +32,7 @@
 #include "spg_gemm.cuh"
 #include <cmath>
 
-static thread_local bool spg_tls_impatient = false;            // spgk_selftest_impatient
+static thread_local int spg_tls_impatient = 0;                // spgk_selftest_impatient
 
 namespace {
 
@@ -565,5 +565,5 @@ extern "C" uint32_t spgk_layer_gemm_sum_steps(const spgk_layer *L, uint32_t N, i
     return spg_gemm_steps(L, N, (uint32_t)a_parts, (uint32_t)w_parts, softmax_fused != 0, dp, dev);
 }
 
-bool spg_gemm_impatient() { return spg_tls_impatient; }
-extern "C" void spgk_selftest_impatient(int on) { spg_tls_impatient = on != 0; }
+int spg_gemm_impatient() { return spg_tls_impatient; }
+extern "C" void spgk_selftest_impatient(int on) { spg_tls_impatient = on; }

@@ -52,41 +52,53 @@ struct LayerParams {
     void *y; int type; uint32_t ldy;
     uint8_t *next_codes, *next_scales; uint32_t next_pitch, next_kt;
     int32_t *status;
-    uint32_t patience, limit;                 // (the check of the failure path) the first tile whose products give up, in clusters their first CTA's; attempts of a pair's waits for a k-block
+    // (the check of the failure path) the first tile whose products give up, in clusters their first CTA's; attempts of a pair's waits for a k-block and for tensor memory
+    uint32_t patience, limit, limit_free;
 };
 constexpr uint32_t DRAIN = 1u << 12;          // attempts of a last wait
 
 __device__ __forceinline__ uint32_t ld_shared(uint32_t addr) { uint32_t v; asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory"); return v; }
 // The products' wait for a k-block, as mbar_wait_uniform.  Where it gives up, `to` and `end`, the barriers that are told of the products, become `nowhere`, others that nobody
-// waits for: the loop runs out with products of whatever lies there, but no place of the ring is given back to copies, and no sums are said to be complete.
+// waits for: what follows makes products of whatever lies there, but no place of the ring is given back to copies, and no sums are said to be complete.  `steps` becomes 0:
+// no products at all where sums that are not taken yet lie in their place.
 // (Found out behind the wait instead, by its result and a branch, that cost 15 cycles a k-block.)
-__device__ __forceinline__ void wait_or_nowhere(uint32_t bar, uint32_t parity, uint32_t aborted, int32_t *status, int code, uint32_t &to, uint32_t &end, uint32_t nowhere,
+// (ASK: a first attempt that returns at once, so that with a limit of 0 nothing is waited for)
+template <bool ASK = false>
+__device__ __forceinline__ void wait_or_nowhere(uint32_t bar, uint32_t parity, uint32_t aborted, int32_t *status, int code, uint32_t &to, uint32_t &end, uint32_t &steps, uint32_t nowhere,
                                                 uint32_t limit = 1u << 16)
 {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p, q;\n\t"
-        ".reg .u32 n, a;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%2], %3;\n\t"
-        "@p bra SPG_MX4_DONE;\n\t"
-        "mov.u32 n, 0;\n\t"
-        "SPG_MX4_LOOP:\n\t"
-        "ld.volatile.shared.u32 a, [%4];\n\t"
-        "setp.ne.u32 q, a, 0;\n\t"
-        "@q bra SPG_MX4_NOWHERE;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%2], %3, %8;\n\t"
-        "@p bra SPG_MX4_DONE;\n\t"
-        "add.u32 n, n, 1;\n\t"
-        "setp.lt.u32 q, n, %7;\n\t"
-        "@q bra SPG_MX4_LOOP;\n\t"
-        "st.volatile.shared.u32 [%4], 1;\n\t"
-        "atom.global.cas.b32 a, [%5], 0, %6;\n\t"
-        "SPG_MX4_NOWHERE:\n\t"
-        "mov.u32 %0, %9;\n\t"
-        "mov.u32 %1, %9;\n\t"
-        "SPG_MX4_DONE:\n\t"
-        "}"
-        : "+r"(to), "+r"(end) : "r"(bar), "r"(parity), "r"(aborted), "l"(status), "r"(code), "r"(limit), "r"(SPG_WAIT_HINT_NS), "r"(nowhere) : "memory");
+#define SPG_MX4_WAIT(FIRST)                                                                                                                                             \
+    asm volatile(                                                                                                                                                       \
+        "{\n\t"                                                                                                                                                         \
+        ".reg .pred p, q;\n\t"                                                                                                                                          \
+        ".reg .u32 n, a;\n\t"                                                                                                                                           \
+        "mbarrier." FIRST ".parity.shared::cta.b64 p, [%3], %4;\n\t"                                                                                                    \
+        "@p bra SPG_MX4_DONE;\n\t"                                                                                                                                      \
+        "mov.u32 n, 0;\n\t"                                                                                                                                             \
+        "SPG_MX4_LOOP:\n\t"                                                                                                                                             \
+        "ld.volatile.shared.u32 a, [%5];\n\t"                                                                                                                           \
+        "setp.ne.u32 q, a, 0;\n\t"                                                                                                                                      \
+        "@q bra SPG_MX4_NOWHERE;\n\t"                                                                                                                                   \
+        "setp.ge.u32 q, n, %8;\n\t"                                                                                                                                     \
+        "@q bra SPG_MX4_LATE;\n\t"                                                                                                                                      \
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%3], %4, %9;\n\t"                                                                                                 \
+        "@p bra SPG_MX4_DONE;\n\t"                                                                                                                                      \
+        "add.u32 n, n, 1;\n\t"                                                                                                                                          \
+        "bra SPG_MX4_LOOP;\n\t"                                                                                                                                         \
+        "SPG_MX4_LATE:\n\t"                                                                                                                                             \
+        "st.volatile.shared.u32 [%5], 1;\n\t"                                                                                                                           \
+        "atom.global.cas.b32 a, [%6], 0, %7;\n\t"                                                                                                                       \
+        "SPG_MX4_NOWHERE:\n\t"                                                                                                                                          \
+        "mov.u32 %0, %10;\n\t"                                                                                                                                          \
+        "mov.u32 %1, %10;\n\t"                                                                                                                                          \
+        "mov.u32 %2, 0;\n\t"                                                                                                                                            \
+        "SPG_MX4_DONE:\n\t"                                                                                                                                             \
+        "}"                                                                                                                                                             \
+        : "+r"(to), "+r"(end), "+r"(steps)                                                                                                                              \
+        : "r"(bar), "r"(parity), "r"(aborted), "l"(status), "r"(code), "r"(limit), "r"(SPG_WAIT_HINT_NS), "r"(nowhere) : "memory")
+    if constexpr (ASK) SPG_MX4_WAIT("test_wait");
+    else SPG_MX4_WAIT("try_wait");
+#undef SPG_MX4_WAIT
 }
 // (the check of the failure path: as if it had)
 __device__ __forceinline__ void give_up_if(uint32_t yes, uint32_t aborted, int32_t *status, int code, uint32_t &to, uint32_t &end, uint32_t nowhere)
@@ -321,11 +333,11 @@ __global__ void __launch_bounds__(THREADS) spg_mx4_layer_kernel(const __grid_con
         // (One lane runs the loop, and the last k-block has one commit, not two: 340 cycles a k-block.  With the lane chosen anew for each, a way of its own for
         // a row's end and a second commit behind the loop it took 445, whatever the copies and products were, and a short layer 0.1 us more.)
         const uint32_t idesc = idesc_mx4(NT);
-        uint32_t to = empty, end = done;
+        uint32_t to = empty, end = done, steps = 0;
         if (elect_one()) {
             give_up_if(p.patience == 0 && rank == 0, aborted, p.status, 2, to, end, nowhere);
             for (uint32_t kb = lo, s = 0, phase = 0; kb < hi; kb++) {
-                wait_or_nowhere(full + 8 * s, phase, aborted, p.status, 2, to, end, nowhere);
+                wait_or_nowhere(full + 8 * s, phase, aborted, p.status, 2, to, end, steps, nowhere);
                 tc_fence_after();
                 const uint32_t at = ring + s * L::STAGE, sf = tmem + L::SFW + ((kb - lo) & 1u) * L::SF_COLS, left = p.cols - kb * KB;
                 const uint32_t sfw = at + W_BYTES + L::X_BYTES, sfx = sfw + SF_BYTES;
@@ -553,11 +565,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_mx4_pair_kernel(const __grid
             uint32_t s = 0, phase = 0, turn = 1, back = empty, end = sums_full;
             for (uint32_t t = pair; t < tiles; t += pairs) {
                 if (t >= p.patience) back = end = nowhere;
-                wait_or_nowhere(sums_free, turn, aborted, p.status, 6, back, end, nowhere);
+                uint32_t kblocks = p.kblocks;
+                wait_or_nowhere<true>(sums_free, turn, aborted, p.status, 6, back, end, kblocks, nowhere, p.limit_free);
                 turn ^= 1u;
                 tc_fence_after();
-                for (uint32_t kb = 0; kb < p.kblocks; kb++) {
-                    wait_or_nowhere(full + 8 * s, phase, aborted, p.status, 2, back, end, nowhere, p.limit);
+                for (uint32_t kb = 0; kb < kblocks; kb++) {
+                    wait_or_nowhere(full + 8 * s, phase, aborted, p.status, 2, back, end, kblocks, nowhere, p.limit);
                     tc_fence_after();
                     const uint32_t at = ring + s * P_STAGE, to = tmem + P_SF + (kb & 1u) * P_SF_COLS;
                     if (elect_one()) {
@@ -809,7 +822,9 @@ extern "C" int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, con
     p.N = X->rows; p.out = W->rows; p.cols = W->cols;
     p.kblocks = (W->cols + KB - 1) / KB; p.kt = spgmx4::tiles4(W->cols);
     p.w_scales = (const uint8_t *)W->scales; p.x_scales = (const uint8_t *)X->scales;
-    p.bias = bias; p.act = act; p.y = y; p.type = type; p.ldy = ldy; p.status = status; p.patience = spg_gemm_impatient() ? 0 : 0xffffffffu; p.limit = spg_gemm_impatient() ? 64 : 1u << 16;
+    p.bias = bias; p.act = act; p.y = y; p.type = type; p.ldy = ldy; p.status = status;
+    const int impatient = spg_gemm_impatient();
+    p.patience = impatient == 1 ? 0 : 0xffffffffu; p.limit = impatient == 1 ? 64 : 1u << 16; p.limit_free = impatient == 2 ? 0 : 1u << 16;
     if (next) { p.next_codes = (uint8_t *)next->codes; p.next_scales = (uint8_t *)next->scales; p.next_pitch = next->pitch; p.next_kt = spgmx4::tiles4(next->cols); }
     cudaStream_t st = (cudaStream_t)stream;
     if (p.N <= 16) return launch<16>(W, X, p, dp, dev, st);

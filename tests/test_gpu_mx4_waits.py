@@ -83,3 +83,34 @@ def test_a_pair_gives_up_its_last_tile_alone(spg, lib, n, out, k, t):
                     assert np.array_equal(y1[rows, units], y[rows, units])
                     assert np.array_equal(codes1[rows, held], codes[rows, held]) and np.array_equal(tiles1[at], tiles[at])
         assert left.sum() == min(PAIRS, left.size)
+
+
+def test_products_do_not_take_the_place_of_sums_that_are_not_taken_yet(spg, lib):
+    """Pairs of seven short tiles that give up the wait for tensor memory where the sums of the tile before still lie there: what is put out is right, the rest is left alone."""
+    import torch
+    n, out, k = 4096, 8192, 512
+    w, x = Packed(spg, out, k), Packed(spg, n, k)
+    for m in (w, x):
+        m.codes.random_()
+        m.tiles.fill_(127)
+    y = torch.empty((n, out), dtype=torch.float32, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def run(impatient):
+        y.fill_(float("nan"))
+        lib.spgk_selftest_impatient(impatient)
+        try:
+            assert lib.spgk_layer_mx4(w.ref, None, 6, x.ref, y.data_ptr(), 2, out, None, status.data_ptr(), None) == 0
+        finally:
+            lib.spgk_selftest_impatient(0)
+        return lib.spgk_gemm_tc_status(status.data_ptr(), None), y.clone()
+    rc, right = run(0)
+    assert rc == 0 and right.isfinite().all()
+    for _ in range(3):
+        rc, got = run(2)
+        assert rc == TIMEOUT and b"bounded wait 6 " in lib.spgk_error_string()
+        put = got.isfinite()
+        assert 0 < int(put.sum()) < n * out
+        assert torch.equal(got[put], right[put])
+    rc, got = run(0)
+    assert rc == 0 and torch.equal(got, right)
