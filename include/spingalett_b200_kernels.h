@@ -615,6 +615,68 @@ SPGK_API int spgk_mx4_dequantize(const spgk_mx4 *src, void *y, int type, uint32_
 SPGK_API int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, const spgk_mx4 *X, void *y, int type, uint32_t ldy,
                             const spgk_mx4 *next, int32_t *status, void *stream);
 
+/* ---- 8-bit floating point with a scale for each block of 128 ----------------
+ * (No counterpart in the reference, whose integer formats have one scale per array.)
+ * A matrix of `rows` x `cols` values in blocks of 128 along a row: an element is E4M3 (4 exponent bits, 3 of mantissa, 448 the largest number, 0x7F and
+ * 0xFF NaN), a block has one E8M0 scale 2^(byte - 127), byte 0xFF meaning that all its values are NaN.
+ *   codes : row r starts at codes + r * pitch.  16-byte aligned; pitch is a multiple of 16 and at least spgk_fp8_pitch(cols).
+ *   scales: 32-bit words of four blocks, a block's byte the higher the later it comes; the word of a row stands beside those of its neighbours, and the
+ *           next four blocks' of all rows behind these: the scale of block b of row r is byte spgk_fp8_scale_index(rows, r, b). 16-byte aligned,
+ *           spgk_fp8_scales_bytes(rows, cols) bytes.  Any run of rows can be taken out of a matrix this way, from any row on.
+ * What lies behind cols in a row, and the scales of blocks behind the last, is not looked at.  Of these functions' operands none may overlap what they write. */
+#define SPGK_FP8_BLOCK 128u
+typedef struct {
+    void    *codes;
+    void    *scales;
+    uint32_t rows, cols;
+    uint32_t pitch;           /* bytes from a row's codes to the next row's */
+} spgk_fp8;
+SPGK_API uint32_t spgk_fp8_pitch(uint32_t cols);
+SPGK_API size_t spgk_fp8_scales_bytes(uint32_t rows, uint32_t cols);
+SPGK_API size_t spgk_fp8_scale_index(uint32_t rows, uint32_t row, uint32_t block);
+/* Row r of dst = row rows_idx[r] of x (x_rows rows of ldx elements of `type`), or row r where rows_idx (dev int32 [dst->rows]) is NULL; a row of zeros where
+ * the index is not one of x's rows.  A block's scale is the least power of two, from 2^-127 on, by which its largest magnitude comes to 448 or less; its elements are
+ * rounded to nearest (ties to the even code).  A block with a NaN or an infinity becomes NaN. */
+SPGK_API int spgk_fp8_quantize(const void *x, int type, uint32_t ldx, uint32_t x_rows, const int32_t *rows_idx, const spgk_fp8 *dst, void *stream);
+/* y (rows of ldy elements of `type`) = the values of src: exact in fp32 (beyond its range infinite), rounded in fp16 and, below its normal range, in bf16. */
+SPGK_API int spgk_fp8_dequantize(const spgk_fp8 *src, void *y, int type, uint32_t ldy, void *stream);
+/* A dense layer whose weights W (out x in) and inputs X (N x in) are both in this form:
+ *   y[n][j] = act(bias[j] + sum_k W[j][k] * X[n][k])        (bias: dev fp32 [out] or NULL)
+ * with exact products and fp32 sums on the tensor cores (at most 2^27 inputs).  y: rows of ldy elements of `type`, rounded once, or NULL; next: the same values quantised
+ * as by spgk_fp8_quantize from fp32 (next->rows == X->rows, next->cols == out; scales of blocks behind the last are left as they were), the operand of the layer
+ * behind, or NULL; one of the two at least.  ACT_SOFTMAX is left to spgk_softmax_rows, and refused with `next`.
+ * status: dev int32, zero before the first call, as for spgk_layer_gemm_tc (read with spgk_gemm_tc_status). Where it says that a wait gave up, the
+ * outputs whose sums were not complete are as they were before the call.
+ * Does forward()'s layer step, reference Network.c:218-247, on another number format. */
+SPGK_API int spgk_layer_fp8(const spgk_fp8 *W, const float *bias, int act, const spgk_fp8 *X, void *y, int type, uint32_t ldy,
+                            const spgk_fp8 *next, int32_t *status, void *stream);
+/* The same for rows in groups, each with a layer of its own: W has the weights of `experts` layers one behind the other (rows = experts * out), bias
+ * likewise (experts * out values), and rows starts[e] to starts[e + 1] - 1 of X, y and next belong to layer e.  starts: dev int32 [experts + 1], read on the device; a group
+ * may have no rows, and rows in front of starts[0] or behind starts[experts] of y and next are left as they were.  A start below zero or an earlier one
+ * counts as the largest before it (zero at first), one beyond X->rows as X->rows. */
+#define SPGK_MAX_EXPERTS 1024u
+SPGK_API int spgk_experts_fp8(const spgk_fp8 *W, uint32_t experts, const float *bias, int act, const spgk_fp8 *X, const int32_t *starts,
+                              void *y, int type, uint32_t ldy, const spgk_fp8 *next, int32_t *status, void *stream);
+
+/* ---- rows to experts and back --------------------------------------------------
+ * (No counterpart in the reference.)
+ * Per row of `experts` logits (rows of ld elements of `type`; a NaN counts as -infinity, which closes an expert to a row): its experts are the first top_k
+ * in the order (logit, falling; index, rising) that are above -infinity; with m the row's largest logit and w_i = exp(l_i - m) -- where m is +infinity, 1 for its equals and 0 for
+ * the rest -- an expert's gate is w_i over the sum of all w, or, with `normalise`, of those chosen.
+ *   chosen: dev int32 [N][top_k], the experts in that order, -1 behind the last;  gates: dev fp32 [N][top_k], 0 there.
+ *   The pairs (row, expert) in the order (expert; row) are what the experts' layers work on:
+ *   starts: dev int32 [experts + 1], where each expert's begin; starts[experts] is how many there are;
+ *   order : dev int32 [N * top_k], their rows, -1 behind the last: rows_idx of spgk_fp8_quantize;
+ *   places: dev int32 [N][top_k], the place of (row, chosen expert) in that order, -1 where none was chosen: for spgk_combine_rows.
+ * No two of the five may be the same memory.  N * top_k is below 2^30. */
+#define SPGK_ROUTE_MAX_TOP 32u
+SPGK_API int spgk_route_rows(const void *logits, int type, uint32_t ld, uint32_t N, uint32_t experts, uint32_t top_k, int normalise,
+                             int32_t *chosen, float *gates, int32_t *starts, int32_t *order, int32_t *places, void *stream);
+/* out[n][c] = sum over j of gates[n][j] * y[places[n][j]][c], in fp32 and in the order of j, rounded once; a place that is none of y's y_rows rows counts as a
+ * row of zeros, whatever its gate.  y: rows of ldy elements of `type`; places, gates: dev [N][top_k]; out: rows of ldo elements of out_type. */
+SPGK_API int spgk_combine_rows(const void *y, int type, uint32_t ldy, uint32_t y_rows, const int32_t *places, const float *gates, uint32_t N, uint32_t top_k,
+                               uint32_t width, void *out, int out_type, uint32_t ldo, void *stream);
+
 /* ---- an answer drawn from rows of logits ------------------------------------
  * (No counterpart in the reference, which leaves the choice to the caller.)
  * Per row of `width` logits (rows of ld elements of `type`; a NaN counts as -infinity, which masks):

@@ -20,6 +20,7 @@ OK, ERR_ALLOC, ERR_INVALID, ERR_DEVICE = 0, 1, 2, 3
 
 TYPE_F16, TYPE_BF16, TYPE_F32 = range(3)               # SPGK_T_*
 MX4_BLOCK, SAMPLE_MAX_WIDTH = 32, 262144
+FP8_BLOCK, MAX_EXPERTS, ROUTE_MAX_TOP = 128, 1024, 32
 
 PRECISION_NAMES = {"fp32": 0, "fp16": 1, "bf16": 2, "int8": 3, "int4": 4, "int2": 5}
 
@@ -87,6 +88,11 @@ class KLayer(C.Structure):
 
 class Mx4(C.Structure):
     """spgk_mx4 of include/spingalett_b200_kernels.h: a matrix of microscaled 4-bit numbers"""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_uint32), ("cols", C.c_uint32), ("pitch", C.c_uint32)]
+
+
+class Fp8(C.Structure):
+    """spgk_fp8 of include/spingalett_b200_kernels.h: a matrix of 8-bit floating-point numbers with a scale for each block of 128"""
     _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_uint32), ("cols", C.c_uint32), ("pitch", C.c_uint32)]
 
 
@@ -203,8 +209,9 @@ def bind_extensions(lib):
 
 
 def bind_operators(lib):
-    """The kernel-level operators on device pointers (microscaled 4-bit numbers, draws from logits); 0 or a negative SPGK_E_* code."""
-    vp, u32, mx4 = C.c_void_p, C.c_uint32, C.POINTER(Mx4)
+    """The kernel-level operators on device pointers (microscaled 4-bit numbers, 8-bit numbers in blocks, rows to experts and back, draws from logits); 0 or a
+    negative SPGK_E_* code."""
+    vp, u32, mx4, fp8 = C.c_void_p, C.c_uint32, C.POINTER(Mx4), C.POINTER(Fp8)
     lib.spgk_error_string.argtypes = []
     lib.spgk_error_string.restype = C.c_char_p
     lib.spgk_mx4_pitch.argtypes = [u32]
@@ -216,6 +223,18 @@ def bind_operators(lib):
     lib.spgk_mx4_quantize.argtypes = [vp, C.c_int, u32, mx4, vp]
     lib.spgk_mx4_dequantize.argtypes = [mx4, vp, C.c_int, u32, vp]
     lib.spgk_layer_mx4.argtypes = [mx4, vp, C.c_int, mx4, vp, C.c_int, u32, mx4, vp, vp]
+    lib.spgk_fp8_pitch.argtypes = [u32]
+    lib.spgk_fp8_pitch.restype = u32
+    lib.spgk_fp8_scales_bytes.argtypes = [u32, u32]
+    lib.spgk_fp8_scales_bytes.restype = C.c_size_t
+    lib.spgk_fp8_scale_index.argtypes = [u32, u32, u32]
+    lib.spgk_fp8_scale_index.restype = C.c_size_t
+    lib.spgk_fp8_quantize.argtypes = [vp, C.c_int, u32, u32, vp, fp8, vp]
+    lib.spgk_fp8_dequantize.argtypes = [fp8, vp, C.c_int, u32, vp]
+    lib.spgk_layer_fp8.argtypes = [fp8, vp, C.c_int, fp8, vp, C.c_int, u32, fp8, vp, vp]
+    lib.spgk_experts_fp8.argtypes = [fp8, u32, vp, C.c_int, fp8, vp, vp, C.c_int, u32, fp8, vp, vp]
+    lib.spgk_route_rows.argtypes = [vp, C.c_int, u32, u32, u32, u32, C.c_int, vp, vp, vp, vp, vp, vp]
+    lib.spgk_combine_rows.argtypes = [vp, C.c_int, u32, u32, vp, vp, u32, u32, u32, vp, C.c_int, u32, vp]
     lib.spgk_gemm_tc_status.argtypes = [vp, vp]
     lib.spgk_sample_rows.argtypes = [vp, C.c_int, u32, u32, u32, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     return lib
