@@ -1,113 +1,897 @@
-// spg_fp8_layer.cu -- dense layers on 8-bit operands with a scale for each block of 128, one layer or one for each group of rows.
+// spg_fp8_layer.cu -- dense layers on 8-bit operands with a scale for each block of 128, one layer for all rows or one for each group of them.
 //
 //   y[n][j] = act(bias[j] + sum_b 2^(Ew[j,b] + Ex[n,b]) * sum_{k in block b} w[j][k] x[n][k])
 //
-// A block of threads has 32 rows and 128 units, a thread four by four of them; elements go through shared memory as fp32, and a block's sum is scaled as a whole, by
-// 2^(Ew + Ex) in two factors (neither operand's values need fit fp32).
+// tcgen05.mma kind::mxf8f6f4 multiplies E4M3 elements and their E8M0 scales as they lie in memory: nothing is unpacked.  It takes a scale for 32 elements; four products
+// in a row are given the same one.  A word of scales has those of four k-blocks of 128, so it goes to tensor memory once for all four (tcgen05.cp, issued in
+// front of the products by the same thread, runs in order with them) and the instruction's scale ids say which byte.
+// The weights are the 128-row side of a tile, rows of the batch its columns (16 to 256): a batch of one costs no more products than one of sixteen, a lane of the epilogue has
+// one output unit, and a tile's units are one block of the next layer's input.
+// Groups of rows begin anywhere: a tile's codes come by boxes from any row on, and its scales by a warp that reads the words of its rows and lays them out as tcgen05.cp wants
+// them.  What a box brings beyond a group's last row belongs to other columns and is not put out.
+// The grid has no more CTAs than the GPU has SMs; each walks the tiles of all groups, copies running ahead over a tile's end.  Where there are few tiles, up to eight CTAs of
+// a cluster share one, each with its part of the k-blocks, and send one another their sums, which are added in rank order.
+//
+// Every wait on an mbarrier is bounded.  A role whose wait gave up records a code in `status`, raises a flag that ends all other waits, and is not told of what follows; outputs are
+// put out only of sums that are said to be complete.  Copies and products under way end, again waited for with a limit, before the memory that they write to is given back.
 #include "spg_fp8.cuh"
+#include "spg_gemm.cuh"
+#include "spg_tc.cuh"
+#include <cstdio>
+#include <mutex>
 
 namespace {
 
+using namespace spgtc;
 using namespace spgfp8;
 
-constexpr uint32_t TM = 128, TN = 32, TK = 32, THREADS = 256;
+constexpr uint32_t TM = 128;                  // output units of a tile
+constexpr uint32_t KB = 128;                  // elements of a k-block: one block, four products
+constexpr uint32_t W_BYTES = TM * KB;         // codes of a tile's weights
+constexpr uint32_t SF_TILE = 512;             // words of scales of 128 rows
+constexpr uint32_t SF_SLOTS = 4;              // words on their way, four k-blocks each
+constexpr uint32_t ROLES = 3;                 // warp 0: copies, warp 1: products, warp 2: scales; the rest: outputs
+constexpr uint32_t EPI = 8, THREADS = 32 * (ROLES + EPI);
+constexpr uint32_t MAX_STAGES = 12;
+constexpr uint32_t MAX_SPLIT = 8;
+constexpr uint32_t AHEAD = 2;
+constexpr uint32_t PART = 8 * TM * 4;         // a CTA's sums of eight rows
+constexpr uint32_t HEAD = 2048;
+constexpr uint32_t ROOM = 180 * 1024;         // of shared memory for a CTA (the rest of an SM's is its cache)
+constexpr uint32_t DRAIN = 1u << 12;          // attempts of a last wait
 
 struct LayerParams {
-    uint32_t N, out, cols, experts, w_rows;
-    const uint8_t *w, *x; uint32_t w_pitch, x_pitch;
-    const uint8_t *w_scales, *x_scales;
-    const int32_t *starts;
+    uint32_t N, out, cols, experts;           // rows, units and inputs of a layer, layers
+    uint32_t w_rows, kblocks, j_tiles, split, stages;
+    const uint32_t *w_words, *x_words;        // scales
+    const int32_t *starts;                    // of the groups, or NULL: one group
     const float *bias;
     int act;
     void *y; int type; uint32_t ldy;
     uint8_t *next_codes, *next_scales; uint32_t next_pitch;
+    int32_t *status;
+    int impatient;                            // (the check of the failure path: spgk_selftest_impatient)
 };
 
-__global__ void __launch_bounds__(THREADS) spg_fp8_layer_kernel(const LayerParams p)
+__device__ __forceinline__ void st_cluster_if(uint32_t addr, float v, uint32_t yes)
 {
-    __shared__ float ws[TK][TM + 4], xs[TK][TN + 4];
-    __shared__ uint32_t bytes[TM + TN];
-    __shared__ uint32_t place[3];
-    spg_grid_trigger();
-    spg_grid_wait();
-    if (threadIdx.x == 0) {
-        // the tile of rows that this block has, of all groups' one behind the other
-        uint32_t t = blockIdx.y, at = 0;
-        place[0] = place[1] = place[2] = 0;
-        for (uint32_t e = 0; e < p.experts; e++) {
-            uint32_t lo = at, hi = p.N;
-            if (p.starts) {
-                lo = max(at, min((uint32_t)max(p.starts[e], 0), p.N));
-                hi = max(lo, min((uint32_t)max(p.starts[e + 1], 0), p.N));
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.shared::cluster.f32 [%0], %1;\n\t}" ::"r"(addr), "f"(v), "r"(yes) : "memory");
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ void cluster_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { __syncwarp(); asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// `id`: which of the CTA's barriers, for this many threads
+__device__ __forceinline__ void some_meet(uint32_t id, uint32_t threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ bool some_agree(uint32_t id, uint32_t threads, bool yes)
+{
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(id), "r"(threads), "r"((uint32_t)yes) : "memory");
+    return all != 0;
+}
+// one look at a barrier's phase
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+
+// kind::mxf8f6f4, E4M3 on both sides, UE8M0 scales
+__host__ __device__ constexpr uint32_t idesc_fp8(uint32_t m, uint32_t n) { return ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24); }
+
+// (predicated: a k-block's products are one way without branches)
+__device__ __forceinline__ void umma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate, uint32_t yes)
+{
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "setp.ne.b32 q, %7, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(yes) : "memory");
+}
+__device__ __forceinline__ void umma_fp8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate, uint32_t yes)
+{
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "setp.ne.b32 q, %7, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(yes) : "memory");
+}
+// 512 bytes (32 rows of 16) -> four columns of tensor memory, once for each quarter of the lanes; of a pair in both CTAs, each from its own shared memory to its own tensor memory
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) { asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory"); }
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) { asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory"); }
+// no swizzle, groups of eight rows of 16 bytes 128 bytes apart
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr)
+{
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(128u >> 4) << 16 | (uint64_t)(128u >> 4) << 32 | (uint64_t)1u << 46;
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
+          "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+          "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void prefetch_l2(const CUtensorMap *map, int c0, int c1)
+{
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
+}
+
+// ---- groups of rows and their tiles -----------------------------------------------------------------------------------------------
+// In shared memory: for each layer the first row of its group and how many tiles of rows the groups in front have; one entry more with the end of both.
+struct Table { uint32_t *row, *first; };
+__host__ __device__ constexpr uint32_t table_bytes(uint32_t experts) { return ((experts + 1) * 8 + 1023) / 1024 * 1024; }
+
+// by one warp; behind the wait for the launch in front where there are starts
+__device__ __forceinline__ void make_table(const LayerParams &p, const Table &tab, uint32_t tile_rows, uint32_t lane)
+{
+    if (!p.starts) {
+        if (lane < 2) { tab.row[lane] = lane * p.N; tab.first[lane] = lane * ((p.N + tile_rows - 1) / tile_rows); }
+        return;
+    }
+    const auto inside = [&](int32_t s) { return min((uint32_t)max(s, 0), p.N); };
+    uint32_t row = inside(p.starts[0]), tiles = 0;
+    for (uint32_t e0 = 0; e0 < p.experts; e0 += 256) {
+        uint32_t end[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) { const uint32_t e = e0 + i * 32 + lane; end[i] = e < p.experts ? inside(p.starts[e + 1]) : 0u; }
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t e = e0 + i * 32 + lane;
+            if (e0 + i * 32 >= p.experts) break;
+            uint32_t hi = max(end[i], row);                                       // no group ends in front of an earlier one
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) { const uint32_t v = __shfl_up_sync(0xffffffffu, hi, o); if (lane >= (uint32_t)o) hi = max(hi, v); }
+            uint32_t lo = __shfl_up_sync(0xffffffffu, hi, 1);
+            if (lane == 0) lo = row;
+            const uint32_t mine = (hi - lo + tile_rows - 1) / tile_rows;
+            uint32_t upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) { const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += v; }
+            if (e < p.experts) {
+                tab.row[e] = lo; tab.first[e] = tiles + upto - mine;
+                if (e + 1 == p.experts) { tab.row[e + 1] = hi; tab.first[e + 1] = tiles + upto; }
             }
-            at = hi;
-            const uint32_t tiles = (hi - lo + TN - 1) / TN;
-            if (t < tiles) { place[0] = e; place[1] = lo + t * TN; place[2] = hi; break; }
-            t -= tiles;
+            row = __shfl_sync(0xffffffffu, hi, 31);
+            tiles += __shfl_sync(0xffffffffu, upto, 31);
         }
     }
-    __syncthreads();
-    const uint32_t e = place[0], n0 = place[1], end = place[2], j0 = blockIdx.x * TM;
-    if (n0 >= end) return;
+}
+
+// Tile t of all: its layer, its tile of units, its first row and how many rows of its group there are from there on.  A group's tiles go in bands of so many tiles of units, the units
+// fastest inside a band: what runs at a time shares weights and rows in L2.
+struct Tile {
+    uint32_t e, j, n0, rows;
+    __device__ __forceinline__ bool find(uint32_t t, const Table &tab, uint32_t experts, uint32_t j_tiles, uint32_t tile_rows, uint32_t band)
+    {
+        const uint32_t q = t / j_tiles;
+        if (q >= tab.first[experts]) return false;
+        uint32_t lo = 0, hi = experts;                                            // first[lo] <= q < first[hi]
+        while (hi - lo > 1) { const uint32_t mid = (lo + hi) / 2; if (tab.first[mid] <= q) lo = mid; else hi = mid; }
+        e = lo;
+        const uint32_t at = tab.first[lo], n_tiles = tab.first[lo + 1] - at, r = t - at * j_tiles, one = band * n_tiles, g = r / one, left = r % one, here = min(band, j_tiles - g * band);
+        j = g * band + left % here;
+        n0 = tab.row[lo] + left / here * tile_rows;
+        rows = tab.row[lo + 1] - n0;
+        return true;
+    }
+};
+
+// ---- outputs ----------------------------------------------------------------------------------------------------------------------
+// (predicated: a branch around each store costs more than the store)
+__device__ __forceinline__ void put(float *y, float v, uint32_t yes)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.f32 [%0], %1;\n\t}" ::"l"(y), "f"(v), "r"(yes) : "memory");
+}
+__device__ __forceinline__ void put16(void *y, uint16_t v, uint32_t yes)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p st.global.u16 [%0], %1;\n\t}" ::"l"(y), "h"(v), "r"(yes) : "memory");
+}
+__device__ __forceinline__ void put(__half *y, float v, uint32_t yes) { put16(y, __half_as_ushort(__float2half_rn(v)), yes); }
+__device__ __forceinline__ void put(__nv_bfloat16 *y, float v, uint32_t yes) { put16(y, __bfloat16_as_ushort(__float2bfloat16_rn(v)), yes); }
+
+// what is chosen -- activation, type -- is chosen outside the loops over the rows: an epilogue's instructions come from L2 as it runs
+template <int C, typename F> __device__ __forceinline__ void each(float (&v)[C], F f)
+{
+#pragma unroll
+    for (int i = 0; i < C; i++) v[i] = f(v[i]);
+}
+template <int C> __device__ __forceinline__ void activate(float (&v)[C], int act)
+{
+    switch (act) {
+        case SPG_ACT_RELU:    each(v, [](float x) { return spg_activate(x, SPG_ACT_RELU); }); break;
+        case SPG_ACT_LEAKY:   each(v, [](float x) { return spg_activate(x, SPG_ACT_LEAKY); }); break;
+        case SPG_ACT_SIGMOID: each(v, [](float x) { return spg_activate(x, SPG_ACT_SIGMOID); }); break;
+        case SPG_ACT_TANH:    each(v, [](float x) { return spg_activate(x, SPG_ACT_TANH); }); break;
+        case SPG_ACT_FOO52:   each(v, [](float x) { return spg_activate(x, SPG_ACT_FOO52); }); break;
+        default: break;
+    }
+}
+template <typename T, int C> __device__ __forceinline__ void put_rows(const LayerParams &p, const float (&v)[C], uint32_t n0, uint32_t rows, uint32_t j)
+{
+    T *y = reinterpret_cast<T *>(p.y) + (uint64_t)n0 * p.ldy + j;
+#pragma unroll
+    for (int i = 0; i < C; i++, y += p.ldy) put(y, v[i], (uint32_t)i < rows && j < p.out);
+}
+
+// The four warps that have the same rows of a tile, its 128 units between them: where they leave their largest magnitudes to one another, eight rows by turns in two places
+struct Four {
+    uint32_t *most;                           // [2][4][8]
+    uint32_t id, quad, turn;                  // their barrier, this warp among them
+};
+// Eight rows' values of this lane's unit, the four warps' 128 units being one block of the next layer's input: scales, codes, stores.
+// Lane i makes row i's scale for all.  A lane's codes are bytes of two words, one a row; two exchanges among four lanes turn each word into four units of one row.
+__device__ __forceinline__ void put_next(const LayerParams &p, const float (&v)[8], uint32_t n0, uint32_t rows, uint32_t j0, uint32_t lane, Four &four)
+{
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t a = __reduce_max_sync(0xffffffffu, __float_as_uint(v[i]) & 0x7fffffffu);
+        if (lane % 8u == (uint32_t)i) most = a;
+    }
+    uint32_t *place = four.most + four.turn * 32u;
+    four.turn ^= 1u;
+    if (lane < 8u) place[four.quad * 8u + lane] = most;
+    some_meet(four.id, 128);
+#pragma unroll
+    for (uint32_t q = 0; q < 4; q++) most = max(most, place[q * 8u + lane % 8u]);
+    const uint32_t mine = scale_byte(most);                                      // row lane % 8
+    const float inv = inverse_scale(mine);
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) q[i] = v[i] * __shfl_sync(0xffffffffu, inv, i);
+    const uint32_t j = j0 + lane / 4u * 4u, block = j0 / TM;
+    const bool there = j < (p.out + 15u) / 16u * 16u;
+#pragma unroll
+    for (uint32_t h = 0; h < 2; h++) {
+        uint32_t w = encode4(q[4 * h], q[4 * h + 1], q[4 * h + 2], q[4 * h + 3]);
+        w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 2), lane & 2u ? 0x3276 : 0x5410);
+        w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 1), lane & 1u ? 0x3715 : 0x6240);
+        const uint32_t i = 4u * h + lane % 4u;                                   // this lane's row now
+        if (__shfl_sync(0xffffffffu, mine, i) == 255u) w = 0;                    // a NaN block
+        if (i < rows && there) *reinterpret_cast<uint32_t *>(p.next_codes + (uint64_t)(n0 + i) * p.next_pitch + j) = w;
+    }
+    if (four.quad == 0 && lane < 8u && lane < rows) p.next_scales[((uint64_t)(block / 4u) * p.N + n0 + lane) * 4u + block % 4u] = (uint8_t)mine;
+}
+// C rows' sums of this lane's unit to outputs (rows: how many of them there are; with none it only brings its instructions to the SM)
+template <int C> __device__ __forceinline__ void finish(const LayerParams &p, float (&v)[C], uint32_t n0, uint32_t rows, uint32_t j0, uint32_t lane, float bias, Four &four)
+{
+    const uint32_t j = j0 + lane;
+    each(v, [bias](float x) { return x + bias; });
+    activate(v, p.act);
+    if (p.y) {
+        if (p.type == SPGK_T_F32) put_rows<float>(p, v, n0, rows, j);
+        else if (p.type == SPGK_T_F16) put_rows<__half>(p, v, n0, rows, j);
+        else put_rows<__nv_bfloat16>(p, v, n0, rows, j);
+    }
+    if (p.next_codes) {
+#pragma unroll
+        for (int i = 0; i < C; i += 8) {
+            float q[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) q[k] = j < p.out ? v[i + k] : 0.0f;
+            put_next(p, q, n0 + i, rows > (uint32_t)i ? rows - i : 0, j0, lane, four);
+        }
+    }
+}
+
+// ---- scales -----------------------------------------------------------------------------------------------------------------------
+// The words of a tile's rows for four k-blocks, R times 32 of them from row `first` on (zero from `rows` on): lane l has rows l, l + 32, ...
+template <uint32_t R> __device__ __forceinline__ void load_words(uint32_t (&v)[R], const uint32_t *words, uint32_t group, uint32_t rows, uint32_t first, uint32_t lane)
+{
+    const uint32_t *at = words + (uint64_t)group * rows;
+#pragma unroll
+    for (uint32_t i = 0; i < R; i++) { const uint32_t r = first + i * 32u + lane; v[i] = r < rows ? at[r] : 0u; }
+}
+// to shared memory, 128 rows a tile of 512 bytes: row r's word is the r % 128 / 32'th of the 16 bytes r % 32
+template <uint32_t R> __device__ __forceinline__ void store_words(uint32_t at, const uint32_t (&v)[R], uint32_t lane)
+{
+#pragma unroll
+    for (uint32_t i = 0; i < R; i += 4)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * (SF_TILE / 4) + lane * 16u), "r"(v[i]), "r"(i + 1 < R ? v[i + 1 < R ? i + 1 : i] : 0u),
+                     "r"(i + 2 < R ? v[i + 2 < R ? i + 2 : i] : 0u), "r"(i + 3 < R ? v[i + 3 < R ? i + 3 : i] : 0u) : "memory");
+}
+
+// ---- single CTAs, and clusters that share a tile ------------------------------------------------------------------------------------
+template <uint32_t NT> struct Shape {
+    static constexpr uint32_t X_BYTES = NT * KB;
+    static constexpr uint32_t STAGE = W_BYTES + X_BYTES;
+    static constexpr uint32_t SFW = 2 * NT, SFX = 4, SF_COLS = 8;             // tensor memory: two sets of sums, two sets of scales
+    static constexpr uint32_t USED = SFW + 2 * SF_COLS;
+    static constexpr uint32_t COLS = USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+    static constexpr uint32_t X_WORDS = (NT + 31) / 32;
+};
+constexpr uint32_t BAND = 16;
+
+// Where CTAs share a tile, chunks of eight of its rows go to them by turns, and each sends its sums of a chunk to the CTA that has it
+__host__ __device__ constexpr uint32_t chunks_of(uint32_t rows, uint32_t nt) { return ((rows < nt ? rows : nt) + 7) / 8; }
+template <uint32_t NT> __host__ __device__ constexpr uint32_t parts_bytes(uint32_t rows, uint32_t split)
+{
+    return split > 1 ? (chunks_of(rows, NT) + split - 1) / split * split * PART : 0;
+}
+
+template <uint32_t NT>
+__global__ void __launch_bounds__(THREADS) spg_fp8_layer_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LayerParams p)
+{
+    using L = Shape<NT>;
+    extern __shared__ uint8_t raw[];
+    uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t head = smem_u32(base), table = head + HEAD, words = table + table_bytes(p.experts), parts = words + SF_SLOTS * 2 * SF_TILE, ring = parts + parts_bytes<NT>(p.N, p.split);
+    const uint32_t full = head, empty = full + 8 * MAX_STAGES, sf_full = empty + 8 * MAX_STAGES, sf_empty = sf_full + 8 * SF_SLOTS, sums_full = sf_empty + 8 * SF_SLOTS, sums_free = sums_full + 16;
+    const uint32_t ended = sums_free + 16, slot = ended + 8, aborted = slot + 4, late = aborted + 4, told = late + 4;
+    // (aborted: a wait of this CTA gave up; late: one of the last waits did; told: one of the cluster's CTAs does not have its sums)
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head)), *told_flag = abort_flag + 2;
+    uint32_t *const most = reinterpret_cast<uint32_t *>(base + 1024);
+    const Table tab = { reinterpret_cast<uint32_t *>(base + HEAD), reinterpret_cast<uint32_t *>(base + HEAD) + p.experts + 1 };
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
-    float acc[4][4] = {}, sub[4][4] = {};
-    for (uint32_t k0 = 0; k0 < p.cols; k0 += TK) {
-        const uint32_t b = k0 / BLOCK;
-        for (uint32_t i = threadIdx.x; i < (TM + TN) * (TK / 4); i += THREADS) {
-            const uint32_t r = i / (TK / 4), c = i % (TK / 4) * 4, k = k0 + c;
-            const bool w = r < TM;
-            const uint64_t row = w ? (uint64_t)e * p.out + j0 + r : (uint64_t)n0 + (r - TM);
-            const bool there = (w ? j0 + r < p.out : n0 + (r - TM) < end) && k < p.cols;
-            float v[4] = {};
-            if (there) {
-                decode4(*reinterpret_cast<const uint32_t *>((w ? p.w + row * p.w_pitch : p.x + row * p.x_pitch) + k), v);
-                for (uint32_t q = 0; q < 4; q++) if (k + q >= p.cols) v[q] = 0.0f;
-                if (c == 0) bytes[r] = (w ? p.w_scales : p.x_scales)[((uint64_t)(b / 4) * (w ? p.w_rows : p.N) + row) * 4 + b % 4];
-            }
-            for (uint32_t q = 0; q < 4; q++) if (w) ws[c + q][r] = v[q]; else xs[c + q][r - TM] = v[q];
+    const uint32_t rank = blockIdx.x % p.split, team = blockIdx.x / p.split, teams = gridDim.x / p.split;
+    // this CTA's k-blocks
+    const uint32_t lo = (uint32_t)((uint64_t)p.kblocks * rank / p.split), hi = (uint32_t)((uint64_t)p.kblocks * (rank + 1) / p.split);
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < p.stages; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (uint32_t s = 0; s < SF_SLOTS; s++) { mbar_init(sf_full + 8 * s, 1); mbar_init(sf_empty + 8 * s, 1); }
+        for (uint32_t a = 0; a < 2; a++) { mbar_init(sums_full + 8 * a, 1); mbar_init(sums_free + 8 * a, EPI); }
+        mbar_init(ended, 1);
+        for (uint32_t i = 0; i < 3; i++) abort_flag[i] = 0;
+        mbar_fence_init();
+    }
+    if (p.split > 1) cluster_arrive();                                           // (behind `told`, and in front of the wait for tensor memory: see below)
+    if (warp == 1) tmem_alloc(slot, L::COLS);
+    if (warp == 0 && elect_one()) { prefetch_map(&map_w); prefetch_map(&map_x); }
+    if (warp == 2 && !p.starts) make_table(p, tab, NT, lane);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
+    spg_grid_trigger();
+    // The first weights to L2 while the kernel in front still runs (whoever writes them: L2 is where writes meet), where it is known which they are
+    if (warp == 0 && !p.starts && elect_one()) {
+        Tile tile;
+        if (tile.find(team, tab, 1, p.j_tiles, NT, BAND))
+            for (uint32_t kb = lo; kb < hi && kb < lo + AHEAD; kb++) prefetch_l2(&map_w, (int)(kb * KB), (int)(tile.j * TM));
+    }
+    __syncwarp();
+    if (warp < ROLES) {
+        spg_grid_wait();
+        if (p.starts) {
+            if (warp == 2) make_table(p, tab, NT, lane);
+            some_meet(1, THREADS);
         }
-        __syncthreads();
-        for (uint32_t k = 0; k < TK; k++) {
-            const float4 a = *reinterpret_cast<const float4 *>(&xs[k][warp * 4]), b4 = *reinterpret_cast<const float4 *>(&ws[k][lane * 4]);
-            const float x[4] = { a.x, a.y, a.z, a.w }, w[4] = { b4.x, b4.y, b4.z, b4.w };
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) sub[i][j] = fmaf(x[i], w[j], sub[i][j]);
-        }
-        if (k0 % BLOCK == BLOCK - TK || k0 + TK >= p.cols) {
-            for (uint32_t i = 0; i < 4; i++)
-                for (uint32_t j = 0; j < 4; j++) {
-                    const uint32_t a = bytes[lane * 4 + j], c = bytes[TM + warp * 4 + i], half = (a + c) / 2;
-                    acc[i][j] += a == 255u || c == 255u ? __uint_as_float(0x7fffffffu) : sub[i][j] * scale_value(half) * scale_value(a + c - half);
-                    sub[i][j] = 0.0f;
+    }
+    Tile tile;
+    uint32_t t = team;
+    if (warp == 0) {
+        uint32_t begun = 0;
+        if (elect_one()) {
+            bool ok = true;
+            for (uint32_t s = 0, phase = 1; ok && tile.find(t, tab, p.experts, p.j_tiles, NT, BAND); t += teams) {
+                for (uint32_t kb = lo; kb < hi; kb++) {
+                    if (!(ok = mbar_wait(empty + 8 * s, phase, abort_flag, p.status, 1))) break;
+                    const uint32_t at = ring + s * L::STAGE;
+                    mbar_expect_tx(full + 8 * s, L::STAGE);
+                    tma_load_2d(at, &map_w, full + 8 * s, (int)(kb * KB), (int)(tile.e * p.out + tile.j * TM));
+                    tma_load_2d(at + W_BYTES, &map_x, full + 8 * s, (int)(kb * KB), (int)tile.n0);
+                    begun++;
+                    if (++s == p.stages) { s = 0; phase ^= 1u; }
                 }
+            }
+            // (the table's place is no longer needed by whoever gave up: the last word of the head says how many copies were begun)
+            *reinterpret_cast<volatile uint32_t *>(base + HEAD - 4) = begun;
         }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (elect_one()) {
+            const uint32_t idesc = idesc_fp8(TM, NT), last = tab.first[p.experts] * p.j_tiles;
+            uint32_t s = 0, phase = 0, q = 0, q_phase = 0, a = 0, a_phase = 1, odd = 0;
+            bool ok = true;
+            for (; ok && t < last; t += teams) {
+                if (p.impatient == 1 && last - t <= teams && rank == 0) { atomicCAS(p.status, 0, 2); *abort_flag = 1; break; }
+                ok = p.impatient != 2 ? mbar_wait(sums_free + 8 * a, a_phase, abort_flag, p.status, 6) : mbar_test(sums_free + 8 * a, a_phase);
+                if (!ok) { atomicCAS(p.status, 0, 6); *abort_flag = 1; break; }
+                tc_fence_after();
+                for (uint32_t kb = lo; kb < hi; kb++) {
+                    if (kb % 4u == 0 || kb == lo) {
+                        if (!(ok = mbar_wait(sf_full + 8 * q, q_phase, abort_flag, p.status, 7))) break;
+                        tc_fence_after();
+                        const uint32_t to = tmem + L::SFW + (odd ^= 1u) * L::SF_COLS;
+                        const uint64_t from = scale_desc(words + q * 2 * SF_TILE);
+                        copy_scales(to, from);
+                        copy_scales(to + L::SFX, from + (SF_TILE >> 4));
+                        umma_commit(sf_empty + 8 * q);
+                        if (++q == SF_SLOTS) { q = 0; q_phase ^= 1u; }
+                    }
+                    if (!(ok = mbar_wait(full + 8 * s, phase, abort_flag, p.status, 2))) break;
+                    tc_fence_after();
+                    const uint32_t at = ring + s * L::STAGE, sf = tmem + L::SFW + odd * L::SF_COLS, left = p.cols - kb * KB, id = (kb % 4u) << 4 | (kb % 4u) << 29;
+                    const uint64_t w = smem_desc_sw128(at), x = smem_desc_sw128(at + W_BYTES);
+                    umma_fp8(tmem + a * NT, w, x, idesc | id, sf, sf + L::SFX, kb > lo, 1);
+                    umma_fp8(tmem + a * NT, w + 2, x + 2, idesc | id, sf, sf + L::SFX, 1, left > 32);
+                    umma_fp8(tmem + a * NT, w + 4, x + 4, idesc | id, sf, sf + L::SFX, 1, left > 64);
+                    umma_fp8(tmem + a * NT, w + 6, x + 6, idesc | id, sf, sf + L::SFX, 1, left > 96);
+                    umma_commit(empty + 8 * s);
+                    if (++s == p.stages) { s = 0; phase ^= 1u; }
+                }
+                if (!ok) break;
+                umma_commit(sums_full + 8 * a);
+                if (++a == 2) { a = 0; a_phase ^= 1u; }
+            }
+        }
+        __syncwarp();
+        if (p.split > 1) {
+            // Given back before this CTA waits for the others: one that has none on its SM, and so cannot finish, may hold up a cluster that holds some elsewhere
+            if (team < tab.first[p.experts] * p.j_tiles) some_meet(2, 32 * (EPI + 1));
+            if (*abort_flag) {
+                if (elect_one()) umma_commit(ended);
+                __syncwarp();
+                mbar_wait_uniform(ended, 0, late, p.status, 5, DRAIN);
+            }
+            tc_fence_after();
+            tmem_free(tmem, L::COLS);
+        }
+    } else if (warp == 2) {
+        uint32_t q = 0, phase = 1, w[4], x[L::X_WORDS], g = lo / 4u;
+        const uint32_t g_end = (hi + 3u) / 4u;
+        bool more = tile.find(t, tab, p.experts, p.j_tiles, NT, BAND);
+        const auto load = [&]() {
+            load_words(w, p.w_words, g, p.w_rows, tile.e * p.out + tile.j * TM, lane);
+            load_words(x, p.x_words, g, p.N, tile.n0, lane);
+        };
+        if (more) load();
+        while (more) {
+            uint32_t w0[4], x0[L::X_WORDS];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) w0[i] = w[i];
+#pragma unroll
+            for (uint32_t i = 0; i < L::X_WORDS; i++) x0[i] = x[i];
+            if (++g == g_end) { g = lo / 4u; t += teams; more = tile.find(t, tab, p.experts, p.j_tiles, NT, BAND); }
+            if (more) load();                                                    // (on their way while these wait for their place)
+            mbar_wait_uniform(sf_empty + 8 * q, phase, aborted, p.status, 8);
+            if (*abort_flag) break;
+            store_words(words + q * 2 * SF_TILE, w0, lane);
+            store_words(words + q * 2 * SF_TILE + SF_TILE, x0, lane);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sf_full + 8 * q);
+            if (++q == SF_SLOTS) { q = 0; phase ^= 1u; }
+        }
+    } else {
+        const uint32_t quad = warp % 4u, half = (warp - ROLES) / 4u;
+        Four four = { most + half * 64u, 3u + half, quad, 0u };
+        uint32_t a = 0, a_phase = 0;
+        // Once without a row before the launch in front has ended: the outputs' instructions come from L2, and would follow the products
+#pragma unroll 1
+        for (uint32_t dry = 1;; dry = 0) {
+            if (!dry) {
+                if (!tile.find(t, tab, p.experts, p.j_tiles, NT, BAND)) break;
+            } else tile = { 0, 0, 0, 0 };
+            const uint32_t j0 = tile.j * TM + quad * 32u, j = j0 + lane, lanes = tmem + a * NT + (quad * 32u << 16), rows = min(tile.rows, NT);
+            float bias = 0.0f;
+            bool ok = true;
+            if (!dry) {
+                if (p.bias && j < p.out) bias = p.bias[(uint64_t)tile.e * p.out + j];
+                // (all four warps of a row go one way)
+                ok = some_agree(3u + half, 128, mbar_wait(sums_full + 8 * a, a_phase, abort_flag, p.status, 3));
+                tc_fence_after();
+                if (p.split > 1) {
+                    // This CTA's sums to those that put them out, [chunk][CTA][row][unit], sent before one barrier
+                    cluster_wait();                                              // all have begun
+                    const uint32_t chunks = ok ? (rows + 7u) / 8u : 0u;
+                    for (uint32_t c = half; c < chunks; c += 2) {
+                        float v[8];
+                        tmem_ld8(lanes + 8 * c, v);
+                        tmem_ld_wait();
+                        const uint32_t to = mapa(parts + (c / p.split * p.split + rank) * PART + (quad * 32u + lane) * 4u, c % p.split), left = rows - 8 * c;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) st_cluster_if(to + i * TM * 4u, v[i], (uint32_t)i < left);
+                    }
+                    if (!ok && lane < p.split) st_cluster_u32(mapa(told, lane), 1);
+                    tc_fence_before();
+                    __syncwarp();
+                    some_meet(2, 32 * (EPI + 1));
+                    cluster_arrive();
+                    cluster_wait();
+                    ok = !__any_sync(0xffffffffu, *told_flag);
+                }
+            }
+            if (ok) {
+                const uint32_t end = dry ? 1u : rows;
+#pragma unroll 1
+                for (uint32_t c = dry ? 0 : (half * p.split + rank) * 8u; c < end; c += p.split * 16u) {
+                    float v[8];
+                    if (p.split == 1 || dry) {
+                        if (!dry) { tmem_ld8(lanes + c, v); tmem_ld_wait(); }
+                        else each(v, [](float) { return 0.0f; });
+                    } else {
+                        const float *part = reinterpret_cast<const float *>(base + (parts - head)) + (c / 8 / p.split * p.split) * (PART / 4) + quad * 32u + lane;
+                        each(v, [](float) { return 0.0f; });
+#pragma unroll 1
+                        for (uint32_t r = 0; r < p.split; r++, part += PART / 4) {   // in rank order
+#pragma unroll
+                            for (int i = 0; i < 8; i++) v[i] += part[i * TM];
+                        }
+                    }
+                    finish(p, v, tile.n0 + c, dry ? 0u : rows - c, j0, lane, bias, four);
+                }
+            }
+            if (dry) {
+                spg_grid_wait();
+                if (p.starts) some_meet(1, THREADS);
+                continue;
+            }
+            if (!ok) break;
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sums_free + 8 * a);
+            if (++a == 2) { a = 0; a_phase ^= 1u; }
+            t += teams;
+        }
+    }
+    if (p.split > 1) {
+        // (a cluster without a tile has been through none of its barriers, one with a tile, whose outputs' warps have been through both, only by these)
+        const bool none = team >= tab.first[p.experts] * p.j_tiles;
+        if (warp < ROLES || none) { cluster_wait(); cluster_arrive(); cluster_wait(); }
+    }
+    __syncwarp();
+    __syncthreads();
+    if (*abort_flag) {
+        // what is under way ends first: the products, which `ended` is told of, and the last copies, each of which has its barrier
+        if (warp == 1 && p.split == 1) {
+            if (elect_one()) umma_commit(ended);
+            __syncwarp();
+            mbar_wait_uniform(ended, 0, late, p.status, 5, DRAIN);
+        }
+        if (warp == 0) {
+            const uint32_t begun = *reinterpret_cast<volatile uint32_t *>(base + HEAD - 4);
+            for (uint32_t i = begun > p.stages ? begun - p.stages : 0; i < begun; i++) mbar_wait_uniform(full + 8 * (i % p.stages), i / p.stages & 1u, late, p.status, 4, DRAIN);
+        }
+        __syncwarp();
         __syncthreads();
     }
-    for (uint32_t i = 0; i < 4; i++) {
-        const uint32_t n = n0 + warp * 4 + i;
-        if (n >= end) break;
-        float v[4];
-        uint32_t most = 0;
-        for (uint32_t q = 0; q < 4; q++) {
-            const uint32_t j = j0 + lane * 4 + q;
-            v[q] = j < p.out ? spg_activate(acc[i][q] + (p.bias ? p.bias[(uint64_t)e * p.out + j] : 0.0f), p.act) : 0.0f;
-            most = max(most, __float_as_uint(v[q]) & 0x7fffffffu);
-            if (!p.y || j >= p.out) continue;
-            const uint64_t at = (uint64_t)n * p.ldy + j;
-            if (p.type == SPGK_T_F32) ((float *)p.y)[at] = v[q];
-            else if (p.type == SPGK_T_F16) ((__half *)p.y)[at] = from_f32<__half>(v[q]);
-            else ((__nv_bfloat16 *)p.y)[at] = from_f32<__nv_bfloat16>(v[q]);
-        }
-        if (p.next_codes) {
-            const uint32_t byte = scale_byte(__reduce_max_sync(0xffffffffu, most)), b = j0 / BLOCK;
-            const float inv = inverse_scale(byte);
-            const uint32_t code = byte == 255u ? 0u : encode4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-            if (j0 + lane * 4 < (p.out + 15) / 16 * 16) *reinterpret_cast<uint32_t *>(p.next_codes + (uint64_t)n * p.next_pitch + j0 + lane * 4) = code;
-            if (lane == 0) p.next_scales[((uint64_t)(b / 4) * p.N + n) * 4 + b % 4] = (uint8_t)byte;
+    if (warp == 1 && p.split == 1) { tc_fence_after(); tmem_free(tmem, L::COLS); }
+}
+
+// ---- pairs of CTAs, many rows -------------------------------------------------------------------------------------------------
+// 256 units x up to 256 rows of a group a tile on a cluster of two (cta_group::2): each CTA holds 128 units' weights and half of the rows, so a k-block costs it 32 KB
+// for 512 cycles of products; a CTA alone would need 48. The last tile of a group multiplies no more rows than it has (in steps of 32).
+// The sixteen epilogue warps take all columns of sums to registers at once (64 a thread), so the next tile's products wait for that alone (there
+// is no room in tensor memory for a second accumulator of 256 columns beside the scales).
+constexpr uint32_t PN = 256;                                   // rows of the batch a tile
+constexpr uint32_t P_EPI = 16, P_THREADS = 32 * (ROLES + P_EPI);
+constexpr uint32_t P_COLS = PN / (P_EPI / 4);                   // columns of an epilogue warp
+constexpr uint32_t P_STAGE = W_BYTES + PN / 2 * KB;
+constexpr uint32_t P_STAGES = 6;
+constexpr uint32_t P_WORDS = 3 * SF_TILE;                       // of 128 units and 256 rows
+constexpr uint32_t P_SF = PN, P_SFX = 4, P_SF_COLS = 16;        // columns of tensor memory: scales behind the sums, twice; those of the rows behind the weights'
+constexpr uint32_t P_BAND = 8;
+__host__ __device__ constexpr uint32_t pair_smem(uint32_t experts) { return 1024 + HEAD + table_bytes(experts) + SF_SLOTS * P_WORDS + P_STAGES * P_STAGE; }
+
+__global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LayerParams p)
+{
+    extern __shared__ uint8_t raw[];
+    uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t head = smem_u32(base), table = head + HEAD, words = table + table_bytes(p.experts), ring = words + SF_SLOTS * P_WORDS;
+    const uint32_t full = head, empty = full + 8 * P_STAGES, sf_full = empty + 8 * P_STAGES, sf_empty = sf_full + 8 * SF_SLOTS, sums_full = sf_empty + 8 * SF_SLOTS, sums_free = sums_full + 8;
+    const uint32_t ended = sums_free + 8, slot = ended + 8, aborted = slot + 4, late = aborted + 4, told = late + 4;
+    // (told: of each of the two CTAs, how many k-blocks' copies it began, and then whether a wait gave up in it)
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head));
+    volatile uint32_t *told_at = reinterpret_cast<volatile uint32_t *>(base + (told - head));
+    uint32_t *const most = reinterpret_cast<uint32_t *>(base + 1024);
+    const Table tab = { reinterpret_cast<uint32_t *>(base + HEAD), reinterpret_cast<uint32_t *>(base + HEAD) + p.experts + 1 };
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = cluster_rank(), pairs = gridDim.x / 2u;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < P_STAGES; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (uint32_t s = 0; s < SF_SLOTS; s++) { mbar_init(sf_full + 8 * s, 2); mbar_init(sf_empty + 8 * s, 1); }
+        mbar_init(sums_full, 1);
+        mbar_init(sums_free, 2 * P_EPI);
+        mbar_init(ended, 1);
+        for (uint32_t i = 0; i < 6; i++) abort_flag[i] = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc_pair(slot, 512);
+    if (warp == 0 && elect_one()) { prefetch_map(&map_w); prefetch_map(&map_x); }
+    if (warp == 2 && !p.starts) make_table(p, tab, PN, lane);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
+    spg_grid_trigger();
+    if (warp < ROLES) {
+        spg_grid_wait();
+        if (p.starts) {
+            if (warp == 2) make_table(p, tab, PN, lane);
+            some_meet(1, P_THREADS);
         }
     }
+    // columns of a tile with so many rows left in its group: each CTA has half of them, in whole eights
+    const auto columns = [](uint32_t rows) { return rows >= PN ? PN : (rows + 31u) / 32u * 32u; };
+    // a wait gave up: the other CTA's waits end as well
+    const auto give_up = [&](int code) {
+        atomicCAS(p.status, 0, code);
+        for (uint32_t r = 0; r < 2; r++) st_cluster_u32(mapa(aborted, r), 1);
+    };
+    Tile tile;
+    uint32_t t = blockIdx.x / 2u;
+    if (warp == 0) {
+        if (elect_one()) {
+            const uint32_t leader = mapa(full, 0);
+            uint32_t begun = 0;
+            bool ok = true;
+            for (uint32_t s = 0, phase = 1; ok && tile.find(t, tab, p.experts, p.j_tiles, PN, P_BAND); t += pairs) {
+                const int row_w = (int)(tile.e * p.out + tile.j * 256u + rank * TM), row_x = (int)(tile.n0 + rank * columns(tile.rows) / 2u);
+                for (uint32_t kb = 0; kb < p.kblocks; kb++) {
+                    if (!(ok = mbar_wait(empty + 8 * s, phase, abort_flag, p.status, 1))) break;
+                    const uint32_t at = ring + s * P_STAGE;
+                    if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * P_STAGE);
+                    tma_load_2d_pair(at, &map_w, leader + 8 * s, (int)(kb * KB), row_w);
+                    tma_load_2d_pair(at + W_BYTES, &map_x, leader + 8 * s, (int)(kb * KB), row_x);
+                    begun++;
+                    if (++s == P_STAGES) { s = 0; phase ^= 1u; }
+                }
+            }
+            for (uint32_t r = 0; r < 2; r++) st_cluster_u32(mapa(told + 8 * rank, r), begun);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            uint32_t s = 0, phase = 0, q = 0, q_phase = 0, turn = 1, odd = 0;
+            const uint32_t last = tab.first[p.experts] * p.j_tiles;
+            bool ok = true;
+            for (; ok && tile.find(t, tab, p.experts, p.j_tiles, PN, P_BAND); t += pairs) {
+                if (p.impatient == 1 && last - t <= pairs) { give_up(2); break; }
+                const uint32_t idesc = idesc_fp8(256, columns(tile.rows));
+                ok = p.impatient != 2 ? mbar_wait(sums_free, turn, abort_flag, p.status, 6) : mbar_test(sums_free, turn);
+                if (!ok) { give_up(6); break; }
+                turn ^= 1u;
+                tc_fence_after();
+                for (uint32_t kb = 0; kb < p.kblocks; kb++) {
+                    if (kb % 4u == 0) {
+                        if (!(ok = mbar_wait(sf_full + 8 * q, q_phase, abort_flag, p.status, 7))) break;
+                        tc_fence_after();
+                        const uint32_t to = tmem + P_SF + (odd ^= 1u) * P_SF_COLS;
+                        const uint64_t from = scale_desc(words + q * P_WORDS);
+                        copy_scales_pair(to, from);
+                        copy_scales_pair(to + P_SFX, from + (SF_TILE >> 4));
+                        copy_scales_pair(to + P_SFX + 4, from + (2 * SF_TILE >> 4));
+                        umma_commit_pair(sf_empty + 8 * q);
+                        if (++q == SF_SLOTS) { q = 0; q_phase ^= 1u; }
+                    }
+                    if (!(ok = mbar_wait(full + 8 * s, phase, abort_flag, p.status, 2))) break;
+                    tc_fence_after();
+                    const uint32_t at = ring + s * P_STAGE, sf = tmem + P_SF + odd * P_SF_COLS, left = p.cols - kb * KB, id = idesc | (kb % 4u) << 4 | (kb % 4u) << 29;
+                    const uint64_t w = smem_desc_sw128(at), x = smem_desc_sw128(at + W_BYTES);
+                    umma_fp8_pair(tmem, w, x, id, sf, sf + P_SFX, kb > 0, 1);
+                    umma_fp8_pair(tmem, w + 2, x + 2, id, sf, sf + P_SFX, 1, left > 32);
+                    umma_fp8_pair(tmem, w + 4, x + 4, id, sf, sf + P_SFX, 1, left > 64);
+                    umma_fp8_pair(tmem, w + 6, x + 6, id, sf, sf + P_SFX, 1, left > 96);
+                    umma_commit_pair(empty + 8 * s);
+                    if (++s == P_STAGES) { s = 0; phase ^= 1u; }
+                }
+                if (!ok) { give_up(2); break; }
+                umma_commit_pair(sums_full);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        const uint32_t leader = mapa(sf_full, 0), groups = (p.kblocks + 3u) / 4u;
+        uint32_t q = 0, phase = 1, w[4], x[8], g = 0;
+        bool more = tile.find(t, tab, p.experts, p.j_tiles, PN, P_BAND);
+        const auto load = [&]() {
+            load_words(w, p.w_words, g, p.w_rows, tile.e * p.out + tile.j * 256u + rank * TM, lane);
+            load_words(x, p.x_words, g, p.N, tile.n0, lane);
+        };
+        if (more) load();
+        while (more) {
+            uint32_t w0[4], x0[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) w0[i] = w[i];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) x0[i] = x[i];
+            if (++g == groups) { g = 0; t += pairs; more = tile.find(t, tab, p.experts, p.j_tiles, PN, P_BAND); }
+            if (more) load();                                                    // (on their way while these wait for their place)
+            mbar_wait_uniform_cluster(sf_empty + 8 * q, phase, aborted, p.status, 8);
+            if (__any_sync(0xffffffffu, *abort_flag)) break;
+            store_words(words + q * P_WORDS, w0, lane);
+            store_words(words + q * P_WORDS + SF_TILE, x0, lane);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(leader + 8 * q);
+            if (++q == SF_SLOTS) { q = 0; phase ^= 1u; }
+        }
+    } else {
+        const uint32_t quad = warp % 4u, part = (warp - ROLES) / 4u, free_at = mapa(sums_free, 0);
+        Four four = { most + part * 64u, 2u + part, quad, 0u };
+        uint32_t turn = 0;
+        // (dry: once without a row, as above)
+#pragma unroll 1
+        for (uint32_t dry = 1;; dry = 0) {
+            if (!dry) {
+                if (!tile.find(t, tab, p.experts, p.j_tiles, PN, P_BAND)) break;
+            } else tile = { 0, 0, 0, 0 };
+            const uint32_t j0 = tile.j * 256u + rank * TM + quad * 32u, j = j0 + lane, n0 = tile.n0 + part * P_COLS;
+            const uint32_t rows = min(tile.rows, PN) > part * P_COLS ? min(tile.rows, PN) - part * P_COLS : 0u;       // this warp's columns
+            const uint32_t from = tmem + (quad * 32u << 16) + part * P_COLS;
+            const bool some = tile.j * 256u + rank * TM < p.out;                 // (the same in the four warps: some of this CTA's units there are)
+            float bias = 0.0f;
+            if (!dry) {
+                if (p.bias && j < p.out) bias = p.bias[(uint64_t)tile.e * p.out + j];
+                // (all four warps of a row go one way)
+                if (!some_agree(2u + part, 128, mbar_wait(sums_full, turn, abort_flag, p.status, 3))) break;
+                turn ^= 1u;
+                tc_fence_after();
+            }
+            const bool last = !dry && t + pairs >= tab.first[p.experts] * p.j_tiles;
+            if (dry || last) {
+                // the last: nobody waits for tensor memory, and a short loop is quicker than 64 columns written out that come from L2
+#pragma unroll 1
+                for (uint32_t c = 0; c < (dry ? 1u : some ? min(rows, P_COLS) : 0u); c += 8) {
+                    float v[8];
+                    if (!dry) { tmem_ld8(from + c, v); tmem_ld_wait(); }
+                    else each(v, [](float) { return 0.0f; });
+                    finish(p, v, n0 + c, dry ? 0u : rows - c, j0, lane, bias, four);
+                }
+                tc_fence_before();
+                if (dry) {
+                    spg_grid_wait();
+                    if (p.starts) some_meet(1, P_THREADS);
+                    continue;
+                }
+            } else {
+                float v[P_COLS];
+#pragma unroll
+                for (int i = 0; i < (int)P_COLS; i += 32) tmem_ld32(from + i, v + i);
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(free_at);
+                if (rows && some) finish(p, v, n0, rows, j0, lane, bias, four);
+            }
+            t += pairs;
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (uint32_t r = 0; r < 2; r++) st_cluster_u32(mapa(told + 8 * rank + 4, r), (uint32_t)*abort_flag);
+    cluster_sync();
+    if (told_at[1] | told_at[3]) {
+        // Products and copies under way end first.  Each k-block's copies are counted for both CTAs at once, by the first one's barrier: where one of them began fewer, as many bytes
+        // are fetched here once more, or expected of the other alone.
+        if (rank == 0 && warp == 1) {
+            if (elect_one()) umma_commit_pair(ended);
+            __syncwarp();
+            mbar_wait_uniform(ended, 0, late, p.status, 5, DRAIN);
+        }
+        if (rank == 0 && warp == 0) {
+            const uint32_t mine = told_at[0], other = told_at[2], end = max(mine, other);
+            for (uint32_t i = min(mine, other); i < end; i++) {
+                const uint32_t s = i % P_STAGES, bar = full + 8 * s, at = ring + s * P_STAGE;
+                if (elect_one()) {
+                    if (i >= mine) mbar_expect_tx(bar, P_STAGE);                 // (the other's)
+                    else {
+                        tma_load_2d_pair(at, &map_w, mapa(bar, 0), 0, 0);
+                        tma_load_2d_pair(at + W_BYTES, &map_x, mapa(bar, 0), 0, 0);
+                    }
+                }
+                __syncwarp();
+            }
+            for (uint32_t i = end > P_STAGES ? end - P_STAGES : 0; i < end; i++) mbar_wait_uniform_cluster(full + 8 * (i % P_STAGES), i / P_STAGES & 1u, late, p.status, 4, DRAIN);
+        }
+        __syncwarp();
+        __syncthreads();
+        cluster_sync();
+    }
+    if (warp == 1) { tc_fence_after(); tmem_free_pair(tmem, 512); }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn()
+{
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(f);
+    });
+    return fn;
+}
+
+// boxes of a k-block x box_rows rows of a matrix' codes; what lies behind its columns and rows is zero
+int codes_map(CUtensorMap *map, const spgk_fp8 *m, uint32_t box_rows)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) { spgk_set_error("cuTensorMapEncodeTiled", "driver entry point not available"); return SPGK_E_CUDA; }
+    const cuuint64_t dims[2] = { m->cols, m->rows }, strides[1] = { m->pitch };
+    const cuuint32_t box[2] = { KB, box_rows }, steps[2] = { 1, 1 };
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, m->codes, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        char msg[64];
+        snprintf(msg, sizeof msg, "CUresult %d", (int)r);
+        spgk_set_error("cuTensorMapEncodeTiled (8-bit operand)", msg);
+        return SPGK_E_CUDA;
+    }
+    return SPGK_OK;
+}
+
+// the most tiles of `tile_rows` rows that p.N rows in any groups make: one for each layer that has some, and one more for every tile_rows of the rest
+uint64_t most_tiles(const LayerParams &p, uint32_t tile_rows)
+{
+    const uint32_t some = p.experts < p.N ? p.experts : p.N;
+    return (some + (uint64_t)(p.N - some) / tile_rows) * p.j_tiles;
+}
+// clusters of this many CTAs that find room at a time, one CTA an SM
+uint32_t at_a_time(uint32_t split, uint32_t sms) { return (split == 8 ? 15u : split == 4 ? 33u : split == 2 ? 74u : 148u) * sms / 148u; }
+
+int launch_as(const char *name, void (*kernel)(CUtensorMap, CUtensorMap, LayerParams), uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, const CUtensorMap &map_w, const CUtensorMap &map_x,
+              const LayerParams &p, cudaStream_t stream)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    SPGK_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, p));
+    return spgk_check_launch(name);
+}
+
+template <uint32_t NT> int launch(const spgk_fp8 *W, const spgk_fp8 *X, LayerParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
+{
+    using L = Shape<NT>;
+    static SpgOncePerDevice once;
+    int rc = once.run(dev, [&]() -> int {
+        SPGK_CUDA(cudaFuncSetAttribute(spg_fp8_layer_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dp.smem_optin));
+        return SPGK_OK;
+    });
+    if (rc) return rc;
+    CUtensorMap map_w, map_x;
+    if ((rc = codes_map(&map_w, W, TM)) || (rc = codes_map(&map_x, X, NT))) return rc;
+    p.j_tiles = (p.out + TM - 1) / TM;
+    const uint32_t sms = (uint32_t)dp.sm_count;
+    const uint64_t tiles = most_tiles(p, NT);
+    if (tiles > 0x3fffffffu) { spgk_set_error("spgk_layer_fp8", "too many tiles"); return SPGK_E_ARG; }
+    p.split = 1;
+    while (p.split < MAX_SPLIT && p.kblocks >= p.split * 4 && tiles <= at_a_time(p.split * 2, sms)) p.split *= 2;
+    const uint32_t fixed = 1024 + HEAD + table_bytes(p.experts) + SF_SLOTS * 2 * SF_TILE + parts_bytes<NT>(p.N, p.split);
+    const uint32_t most = (ROOM - fixed) / L::STAGE;
+    p.stages = most < MAX_STAGES ? most : MAX_STAGES;
+    const uint32_t grid = p.split > 1 ? (uint32_t)tiles * p.split : (tiles < sms ? (uint32_t)tiles : sms);
+    return launch_as("spg_fp8_layer_kernel", spg_fp8_layer_kernel<NT>, grid, THREADS, fixed + p.stages * L::STAGE, p.split, map_w, map_x, p, stream);
+}
+
+int launch_pairs(const spgk_fp8 *W, const spgk_fp8 *X, LayerParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
+{
+    static SpgOncePerDevice once;
+    int rc = once.run(dev, [&]() -> int {
+        SPGK_CUDA(cudaFuncSetAttribute(spg_fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pair_smem(SPGK_MAX_EXPERTS)));
+        return SPGK_OK;
+    });
+    if (rc) return rc;
+    CUtensorMap map_w, map_x;
+    if ((rc = codes_map(&map_w, W, TM)) || (rc = codes_map(&map_x, X, PN / 2))) return rc;
+    p.j_tiles = (p.out + 255) / 256;
+    const uint64_t tiles = most_tiles(p, PN);
+    if (tiles > 0x3fffffffu) { spgk_set_error("spgk_layer_fp8", "too many tiles"); return SPGK_E_ARG; }
+    const uint32_t room = (uint32_t)dp.sm_count / 2, pairs = tiles < room ? (uint32_t)tiles : room;
+    return launch_as("spg_fp8_pair_kernel", spg_fp8_pair_kernel, pairs * 2, P_THREADS, pair_smem(p.experts), 2, map_w, map_x, p, stream);
 }
 
 int refuse(const char *who, const char *why) { spgk_set_error(who, why); return SPGK_E_ARG; }
@@ -131,16 +915,25 @@ int layers(const char *who, const spgk_fp8 *W, uint32_t experts, const float *bi
     if (!status || (uintptr_t)status % 4u) return refuse(who, "no status word");
     if ((uintptr_t)bias % 4u) return refuse(who, "bias not aligned");
     if (X->rows == 0) return SPGK_OK;
+    SpgDeviceProps dp;
+    int dev = 0;
+    if ((rc = spg_device_props(&dp))) return rc;
+    SPGK_CUDA(cudaGetDevice(&dev));
     LayerParams p{};
     p.N = X->rows; p.out = out; p.cols = W->cols; p.experts = experts; p.w_rows = W->rows;
-    p.w = (const uint8_t *)W->codes; p.x = (const uint8_t *)X->codes; p.w_pitch = W->pitch; p.x_pitch = X->pitch;
-    p.w_scales = (const uint8_t *)W->scales; p.x_scales = (const uint8_t *)X->scales;
-    p.starts = starts; p.bias = bias; p.act = act; p.y = y; p.type = type; p.ldy = ldy;
+    p.kblocks = (W->cols + KB - 1) / KB;
+    p.w_words = (const uint32_t *)W->scales; p.x_words = (const uint32_t *)X->scales;
+    p.starts = starts; p.bias = bias; p.act = act; p.y = y; p.type = type; p.ldy = ldy; p.status = status;
     if (next) { p.next_codes = (uint8_t *)next->codes; p.next_scales = (uint8_t *)next->scales; p.next_pitch = next->pitch; }
-    const uint64_t tiles = (uint64_t)p.N / TN + (experts < p.N ? experts : p.N) + 1;
-    if (tiles > 65535u) return refuse(who, "too many tiles of rows");
-    SPGK_CUDA(spg_launch_chained(spg_fp8_layer_kernel, dim3((out + TM - 1) / TM, (uint32_t)tiles), dim3(THREADS), 0, (cudaStream_t)stream, p));
-    return spgk_check_launch("spg_fp8_layer_kernel");
+    p.impatient = spg_gemm_impatient();
+    cudaStream_t st = (cudaStream_t)stream;
+    const uint32_t each = p.N / experts + (p.N % experts != 0);                 // rows of a group, on average
+    const uint32_t nt = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : each <= 128 ? 128 : 256;
+    if (nt <= 16) return launch<16>(W, X, p, dp, dev, st);
+    if (nt <= 32) return launch<32>(W, X, p, dp, dev, st);
+    if (nt <= 64) return launch<64>(W, X, p, dp, dev, st);
+    if (nt <= 128) return launch<128>(W, X, p, dp, dev, st);
+    return launch_pairs(W, X, p, dp, dev, st);
 }
 
 }  // namespace
