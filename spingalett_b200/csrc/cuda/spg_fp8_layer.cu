@@ -571,7 +571,7 @@ constexpr uint32_t P_STAGE = W_BYTES + PN / 2 * KB;
 constexpr uint32_t P_STAGES = 6;
 constexpr uint32_t P_WORDS = 3 * SF_TILE;                       // of 128 units and 256 rows
 constexpr uint32_t P_SF = PN, P_SFX = 4, P_SF_COLS = 16;        // columns of tensor memory: scales behind the sums, twice; those of the rows behind the weights'
-constexpr uint32_t P_BAND = 8;
+constexpr uint32_t P_BAND = 12;
 __host__ __device__ constexpr uint32_t pair_smem(uint32_t experts) { return 1024 + HEAD + table_bytes(experts) + SF_SLOTS * P_WORDS + P_STAGES * P_STAGE; }
 
 __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LayerParams p)

@@ -4,17 +4,20 @@
 //   order  : place(n, j) = starts[e] + how many pairs in front of (n, j), in the order of the rows, have the same expert e = chosen[n][j]
 //   sum    : out[n] = sum_j gate[n][j] * y[place[n][j]]
 //
-// A warp has a row of logits, up to 32 a lane, and takes its largest out one after the other.  The order is a counting sort by one cluster of up to eight
-// blocks: warps count their part of the pairs, what is in front of a warp is summed up in shared memory, what is in front of a block over the cluster, and
-// each warp walks its part once more.  Neither hangs on the order in which anything runs.
+// A warp has a row of logits, up to 32 a lane, and takes its largest out one after the other.  The order is a counting sort that hangs on nothing's timing.  Few rows go
+// through one block of threads, choice and order.  More rows are cut into parts: as each part's choice is made its pairs are counted by expert, one cluster sums the counts up over the
+// parts and experts, and then each part finds its pairs' places from where its experts begin.  The counts lie in the memory of the results on the way: in that of the order,
+// which is written last, and where a part's experts begin in that of its places, which only this part reads and writes.
 #include "spg_fp8.cuh"
 
 namespace {
 
 using namespace spgfp8;
 
-constexpr uint32_t CHOOSE_THREADS = 256;
-constexpr uint32_t SORT_WARPS = 32, SORT_THREADS = 32 * SORT_WARPS, SORT_CLUSTER = 8;
+constexpr uint32_t CHOOSE_THREADS = 512, CHOOSE_WARPS = CHOOSE_THREADS / 32u;
+constexpr uint32_t THREADS = 256, WARPS = THREADS / 32u, LEAST = 64;       // of a part: its order's threads, and the pairs that it has at least
+constexpr uint32_t ONE_THREADS = 1024, ONE_WARPS = ONE_THREADS / 32u, ONE_PAIRS = 4096, ONE_ROWS = 128, ONE_V = 8;   // where one block of threads has all rows, or all pairs
+constexpr uint32_t SUM_THREADS = 1024, SUM_CLUSTER = 8;
 
 // order of floats as that of unsigned numbers; -infinity comes lowest, above 0, which no logit has
 __device__ __forceinline__ uint32_t key_of(float v)
@@ -23,63 +26,246 @@ __device__ __forceinline__ uint32_t key_of(float v)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
-constexpr uint32_t KEY_CLOSED = 0x007fffffu;                    // of -infinity
+__device__ __forceinline__ float closed() { return __int_as_float(0xff800000); }
 
-// one row by one warp; V: logits a lane
-template <typename T, uint32_t V>
-__device__ __forceinline__ void choose(const T *row, uint32_t experts, uint32_t top_k, bool normalise, int32_t *chosen, float *gates, uint32_t lane)
+// V neighbouring logits from e0 on (-infinity beyond the last, and for a NaN); vec: rows lie on what a lane reads
+template <typename T, uint32_t V> __device__ __forceinline__ void load_logits(const T *row, uint32_t e0, uint32_t experts, bool vec, float (&l)[V])
 {
-    uint32_t key[V];
-    uint32_t most = 0;
+    constexpr uint32_t bytes = V * sizeof(T), word = bytes >= 16 ? 16 : bytes;
+    alignas(16) T t[V];
+    if (vec && e0 + V <= experts) {
 #pragma unroll
-    for (uint32_t i = 0; i < V; i++) {
-        const uint32_t e = i * 32u + lane;
-        float l = e < experts ? to_f32(row[e]) : __int_as_float(0xff800000);
-        l = l == l ? l + 0.0f : __int_as_float(0xff800000);     // (-0 is 0)
-        key[i] = e < experts ? key_of(l) : 0u;
-        most = max(most, key[i]);
+        for (uint32_t i = 0; i < bytes / word; i++) {
+            if constexpr (word == 16) reinterpret_cast<uint4 *>(t)[i] = reinterpret_cast<const uint4 *>(row + e0)[i];
+            else if constexpr (word == 8) reinterpret_cast<uint2 *>(t)[i] = reinterpret_cast<const uint2 *>(row + e0)[i];
+            else if constexpr (word == 4) reinterpret_cast<uint32_t *>(t)[i] = reinterpret_cast<const uint32_t *>(row + e0)[i];
+            else t[i] = row[e0 + i];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < V; i++) l[i] = to_f32(t[i]);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < V; i++) l[i] = e0 + i < experts ? to_f32(row[e0 + i]) : closed();
     }
-    const uint32_t first = __reduce_max_sync(0xffffffffu, most);
-    const float m = value_of(first);
-    const auto weight = [&](uint32_t k) { return k == first ? 1.0f : k <= KEY_CLOSED ? 0.0f : expf(value_of(k) - m); };
-    float total = 0.0f;
-    if (!normalise) {
 #pragma unroll
-        for (uint32_t i = 0; i < V; i++) total += weight(key[i]);
-        total = spg_warp_sum(total);
-    }
-    int32_t mine = -1;
-    float w = 0.0f;
-    for (uint32_t j = 0; j < top_k; j++) {
-        uint32_t best = 0, at = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < V; i++) if (key[i] > best) { best = key[i]; at = i; }
-        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-        if (top <= KEY_CLOSED) break;
-        const uint32_t e = __reduce_min_sync(0xffffffffu, best == top ? at * 32u + lane : 0xffffffffu);
-#pragma unroll
-        for (uint32_t i = 0; i < V; i++) if (i * 32u + lane == e) key[i] = 0;
-        const float v = weight(top);
-        if (normalise) total += v;
-        if (lane == j) { mine = (int32_t)e; w = v; }
-    }
-    if (lane < top_k) { chosen[lane] = mine; gates[lane] = mine >= 0 ? w / total : 0.0f; }
+    for (uint32_t i = 0; i < V; i++) l[i] = fmaxf(l[i], closed()) + 0.0f;                         // (the larger of a NaN and another is the other; -0 is 0)
 }
 
-template <typename T, uint32_t V>
-__global__ void __launch_bounds__(CHOOSE_THREADS) spg_route_choose_kernel(const T *logits, uint32_t ld, uint32_t N, uint32_t experts, uint32_t top_k, int normalise, int32_t *chosen, float *gates)
+// Falling order in a lane: exchanges whose places are known when this is compiled (Batcher's merges of odd and even places).  Equal keys change places only
+// where LATER, the index behind the key, says so.
+template <uint32_t V, bool LATER> __device__ __forceinline__ void sort_lane(uint32_t (&key)[V], uint32_t (&at)[V])
 {
+#pragma unroll
+    for (uint32_t run = 1; run < V; run *= 2)
+#pragma unroll
+        for (uint32_t gap = run; gap >= 1; gap /= 2)
+#pragma unroll
+            for (uint32_t j = gap % run; j + gap < V; j += 2 * gap)
+#pragma unroll
+                for (uint32_t i = 0; i < gap; i++) {
+                    const uint32_t a = i + j, b = i + j + gap;
+                    if (b >= V || a / (2 * run) != b / (2 * run)) continue;
+                    if constexpr (!LATER) {
+                        const uint32_t hi = max(key[a], key[b]), lo = min(key[a], key[b]);
+                        key[a] = hi; key[b] = lo;
+                    } else {
+                        const bool turn = key[b] > key[a] || (key[b] == key[a] && at[b] < at[a]);
+                        const uint32_t k = key[a], n = at[a];
+                        key[a] = turn ? key[b] : k; key[b] = turn ? k : key[b];
+                        at[a] = turn ? at[b] : n; at[b] = turn ? n : at[b];
+                    }
+                }
+}
+
+// One row by one warp: lane j's expert and gate (-1, 0 where there are fewer).  V: logits a lane, whose order it makes first; then the largest of the lanes' first is the next,
+// top_k times.  16-bit logits are searched as keys with the index behind them, so that the maximum over the warp names the expert too; of 32-bit ones that are equal the first
+// lane's is the first.
+template <typename T, uint32_t V>
+__device__ __forceinline__ int32_t choose(const T *row, uint32_t experts, uint32_t top_k, bool normalise, bool vec, uint32_t lane, float &gate)
+{
+    constexpr bool SHORT = sizeof(T) == 2;
+    float l[V];
+    load_logits<T, V>(row, lane * V, experts, vec, l);
+    uint32_t key[V], at[V];
+#pragma unroll
+    for (uint32_t i = 0; i < V; i++) {
+        const uint32_t e = lane * V + i;
+        at[i] = e;
+        if constexpr (SHORT) {
+            const T t = from_f32<T>(l[i]);
+            const uint32_t b = *reinterpret_cast<const uint16_t *>(&t);
+            key[i] = (b ^ (b & 0x8000u ? 0xffffu : 0x8000u)) << 16 | (0xffffu - e);
+        } else key[i] = key_of(l[i]);
+    }
+    const auto of = [](uint32_t k) {
+        if constexpr (SHORT) {
+            const uint16_t b = (uint16_t)(k & 0x80000000u ? k >> 16 & 0x7fffu : ~(k >> 16));
+            return to_f32(*reinterpret_cast<const T *>(&b));
+        } else return value_of(k);
+    };
+    // the largest logit, of which all weights are fractions
+    uint32_t most = key[0];
+#pragma unroll
+    for (uint32_t i = 1; i < V; i++) most = max(most, key[i]);
+    const float m = of(__reduce_max_sync(0xffffffffu, most));
+    float total = 0.0f;
+    if (!normalise) {
+        if (m < __int_as_float(0x7f800000)) {
+#pragma unroll
+            for (uint32_t i = 0; i < V; i++) total += expf(l[i] - m);             // (0 for those closed; where all are, nobody asks)
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < V; i++) total += l[i] == m ? 1.0f : 0.0f;
+        }
+        total = spg_warp_sum(total);
+    }
+    sort_lane<V, !SHORT>(key, at);
+    uint32_t mine = 0, place = 0;
+    for (uint32_t j = 0; j < top_k; j++) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, key[0]);
+        bool first = key[0] == top;
+        uint32_t e = 0;
+        if constexpr (!SHORT) {
+            const uint32_t lanes = __ballot_sync(0xffffffffu, first), one = __ffs(lanes) - 1;
+            e = __shfl_sync(0xffffffffu, at[0], one);
+            first = lane == one;
+        }
+        if (lane == j) { mine = top; place = e; }
+        if (first) {
+#pragma unroll
+            for (uint32_t i = 0; i + 1 < V; i++) { key[i] = key[i + 1]; at[i] = at[i + 1]; }
+            key[V - 1] = 0;
+        }
+    }
+    const float best = of(mine);
+    const bool open = lane < top_k && best > closed();                            // (no key: a NaN)
+    const float w = !open ? 0.0f : best == m ? 1.0f : expf(best - m);
+    if (normalise) total = spg_warp_sum(w);
+    gate = open ? w / total : 0.0f;
+    return open ? (int32_t)(SHORT ? 0xffffu - (mine & 0xffffu) : place) : -1;
+}
+
+// Where the `count` pairs in `chosen` (shared memory), the first of them pair `first` of all, go: each behind those of its expert that come earlier; place[e] is that of the expert's
+// first.  counts: `warps` times `experts` words; pairs: of all parts.  All threads of the block call it; `warps` of them have a run of pairs each.
+// (What was written to the results' memory on the way is read back here: calls that wrongly share it read one another's, so nothing is indexed by it unchecked.)
+__device__ __forceinline__ void order_pairs(const int32_t *chosen, uint32_t count, uint32_t first, uint32_t pairs, const uint32_t *place, uint32_t *counts, uint32_t warps, uint32_t experts, uint32_t top_k,
+                                            int32_t *order, int32_t *places)
+{
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, turns = (count + 31u) / 32u, per = (turns + warps - 1) / warps;
+    const uint32_t lo = warp < warps ? min(turns, warp * per) * 32u : turns * 32u, hi = warp < warps ? min(count, lo + per * 32u) : 0u;
+    uint32_t *mine = counts + warp * experts;
+    for (uint32_t i = threadIdx.x; i < warps * experts; i += blockDim.x) counts[i] = 0;
+    __syncthreads();
+    for (uint32_t i = lo + lane; i < hi; i += 32u) {
+        const uint32_t e = (uint32_t)chosen[i];
+        if (e < experts) atomicAdd(mine + e, 1u);
+    }
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x) {
+        uint32_t at = place[e];
+        for (uint32_t w = 0; w < warps; w++) { const uint32_t c = counts[w * experts + e]; counts[w * experts + e] = at; at += c; }
+    }
+    __syncthreads();
+    for (uint32_t i0 = lo; i0 < hi; i0 += 32u) {
+        const uint32_t i = i0 + lane;
+        const uint32_t e = i < hi ? (uint32_t)chosen[i] : 0xffffffffu;
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        const uint32_t at = e < experts ? mine[e] + __popc(same & ((1u << lane) - 1u)) : 0u;
+        __syncwarp();
+        if (e < experts && (same >> lane) == 1u) mine[e] = at + 1u;              // (the last of its kind)
+        __syncwarp();
+        if (i < hi) places[first + i] = e < experts ? (int32_t)at : -1;
+        if (e < experts && at < pairs) order[at] = (int32_t)((first + i) / top_k);
+    }
+}
+
+// Sum over the threads in front and over all, of one value a thread (sums: a word for each of the block's warps)
+__device__ __forceinline__ uint32_t scan_block(uint32_t v, uint32_t *sums, uint32_t &all)
+{
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+    uint32_t upto = v;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) { const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += u; }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    uint32_t front = 0;
+    all = 0;
+    for (uint32_t w = 0; w < blockDim.x / 32u; w++) { const uint32_t s = sums[w]; if (w < warp) front += s; all += s; }
+    return front + upto - v;
+}
+
+// Few rows, choice and order; or, with `made`, the order alone (of more than 256 experts always: a row's logits need more registers than so many threads have).  Shared memory: chosen, counts of the warps, places of the experts
+template <typename T, uint32_t V>
+__global__ void __launch_bounds__(ONE_THREADS) spg_route_one_kernel(const T *logits, uint32_t ld, uint32_t N, uint32_t experts, uint32_t top_k, int normalise, bool vec, bool made, uint32_t warps,
+                                                                    int32_t *chosen, float *gates, int32_t *starts, int32_t *order, int32_t *places)
+{
+    extern __shared__ uint32_t sh[];
+    __shared__ uint32_t sums[ONE_WARPS];
+    const uint32_t pairs = N * top_k, warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+    int32_t *mine = reinterpret_cast<int32_t *>(sh);
+    uint32_t *counts = sh + (pairs + 31u) / 32u * 32u, *place = counts + warps * experts;
     spg_grid_trigger();
+    for (uint32_t e = threadIdx.x; e < experts; e += ONE_THREADS) place[e] = 0;
     spg_grid_wait();
-    const uint32_t n = blockIdx.x * (CHOOSE_THREADS / 32u) + threadIdx.x / 32u;
-    if (n < N) choose<T, V>(logits + (uint64_t)n * ld, experts, top_k, normalise, chosen + (uint64_t)n * top_k, gates + (uint64_t)n * top_k, threadIdx.x % 32u);
+    __syncthreads();
+    if (made) {
+        for (uint32_t i = threadIdx.x; i < pairs; i += ONE_THREADS) {
+            const int32_t e = chosen[i];
+            mine[i] = e;
+            if ((uint32_t)e < experts) atomicAdd(place + e, 1u);
+        }
+    } else if constexpr (V <= ONE_V) {
+        for (uint32_t n = warp; n < N; n += ONE_WARPS) {
+            float gate;
+            const int32_t e = choose<T, V>(logits + (uint64_t)n * ld, experts, top_k, normalise, vec, lane, gate);
+            if (lane < top_k) {
+                const uint32_t i = n * top_k + lane;
+                chosen[i] = mine[i] = e;
+                gates[i] = gate;
+                if (e >= 0) atomicAdd(place + e, 1u);
+            }
+        }
+    }
+    __syncthreads();
+    uint32_t all;
+    const uint32_t begin = scan_block(threadIdx.x < experts ? place[threadIdx.x] : 0u, sums, all);
+    if (threadIdx.x < experts) { place[threadIdx.x] = begin; starts[threadIdx.x] = (int32_t)begin; }
+    if (threadIdx.x == 0) starts[experts] = (int32_t)all;
+    __syncthreads();
+    order_pairs(mine, pairs, 0, pairs, place, counts, warps, experts, top_k, order, places);
+    for (uint32_t i = all + threadIdx.x; i < pairs; i += ONE_THREADS) order[i] = -1;
+}
+
+// A part's choice (rows `share` times blockIdx.x on; the last part has the rest), and how many of its pairs each expert has
+template <typename T, uint32_t V>
+__global__ void __launch_bounds__(CHOOSE_THREADS) spg_route_choose_kernel(const T *logits, uint32_t ld, uint32_t N, uint32_t experts, uint32_t top_k, int normalise, bool vec, uint32_t share, bool count,
+                                                                   int32_t *chosen, float *gates, uint32_t *counts)
+{
+    extern __shared__ uint32_t sh[];
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, lo = blockIdx.x * share, hi = blockIdx.x + 1 == gridDim.x ? N : lo + share;
+    spg_grid_trigger();
+    if (count) for (uint32_t e = threadIdx.x; e < experts; e += CHOOSE_THREADS) sh[e] = 0;
+    spg_grid_wait();
+    __syncthreads();
+    for (uint32_t n = lo + warp; n < hi; n += CHOOSE_WARPS) {
+        float gate;
+        const int32_t e = choose<T, V>(logits + (uint64_t)n * ld, experts, top_k, normalise, vec, lane, gate);
+        if (lane < top_k) {
+            chosen[n * top_k + lane] = e;
+            gates[n * top_k + lane] = gate;
+            if (count && e >= 0) atomicAdd(sh + e, 1u);
+        }
+    }
+    if (!count) return;
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < experts; e += CHOOSE_THREADS) counts[(uint64_t)blockIdx.x * experts + e] = sh[e];
 }
 
 __device__ __forceinline__ uint32_t ld_cluster(const uint32_t *here, uint32_t rank)
 {
     uint32_t addr = (uint32_t)__cvta_generic_to_shared(here), v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
     return v;
 }
 __device__ __forceinline__ void cluster_sync()
@@ -89,107 +275,151 @@ __device__ __forceinline__ void cluster_sync()
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// shared memory: [SORT_WARPS][experts] pairs in front of a warp, [experts] pairs of the block, [experts] first places, [SORT_WARPS] sums of warps
-__global__ void __launch_bounds__(SORT_THREADS) spg_route_order_kernel(const int32_t *chosen, uint32_t pairs, uint32_t experts, uint32_t top_k, int32_t *starts, int32_t *order, int32_t *places)
+// Counts [parts][experts] to where each part's pairs of each expert begin (first[part * stride + expert]), and where each expert's do.  A cluster: its blocks have the parts in
+// runs, a block's threads an expert each and, where there are few experts, a run of the block's parts.
+__global__ void __launch_bounds__(SUM_THREADS) spg_route_sum_kernel(const uint32_t *counts, uint32_t parts, uint32_t experts, uint32_t wide, uint32_t stride, uint32_t *first, int32_t *starts)
 {
-    extern __shared__ uint32_t sh[];
-    uint32_t *counts = sh, *all = counts + SORT_WARPS * experts, *base = all + experts, *sums = base + experts;
-    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = blockIdx.x, blocks = gridDim.x;
+    __shared__ uint32_t run[SUM_THREADS], all[SPGK_MAX_EXPERTS], begin[SPGK_MAX_EXPERTS], sums[SUM_THREADS / 32u];
+    const uint32_t rank = blockIdx.x, e = threadIdx.x % wide, slice = threadIdx.x / wide, slices = SUM_THREADS / wide;      // wide: experts, up to a whole warp
+    const uint32_t per = (parts + SUM_CLUSTER * slices - 1) / (SUM_CLUSTER * slices), lo = min(parts, (rank * slices + slice) * per), hi = e < experts && slice < slices ? min(parts, lo + per) : lo;
+    constexpr uint32_t KEPT = 16;                                // of a run, on their way at a time and at hand the second time
+    uint32_t c[KEPT];
+    const auto load = [&](uint32_t b0) {
+#pragma unroll
+        for (uint32_t i = 0; i < KEPT; i++) c[i] = b0 + i < hi ? counts[(uint64_t)(b0 + i) * experts + e] : 0u;
+    };
     spg_grid_trigger();
-    for (uint32_t i = threadIdx.x; i < SORT_WARPS * experts; i += SORT_THREADS) counts[i] = 0;
-    __syncthreads();
     spg_grid_wait();
-    // this warp's pairs: whole turns of 32
-    const uint32_t turns = (pairs + 31u) / 32u, per = (turns + blocks * SORT_WARPS - 1) / (blocks * SORT_WARPS);
-    const uint32_t lo = min(turns, (rank * SORT_WARPS + warp) * per) * 32u, hi = min(pairs, lo + per * 32u);
-    uint32_t *mine = counts + warp * experts;
-    for (uint32_t i = lo + lane; i < hi; i += 32u) {
-        const int32_t e = chosen[i];
-        if (e >= 0) atomicAdd(mine + e, 1u);
+    uint32_t sum = 0;
+    for (uint32_t b = lo; b < hi; b += KEPT) {
+        load(b);
+#pragma unroll
+        for (uint32_t i = 0; i < KEPT; i++) sum += c[i];
     }
+    run[threadIdx.x] = sum;
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < experts; e += SORT_THREADS) {
-        uint32_t sum = 0;
-        for (uint32_t w = 0; w < SORT_WARPS; w++) { const uint32_t c = counts[w * experts + e]; counts[w * experts + e] = sum; sum += c; }
-        all[e] = sum;
+    if (threadIdx.x < experts) {
+        uint32_t upto = 0;
+#pragma unroll 4
+        for (uint32_t s = 0; s < slices; s++) { const uint32_t v = run[s * wide + threadIdx.x]; run[s * wide + threadIdx.x] = upto; upto += v; }
+        all[threadIdx.x] = upto;
     }
     cluster_sync();
-    // first places: the experts in front (a scan; thread e has expert e), then the blocks in front
-    uint32_t before = 0, whole = 0;
-    if (threadIdx.x < experts)
-        for (uint32_t r = 0; r < blocks; r++) {
-            const uint32_t c = ld_cluster(all + threadIdx.x, r);
-            whole += c;
-            if (r < rank) before += c;
-        }
-    uint32_t upto = whole;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) { const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += v; }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    uint32_t front = 0, total = 0;
-    for (uint32_t w = 0; w < SORT_WARPS; w++) { const uint32_t s = sums[w]; if (w < warp) front += s; total += s; }
+    uint32_t before = 0, whole = 0, total;
     if (threadIdx.x < experts) {
-        base[threadIdx.x] = front + upto - whole + before;
-        if (rank == 0) starts[threadIdx.x] = (int32_t)(front + upto - whole);
+        uint32_t v[SUM_CLUSTER];
+#pragma unroll
+        for (uint32_t r = 0; r < SUM_CLUSTER; r++) v[r] = ld_cluster(all + threadIdx.x, r);
+#pragma unroll
+        for (uint32_t r = 0; r < SUM_CLUSTER; r++) { whole += v[r]; if (r < rank) before += v[r]; }
+    }
+    const uint32_t at = scan_block(whole, sums, total);
+    if (threadIdx.x < experts) {
+        begin[threadIdx.x] = at + before;
+        if (rank == 0) starts[threadIdx.x] = (int32_t)at;
     }
     if (rank == 0 && threadIdx.x == 0) starts[experts] = (int32_t)total;
     __syncthreads();
-    for (uint32_t i0 = lo; i0 < hi; i0 += 32u) {
-        const uint32_t i = i0 + lane;
-        const int32_t e = i < hi ? chosen[i] : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        uint32_t at = 0;
-        if (e >= 0) at = base[e] + mine[e] + __popc(same & ((1u << lane) - 1u));
-        __syncwarp();
-        if (e >= 0 && (same >> lane) == 1u) mine[e] += __popc(same);              // (the last of its kind)
-        __syncwarp();
-        if (i < hi) places[i] = e >= 0 ? (int32_t)at : -1;
-        if (e >= 0) order[at] = (int32_t)(i / top_k);
+    if (lo < hi) {
+        uint32_t upto = begin[e] + run[slice * wide + e];
+        for (uint32_t b = lo; b < hi; b += KEPT) {
+            if (per > KEPT) load(b);
+#pragma unroll
+            for (uint32_t i = 0; i < KEPT; i++) if (b + i < hi) { first[(uint64_t)(b + i) * stride + e] = upto; upto += c[i]; }
+        }
     }
-    for (uint32_t i = total + rank * SORT_THREADS + threadIdx.x; i < pairs; i += blocks * SORT_THREADS) order[i] = -1;
     cluster_sync();                                              // (the others may still read this block's sums)
 }
 
-// A thread has 16 bytes of a row's output, or one element where rows do not lie on 16 bytes.
-template <typename T, typename O, uint32_t W>
-__global__ void __launch_bounds__(256) spg_combine_kernel(const T *y, uint32_t ldy, uint32_t y_rows, const int32_t *places, const float *gates, uint32_t N, uint32_t top_k, uint32_t width,
+// A part's pairs to their places.  Shared memory: chosen, counts of the warps, places of the experts
+__global__ void __launch_bounds__(THREADS) spg_route_order_kernel(const int32_t *chosen, uint32_t N, uint32_t experts, uint32_t top_k, uint32_t share, const int32_t *starts, int32_t *order, int32_t *places)
+{
+    extern __shared__ uint32_t sh[];
+    const uint32_t lo = blockIdx.x * share * top_k, pairs = N * top_k, count = (blockIdx.x + 1 == gridDim.x ? pairs : lo + share * top_k) - lo;
+    int32_t *mine = reinterpret_cast<int32_t *>(sh);
+    uint32_t *counts = sh + (count + 31u) / 32u * 32u, *place = counts + WARPS * experts;
+    spg_grid_trigger();
+    spg_grid_wait();
+    for (uint32_t i = threadIdx.x; i < count; i += THREADS) mine[i] = chosen[lo + i];
+    for (uint32_t e = threadIdx.x; e < experts; e += THREADS) place[e] = (uint32_t)places[lo + e];     // (where the sums left them; this part's places go there)
+    __syncthreads();
+    order_pairs(mine, count, lo, pairs, place, counts, WARPS, experts, top_k, order, places);
+    for (uint64_t i = (uint64_t)(uint32_t)starts[experts] + blockIdx.x * THREADS + threadIdx.x; i < pairs; i += gridDim.x * THREADS) order[i] = -1;
+}
+
+// A thread has U times W neighbouring columns of a row: W are 16 bytes of the narrower type, or one where rows do not lie on 16 bytes; U is 1, and the rows' pieces
+// go to threads one behind the other, or 2 or 4 where a row has enough of them for a block of threads of its own.  ROWS of the rows that are added up are on their way at a time.
+// What bounds it is how many bytes are: a place, then the rows, then the sum is a way of three latencies.  us with U = 1, 2 and 4: 16384 x 2 rows of 8192 bf16 163, 126 and 120
+// (6.7 TB/s; 145 through the caches as usual), 4096 x 2 of 4096 19.7, 14.2 and, half of the threads idle, 19.3.
+template <typename T, typename O, uint32_t W, uint32_t U, uint32_t ROWS>
+__global__ void __launch_bounds__(256) spg_combine_kernel(const T *y, uint32_t ldy, uint32_t y_rows, const int32_t *places, const float *gates, uint32_t N, uint32_t top_k,
                                                           O *out, uint32_t ldo, uint32_t pieces)
 {
     spg_grid_trigger();
     spg_grid_wait();
-    const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
-    const uint32_t n = (uint32_t)(i / pieces), c = (uint32_t)(i % pieces) * W;
+    uint32_t n, first;                                           // the row, and the first of this thread's pieces, the next 256 from it
+    if constexpr (U == 1) {
+        const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+        if (i >> 32) { n = (uint32_t)(i / pieces); first = (uint32_t)(i % pieces); }
+        else { n = (uint32_t)i / pieces; first = (uint32_t)i % pieces; }
+    } else {
+        const uint32_t blocks = (pieces - 1) / (256u * U) + 1;
+        n = blockIdx.x / blocks; first = blockIdx.x % blocks * 256u * U + threadIdx.x;
+    }
     if (n >= N) return;
-    float v[W];
+    float v[U][W];
 #pragma unroll
-    for (uint32_t q = 0; q < W; q++) v[q] = 0.0f;
-    for (uint32_t j = 0; j < top_k; j++) {
-        const uint32_t p = (uint32_t)places[(uint64_t)n * top_k + j];
-        if (p >= y_rows) continue;
-        const float g = gates[(uint64_t)n * top_k + j];
-        const T *row = y + (uint64_t)p * ldy + c;
-        alignas(16) T t[W];
-        if constexpr (W * sizeof(T) % 16 == 0) {
+    for (uint32_t u = 0; u < U; u++)
 #pragma unroll
-            for (uint32_t q = 0; q < W * sizeof(T) / 16; q++) reinterpret_cast<uint4 *>(t)[q] = reinterpret_cast<const uint4 *>(row)[q];
-        } else {
+        for (uint32_t q = 0; q < W; q++) v[u][q] = 0.0f;
+    for (uint32_t j = 0; j < top_k; j += ROWS) {
+        alignas(16) T t[ROWS][U][W];
+        float g[ROWS];
+        bool there[ROWS];
 #pragma unroll
-            for (uint32_t q = 0; q < W; q++) t[q] = row[q];
+        for (uint32_t k = 0; k < ROWS; k++) {
+            const uint64_t at = (uint64_t)n * top_k + j + k;
+            const uint32_t p = j + k < top_k ? (uint32_t)places[at] : 0xffffffffu;
+            there[k] = p < y_rows;
+            g[k] = there[k] ? gates[at] : 0.0f;
+            const T *row = y + (uint64_t)(there[k] ? p : 0u) * ldy;
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++) {
+                const uint32_t c = (first + u * 256u) * W;
+                if (!there[k] || (U > 1 && first + u * 256u >= pieces)) continue;
+                if constexpr (W * sizeof(T) % 16 == 0) {
+#pragma unroll
+                    for (uint32_t q = 0; q < W * sizeof(T) / 16; q++) reinterpret_cast<uint4 *>(t[k][u])[q] = __ldcs(reinterpret_cast<const uint4 *>(row + c) + q);
+                } else {
+#pragma unroll
+                    for (uint32_t q = 0; q < W; q++) t[k][u][q] = row[c + q];
+                }
+            }
         }
 #pragma unroll
-        for (uint32_t q = 0; q < W; q++) v[q] = fmaf(g, to_f32(t[q]), v[q]);
+        for (uint32_t k = 0; k < ROWS; k++) {
+            if (!there[k]) continue;
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++)
+#pragma unroll
+                for (uint32_t q = 0; q < W; q++) v[u][q] = fmaf(g[k], to_f32(t[k][u][q]), v[u][q]);
+        }
     }
-    O *dst = out + (uint64_t)n * ldo + c;
-    alignas(16) O o[W];
 #pragma unroll
-    for (uint32_t q = 0; q < W; q++) o[q] = from_f32<O>(v[q]);
-    if constexpr (W * sizeof(O) % 16 == 0) {
+    for (uint32_t u = 0; u < U; u++) {
+        const uint32_t c = (first + u * 256u) * W;
+        if (U > 1 && first + u * 256u >= pieces) continue;
+        O *dst = out + (uint64_t)n * ldo + c;
+        alignas(16) O o[W];
 #pragma unroll
-        for (uint32_t q = 0; q < W * sizeof(O) / 16; q++) reinterpret_cast<uint4 *>(dst)[q] = reinterpret_cast<const uint4 *>(o)[q];
-    } else {
+        for (uint32_t q = 0; q < W; q++) o[q] = from_f32<O>(v[u][q]);
+        if constexpr (W * sizeof(O) % 16 == 0) {
 #pragma unroll
-        for (uint32_t q = 0; q < W; q++) dst[q] = o[q];
+            for (uint32_t q = 0; q < W * sizeof(O) / 16; q++) __stcs(reinterpret_cast<uint4 *>(dst) + q, reinterpret_cast<const uint4 *>(o)[q]);
+        } else {
+#pragma unroll
+            for (uint32_t q = 0; q < W; q++) dst[q] = o[q];
+        }
     }
 }
 
@@ -197,19 +427,69 @@ int refuse(const char *who, const char *why) { spgk_set_error(who, why); return 
 bool known(int type) { return type == SPGK_T_F16 || type == SPGK_T_BF16 || type == SPGK_T_F32; }
 uint32_t size_of(int type) { return type == SPGK_T_F32 ? 4u : 2u; }
 
-template <typename T, uint32_t V>
-int choose_all(const void *logits, uint32_t ld, uint32_t N, uint32_t experts, uint32_t top_k, int normalise, int32_t *chosen, float *gates, cudaStream_t stream)
+struct Route {
+    uint32_t ld, N, experts, top_k; int normalise;
+    int32_t *chosen; float *gates; int32_t *starts, *order, *places;
+    int dev; cudaStream_t stream;
+};
+constexpr size_t ONE_SMEM = ((size_t)ONE_PAIRS + (size_t)ONE_WARPS * SPGK_MAX_EXPERTS + SPGK_MAX_EXPERTS) * 4u;
+
+// One block of threads has all rows, or only all pairs; or rows in parts of as many pairs as there are experts at least (their counts lie in the memory of the pairs' results)
+template <typename T, uint32_t V> int route(const void *logits, const Route &r)
 {
-    constexpr uint32_t rows = CHOOSE_THREADS / 32u;
-    SPGK_CUDA(spg_launch_chained(spg_route_choose_kernel<T, V>, dim3((N + rows - 1) / rows), dim3(CHOOSE_THREADS), 0, stream, (const T *)logits, ld, N, experts, top_k, normalise, chosen, gates));
-    return spgk_check_launch("spg_route_choose_kernel");
+    const uint32_t pairs = r.N * r.top_k, share = ((r.experts > LEAST ? r.experts : LEAST) + r.top_k - 1) / r.top_k, parts = r.N / share;
+    const bool vec = (uintptr_t)logits % 16 == 0 && (uint64_t)r.ld * sizeof(T) % 16 == 0, few = r.N <= ONE_ROWS && V <= ONE_V, one = pairs <= ONE_PAIRS || parts == 0;
+    const T *x = (const T *)logits;
+    if (!one || !few) {
+        constexpr uint32_t rows = CHOOSE_WARPS;
+        SPGK_CUDA(spg_launch_chained(spg_route_choose_kernel<T, V>, dim3(one ? (r.N + rows - 1) / rows : parts), dim3(CHOOSE_THREADS), one ? 0 : r.experts * 4u, r.stream,
+                                     x, r.ld, r.N, r.experts, r.top_k, r.normalise, vec, one ? rows : share, !one, r.chosen, r.gates, (uint32_t *)r.order));
+        const int rc = spgk_check_launch("spg_route_choose_kernel");
+        if (rc) return rc;
+    }
+    if (one) {
+        static SpgOncePerDevice once;
+        const int rc = once.run(r.dev, [&]() -> int {
+            SPGK_CUDA(cudaFuncSetAttribute(spg_route_one_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ONE_SMEM));
+            return SPGK_OK;
+        });
+        if (rc) return rc;
+        const uint32_t turns = (pairs + 31u) / 32u, warps = turns < 1 ? 1 : turns < ONE_WARPS ? turns : ONE_WARPS;
+        SPGK_CUDA(spg_launch_chained(spg_route_one_kernel<T, V>, dim3(1), dim3(ONE_THREADS), ((size_t)turns * 32u + (size_t)(warps + 1) * r.experts) * 4u, r.stream,
+                                     x, r.ld, r.N, r.experts, r.top_k, r.normalise, vec, !few, warps, r.chosen, r.gates, r.starts, r.order, r.places));
+        return spgk_check_launch("spg_route_one_kernel");
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(SUM_CLUSTER); cfg.blockDim = dim3(SUM_THREADS); cfg.stream = r.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = SUM_CLUSTER; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    SPGK_CUDA(cudaLaunchKernelEx(&cfg, spg_route_sum_kernel, (const uint32_t *)r.order, parts, r.experts, (r.experts + 31u) / 32u * 32u, share * r.top_k, (uint32_t *)r.places, r.starts));
+    int rc = spgk_check_launch("spg_route_sum_kernel");
+    if (rc) return rc;
+    static SpgOncePerDevice once;
+    const size_t most = (2 * (size_t)(SPGK_MAX_EXPERTS + SPGK_ROUTE_MAX_TOP) + 32u + (WARPS + 1) * SPGK_MAX_EXPERTS) * 4u;
+    rc = once.run(r.dev, [&]() -> int {
+        SPGK_CUDA(cudaFuncSetAttribute(spg_route_order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+        return SPGK_OK;
+    });
+    if (rc) return rc;
+    const uint32_t last = (r.N - (parts - 1) * share) * r.top_k;                 // the most pairs of a part
+    SPGK_CUDA(spg_launch_chained(spg_route_order_kernel, dim3(parts), dim3(THREADS), ((size_t)(last + 31u) / 32u * 32u + (size_t)(WARPS + 1) * r.experts) * 4u, r.stream,
+                                 (const int32_t *)r.chosen, r.N, r.experts, r.top_k, share, (const int32_t *)r.starts, r.order, r.places));
+    return spgk_check_launch("spg_route_order_kernel");
 }
-template <typename T>
-int choose_all(const void *logits, uint32_t ld, uint32_t N, uint32_t experts, uint32_t top_k, int normalise, int32_t *chosen, float *gates, cudaStream_t stream)
+template <typename T> int route(const void *logits, const Route &r)
 {
-    if (experts <= 64) return choose_all<T, 2>(logits, ld, N, experts, top_k, normalise, chosen, gates, stream);
-    if (experts <= 256) return choose_all<T, 8>(logits, ld, N, experts, top_k, normalise, chosen, gates, stream);
-    return choose_all<T, 32>(logits, ld, N, experts, top_k, normalise, chosen, gates, stream);
+    if (r.experts <= 32) return route<T, 1>(logits, r);
+    if (r.experts <= 64) return route<T, 2>(logits, r);
+    if (r.experts <= 128) return route<T, 4>(logits, r);
+    if (r.experts <= 256) return route<T, 8>(logits, r);
+    if (r.experts <= 512) return route<T, 16>(logits, r);
+    return route<T, 32>(logits, r);
 }
 
 template <typename T, typename O>
@@ -218,10 +498,12 @@ int combine(const void *y, uint32_t ldy, uint32_t y_rows, const int32_t *places,
     constexpr uint32_t W = 16 / (sizeof(T) < sizeof(O) ? sizeof(T) : sizeof(O));
     const bool wide = width % W == 0 && (uint64_t)ldy * sizeof(T) % 16 == 0 && (uint64_t)ldo * sizeof(O) % 16 == 0 && ((uintptr_t)y | (uintptr_t)out) % 16 == 0;
     const uint32_t pieces = wide ? width / W : width;
-    const uint64_t blocks = ((uint64_t)N * pieces + 255) / 256;
+    const uint32_t over = pieces % 1024u, u = pieces >= 640u && (over == 0 || over >= 640u) ? 4u : pieces >= 384u ? 2u : 1u;
+    const uint64_t blocks = u > 1 ? (uint64_t)N * ((pieces - 1) / (256u * u) + 1) : ((uint64_t)N * pieces + 255) / 256;
     if (blocks > 0x7fffffffu) return refuse("spgk_combine_rows", "too many rows and columns for one call");
-    SPGK_CUDA(spg_launch_chained(wide ? spg_combine_kernel<T, O, W> : spg_combine_kernel<T, O, 1>, dim3((uint32_t)blocks), dim3(256), 0, stream,
-                                 (const T *)y, ldy, y_rows, places, gates, N, top_k, width, (O *)out, ldo, pieces));
+    const auto kernel = wide ? (u == 4 ? spg_combine_kernel<T, O, W, 4, 2> : u == 2 ? spg_combine_kernel<T, O, W, 2, 2> : spg_combine_kernel<T, O, W, 1, 4>)
+                             : (u == 4 ? spg_combine_kernel<T, O, 1, 4, 2> : u == 2 ? spg_combine_kernel<T, O, 1, 2, 2> : spg_combine_kernel<T, O, 1, 1, 4>);
+    SPGK_CUDA(spg_launch_chained(kernel, dim3((uint32_t)blocks), dim3(256), 0, stream, (const T *)y, ldy, y_rows, places, gates, N, top_k, (O *)out, ldo, pieces));
     return spgk_check_launch("spg_combine_kernel");
 }
 template <typename T>
@@ -247,34 +529,11 @@ int spgk_route_rows(const void *logits, int type, uint32_t ld, uint32_t N, uint3
     if (!starts || (N && (!logits || !chosen || !gates || !order || !places))) return refuse(who, "no logits, or no place for a result");
     if ((uintptr_t)logits % size_of(type) || ((uintptr_t)chosen | (uintptr_t)gates | (uintptr_t)starts | (uintptr_t)order | (uintptr_t)places) % 4u) return refuse(who, "not aligned");
     if (N > 1 && ld < experts) return refuse(who, "rows overlap");
-    cudaStream_t st = (cudaStream_t)stream;
-    int rc = SPGK_OK;
-    if (N) {
-        if (type == SPGK_T_F32) rc = choose_all<float>(logits, ld, N, experts, top_k, normalise, chosen, gates, st);
-        else if (type == SPGK_T_F16) rc = choose_all<__half>(logits, ld, N, experts, top_k, normalise, chosen, gates, st);
-        else rc = choose_all<__nv_bfloat16>(logits, ld, N, experts, top_k, normalise, chosen, gates, st);
-        if (rc) return rc;
-    }
-    const uint32_t pairs = N * top_k, cluster = pairs > 4096u ? SORT_CLUSTER : 1u;
-    const size_t bytes = ((size_t)(SORT_WARPS + 2) * experts + SORT_WARPS) * 4u;
-    int dev = 0;
-    SPGK_CUDA(cudaGetDevice(&dev));
-    static SpgOncePerDevice once;
-    rc = once.run(dev, [&]() -> int {
-        SPGK_CUDA(cudaFuncSetAttribute(spg_route_order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(((SORT_WARPS + 2) * SPGK_MAX_EXPERTS + SORT_WARPS) * 4u)));
-        return SPGK_OK;
-    });
-    if (rc) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cluster); cfg.blockDim = dim3(SORT_THREADS); cfg.dynamicSmemBytes = bytes; cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = 2;
-    SPGK_CUDA(cudaLaunchKernelEx(&cfg, spg_route_order_kernel, (const int32_t *)chosen, pairs, experts, top_k, starts, order, places));
-    return spgk_check_launch("spg_route_order_kernel");
+    Route r = { ld, N, experts, top_k, normalise, chosen, gates, starts, order, places, 0, (cudaStream_t)stream };
+    SPGK_CUDA(cudaGetDevice(&r.dev));
+    if (type == SPGK_T_F32) return route<float>(logits, r);
+    if (type == SPGK_T_F16) return route<__half>(logits, r);
+    return route<__nv_bfloat16>(logits, r);
 }
 
 int spgk_combine_rows(const void *y, int type, uint32_t ldy, uint32_t y_rows, const int32_t *places, const float *gates, uint32_t N, uint32_t top_k,
