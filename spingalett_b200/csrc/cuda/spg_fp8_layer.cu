@@ -34,7 +34,7 @@ constexpr uint32_t ROLES = 3;                 // warp 0: copies, warp 1: product
 constexpr uint32_t EPI = 8, THREADS = 32 * (ROLES + EPI);
 constexpr uint32_t MAX_STAGES = 12;
 constexpr uint32_t MAX_SPLIT = 8;
-constexpr uint32_t AHEAD = 2;
+constexpr uint32_t AHEAD = 8;
 constexpr uint32_t PART = 8 * TM * 4;         // a CTA's sums of eight rows
 constexpr uint32_t HEAD = 2048;
 constexpr uint32_t ROOM = 180 * 1024;         // of shared memory for a CTA (the rest of an SM's is its cache)
@@ -42,7 +42,7 @@ constexpr uint32_t DRAIN = 1u << 12;          // attempts of a last wait
 
 struct LayerParams {
     uint32_t N, out, cols, experts;           // rows, units and inputs of a layer, layers
-    uint32_t w_rows, kblocks, j_tiles, split, stages;
+    uint32_t w_rows, kblocks, j_tiles, j_inverse, split, stages;
     const uint32_t *w_words, *x_words;        // scales
     const int32_t *starts;                    // of the groups, or NULL: one group
     const float *bias;
@@ -130,19 +130,19 @@ __device__ __forceinline__ void prefetch_l2(const CUtensorMap *map, int c0, int 
 struct Table { uint32_t *row, *first; };
 __host__ __device__ constexpr uint32_t table_bytes(uint32_t experts) { return ((experts + 1) * 8 + 1023) / 1024 * 1024; }
 
-// by one warp; behind the wait for the launch in front where there are starts
+__device__ __forceinline__ uint32_t start_of(const LayerParams &p, uint32_t e) { return min((uint32_t)max(__ldcg(p.starts + e), 0), p.N); }     // (past the SM's own cache: see below)
+// by one warp
 __device__ __forceinline__ void make_table(const LayerParams &p, const Table &tab, uint32_t tile_rows, uint32_t lane)
 {
     if (!p.starts) {
         if (lane < 2) { tab.row[lane] = lane * p.N; tab.first[lane] = lane * ((p.N + tile_rows - 1) / tile_rows); }
         return;
     }
-    const auto inside = [&](int32_t s) { return min((uint32_t)max(s, 0), p.N); };
-    uint32_t row = inside(p.starts[0]), tiles = 0;
+    uint32_t row = start_of(p, 0), tiles = 0;
     for (uint32_t e0 = 0; e0 < p.experts; e0 += 256) {
         uint32_t end[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++) { const uint32_t e = e0 + i * 32 + lane; end[i] = e < p.experts ? inside(p.starts[e + 1]) : 0u; }
+        for (uint32_t i = 0; i < 8; i++) { const uint32_t e = e0 + i * 32 + lane; end[i] = e < p.experts ? start_of(p, e + 1) : 0u; }
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
             const uint32_t e = e0 + i * 32 + lane;
@@ -165,25 +165,48 @@ __device__ __forceinline__ void make_table(const LayerParams &p, const Table &ta
         }
     }
 }
-
-// Tile t of all: its layer, its tile of units, its first row and how many rows of its group there are from there on.  A group's tiles go in bands of so many tiles of units, the units
-// fastest inside a band: what runs at a time shares weights and rows in L2.
-struct Tile {
-    uint32_t e, j, n0, rows;
-    __device__ __forceinline__ bool find(uint32_t t, const Table &tab, uint32_t experts, uint32_t j_tiles, uint32_t tile_rows, uint32_t band)
-    {
-        const uint32_t q = t / j_tiles;
-        if (q >= tab.first[experts]) return false;
-        uint32_t lo = 0, hi = experts;                                            // first[lo] <= q < first[hi]
-        while (hi - lo > 1) { const uint32_t mid = (lo + hi) / 2; if (tab.first[mid] <= q) lo = mid; else hi = mid; }
-        e = lo;
-        const uint32_t at = tab.first[lo], n_tiles = tab.first[lo + 1] - at, r = t - at * j_tiles, one = band * n_tiles, g = r / one, left = r % one, here = min(band, j_tiles - g * band);
-        j = g * band + left % here;
-        n0 = tab.row[lo] + left / here * tile_rows;
-        rows = tab.row[lo + 1] - n0;
-        return true;
+// Where there are starts the table is made in front of the wait for the launch in front, out of what then lies there, which is right where an earlier launch wrote them: it serves to
+// fetch weights ahead.  Behind the wait they are looked at again, and the table is made anew if it shows that they are others: its ends of groups are then not
+// the larger of the start and the end of the group before, one by one, which is how they come about.
+__device__ __forceinline__ bool same_starts(const LayerParams &p, const Table &tab, uint32_t lane)
+{
+    uint32_t row = start_of(p, 0);
+    bool same = tab.row[0] == row;
+    for (uint32_t e0 = 0; e0 < p.experts; e0 += 256) {
+        uint32_t end[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) { const uint32_t e = e0 + i * 32 + lane; end[i] = e < p.experts ? start_of(p, e + 1) : 0u; }
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t e = e0 + i * 32 + lane;
+            if (e < p.experts) same = same && tab.row[e + 1] == max(end[i], tab.row[e]);
+        }
     }
-};
+    return __all_sync(0xffffffffu, same);
+}
+
+// Tile t of all: its layer, its tile of units, its first row and how many rows of its group there are from there on (none: there is no such tile).  A group's tiles go in bands of so many
+// tiles of units, the units fastest inside a band: what runs at a time shares weights and rows in L2.
+// (A call, and few instructions for groups of one tile of rows: all roles look for their first tile when their own instructions are still on their way from L2.  Written out in each, a layer of one
+// row's first copy left 0.9 us behind the wait for the launch in front, one of two groups' 1.7.)
+struct Tile { uint32_t e, j, n0, rows; };
+__device__ __noinline__ Tile find_tile(uint32_t t, const uint32_t *row, const uint32_t *first, uint32_t experts, uint32_t j_tiles, uint32_t j_inverse, uint32_t tile_rows, uint32_t band)
+{
+    uint32_t q = __umulhi(t, j_inverse), r = t - q * j_tiles;                    // t / j_tiles: j_inverse is 2^32 / j_tiles, rounded down, so q is at most one too small
+    if (r >= j_tiles) { q++; r -= j_tiles; }
+    if (q >= first[experts]) return { 0, 0, 0, 0 };
+    uint32_t lo = 0, hi = experts;                                                // first[lo] <= q < first[hi]
+    while (hi - lo > 1) { const uint32_t mid = (lo + hi) / 2; if (first[mid] <= q) lo = mid; else hi = mid; }
+    const uint32_t at = first[lo], n_tiles = first[lo + 1] - at;
+    uint32_t j = r, n = 0;
+    if (n_tiles > 1) {
+        r += (q - at) * j_tiles;
+        const uint32_t one = band * n_tiles, g = r / one, left = r % one, here = min(band, j_tiles - g * band);
+        j = g * band + left % here; n = left / here;
+    }
+    const uint32_t n0 = row[lo] + n * tile_rows;
+    return { lo, j, n0, row[lo + 1] - n0 };
+}
 
 // ---- outputs ----------------------------------------------------------------------------------------------------------------------
 // (predicated: a branch around each store costs more than the store)
@@ -327,12 +350,13 @@ __global__ void __launch_bounds__(THREADS) spg_fp8_layer_kernel(const __grid_con
     const uint32_t head = smem_u32(base), table = head + HEAD, words = table + table_bytes(p.experts), parts = words + SF_SLOTS * 2 * SF_TILE, ring = parts + parts_bytes<NT>(p.N, p.split);
     const uint32_t full = head, empty = full + 8 * MAX_STAGES, sf_full = empty + 8 * MAX_STAGES, sf_empty = sf_full + 8 * SF_SLOTS, sums_full = sf_empty + 8 * SF_SLOTS, sums_free = sums_full + 16;
     const uint32_t ended = sums_free + 16, slot = ended + 8, aborted = slot + 4, late = aborted + 4, told = late + 4;
-    // (aborted: a wait of this CTA gave up; late: one of the last waits did; told: one of the cluster's CTAs does not have its sums)
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head)), *told_flag = abort_flag + 2;
+    // (aborted: a wait of this CTA gave up; late: one of the last waits did; told: one of the cluster's CTAs does not have its sums; behind them: the table was made anew)
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head)), *told_flag = abort_flag + 2, *anew_flag = abort_flag + 3;
     uint32_t *const most = reinterpret_cast<uint32_t *>(base + 1024);
     const Table tab = { reinterpret_cast<uint32_t *>(base + HEAD), reinterpret_cast<uint32_t *>(base + HEAD) + p.experts + 1 };
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
     const uint32_t rank = blockIdx.x % p.split, team = blockIdx.x / p.split, teams = gridDim.x / p.split;
+    const auto find = [&](uint32_t i) { return find_tile(i, tab.row, tab.first, p.experts, p.j_tiles, p.j_inverse, NT, BAND); };
     // this CTA's k-blocks
     const uint32_t lo = (uint32_t)((uint64_t)p.kblocks * rank / p.split), hi = (uint32_t)((uint64_t)p.kblocks * (rank + 1) / p.split);
 
@@ -341,39 +365,44 @@ __global__ void __launch_bounds__(THREADS) spg_fp8_layer_kernel(const __grid_con
         for (uint32_t s = 0; s < SF_SLOTS; s++) { mbar_init(sf_full + 8 * s, 1); mbar_init(sf_empty + 8 * s, 1); }
         for (uint32_t a = 0; a < 2; a++) { mbar_init(sums_full + 8 * a, 1); mbar_init(sums_free + 8 * a, EPI); }
         mbar_init(ended, 1);
-        for (uint32_t i = 0; i < 3; i++) abort_flag[i] = 0;
+        for (uint32_t i = 0; i < 4; i++) abort_flag[i] = 0;
         mbar_fence_init();
     }
     if (p.split > 1) cluster_arrive();                                           // (behind `told`, and in front of the wait for tensor memory: see below)
     if (warp == 1) tmem_alloc(slot, L::COLS);
     if (warp == 0 && elect_one()) { prefetch_map(&map_w); prefetch_map(&map_x); }
-    if (warp == 2 && !p.starts) make_table(p, tab, NT, lane);
+    if (warp == 2) make_table(p, tab, NT, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base + (slot - head));
     spg_grid_trigger();
-    // The first weights to L2 while the kernel in front still runs (whoever writes them: L2 is where writes meet), where it is known which they are
-    if (warp == 0 && !p.starts && elect_one()) {
-        Tile tile;
-        if (tile.find(team, tab, 1, p.j_tiles, NT, BAND))
-            for (uint32_t kb = lo; kb < hi && kb < lo + AHEAD; kb++) prefetch_l2(&map_w, (int)(kb * KB), (int)(tile.j * TM));
+    // The first weights to L2 while the kernel in front still runs (whoever writes them: L2 is where writes meet)
+    Tile tile = { 0, 0, 0, 0 };
+    if (warp < ROLES) tile = find(team);
+    if (warp == 0 && elect_one()) {
+        if (tile.rows)
+            for (uint32_t kb = lo; kb < hi && kb < lo + AHEAD; kb++) prefetch_l2(&map_w, (int)(kb * KB), (int)(tile.e * p.out + tile.j * TM));
     }
     __syncwarp();
     if (warp < ROLES) {
         spg_grid_wait();
         if (p.starts) {
-            if (warp == 2) make_table(p, tab, NT, lane);
+            some_meet(5, 32 * ROLES);                                            // (all have found their first tile)
+            if (warp == 2 && !same_starts(p, tab, lane)) {
+                make_table(p, tab, NT, lane);
+                *anew_flag = 1;
+            }
             some_meet(1, THREADS);
+            if (*anew_flag) tile = find(team);
         }
     }
-    Tile tile;
     uint32_t t = team;
     if (warp == 0) {
         uint32_t begun = 0;
         if (elect_one()) {
             bool ok = true;
-            for (uint32_t s = 0, phase = 1; ok && tile.find(t, tab, p.experts, p.j_tiles, NT, BAND); t += teams) {
+            for (uint32_t s = 0, phase = 1; ok && tile.rows; tile = find(t += teams)) {
                 for (uint32_t kb = lo; kb < hi; kb++) {
                     if (!(ok = mbar_wait(empty + 8 * s, phase, abort_flag, p.status, 1))) break;
                     const uint32_t at = ring + s * L::STAGE;
@@ -440,7 +469,7 @@ __global__ void __launch_bounds__(THREADS) spg_fp8_layer_kernel(const __grid_con
     } else if (warp == 2) {
         uint32_t q = 0, phase = 1, w[4], x[L::X_WORDS], g = lo / 4u;
         const uint32_t g_end = (hi + 3u) / 4u;
-        bool more = tile.find(t, tab, p.experts, p.j_tiles, NT, BAND);
+        bool more = tile.rows;
         const auto load = [&]() {
             load_words(w, p.w_words, g, p.w_rows, tile.e * p.out + tile.j * TM, lane);
             load_words(x, p.x_words, g, p.N, tile.n0, lane);
@@ -452,7 +481,7 @@ __global__ void __launch_bounds__(THREADS) spg_fp8_layer_kernel(const __grid_con
             for (uint32_t i = 0; i < 4; i++) w0[i] = w[i];
 #pragma unroll
             for (uint32_t i = 0; i < L::X_WORDS; i++) x0[i] = x[i];
-            if (++g == g_end) { g = lo / 4u; t += teams; more = tile.find(t, tab, p.experts, p.j_tiles, NT, BAND); }
+            if (++g == g_end) { g = lo / 4u; t += teams; tile = find(t); more = tile.rows; }
             if (more) load();                                                    // (on their way while these wait for their place)
             mbar_wait_uniform(sf_empty + 8 * q, phase, aborted, p.status, 8);
             if (*abort_flag) break;
@@ -471,7 +500,7 @@ __global__ void __launch_bounds__(THREADS) spg_fp8_layer_kernel(const __grid_con
 #pragma unroll 1
         for (uint32_t dry = 1;; dry = 0) {
             if (!dry) {
-                if (!tile.find(t, tab, p.experts, p.j_tiles, NT, BAND)) break;
+                if (!(tile = find(t)).rows) break;
             } else tile = { 0, 0, 0, 0 };
             const uint32_t j0 = tile.j * TM + quad * 32u, j = j0 + lane, lanes = tmem + a * NT + (quad * 32u << 16), rows = min(tile.rows, NT);
             float bias = 0.0f;
@@ -587,6 +616,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
     uint32_t *const most = reinterpret_cast<uint32_t *>(base + 1024);
     const Table tab = { reinterpret_cast<uint32_t *>(base + HEAD), reinterpret_cast<uint32_t *>(base + HEAD) + p.experts + 1 };
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = cluster_rank(), pairs = gridDim.x / 2u;
+    const auto find = [&](uint32_t i) { return find_tile(i, tab.row, tab.first, p.experts, p.j_tiles, p.j_inverse, PN, P_BAND); };
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < P_STAGES; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
@@ -627,7 +657,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
             const uint32_t leader = mapa(full, 0);
             uint32_t begun = 0;
             bool ok = true;
-            for (uint32_t s = 0, phase = 1; ok && tile.find(t, tab, p.experts, p.j_tiles, PN, P_BAND); t += pairs) {
+            for (uint32_t s = 0, phase = 1; ok && (tile = find(t)).rows; t += pairs) {
                 const int row_w = (int)(tile.e * p.out + tile.j * 256u + rank * TM), row_x = (int)(tile.n0 + rank * columns(tile.rows) / 2u);
                 for (uint32_t kb = 0; kb < p.kblocks; kb++) {
                     if (!(ok = mbar_wait(empty + 8 * s, phase, abort_flag, p.status, 1))) break;
@@ -647,7 +677,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
             uint32_t s = 0, phase = 0, q = 0, q_phase = 0, turn = 1, odd = 0;
             const uint32_t last = tab.first[p.experts] * p.j_tiles;
             bool ok = true;
-            for (; ok && tile.find(t, tab, p.experts, p.j_tiles, PN, P_BAND); t += pairs) {
+            for (; ok && (tile = find(t)).rows; t += pairs) {
                 if (p.impatient == 1 && last - t <= pairs) { give_up(2); break; }
                 const uint32_t idesc = idesc_fp8(256, columns(tile.rows));
                 ok = p.impatient != 2 ? mbar_wait(sums_free, turn, abort_flag, p.status, 6) : mbar_test(sums_free, turn);
@@ -685,7 +715,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
     } else if (warp == 2) {
         const uint32_t leader = mapa(sf_full, 0), groups = (p.kblocks + 3u) / 4u;
         uint32_t q = 0, phase = 1, w[4], x[8], g = 0;
-        bool more = tile.find(t, tab, p.experts, p.j_tiles, PN, P_BAND);
+        tile = find(t);
+        bool more = tile.rows;
         const auto load = [&]() {
             load_words(w, p.w_words, g, p.w_rows, tile.e * p.out + tile.j * 256u + rank * TM, lane);
             load_words(x, p.x_words, g, p.N, tile.n0, lane);
@@ -697,7 +728,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
             for (uint32_t i = 0; i < 4; i++) w0[i] = w[i];
 #pragma unroll
             for (uint32_t i = 0; i < 8; i++) x0[i] = x[i];
-            if (++g == groups) { g = 0; t += pairs; more = tile.find(t, tab, p.experts, p.j_tiles, PN, P_BAND); }
+            if (++g == groups) { g = 0; t += pairs; tile = find(t); more = tile.rows; }
             if (more) load();                                                    // (on their way while these wait for their place)
             mbar_wait_uniform_cluster(sf_empty + 8 * q, phase, aborted, p.status, 8);
             if (__any_sync(0xffffffffu, *abort_flag)) break;
@@ -716,7 +747,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
 #pragma unroll 1
         for (uint32_t dry = 1;; dry = 0) {
             if (!dry) {
-                if (!tile.find(t, tab, p.experts, p.j_tiles, PN, P_BAND)) break;
+                if (!(tile = find(t)).rows) break;
             } else tile = { 0, 0, 0, 0 };
             const uint32_t j0 = tile.j * 256u + rank * TM + quad * 32u, j = j0 + lane, n0 = tile.n0 + part * P_COLS;
             const uint32_t rows = min(tile.rows, PN) > part * P_COLS ? min(tile.rows, PN) - part * P_COLS : 0u;       // this warp's columns
@@ -829,6 +860,9 @@ int codes_map(CUtensorMap *map, const spgk_fp8 *m, uint32_t box_rows)
     return SPGK_OK;
 }
 
+// 2^32 / n, rounded down (of 1: the largest there is)
+uint32_t inverse(uint32_t n) { return n == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / n); }
+
 // the most tiles of `tile_rows` rows that p.N rows in any groups make: one for each layer that has some, and one more for every tile_rows of the rest
 uint64_t most_tiles(const LayerParams &p, uint32_t tile_rows)
 {
@@ -864,7 +898,7 @@ template <uint32_t NT> int launch(const spgk_fp8 *W, const spgk_fp8 *X, LayerPar
     if (rc) return rc;
     CUtensorMap map_w, map_x;
     if ((rc = codes_map(&map_w, W, TM)) || (rc = codes_map(&map_x, X, NT))) return rc;
-    p.j_tiles = (p.out + TM - 1) / TM;
+    p.j_tiles = (p.out + TM - 1) / TM; p.j_inverse = inverse(p.j_tiles);
     const uint32_t sms = (uint32_t)dp.sm_count;
     const uint64_t tiles = most_tiles(p, NT);
     if (tiles > 0x3fffffffu) { spgk_set_error("spgk_layer_fp8", "too many tiles"); return SPGK_E_ARG; }
@@ -887,7 +921,7 @@ int launch_pairs(const spgk_fp8 *W, const spgk_fp8 *X, LayerParams p, const SpgD
     if (rc) return rc;
     CUtensorMap map_w, map_x;
     if ((rc = codes_map(&map_w, W, TM)) || (rc = codes_map(&map_x, X, PN / 2))) return rc;
-    p.j_tiles = (p.out + 255) / 256;
+    p.j_tiles = (p.out + 255) / 256; p.j_inverse = inverse(p.j_tiles);
     const uint64_t tiles = most_tiles(p, PN);
     if (tiles > 0x3fffffffu) { spgk_set_error("spgk_layer_fp8", "too many tiles"); return SPGK_E_ARG; }
     const uint32_t room = (uint32_t)dp.sm_count / 2, pairs = tiles < room ? (uint32_t)tiles : room;
