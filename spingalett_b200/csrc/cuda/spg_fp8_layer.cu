@@ -17,6 +17,7 @@
 #include "spg_fp8.cuh"
 #include "spg_gemm.cuh"
 #include "spg_tc.cuh"
+#include <cmath>
 #include <cstdio>
 #include <mutex>
 
@@ -118,6 +119,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *v)
         : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
           "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
           "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[8]) { tmem_ld8(taddr, v); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
+          "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
         : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void prefetch_l2(const CUtensorMap *map, int c0, int c1)
@@ -331,6 +341,7 @@ template <uint32_t NT> struct Shape {
     static constexpr uint32_t USED = SFW + 2 * SF_COLS;
     static constexpr uint32_t COLS = USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
     static constexpr uint32_t X_WORDS = (NT + 31) / 32;
+    static constexpr uint32_t CHUNK = NT >= 64 ? 16 : 8;                      // columns that an epilogue warp puts out at a time
 };
 constexpr uint32_t BAND = 16;
 
@@ -342,7 +353,7 @@ template <uint32_t NT> __host__ __device__ constexpr uint32_t parts_bytes(uint32
 }
 
 template <uint32_t NT>
-__global__ void __launch_bounds__(THREADS) spg_fp8_layer_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LayerParams p)
+__global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LayerParams p)
 {
     using L = Shape<NT>;
     extern __shared__ uint8_t raw[];
@@ -531,24 +542,27 @@ __global__ void __launch_bounds__(THREADS) spg_fp8_layer_kernel(const __grid_con
                     ok = !__any_sync(0xffffffffu, *told_flag);
                 }
             }
-            if (ok) {
-                const uint32_t end = dry ? 1u : rows;
+            if (p.split == 1 || dry) {
+                const uint32_t end = dry ? 1u : ok ? rows : 0u;
 #pragma unroll 1
-                for (uint32_t c = dry ? 0 : (half * p.split + rank) * 8u; c < end; c += p.split * 16u) {
-                    float v[8];
-                    if (p.split == 1 || dry) {
-                        if (!dry) { tmem_ld8(lanes + c, v); tmem_ld_wait(); }
-                        else each(v, [](float) { return 0.0f; });
-                    } else {
-                        const float *part = reinterpret_cast<const float *>(base + (parts - head)) + (c / 8 / p.split * p.split) * (PART / 4) + quad * 32u + lane;
-                        each(v, [](float) { return 0.0f; });
-#pragma unroll 1
-                        for (uint32_t r = 0; r < p.split; r++, part += PART / 4) {   // in rank order
-#pragma unroll
-                            for (int i = 0; i < 8; i++) v[i] += part[i * TM];
-                        }
-                    }
+                for (uint32_t c = dry ? 0 : half * L::CHUNK; c < end; c += 2 * L::CHUNK) {
+                    float v[L::CHUNK];
+                    each(v, [](float) { return 0.0f; });
+                    if (!dry) { tmem_ld(lanes + c, v); tmem_ld_wait(); }
                     finish(p, v, tile.n0 + c, dry ? 0u : rows - c, j0, lane, bias, four);
+                }
+            } else if (ok) {
+#pragma unroll 1
+                for (uint32_t c = (half * p.split + rank) * 8u; c < rows; c += p.split * 16u) {
+                    float v[8];
+                    const float *part = reinterpret_cast<const float *>(base + (parts - head)) + (c / 8 / p.split * p.split) * (PART / 4) + quad * 32u + lane;
+                    each(v, [](float) { return 0.0f; });
+#pragma unroll 1
+                    for (uint32_t r = 0; r < p.split; r++, part += PART / 4) {   // in rank order
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v[i] += part[i * TM];
+                    }
+                    finish(p, v, tile.n0 + c, rows - c, j0, lane, bias, four);
                 }
             }
             if (dry) {
@@ -872,6 +886,41 @@ uint64_t most_tiles(const LayerParams &p, uint32_t tile_rows)
 // clusters of this many CTAs that find room at a time, one CTA an SM
 uint32_t at_a_time(uint32_t split, uint32_t sms) { return (split == 8 ? 15u : split == 4 ? 33u : split == 2 ? 74u : 148u) * sms / 148u; }
 
+// How a call is arranged: rows of a tile (256: pairs of CTAs), CTAs that share one.  What each takes is estimated in us on a B200 (with groups of equal sizes, for want of the real ones), fitted to 1400
+// arrangements of 154 products: 1 to 1024 rows and 8 to 5000 in up to 64 groups, 512 to 8192 inputs, 512 to 8192 units.  What it picks takes 1 % longer on average than the best of
+// them, 15 % at most.  Both ends of it, us: 64 rows x 8192 x 8192 by tiles of 64 rows, two CTAs each, 17.4, by tiles of 16 28.5, in pairs 22.8; 1 x 1024 x 8192 alone 4.8, two CTAs a tile 6.2;
+// 1 x 8192 x 1024 14.7 and, eight a tile, 6.0; 512 x 8192 x 8192 in pairs 31.4, by 128 rows 38.4; 512 x 784 x 512 9.9 and 7.3.
+struct Plan { uint32_t rows, split; float us; };
+float tiles_of(const LayerParams &p, uint32_t rows)
+{
+    const uint32_t groups = p.experts < p.N ? p.experts : p.N;
+    if (groups == 1) return (float)(p.N / rows + (p.N % rows != 0));
+    const float each = (float)p.N / (float)groups / (float)rows + 0.5f;          // (half of a last tile is empty)
+    return (float)groups * (each > 1.0f ? each : 1.0f);
+}
+float whole(float v) { const float w = ceilf(v - 0.02f); return w > 1.0f ? w : 1.0f; }
+Plan plan_of(const LayerParams &p, uint32_t sms)
+{
+    const float k = (float)p.kblocks, j_pairs = (float)((p.out + 255u) / 256u), j_tiles = (float)((p.out + TM - 1) / TM), each = (float)p.N / (float)(p.experts < p.N ? p.experts : p.N);
+    Plan best = { PN, 1, 5.29f + whole(tiles_of(p, PN) * j_pairs / (float)(sms / 2)) * (k * 0.331f + 3.06f) };
+    for (uint32_t rows = 16; rows <= 128; rows *= 2) {
+        LayerParams q = p;
+        q.j_tiles = (p.out + TM - 1) / TM;
+        const uint64_t bound = most_tiles(q, rows);
+        const float tiles = tiles_of(p, rows) * j_tiles, used = each < (float)rows ? each : (float)rows, outputs = 0.372f + used * 0.0078f;
+        for (uint32_t s = 1; s <= MAX_SPLIT && s <= p.kblocks; s *= 2) {
+            if (s > 1 && bound > at_a_time(s, sms)) break;
+            const float at_work = tiles * (float)s < (float)sms ? tiles * (float)s : (float)sms, alone = 0.151f + (float)rows * 0.00043f, drawn = (float)(TM + rows) * at_work * 9.83e-6f;
+            const float products = ceilf(k / (float)s) * (alone > drawn ? alone : drawn);
+            float us = 3.55f + outputs;
+            if (s == 1) us += whole(tiles / (float)sms) * (products > 0.9f * outputs ? products : 0.9f * outputs);
+            else us += products + 0.40f + 0.049f * (float)s + 0.0123f * used + (tiles * (float)s > (float)sms / 2.0f ? 0.71f : 0.0f);
+            if (us < best.us) best = { rows, s, us };
+        }
+    }
+    return best;
+}
+
 int launch_as(const char *name, void (*kernel)(CUtensorMap, CUtensorMap, LayerParams), uint32_t grid, uint32_t threads, uint32_t smem, uint32_t cluster, const CUtensorMap &map_w, const CUtensorMap &map_x,
               const LayerParams &p, cudaStream_t stream)
 {
@@ -887,7 +936,7 @@ int launch_as(const char *name, void (*kernel)(CUtensorMap, CUtensorMap, LayerPa
     return spgk_check_launch(name);
 }
 
-template <uint32_t NT> int launch(const spgk_fp8 *W, const spgk_fp8 *X, LayerParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
+template <uint32_t NT> int launch(const spgk_fp8 *W, const spgk_fp8 *X, LayerParams p, uint32_t split, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
 {
     using L = Shape<NT>;
     static SpgOncePerDevice once;
@@ -902,8 +951,7 @@ template <uint32_t NT> int launch(const spgk_fp8 *W, const spgk_fp8 *X, LayerPar
     const uint32_t sms = (uint32_t)dp.sm_count;
     const uint64_t tiles = most_tiles(p, NT);
     if (tiles > 0x3fffffffu) { spgk_set_error("spgk_layer_fp8", "too many tiles"); return SPGK_E_ARG; }
-    p.split = 1;
-    while (p.split < MAX_SPLIT && p.kblocks >= p.split * 4 && tiles <= at_a_time(p.split * 2, sms)) p.split *= 2;
+    p.split = split;
     const uint32_t fixed = 1024 + HEAD + table_bytes(p.experts) + SF_SLOTS * 2 * SF_TILE + parts_bytes<NT>(p.N, p.split);
     const uint32_t most = (ROOM - fixed) / L::STAGE;
     p.stages = most < MAX_STAGES ? most : MAX_STAGES;
@@ -961,12 +1009,14 @@ int layers(const char *who, const spgk_fp8 *W, uint32_t experts, const float *bi
     if (next) { p.next_codes = (uint8_t *)next->codes; p.next_scales = (uint8_t *)next->scales; p.next_pitch = next->pitch; }
     p.impatient = spg_gemm_impatient();
     cudaStream_t st = (cudaStream_t)stream;
-    const uint32_t each = p.N / experts + (p.N % experts != 0);                 // rows of a group, on average
-    const uint32_t nt = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : each <= 128 ? 128 : 256;
-    if (nt <= 16) return launch<16>(W, X, p, dp, dev, st);
-    if (nt <= 32) return launch<32>(W, X, p, dp, dev, st);
-    if (nt <= 64) return launch<64>(W, X, p, dp, dev, st);
-    if (nt <= 128) return launch<128>(W, X, p, dp, dev, st);
+    const Plan plan = plan_of(p, (uint32_t)dp.sm_count);
+    switch (plan.rows) {
+        case 16: return launch<16>(W, X, p, plan.split, dp, dev, st);
+        case 32: return launch<32>(W, X, p, plan.split, dp, dev, st);
+        case 64: return launch<64>(W, X, p, plan.split, dp, dev, st);
+        case 128: return launch<128>(W, X, p, plan.split, dp, dev, st);
+        default: break;
+    }
     return launch_pairs(W, X, p, dp, dev, st);
 }
 
