@@ -348,8 +348,9 @@ __global__ void __launch_bounds__(THREADS) spg_route_order_kernel(const int32_t 
 }
 
 // A thread has U times W neighbouring columns of a row: W are 16 bytes of the narrower type, or one where rows do not lie on 16 bytes; U is 1, and the rows' pieces
-// go to threads one behind the other, or 2 or 4 where a row has enough of them for a block of threads of its own.  ROWS of the rows that are added up are on their way at a time.
-// What bounds it is how many bytes are: a place, then the rows, then the sum is a way of three latencies.  us with U = 1, 2 and 4: 16384 x 2 rows of 8192 bf16 163, 126 and 120
+// go to threads one behind the other, or 2 or 4 where a row has enough of them for a block of threads of its own.  ROWS of the rows that are added up are on their way at a time; where a block has
+// one row, a warp's lanes have its places, and those that are none are passed over.
+// What bounds it is how many bytes are on their way: a place, then the rows, then the sum is a way of three latencies.  us with U = 1, 2 and 4: 16384 x 2 rows of 8192 bf16 163, 126 and 120
 // (6.7 TB/s; 145 through the caches as usual), 4096 x 2 of 4096 19.7, 14.2 and, half of the threads idle, 19.3.
 template <typename T, typename O, uint32_t W, uint32_t U, uint32_t ROWS>
 __global__ void __launch_bounds__(256) spg_combine_kernel(const T *y, uint32_t ldy, uint32_t y_rows, const int32_t *places, const float *gates, uint32_t N, uint32_t top_k,
@@ -362,31 +363,26 @@ __global__ void __launch_bounds__(256) spg_combine_kernel(const T *y, uint32_t l
         const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
         if (i >> 32) { n = (uint32_t)(i / pieces); first = (uint32_t)(i % pieces); }
         else { n = (uint32_t)i / pieces; first = (uint32_t)i % pieces; }
+        if (n >= N) return;
     } else {
         const uint32_t blocks = (pieces - 1) / (256u * U) + 1;
         n = blockIdx.x / blocks; first = blockIdx.x % blocks * 256u * U + threadIdx.x;
     }
-    if (n >= N) return;
     float v[U][W];
 #pragma unroll
     for (uint32_t u = 0; u < U; u++)
 #pragma unroll
         for (uint32_t q = 0; q < W; q++) v[u][q] = 0.0f;
-    for (uint32_t j = 0; j < top_k; j += ROWS) {
+    // rows p[k] with gates g[k], those that there are
+    const auto add = [&](const uint32_t (&p)[ROWS], const float (&g)[ROWS]) {
         alignas(16) T t[ROWS][U][W];
-        float g[ROWS];
-        bool there[ROWS];
 #pragma unroll
         for (uint32_t k = 0; k < ROWS; k++) {
-            const uint64_t at = (uint64_t)n * top_k + j + k;
-            const uint32_t p = j + k < top_k ? (uint32_t)places[at] : 0xffffffffu;
-            there[k] = p < y_rows;
-            g[k] = there[k] ? gates[at] : 0.0f;
-            const T *row = y + (uint64_t)(there[k] ? p : 0u) * ldy;
+            const T *row = y + (uint64_t)(p[k] < y_rows ? p[k] : 0u) * ldy;
 #pragma unroll
             for (uint32_t u = 0; u < U; u++) {
                 const uint32_t c = (first + u * 256u) * W;
-                if (!there[k] || (U > 1 && first + u * 256u >= pieces)) continue;
+                if (p[k] >= y_rows || (U > 1 && first + u * 256u >= pieces)) continue;
                 if constexpr (W * sizeof(T) % 16 == 0) {
 #pragma unroll
                     for (uint32_t q = 0; q < W * sizeof(T) / 16; q++) reinterpret_cast<uint4 *>(t[k][u])[q] = __ldcs(reinterpret_cast<const uint4 *>(row + c) + q);
@@ -398,11 +394,43 @@ __global__ void __launch_bounds__(256) spg_combine_kernel(const T *y, uint32_t l
         }
 #pragma unroll
         for (uint32_t k = 0; k < ROWS; k++) {
-            if (!there[k]) continue;
+            if (p[k] >= y_rows) continue;
 #pragma unroll
             for (uint32_t u = 0; u < U; u++)
 #pragma unroll
                 for (uint32_t q = 0; q < W; q++) v[u][q] = fmaf(g[k], to_f32(t[k][u][q]), v[u][q]);
+        }
+    };
+    const uint64_t at = (uint64_t)n * top_k;
+    if constexpr (U == 1) {
+        for (uint32_t j = 0; j < top_k; j += ROWS) {
+            uint32_t p[ROWS];
+            float g[ROWS];
+#pragma unroll
+            for (uint32_t k = 0; k < ROWS; k++) {
+                p[k] = j + k < top_k ? (uint32_t)places[at + j + k] : 0xffffffffu;
+                g[k] = j + k < top_k ? gates[at + j + k] : 0.0f;
+            }
+            add(p, g);
+        }
+    } else {
+        const uint32_t lane = threadIdx.x % 32u;
+        for (uint32_t j = 0; j < top_k; j += 32u) {
+            const uint32_t place = j + lane < top_k ? (uint32_t)places[at + j + lane] : 0xffffffffu;
+            const float gate = j + lane < top_k ? gates[at + j + lane] : 0.0f;
+            for (uint32_t left = __ballot_sync(0xffffffffu, place < y_rows); left;) {
+                uint32_t p[ROWS];
+                float g[ROWS];
+#pragma unroll
+                for (uint32_t k = 0; k < ROWS; k++) {
+                    const uint32_t one = left ? __ffs(left) - 1 : 0u;
+                    p[k] = __shfl_sync(0xffffffffu, place, one);
+                    g[k] = __shfl_sync(0xffffffffu, gate, one);
+                    if (!left) p[k] = 0xffffffffu;
+                    left &= left - 1;
+                }
+                add(p, g);
+            }
         }
     }
 #pragma unroll
@@ -498,11 +526,17 @@ int combine(const void *y, uint32_t ldy, uint32_t y_rows, const int32_t *places,
     constexpr uint32_t W = 16 / (sizeof(T) < sizeof(O) ? sizeof(T) : sizeof(O));
     const bool wide = width % W == 0 && (uint64_t)ldy * sizeof(T) % 16 == 0 && (uint64_t)ldo * sizeof(O) % 16 == 0 && ((uintptr_t)y | (uintptr_t)out) % 16 == 0;
     const uint32_t pieces = wide ? width / W : width;
-    const uint32_t over = pieces % 1024u, u = pieces >= 640u && (over == 0 || over >= 640u) ? 4u : pieces >= 384u ? 2u : 1u;
+    // as many pieces a thread as leave few of them without one and blocks for all SMs (us with 2 and 4, single columns: 1942 x 1 rows of 2061 bf16 17 and 11.5)
+    uint32_t u = wide ? 4u : 8u;
+    for (; u > 2; u /= 2) {
+        const uint64_t each = (pieces - 1) / (256u * u) + 1;
+        if (pieces * 10ull >= each * 256u * u * 6u && each * N >= 148u * 4u) break;
+    }
+    if (u == 2 && pieces < 384u) u = 1;
     const uint64_t blocks = u > 1 ? (uint64_t)N * ((pieces - 1) / (256u * u) + 1) : ((uint64_t)N * pieces + 255) / 256;
     if (blocks > 0x7fffffffu) return refuse("spgk_combine_rows", "too many rows and columns for one call");
     const auto kernel = wide ? (u == 4 ? spg_combine_kernel<T, O, W, 4, 2> : u == 2 ? spg_combine_kernel<T, O, W, 2, 2> : spg_combine_kernel<T, O, W, 1, 4>)
-                             : (u == 4 ? spg_combine_kernel<T, O, 1, 4, 2> : u == 2 ? spg_combine_kernel<T, O, 1, 2, 2> : spg_combine_kernel<T, O, 1, 1, 4>);
+                             : (u == 8 ? spg_combine_kernel<T, O, 1, 8, 2> : u == 4 ? spg_combine_kernel<T, O, 1, 4, 4> : u == 2 ? spg_combine_kernel<T, O, 1, 2, 4> : spg_combine_kernel<T, O, 1, 1, 4>);
     SPGK_CUDA(spg_launch_chained(kernel, dim3((uint32_t)blocks), dim3(256), 0, stream, (const T *)y, ldy, y_rows, places, gates, N, top_k, (O *)out, ldo, pieces));
     return spgk_check_launch("spg_combine_kernel");
 }
