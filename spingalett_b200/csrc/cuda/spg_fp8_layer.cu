@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_
     } else if (warp == 1) {
         if (elect_one()) {
             const uint32_t idesc = idesc_fp8(TM, NT), last = tab.first[p.experts] * p.j_tiles;
+            const uint64_t w0 = smem_desc_sw128(ring), x0 = smem_desc_sw128(ring + W_BYTES), words0 = scale_desc(words);
             uint32_t s = 0, phase = 0, q = 0, q_phase = 0, a = 0, a_phase = 1, odd = 0;
             bool ok = true;
             for (; ok && t < last; t += teams) {
@@ -443,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_
                         if (!(ok = mbar_wait(sf_full + 8 * q, q_phase, abort_flag, p.status, 7))) break;
                         tc_fence_after();
                         const uint32_t to = tmem + L::SFW + (odd ^= 1u) * L::SF_COLS;
-                        const uint64_t from = scale_desc(words + q * 2 * SF_TILE);
+                        const uint64_t from = words0 + q * (2 * SF_TILE >> 4);
                         copy_scales(to, from);
                         copy_scales(to + L::SFX, from + (SF_TILE >> 4));
                         umma_commit(sf_empty + 8 * q);
@@ -451,8 +452,8 @@ __global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_
                     }
                     if (!(ok = mbar_wait(full + 8 * s, phase, abort_flag, p.status, 2))) break;
                     tc_fence_after();
-                    const uint32_t at = ring + s * L::STAGE, sf = tmem + L::SFW + odd * L::SF_COLS, left = p.cols - kb * KB, id = (kb % 4u) << 4 | (kb % 4u) << 29;
-                    const uint64_t w = smem_desc_sw128(at), x = smem_desc_sw128(at + W_BYTES);
+                    const uint32_t sf = tmem + L::SFW + odd * L::SF_COLS, left = p.cols - kb * KB, id = (kb % 4u) << 4 | (kb % 4u) << 29;
+                    const uint64_t w = w0 + s * (L::STAGE >> 4), x = x0 + s * (L::STAGE >> 4);
                     umma_fp8(tmem + a * NT, w, x, idesc | id, sf, sf + L::SFX, kb > lo, 1);
                     umma_fp8(tmem + a * NT, w + 2, x + 2, idesc | id, sf, sf + L::SFX, 1, left > 32);
                     umma_fp8(tmem + a * NT, w + 4, x + 4, idesc | id, sf, sf + L::SFX, 1, left > 64);
