@@ -5,9 +5,12 @@
 //   sum    : out[n] = sum_j gate[n][j] * y[place[n][j]]
 //
 // A warp has a row of logits, up to 32 a lane, and takes its largest out one after the other.  The order is a counting sort that hangs on nothing's timing.  Few rows go
-// through one block of threads, choice and order.  More rows are cut into parts: as each part's choice is made its pairs are counted by expert, one cluster sums the counts up over the
+// through one block of threads, choice and order (more than 256 experts do not: a row's logits need more registers than so many threads have); more rows' pairs, their choice made by all SMs,
+// through a cluster.  Many pairs are cut into parts: as each part's choice is made its pairs are counted by expert, one cluster sums the counts up over the
 // parts and experts, and then each part finds its pairs' places from where its experts begin.  The counts lie in the memory of the results on the way: in that of the order,
 // which is written last, and where a part's experts begin in that of its places, which only this part reads and writes.
+// What bounds it: latency, of three ways from memory to memory, and 470 instructions a row of 256 logits (us, bf16: 16384 rows to 8 of 256 experts 22.9, 12 of them the choice; 16384 to 2 of 64 13.1,
+// the pairs in one cluster 14.5; 2000 to 8 of 256 14.3 in parts, 11.1 in one cluster; 32 to 2 of 8 4.6 in one block, 6.1 in two launches; one row 3.8).
 #include "spg_fp8.cuh"
 
 namespace {
@@ -16,8 +19,8 @@ using namespace spgfp8;
 
 constexpr uint32_t CHOOSE_THREADS = 512, CHOOSE_WARPS = CHOOSE_THREADS / 32u;
 constexpr uint32_t THREADS = 256, WARPS = THREADS / 32u, LEAST = 64;       // of a part: its order's threads, and the pairs that it has at least
-constexpr uint32_t ONE_THREADS = 1024, ONE_WARPS = ONE_THREADS / 32u, ONE_PAIRS = 4096, ONE_ROWS = 128, ONE_V = 8;   // where one block of threads has all rows, or all pairs
-constexpr uint32_t SUM_THREADS = 1024, SUM_CLUSTER = 8;
+constexpr uint32_t ONE_THREADS = 1024, ONE_WARPS = ONE_THREADS / 32u, ONE_ROWS = 32, ONE_V = 8;      // where one block of threads has all rows
+constexpr uint32_t SUM_THREADS = 1024, SUM_CLUSTER = 8, SUM_PAIRS = 16384;    // up to so many pairs, one cluster has all of them
 
 // order of floats as that of unsigned numbers; -infinity comes lowest, above 0, which no logit has
 __device__ __forceinline__ uint32_t key_of(float v)
@@ -28,27 +31,23 @@ __device__ __forceinline__ uint32_t key_of(float v)
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 __device__ __forceinline__ float closed() { return __int_as_float(0xff800000); }
 
-// V neighbouring logits from e0 on (-infinity beyond the last, and for a NaN); vec: rows lie on what a lane reads
-template <typename T, uint32_t V> __device__ __forceinline__ void load_logits(const T *row, uint32_t e0, uint32_t experts, bool vec, float (&l)[V])
+// V neighbouring logits from e0 on (-infinity beyond the last); vec: rows lie on what a lane reads
+template <typename T, uint32_t V> struct Logits { alignas(16) T t[V]; };
+template <typename T, uint32_t V> __device__ __forceinline__ void load_logits(const T *row, uint32_t e0, uint32_t experts, bool vec, Logits<T, V> &l)
 {
     constexpr uint32_t bytes = V * sizeof(T), word = bytes >= 16 ? 16 : bytes;
-    alignas(16) T t[V];
     if (vec && e0 + V <= experts) {
 #pragma unroll
         for (uint32_t i = 0; i < bytes / word; i++) {
-            if constexpr (word == 16) reinterpret_cast<uint4 *>(t)[i] = reinterpret_cast<const uint4 *>(row + e0)[i];
-            else if constexpr (word == 8) reinterpret_cast<uint2 *>(t)[i] = reinterpret_cast<const uint2 *>(row + e0)[i];
-            else if constexpr (word == 4) reinterpret_cast<uint32_t *>(t)[i] = reinterpret_cast<const uint32_t *>(row + e0)[i];
-            else t[i] = row[e0 + i];
+            if constexpr (word == 16) reinterpret_cast<uint4 *>(l.t)[i] = reinterpret_cast<const uint4 *>(row + e0)[i];
+            else if constexpr (word == 8) reinterpret_cast<uint2 *>(l.t)[i] = reinterpret_cast<const uint2 *>(row + e0)[i];
+            else if constexpr (word == 4) reinterpret_cast<uint32_t *>(l.t)[i] = reinterpret_cast<const uint32_t *>(row + e0)[i];
+            else l.t[i] = row[e0 + i];
         }
-#pragma unroll
-        for (uint32_t i = 0; i < V; i++) l[i] = to_f32(t[i]);
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < V; i++) l[i] = e0 + i < experts ? to_f32(row[e0 + i]) : closed();
+        for (uint32_t i = 0; i < V; i++) l.t[i] = e0 + i < experts ? row[e0 + i] : from_f32<T>(closed());
     }
-#pragma unroll
-    for (uint32_t i = 0; i < V; i++) l[i] = fmaxf(l[i], closed()) + 0.0f;                         // (the larger of a NaN and another is the other; -0 is 0)
 }
 
 // Falling order in a lane: exchanges whose places are known when this is compiled (Batcher's merges of odd and even places).  Equal keys change places only
@@ -81,11 +80,12 @@ template <uint32_t V, bool LATER> __device__ __forceinline__ void sort_lane(uint
 // top_k times.  16-bit logits are searched as keys with the index behind them, so that the maximum over the warp names the expert too; of 32-bit ones that are equal the first
 // lane's is the first.
 template <typename T, uint32_t V>
-__device__ __forceinline__ int32_t choose(const T *row, uint32_t experts, uint32_t top_k, bool normalise, bool vec, uint32_t lane, float &gate)
+__device__ __forceinline__ int32_t choose(const Logits<T, V> &logits, uint32_t top_k, bool normalise, uint32_t lane, float &gate)
 {
     constexpr bool SHORT = sizeof(T) == 2;
     float l[V];
-    load_logits<T, V>(row, lane * V, experts, vec, l);
+#pragma unroll
+    for (uint32_t i = 0; i < V; i++) l[i] = fmaxf(to_f32(logits.t[i]), closed()) + 0.0f;          // (the larger of a NaN and another is the other; -0 is 0)
     uint32_t key[V], at[V];
 #pragma unroll
     for (uint32_t i = 0; i < V; i++) {
@@ -194,9 +194,9 @@ __device__ __forceinline__ uint32_t scan_block(uint32_t v, uint32_t *sums, uint3
     return front + upto - v;
 }
 
-// Few rows, choice and order; or, with `made`, the order alone (of more than 256 experts always: a row's logits need more registers than so many threads have).  Shared memory: chosen, counts of the warps, places of the experts
+// Few rows, choice and order.  Shared memory: chosen, counts of the warps, places of the experts
 template <typename T, uint32_t V>
-__global__ void __launch_bounds__(ONE_THREADS) spg_route_one_kernel(const T *logits, uint32_t ld, uint32_t N, uint32_t experts, uint32_t top_k, int normalise, bool vec, bool made, uint32_t warps,
+__global__ void __launch_bounds__(ONE_THREADS) spg_route_one_kernel(const T *logits, uint32_t ld, uint32_t N, uint32_t experts, uint32_t top_k, int normalise, bool vec, uint32_t warps,
                                                                     int32_t *chosen, float *gates, int32_t *starts, int32_t *order, int32_t *places)
 {
     extern __shared__ uint32_t sh[];
@@ -208,22 +208,16 @@ __global__ void __launch_bounds__(ONE_THREADS) spg_route_one_kernel(const T *log
     for (uint32_t e = threadIdx.x; e < experts; e += ONE_THREADS) place[e] = 0;
     spg_grid_wait();
     __syncthreads();
-    if (made) {
-        for (uint32_t i = threadIdx.x; i < pairs; i += ONE_THREADS) {
-            const int32_t e = chosen[i];
-            mine[i] = e;
-            if ((uint32_t)e < experts) atomicAdd(place + e, 1u);
-        }
-    } else if constexpr (V <= ONE_V) {
-        for (uint32_t n = warp; n < N; n += ONE_WARPS) {
-            float gate;
-            const int32_t e = choose<T, V>(logits + (uint64_t)n * ld, experts, top_k, normalise, vec, lane, gate);
-            if (lane < top_k) {
-                const uint32_t i = n * top_k + lane;
-                chosen[i] = mine[i] = e;
-                gates[i] = gate;
-                if (e >= 0) atomicAdd(place + e, 1u);
-            }
+    for (uint32_t n = warp; n < N; n += ONE_WARPS) {
+        Logits<T, V> l;
+        load_logits(logits + (uint64_t)n * ld, lane * V, experts, vec, l);
+        float gate;
+        const int32_t e = choose(l, top_k, normalise, lane, gate);
+        if (lane < top_k) {
+            const uint32_t i = n * top_k + lane;
+            chosen[i] = mine[i] = e;
+            gates[i] = gate;
+            if (e >= 0) atomicAdd(place + e, 1u);
         }
     }
     __syncthreads();
@@ -247,9 +241,15 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) spg_route_choose_kernel(const 
     if (count) for (uint32_t e = threadIdx.x; e < experts; e += CHOOSE_THREADS) sh[e] = 0;
     spg_grid_wait();
     __syncthreads();
+    constexpr bool EARLY = V <= 16;                              // (more would not fit the registers)
+    Logits<T, V> next;
+    if (EARLY && lo + warp < hi) load_logits(logits + (uint64_t)(lo + warp) * ld, lane * V, experts, vec, next);
     for (uint32_t n = lo + warp; n < hi; n += CHOOSE_WARPS) {
+        if constexpr (!EARLY) load_logits(logits + (uint64_t)n * ld, lane * V, experts, vec, next);
+        const Logits<T, V> l = next;
+        if (EARLY && n + CHOOSE_WARPS < hi) load_logits(logits + (uint64_t)(n + CHOOSE_WARPS) * ld, lane * V, experts, vec, next);     // (on its way while this one is worked on)
         float gate;
-        const int32_t e = choose<T, V>(logits + (uint64_t)n * ld, experts, top_k, normalise, vec, lane, gate);
+        const int32_t e = choose(l, top_k, normalise, lane, gate);
         if (lane < top_k) {
             chosen[n * top_k + lane] = e;
             gates[n * top_k + lane] = gate;
@@ -273,6 +273,53 @@ __device__ __forceinline__ void cluster_sync()
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Where one expert's pairs begin, over all blocks of a cluster and for this one, out of how many each block has (all: this thread's expert's; 0 from `experts` on).  blocks: SUM_CLUSTER at most
+__device__ __forceinline__ uint32_t scan_cluster(const uint32_t *all, uint32_t experts, uint32_t blocks, uint32_t rank, uint32_t *sums, int32_t *starts, uint32_t &total)
+{
+    uint32_t before = 0, whole = 0;
+    if (threadIdx.x < experts) {
+        uint32_t v[SUM_CLUSTER];
+#pragma unroll
+        for (uint32_t r = 0; r < SUM_CLUSTER; r++) v[r] = r < blocks ? ld_cluster(all + threadIdx.x, r) : 0u;
+#pragma unroll
+        for (uint32_t r = 0; r < SUM_CLUSTER; r++) { whole += v[r]; if (r < rank) before += v[r]; }
+    }
+    const uint32_t at = scan_block(whole, sums, total);
+    if (rank == 0 && threadIdx.x < experts) starts[threadIdx.x] = (int32_t)at;
+    if (rank == 0 && threadIdx.x == 0) starts[experts] = (int32_t)total;
+    return at + before;
+}
+
+// The order of pairs that are not many, their choice made: a cluster has them, its blocks a run each.  Shared memory: chosen, counts of the warps, places of the experts, and how many
+// pairs of each the block has
+__global__ void __launch_bounds__(ONE_THREADS) spg_route_pairs_kernel(const int32_t *chosen, uint32_t pairs, uint32_t experts, uint32_t top_k, uint32_t per, uint32_t warps,
+                                                                      int32_t *starts, int32_t *order, int32_t *places)
+{
+    extern __shared__ uint32_t sh[];
+    __shared__ uint32_t sums[ONE_WARPS];
+    const uint32_t rank = blockIdx.x, blocks = gridDim.x, lo = min(pairs, rank * per), count = min(pairs, lo + per) - lo;
+    int32_t *mine = reinterpret_cast<int32_t *>(sh);
+    uint32_t *counts = sh + per, *place = counts + warps * experts, *all = place + experts;
+    spg_grid_trigger();
+    for (uint32_t e = threadIdx.x; e < experts; e += ONE_THREADS) all[e] = 0;
+    spg_grid_wait();
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < count; i += ONE_THREADS) {
+        const uint32_t e = (uint32_t)chosen[lo + i];
+        mine[i] = (int32_t)e;
+        if (e < experts) atomicAdd(all + e, 1u);
+    }
+    __syncthreads();
+    cluster_sync();
+    uint32_t total;
+    const uint32_t at = scan_cluster(all, experts, blocks, rank, sums, starts, total);
+    if (threadIdx.x < experts) place[threadIdx.x] = at;
+    __syncthreads();
+    order_pairs(mine, count, lo, pairs, place, counts, warps, experts, top_k, order, places);
+    for (uint64_t i = (uint64_t)total + rank * ONE_THREADS + threadIdx.x; i < pairs; i += blocks * ONE_THREADS) order[i] = -1;
+    cluster_sync();                                              // (the others may still read this block's counts)
 }
 
 // Counts [parts][experts] to where each part's pairs of each expert begin (first[part * stride + expert]), and where each expert's do.  A cluster: its blocks have the parts in
@@ -305,20 +352,9 @@ __global__ void __launch_bounds__(SUM_THREADS) spg_route_sum_kernel(const uint32
         all[threadIdx.x] = upto;
     }
     cluster_sync();
-    uint32_t before = 0, whole = 0, total;
-    if (threadIdx.x < experts) {
-        uint32_t v[SUM_CLUSTER];
-#pragma unroll
-        for (uint32_t r = 0; r < SUM_CLUSTER; r++) v[r] = ld_cluster(all + threadIdx.x, r);
-#pragma unroll
-        for (uint32_t r = 0; r < SUM_CLUSTER; r++) { whole += v[r]; if (r < rank) before += v[r]; }
-    }
-    const uint32_t at = scan_block(whole, sums, total);
-    if (threadIdx.x < experts) {
-        begin[threadIdx.x] = at + before;
-        if (rank == 0) starts[threadIdx.x] = (int32_t)at;
-    }
-    if (rank == 0 && threadIdx.x == 0) starts[experts] = (int32_t)total;
+    uint32_t total;
+    const uint32_t at = scan_cluster(all, experts, SUM_CLUSTER, rank, sums, starts, total);
+    if (threadIdx.x < experts) begin[threadIdx.x] = at;
     __syncthreads();
     if (lo < hi) {
         uint32_t upto = begin[e] + run[slice * wide + e];
@@ -460,44 +496,61 @@ struct Route {
     int32_t *chosen; float *gates; int32_t *starts, *order, *places;
     int dev; cudaStream_t stream;
 };
-constexpr size_t ONE_SMEM = ((size_t)ONE_PAIRS + (size_t)ONE_WARPS * SPGK_MAX_EXPERTS + SPGK_MAX_EXPERTS) * 4u;
-
-// One block of threads has all rows, or only all pairs; or rows in parts of as many pairs as there are experts at least (their counts lie in the memory of the pairs' results)
-template <typename T, uint32_t V> int route(const void *logits, const Route &r)
+void launch_cluster(cudaLaunchConfig_t &cfg, cudaLaunchAttribute (&attr)[2], uint32_t blocks, uint32_t threads, size_t smem, cudaStream_t stream)
 {
-    const uint32_t pairs = r.N * r.top_k, share = ((r.experts > LEAST ? r.experts : LEAST) + r.top_k - 1) / r.top_k, parts = r.N / share;
-    const bool vec = (uintptr_t)logits % 16 == 0 && (uint64_t)r.ld * sizeof(T) % 16 == 0, few = r.N <= ONE_ROWS && V <= ONE_V, one = pairs <= ONE_PAIRS || parts == 0;
-    const T *x = (const T *)logits;
-    if (!one || !few) {
-        constexpr uint32_t rows = CHOOSE_WARPS;
-        SPGK_CUDA(spg_launch_chained(spg_route_choose_kernel<T, V>, dim3(one ? (r.N + rows - 1) / rows : parts), dim3(CHOOSE_THREADS), one ? 0 : r.experts * 4u, r.stream,
-                                     x, r.ld, r.N, r.experts, r.top_k, r.normalise, vec, one ? rows : share, !one, r.chosen, r.gates, (uint32_t *)r.order));
-        const int rc = spgk_check_launch("spg_route_choose_kernel");
-        if (rc) return rc;
-    }
-    if (one) {
-        static SpgOncePerDevice once;
-        const int rc = once.run(r.dev, [&]() -> int {
-            SPGK_CUDA(cudaFuncSetAttribute(spg_route_one_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ONE_SMEM));
-            return SPGK_OK;
-        });
-        if (rc) return rc;
-        const uint32_t turns = (pairs + 31u) / 32u, warps = turns < 1 ? 1 : turns < ONE_WARPS ? turns : ONE_WARPS;
-        SPGK_CUDA(spg_launch_chained(spg_route_one_kernel<T, V>, dim3(1), dim3(ONE_THREADS), ((size_t)turns * 32u + (size_t)(warps + 1) * r.experts) * 4u, r.stream,
-                                     x, r.ld, r.N, r.experts, r.top_k, r.normalise, vec, !few, warps, r.chosen, r.gates, r.starts, r.order, r.places));
-        return spgk_check_launch("spg_route_one_kernel");
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(SUM_CLUSTER); cfg.blockDim = dim3(SUM_THREADS); cfg.stream = r.stream;
-    cudaLaunchAttribute attr[2];
+    cfg.gridDim = dim3(blocks); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = SUM_CLUSTER; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = blocks; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
+}
+
+// One block of threads has all rows; or the rows are cut and one cluster has all pairs; or rows go in parts of as many pairs as there are experts at least (their counts lie in the memory
+// of the pairs' results) and the pairs in the same parts.
+template <typename T, uint32_t V> int route(const void *logits, const Route &r)
+{
+    const uint32_t pairs = r.N * r.top_k, share = ((r.experts > LEAST ? r.experts : LEAST) + r.top_k - 1) / r.top_k, parts = r.N / share;
+    const bool vec = (uintptr_t)logits % 16 == 0 && (uint64_t)r.ld * sizeof(T) % 16 == 0, few = r.N <= ONE_ROWS && V <= ONE_V, some = pairs <= SUM_PAIRS;
+    const T *x = (const T *)logits;
+    int rc;
+    if constexpr (V <= ONE_V) {
+        if (few) {
+            static SpgOncePerDevice once;
+            rc = once.run(r.dev, [&]() -> int {
+                SPGK_CUDA(cudaFuncSetAttribute(spg_route_one_kernel<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((ONE_ROWS * SPGK_ROUTE_MAX_TOP + (ONE_WARPS + 1) * ONE_V * 32u) * 4u)));
+                return SPGK_OK;
+            });
+            if (rc) return rc;
+            const uint32_t turns = (pairs + 31u) / 32u, warps = turns < 1 ? 1 : turns < ONE_WARPS ? turns : ONE_WARPS;
+            SPGK_CUDA(spg_launch_chained(spg_route_one_kernel<T, V>, dim3(1), dim3(ONE_THREADS), ((size_t)turns * 32u + (size_t)(warps + 1) * r.experts) * 4u, r.stream,
+                                         x, r.ld, r.N, r.experts, r.top_k, r.normalise, vec, warps, r.chosen, r.gates, r.starts, r.order, r.places));
+            return spgk_check_launch("spg_route_one_kernel");
+        }
+    }
+    if (r.N) SPGK_CUDA(spg_launch_chained(spg_route_choose_kernel<T, V>, dim3(some ? (r.N + CHOOSE_WARPS - 1) / CHOOSE_WARPS : parts), dim3(CHOOSE_THREADS), some ? 0 : r.experts * 4u, r.stream,
+                                 x, r.ld, r.N, r.experts, r.top_k, r.normalise, vec, some ? CHOOSE_WARPS : share, !some, r.chosen, r.gates, (uint32_t *)r.order));
+    if ((rc = spgk_check_launch("spg_route_choose_kernel"))) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    if (some) {
+        static SpgOncePerDevice once;
+        rc = once.run(r.dev, [&]() -> int {
+            SPGK_CUDA(cudaFuncSetAttribute(spg_route_pairs_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((SUM_PAIRS / SUM_CLUSTER + 32u + (ONE_WARPS + 2) * SPGK_MAX_EXPERTS) * 4u)));
+            return SPGK_OK;
+        });
+        if (rc) return rc;
+        const uint32_t turns = pairs ? (pairs + 31u) / 32u : 1u;
+        uint32_t blocks = 1;
+        while (blocks < SUM_CLUSTER && turns > blocks * ONE_WARPS) blocks *= 2;
+        const uint32_t each = (turns + blocks - 1) / blocks, warps = each < ONE_WARPS ? each : ONE_WARPS;
+        launch_cluster(cfg, attr, blocks, ONE_THREADS, ((size_t)each * 32u + (size_t)(warps + 2) * r.experts) * 4u, r.stream);
+        SPGK_CUDA(cudaLaunchKernelEx(&cfg, spg_route_pairs_kernel, (const int32_t *)r.chosen, pairs, r.experts, r.top_k, each * 32u, warps, r.starts, r.order, r.places));
+        return spgk_check_launch("spg_route_pairs_kernel");
+    }
+    launch_cluster(cfg, attr, SUM_CLUSTER, SUM_THREADS, 0, r.stream);
     SPGK_CUDA(cudaLaunchKernelEx(&cfg, spg_route_sum_kernel, (const uint32_t *)r.order, parts, r.experts, (r.experts + 31u) / 32u * 32u, share * r.top_k, (uint32_t *)r.places, r.starts));
-    int rc = spgk_check_launch("spg_route_sum_kernel");
-    if (rc) return rc;
+    if ((rc = spgk_check_launch("spg_route_sum_kernel"))) return rc;
     static SpgOncePerDevice once;
     const size_t most = (2 * (size_t)(SPGK_MAX_EXPERTS + SPGK_ROUTE_MAX_TOP) + 32u + (WARPS + 1) * SPGK_MAX_EXPERTS) * 4u;
     rc = once.run(r.dev, [&]() -> int {
