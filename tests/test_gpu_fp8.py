@@ -358,3 +358,66 @@ def test_on_another_stream_and_replayed(spg, lib):
         c.starts.copy_(torch.tensor([0, 30, 30, 69], dtype=torch.int32))
         c.groups = plain.ranges([0, 30, 30, 69], 70)
         want = np.where(c.want(1)[0] == -3, want, c.want(1)[0])
+
+
+def test_offsets_beyond_32_bits(spg, lib):
+    """Weights of 5 GB of which the last layer is used, rows of the output and of what is quantised 4 GB apart."""
+    import torch
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("less than 40 GB free")
+    rng = np.random.default_rng(8)
+    experts, out, k, n = 610, 1024, 8192, 5
+    w = Packed(spg, experts * out, k)
+    code = rng.choice(np.flatnonzero((plain.SIZES[:127] <= 8) & (plain.SIZES[:127] * 4 % 1 == 0)), (out, k)).astype(np.uint8)
+    w.codes[(experts - 1) * out:experts * out] = torch.from_numpy(code).cuda()
+    words = w.words[:-16].view(-1, experts * out, 4)
+    words.fill_(127)
+    assert w.codes.numel() > 2 ** 32 and w.codes[-1:].data_ptr() - w.codes.data_ptr() > 2 ** 32
+    x, xv = _random(spg, n, k, rng, True)
+    starts = torch.full((experts + 1,), 2, dtype=torch.int32, device="cuda")
+    starts[0], starts[-1] = 0, n                                   # two rows to the first layer, the rest to the last
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ldy = 1 << 30
+    y = torch.zeros((n - 1) * ldy + out, dtype=torch.float16, device="cuda")
+    assert lib.spgk_experts_fp8(w.ref, experts, None, 6, x.ref, starts.data_ptr(), y.data_ptr(), 0, ldy, None, status.data_ptr(), None) == 0, lib.spgk_error_string()
+    assert lib.spgk_gemm_tc_status(status.data_ptr(), None) == 0
+    want = (torch.from_numpy(xv[2:]) @ torch.from_numpy(plain.SIZES[code]).T).to(torch.float16)
+    got = torch.stack([y[r * ldy:r * ldy + out] for r in range(2, n)]).cpu()
+    assert torch.equal(got, want)
+    # the same rows quantised from where they lie, taken by index, and added up
+    index = torch.tensor([4, 2], dtype=torch.int32, device="cuda")
+    m = Packed(spg, 2, out)
+    assert lib.spgk_fp8_quantize(y.data_ptr(), 0, ldy, n, index.data_ptr(), m.ref, None) == 0
+    torch.cuda.synchronize()
+    code_w, scale_w = plain.quantize(got.double().numpy()[[2, 0]])
+    code, scale = m.host()
+    assert np.array_equal(code, code_w) and np.array_equal(scale, scale_w)
+    places, gates = torch.tensor([[3, 4]], dtype=torch.int32, device="cuda"), torch.tensor([[0.5, 0.25]], device="cuda")
+    total = torch.zeros(out, device="cuda")
+    assert lib.spgk_combine_rows(y.data_ptr(), 0, ldy, n, places.data_ptr(), gates.data_ptr(), 1, 2, out, total.data_ptr(), 2, out, None) == 0
+    assert torch.allclose(total.cpu(), 0.5 * got[1].float() + 0.25 * got[2].float(), rtol=2.0 ** -22, atol=0)
+
+
+def test_operands_that_are_views(spg, lib):
+    """Rows taken out of a larger matrix, from any row on: its own codes and the scales' pitch, in a matrix of their own made by an index."""
+    import torch
+    rng = np.random.default_rng(4)
+    x = torch.from_numpy(rng.standard_normal((50, 900)).astype(np.float32)).cuda()
+    part = x[7:40, 100:877]                                        # neither its first row nor its column lies on 16 bytes
+    m = Packed(spg, 33, 777)
+    assert lib.spgk_fp8_quantize(part.data_ptr(), 2, x.stride(0), 33, None, m.ref, None) == 0
+    torch.cuda.synchronize()
+    code_w, scale_w = plain.quantize(part.double().cpu().numpy())
+    code, scale = m.host()
+    assert np.array_equal(code, code_w) and np.array_equal(scale, scale_w)
+    w, wv = _random(spg, 70, 777, rng)
+    y = torch.full((40, 80), 5.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    into = y[3:36, 5:75]
+    assert lib.spgk_layer_fp8(w.ref, None, 6, m.ref, into.data_ptr(), 2, 80, None, status.data_ptr(), None) == 0
+    assert lib.spgk_gemm_tc_status(status.data_ptr(), None) == 0
+    want = plain.values(code_w, scale_w) @ wv.T
+    size = np.abs(plain.values(code_w, scale_w)) @ np.abs(wv).T
+    assert (np.abs(into.double().cpu().numpy() - want) <= size * 26 * 33 * 2.0 ** -24).all()
+    into.fill_(5.0)
+    assert (y == 5).all()                                          # nothing beside it was written
