@@ -32,7 +32,6 @@ constexpr uint32_t W_BYTES = TM * KB;         // codes of a tile's weights
 constexpr uint32_t SF_TILE = 512;             // words of scales of 128 rows
 constexpr uint32_t SF_SLOTS = 4;              // words on their way, four k-blocks each
 constexpr uint32_t ROLES = 3;                 // warp 0: copies, warp 1: products, warp 2: scales; the rest: outputs
-constexpr uint32_t EPI = 8, THREADS = 32 * (ROLES + EPI);
 constexpr uint32_t MAX_STAGES = 12;
 constexpr uint32_t MAX_SPLIT = 8;
 constexpr uint32_t AHEAD = 8;
@@ -341,7 +340,8 @@ template <uint32_t NT> struct Shape {
     static constexpr uint32_t USED = SFW + 2 * SF_COLS;
     static constexpr uint32_t COLS = USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
     static constexpr uint32_t X_WORDS = (NT + 31) / 32;
-    static constexpr uint32_t CHUNK = NT >= 64 ? 16 : 8;                      // columns that an epilogue warp puts out at a time
+    static constexpr uint32_t EPI = NT >= 64 ? 16 : 8, THREADS = 32 * (ROLES + EPI), PARTS = EPI / 4;      // warps that put out, four of them all units of the same rows
+    static constexpr uint32_t CHUNK = NT >= 128 ? 16 : 8;                     // columns that such a warp puts out at a time
 };
 constexpr uint32_t BAND = 16;
 
@@ -353,16 +353,18 @@ template <uint32_t NT> __host__ __device__ constexpr uint32_t parts_bytes(uint32
 }
 
 template <uint32_t NT>
-__global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LayerParams p)
+__global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LayerParams p)
 {
     using L = Shape<NT>;
+    constexpr uint32_t EPI = L::EPI, THREADS = L::THREADS;
     extern __shared__ uint8_t raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     const uint32_t head = smem_u32(base), table = head + HEAD, words = table + table_bytes(p.experts), parts = words + SF_SLOTS * 2 * SF_TILE, ring = parts + parts_bytes<NT>(p.N, p.split);
     const uint32_t full = head, empty = full + 8 * MAX_STAGES, sf_full = empty + 8 * MAX_STAGES, sf_empty = sf_full + 8 * SF_SLOTS, sums_full = sf_empty + 8 * SF_SLOTS, sums_free = sums_full + 16;
     const uint32_t ended = sums_free + 16, slot = ended + 8, aborted = slot + 4, late = aborted + 4, told = late + 4;
-    // (aborted: a wait of this CTA gave up; late: one of the last waits did; told: one of the cluster's CTAs does not have its sums; behind them: the table was made anew)
+    // (aborted: a wait of this CTA gave up; late: one of the last waits did; told: one of the cluster's CTAs does not have its sums; behind them: the table was made anew; copies that were begun)
     volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head)), *told_flag = abort_flag + 2, *anew_flag = abort_flag + 3;
+    volatile uint32_t *const begun_at = reinterpret_cast<volatile uint32_t *>(abort_flag + 4);
     uint32_t *const most = reinterpret_cast<uint32_t *>(base + 1024);
     const Table tab = { reinterpret_cast<uint32_t *>(base + HEAD), reinterpret_cast<uint32_t *>(base + HEAD) + p.experts + 1 };
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
@@ -424,8 +426,7 @@ __global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_
                     if (++s == p.stages) { s = 0; phase ^= 1u; }
                 }
             }
-            // (the table's place is no longer needed by whoever gave up: the last word of the head says how many copies were begun)
-            *reinterpret_cast<volatile uint32_t *>(base + HEAD - 4) = begun;
+            *begun_at = begun;
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -439,27 +440,32 @@ __global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_
                 ok = p.impatient != 2 ? mbar_wait(sums_free + 8 * a, a_phase, abort_flag, p.status, 6) : mbar_test(sums_free + 8 * a, a_phase);
                 if (!ok) { atomicCAS(p.status, 0, 6); *abort_flag = 1; break; }
                 tc_fence_after();
-                for (uint32_t kb = lo; kb < hi; kb++) {
-                    if (kb % 4u == 0 || kb == lo) {
-                        if (!(ok = mbar_wait(sf_full + 8 * q, q_phase, abort_flag, p.status, 7))) break;
-                        tc_fence_after();
-                        const uint32_t to = tmem + L::SFW + (odd ^= 1u) * L::SF_COLS;
-                        const uint64_t from = words0 + q * (2 * SF_TILE >> 4);
-                        copy_scales(to, from);
-                        copy_scales(to + L::SFX, from + (SF_TILE >> 4));
-                        umma_commit(sf_empty + 8 * q);
-                        if (++q == SF_SLOTS) { q = 0; q_phase ^= 1u; }
-                    }
-                    if (!(ok = mbar_wait(full + 8 * s, phase, abort_flag, p.status, 2))) break;
+                // (Written out for the four blocks of a word: 260 cycles a k-block, 330 in a loop over them one by one; 27 of them are an instruction of products, 54 a wait, 6 a commit.)
+                for (uint32_t kb = lo; ok && kb < hi;) {
+                    if (!(ok = mbar_wait(sf_full + 8 * q, q_phase, abort_flag, p.status, 7))) break;
                     tc_fence_after();
-                    const uint32_t sf = tmem + L::SFW + odd * L::SF_COLS, left = p.cols - kb * KB, id = (kb % 4u) << 4 | (kb % 4u) << 29;
-                    const uint64_t w = w0 + s * (L::STAGE >> 4), x = x0 + s * (L::STAGE >> 4);
-                    umma_fp8(tmem + a * NT, w, x, idesc | id, sf, sf + L::SFX, kb > lo, 1);
-                    umma_fp8(tmem + a * NT, w + 2, x + 2, idesc | id, sf, sf + L::SFX, 1, left > 32);
-                    umma_fp8(tmem + a * NT, w + 4, x + 4, idesc | id, sf, sf + L::SFX, 1, left > 64);
-                    umma_fp8(tmem + a * NT, w + 6, x + 6, idesc | id, sf, sf + L::SFX, 1, left > 96);
-                    umma_commit(empty + 8 * s);
-                    if (++s == p.stages) { s = 0; phase ^= 1u; }
+                    odd ^= 1u;
+                    const uint32_t sf = tmem + L::SFW + odd * L::SF_COLS, d = tmem + a * NT;
+                    const uint64_t from = words0 + q * (2 * SF_TILE >> 4);
+                    copy_scales(sf, from);
+                    copy_scales(sf + L::SFX, from + (SF_TILE >> 4));
+                    umma_commit(sf_empty + 8 * q);
+                    if (++q == SF_SLOTS) { q = 0; q_phase ^= 1u; }
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++) {
+                        if (kb % 4u != i || kb >= hi) continue;
+                        if (!(ok = mbar_wait(full + 8 * s, phase, abort_flag, p.status, 2))) break;
+                        tc_fence_after();
+                        const uint32_t left = p.cols - kb * KB, id = idesc | i << 4 | i << 29;
+                        const uint64_t w = w0 + s * (L::STAGE >> 4), x = x0 + s * (L::STAGE >> 4);
+                        umma_fp8(d, w, x, id, sf, sf + L::SFX, kb > lo, 1);
+                        umma_fp8(d, w + 2, x + 2, id, sf, sf + L::SFX, 1, left > 32);
+                        umma_fp8(d, w + 4, x + 4, id, sf, sf + L::SFX, 1, left > 64);
+                        umma_fp8(d, w + 6, x + 6, id, sf, sf + L::SFX, 1, left > 96);
+                        umma_commit(empty + 8 * s);
+                        if (++s == p.stages) { s = 0; phase ^= 1u; }
+                        kb++;
+                    }
                 }
                 if (!ok) break;
                 umma_commit(sums_full + 8 * a);
@@ -505,8 +511,8 @@ __global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_
             if (++q == SF_SLOTS) { q = 0; phase ^= 1u; }
         }
     } else {
-        const uint32_t quad = warp % 4u, half = (warp - ROLES) / 4u;
-        Four four = { most + half * 64u, 3u + half, quad, 0u };
+        const uint32_t quad = warp % 4u, part = (warp - ROLES) / 4u;
+        Four four = { most + part * 64u, 6u + part, quad, 0u };
         uint32_t a = 0, a_phase = 0;
         // Once without a row before the launch in front has ended: the outputs' instructions come from L2, and would follow the products
 #pragma unroll 1
@@ -520,13 +526,13 @@ __global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_
             if (!dry) {
                 if (p.bias && j < p.out) bias = p.bias[(uint64_t)tile.e * p.out + j];
                 // (all four warps of a row go one way)
-                ok = some_agree(3u + half, 128, mbar_wait(sums_full + 8 * a, a_phase, abort_flag, p.status, 3));
+                ok = some_agree(6u + part, 128, mbar_wait(sums_full + 8 * a, a_phase, abort_flag, p.status, 3));
                 tc_fence_after();
                 if (p.split > 1) {
                     // This CTA's sums to those that put them out, [chunk][CTA][row][unit], sent before one barrier
                     cluster_wait();                                              // all have begun
                     const uint32_t chunks = ok ? (rows + 7u) / 8u : 0u;
-                    for (uint32_t c = half; c < chunks; c += 2) {
+                    for (uint32_t c = part; c < chunks; c += L::PARTS) {
                         float v[8];
                         tmem_ld8(lanes + 8 * c, v);
                         tmem_ld_wait();
@@ -546,7 +552,7 @@ __global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_
             if (p.split == 1 || dry) {
                 const uint32_t end = dry ? 1u : ok ? rows : 0u;
 #pragma unroll 1
-                for (uint32_t c = dry ? 0 : half * L::CHUNK; c < end; c += 2 * L::CHUNK) {
+                for (uint32_t c = dry ? 0 : part * L::CHUNK; c < end; c += L::PARTS * L::CHUNK) {
                     float v[L::CHUNK];
                     each(v, [](float) { return 0.0f; });
                     if (!dry) { tmem_ld(lanes + c, v); tmem_ld_wait(); }
@@ -554,14 +560,14 @@ __global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_
                 }
             } else if (ok) {
 #pragma unroll 1
-                for (uint32_t c = (half * p.split + rank) * 8u; c < rows; c += p.split * 16u) {
+                for (uint32_t c = (part * p.split + rank) * 8u; c < rows; c += p.split * L::PARTS * 8u) {
                     float v[8];
-                    const float *part = reinterpret_cast<const float *>(base + (parts - head)) + (c / 8 / p.split * p.split) * (PART / 4) + quad * 32u + lane;
+                    const float *sums = reinterpret_cast<const float *>(base + (parts - head)) + (c / 8 / p.split * p.split) * (PART / 4) + quad * 32u + lane;
                     each(v, [](float) { return 0.0f; });
 #pragma unroll 1
-                    for (uint32_t r = 0; r < p.split; r++, part += PART / 4) {   // in rank order
+                    for (uint32_t r = 0; r < p.split; r++, sums += PART / 4) {   // in rank order
 #pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] += part[i * TM];
+                        for (int i = 0; i < 8; i++) v[i] += sums[i * TM];
                     }
                     finish(p, v, tile.n0 + c, rows - c, j0, lane, bias, four);
                 }
@@ -594,7 +600,7 @@ __global__ void __launch_bounds__(THREADS, 1) spg_fp8_layer_kernel(const __grid_
             mbar_wait_uniform(ended, 0, late, p.status, 5, DRAIN);
         }
         if (warp == 0) {
-            const uint32_t begun = *reinterpret_cast<volatile uint32_t *>(base + HEAD - 4);
+            const uint32_t begun = *begun_at;
             for (uint32_t i = begun > p.stages ? begun - p.stages : 0; i < begun; i++) mbar_wait_uniform(full + 8 * (i % p.stages), i / p.stages & 1u, late, p.status, 4, DRAIN);
         }
         __syncwarp();
@@ -957,7 +963,7 @@ template <uint32_t NT> int launch(const spgk_fp8 *W, const spgk_fp8 *X, LayerPar
     const uint32_t most = (ROOM - fixed) / L::STAGE;
     p.stages = most < MAX_STAGES ? most : MAX_STAGES;
     const uint32_t grid = p.split > 1 ? (uint32_t)tiles * p.split : (tiles < sms ? (uint32_t)tiles : sms);
-    return launch_as("spg_fp8_layer_kernel", spg_fp8_layer_kernel<NT>, grid, THREADS, fixed + p.stages * L::STAGE, p.split, map_w, map_x, p, stream);
+    return launch_as("spg_fp8_layer_kernel", spg_fp8_layer_kernel<NT>, grid, L::THREADS, fixed + p.stages * L::STAGE, p.split, map_w, map_x, p, stream);
 }
 
 int launch_pairs(const spgk_fp8 *W, const spgk_fp8 *X, LayerParams p, const SpgDeviceProps &dp, int dev, cudaStream_t stream)
