@@ -893,10 +893,10 @@ uint64_t most_tiles(const LayerParams &p, uint32_t tile_rows)
 // clusters of this many CTAs that find room at a time, one CTA an SM
 uint32_t at_a_time(uint32_t split, uint32_t sms) { return (split == 8 ? 15u : split == 4 ? 33u : split == 2 ? 74u : 148u) * sms / 148u; }
 
-// How a call is arranged: rows of a tile (256: pairs of CTAs), CTAs that share one.  What each takes is estimated in us on a B200 (with groups of equal sizes, for want of the real ones), fitted to 1400
-// arrangements of 154 products: 1 to 1024 rows and 8 to 5000 in up to 64 groups, 512 to 8192 inputs, 512 to 8192 units.  What it picks takes 1 % longer on average than the best of
-// them, 15 % at most.  Both ends of it, us: 64 rows x 8192 x 8192 by tiles of 64 rows, two CTAs each, 17.4, by tiles of 16 28.5, in pairs 22.8; 1 x 1024 x 8192 alone 4.8, two CTAs a tile 6.2;
-// 1 x 8192 x 1024 14.7 and, eight a tile, 6.0; 512 x 8192 x 8192 in pairs 31.4, by 128 rows 38.4; 512 x 784 x 512 9.9 and 7.3.
+// How a call is arranged: rows of a tile (256: pairs of CTAs), CTAs that share one.  What each takes is estimated in us on a B200 (with groups of equal sizes, for want of the real ones), fitted to 1285
+// arrangements of 205 products: 1 to 5000 rows, in up to 200 groups, 128 to 16384 inputs, 128 to 8192 units.  What it picks takes 1 % longer on average than the best of
+// them, 15 % at most.  Both ends of it, us: 64 rows x 8192 x 8192 by tiles of 64 rows, two CTAs each, 16.6, by tiles of 16 24.8, in pairs 23.1; 1 x 1024 x 8192 alone 4.6, two CTAs a tile 6.2;
+// 1 x 8192 x 1024 12.0 and, eight a tile, 5.9; 512 x 8192 x 8192 in pairs 31.1, by 128 rows 38.3; 512 x 784 x 512 9.6 and 7.2.
 struct Plan { uint32_t rows, split; float us; };
 float tiles_of(const LayerParams &p, uint32_t rows)
 {
@@ -909,19 +909,19 @@ float whole(float v) { const float w = ceilf(v - 0.02f); return w > 1.0f ? w : 1
 Plan plan_of(const LayerParams &p, uint32_t sms)
 {
     const float k = (float)p.kblocks, j_pairs = (float)((p.out + 255u) / 256u), j_tiles = (float)((p.out + TM - 1) / TM), each = (float)p.N / (float)(p.experts < p.N ? p.experts : p.N);
-    Plan best = { PN, 1, 5.29f + whole(tiles_of(p, PN) * j_pairs / (float)(sms / 2)) * (k * 0.331f + 3.06f) };
+    Plan best = { PN, 1, 5.77f + whole(tiles_of(p, PN) * j_pairs / (float)(sms / 2)) * (k * 0.334f + 1.79f) };
     for (uint32_t rows = 16; rows <= 128; rows *= 2) {
         LayerParams q = p;
         q.j_tiles = (p.out + TM - 1) / TM;
         const uint64_t bound = most_tiles(q, rows);
-        const float tiles = tiles_of(p, rows) * j_tiles, used = each < (float)rows ? each : (float)rows, outputs = 0.372f + used * 0.0078f;
+        const float tiles = tiles_of(p, rows) * j_tiles, used = each < (float)rows ? each : (float)rows, outputs = 0.33f + used * 0.0092f;
         for (uint32_t s = 1; s <= MAX_SPLIT && s <= p.kblocks; s *= 2) {
             if (s > 1 && bound > at_a_time(s, sms)) break;
-            const float at_work = tiles * (float)s < (float)sms ? tiles * (float)s : (float)sms, alone = 0.151f + (float)rows * 0.00043f, drawn = (float)(TM + rows) * at_work * 9.83e-6f;
+            const float at_work = tiles * (float)s < (float)sms ? tiles * (float)s : (float)sms, alone = 0.119f + (float)rows * 0.00068f, drawn = (float)(TM + rows) * at_work * 9.08e-6f;
             const float products = ceilf(k / (float)s) * (alone > drawn ? alone : drawn);
-            float us = 3.55f + outputs;
+            float us = 3.22f + outputs;
             if (s == 1) us += whole(tiles / (float)sms) * (products > 0.9f * outputs ? products : 0.9f * outputs);
-            else us += products + 0.40f + 0.049f * (float)s + 0.0123f * used + (tiles * (float)s > (float)sms / 2.0f ? 0.71f : 0.0f);
+            else us += products + 0.40f + 0.116f * (float)s + 0.0108f * used + (tiles * (float)s > (float)sms / 2.0f ? 0.99f : 0.0f);
             if (us < best.us) best = { rows, s, us };
         }
     }
