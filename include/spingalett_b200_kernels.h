@@ -668,12 +668,13 @@ SPGK_API int spgk_experts_fp8(const spgk_fp8 *W, uint32_t experts, const float *
  *   starts: dev int32 [experts + 1], where each expert's begin; starts[experts] is how many there are;
  *   order : dev int32 [N * top_k], their rows, -1 behind the last: rows_idx of spgk_fp8_quantize;
  *   places: dev int32 [N][top_k], the place of (row, chosen expert) in that order, -1 where none was chosen: for spgk_combine_rows.
- * No two of the five may be the same memory.  N * top_k is below 2^30. */
+ * The five are memory of their own, each, and not the logits' (they hold counts on the way).  N * top_k is below 2^30. */
 #define SPGK_ROUTE_MAX_TOP 32u
 SPGK_API int spgk_route_rows(const void *logits, int type, uint32_t ld, uint32_t N, uint32_t experts, uint32_t top_k, int normalise,
                              int32_t *chosen, float *gates, int32_t *starts, int32_t *order, int32_t *places, void *stream);
 /* out[n][c] = sum over j of gates[n][j] * y[places[n][j]][c], in fp32 and in the order of j, rounded once; a place that is none of y's y_rows rows counts as a
- * row of zeros, whatever its gate.  y: rows of ldy elements of `type`; places, gates: dev [N][top_k]; out: rows of ldo elements of out_type. */
+ * row of zeros, whatever its gate.  y: rows of ldy elements of `type`; places, gates: dev [N][top_k]; out: rows of ldo elements of out_type, which overlap nothing that
+ * is read. */
 SPGK_API int spgk_combine_rows(const void *y, int type, uint32_t ldy, uint32_t y_rows, const int32_t *places, const float *gates, uint32_t N, uint32_t top_k,
                                uint32_t width, void *out, int out_type, uint32_t ldo, void *stream);
 

@@ -616,6 +616,9 @@ int spgk_route_rows(const void *logits, int type, uint32_t ld, uint32_t N, uint3
     if (!starts || (N && (!logits || !chosen || !gates || !order || !places))) return refuse(who, "no logits, or no place for a result");
     if ((uintptr_t)logits % size_of(type) || ((uintptr_t)chosen | (uintptr_t)gates | (uintptr_t)starts | (uintptr_t)order | (uintptr_t)places) % 4u) return refuse(who, "not aligned");
     if (N > 1 && ld < experts) return refuse(who, "rows overlap");
+    const void *const results[] = { chosen, gates, starts, order, places };      // (they hold counts on the way)
+    for (uint32_t i = 0; N && i < 5; i++)
+        for (uint32_t j = 0; j < i; j++) if (results[i] == results[j]) return refuse(who, "two results in one place");
     Route r = { ld, N, experts, top_k, normalise, chosen, gates, starts, order, places, 0, (cudaStream_t)stream };
     SPGK_CUDA(cudaGetDevice(&r.dev));
     if (type == SPGK_T_F32) return route<float>(logits, r);

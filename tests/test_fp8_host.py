@@ -110,11 +110,12 @@ def test_bad_layers_are_refused(spg, lib):
 
 
 def test_bad_routes_are_refused(lib):
-    def call(logits=SOME, kind=2, ld=10, n=2, experts=10, top=2, chosen=SOME, gates=SOME, starts=SOME, order=SOME, places=SOME):
+    def call(logits=SOME, kind=2, ld=10, n=2, experts=10, top=2, chosen=SOME, gates=2 * SOME, starts=3 * SOME, order=4 * SOME, places=5 * SOME):
         return lib.spgk_route_rows(logits, kind, ld, n, experts, top, 0, chosen, gates, starts, order, places, None)
     for bad in (dict(kind=3), dict(kind=-1), dict(experts=0), dict(experts=1025, ld=1025), dict(top=0), dict(top=11), dict(top=33, experts=64, ld=64), dict(logits=0), dict(chosen=0), dict(gates=0),
                 dict(starts=0), dict(order=0), dict(places=0), dict(logits=SOME + 2), dict(logits=SOME + 1, kind=0), dict(ld=9), dict(chosen=SOME + 1), dict(gates=SOME + 2), dict(starts=SOME + 2),
-                dict(order=SOME + 2), dict(places=SOME + 3), dict(n=1 << 29), dict(n=0, starts=0)):
+                dict(order=SOME + 2), dict(places=SOME + 3), dict(n=1 << 29), dict(n=0, starts=0),
+                dict(places=SOME), dict(order=2 * SOME), dict(starts=5 * SOME)):
         assert call(**bad) == -2, bad
         assert b"spgk_route_rows" in lib.spgk_error_string()
 

@@ -253,6 +253,16 @@ def test_experts_sums_that_need_no_rounding(spg, lib, n, out, k, experts):
     assert np.array_equal(c.rows(6, 2), c.want(6)[0])
 
 
+@pytest.mark.parametrize("n,out,k,experts", [(4, 200, 8192, 3), (70, 4000, 300, 20), (3000, 1000, 384, 2), (200, 64, 64, 1000)])
+def test_groups_without_any_rows(spg, lib, n, out, k, experts):
+    """No row belongs to a group, or one alone: the last, a middle one, to the last layer or a middle one."""
+    for first, e in ((None, 0), (n - 1, experts - 1), (n // 2, experts // 2), (0, 0)):
+        starts = [n if first is None else first] * (experts + 1) if first is None else [first] * (e + 1) + [first + 1] * (experts - e)
+        c = Call(spg, lib, np.random.default_rng(n), n, out, k, starts, exact=True, bias=False)
+        got = c.rows(6, 2)
+        assert np.array_equal(got, c.want(6)[0]) and (got == -3).all(1).sum() == (n if first is None else n - 1)
+
+
 def test_starts_that_fall_or_leave_the_rows(spg, lib):
     """A start below zero or an earlier one counts as the largest before it, one beyond the last row as that."""
     for starts in ([-5, 3, 2, 9, 8, 40], [2 ** 31 - 1, 0, 5, 7], [-2 ** 31, 4, -1, 2 ** 31 - 1], [20, 10, 5, 0]):
@@ -358,6 +368,71 @@ def test_on_another_stream_and_replayed(spg, lib):
         c.starts.copy_(torch.tensor([0, 30, 30, 69], dtype=torch.int32))
         c.groups = plain.ranges([0, 30, 30, 69], 70)
         want = np.where(c.want(1)[0] == -3, want, c.want(1)[0])
+
+
+def test_starts_that_the_launch_in_front_writes(spg, lib):
+    """Starts and rows written by the launch directly in front, other ones every time, without a wait in between: none of what a layer looked at ahead is used."""
+    import torch
+    rng = np.random.default_rng(6)
+    for n, out, k, experts in ((48, 300, 2048, 5), (900, 700, 256, 9), (5, 4000, 1024, 4)):
+        c = Call(spg, lib, rng, n, out, k, [0] * experts + [n], exact=True)
+        tables = [np.concatenate(([0], np.sort(rng.integers(0, n + 1, experts - 1)), [n])) for _ in range(12)]
+        sources = [torch.tensor(t, dtype=torch.int32, device="cuda") for t in tables]
+        outs = [torch.zeros(n, out, device="cuda") for _ in tables]
+        torch.cuda.synchronize()
+        for src, y in zip(sources, outs):
+            c.starts.copy_(src)
+            assert lib.spgk_experts_fp8(c.w.ref, experts, c.bd.data_ptr(), 6, c.x.ref, c.starts.data_ptr(), y.data_ptr(), 2, out, None, c.status.data_ptr(), None) == 0
+        assert lib.spgk_gemm_tc_status(c.status.data_ptr(), None) == 0
+        for t, y in zip(tables, outs):
+            c.groups = plain.ranges(t, n)
+            assert np.array_equal(y.double().cpu().numpy(), c.want(6)[0])
+
+
+FIRST = """
+import ctypes, sys, torch
+sys.path.insert(0, {root!r})
+import spingalett_b200 as spg
+lib = spg.lib()
+n, experts, top, k = 300, 6, 2, 512
+x, logits = torch.randn(n, k, device="cuda"), torch.randn(n, experts, device="cuda")
+def ints(m): return torch.zeros(m, dtype=torch.int32, device="cuda")
+chosen, gates, starts, order, places, status = ints(n * top), torch.zeros(n * top, device="cuda"), ints(experts + 1), ints(n * top), ints(n * top), ints(1)
+def matrix(rows, cols):
+    m = (torch.zeros(rows, cols, dtype=torch.uint8, device="cuda"), torch.zeros(rows * 4 * (-(-cols // 512)), dtype=torch.uint8, device="cuda"))
+    return m, ctypes.byref(spg.abi.Fp8(m[0].data_ptr(), m[1].data_ptr(), rows, cols, cols))
+(wm, w), (xm, x8) = matrix(experts * 128, k), matrix(n * top, k)
+wv = torch.randn(experts * 128, k, device="cuda")
+y, out = torch.zeros(n * top, 128, device="cuda"), torch.zeros(n, 128, device="cuda")
+def way():
+    st = torch.cuda.current_stream().cuda_stream
+    for call, args in ((lib.spgk_fp8_quantize, (wv.data_ptr(), 2, k, experts * 128, None, w)),
+                       (lib.spgk_route_rows, (logits.data_ptr(), 2, experts, n, experts, top, 1, chosen.data_ptr(), gates.data_ptr(), starts.data_ptr(), order.data_ptr(), places.data_ptr())),
+                       (lib.spgk_fp8_quantize, (x.data_ptr(), 2, k, n, order.data_ptr(), x8)),
+                       (lib.spgk_experts_fp8, (w, experts, None, 1, x8, starts.data_ptr(), y.data_ptr(), 2, 128, None, status.data_ptr())),
+                       (lib.spgk_combine_rows, (y.data_ptr(), 2, 128, n * top, places.data_ptr(), gates.data_ptr(), n, top, 128, out.data_ptr(), 2, 128))):
+        assert call(*args, st) == 0, lib.spgk_error_string()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    way()
+graph.replay()
+torch.cuda.synchronize()
+got = out.clone()
+out.zero_()
+way()
+torch.cuda.synchronize()
+assert status.item() == 0 and torch.equal(got, out) and got.abs().max() > 1
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture(lib):
+    import subprocess
+    import sys
+    from conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST.format(root=ROOT)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
 
 
 def test_offsets_beyond_32_bits(spg, lib):
