@@ -619,7 +619,8 @@ SPGK_API int spgk_layer_mx4(const spgk_mx4 *W, const float *bias, int act, const
  * (No counterpart in the reference, whose integer formats have one scale per array.)
  * A matrix of `rows` x `cols` values in blocks of 128 along a row: an element is E4M3 (4 exponent bits, 3 of mantissa, 448 the largest number, 0x7F and
  * 0xFF NaN), a block has one E8M0 scale 2^(byte - 127), byte 0xFF meaning that all its values are NaN.
- *   codes : row r starts at codes + r * pitch.  16-byte aligned; pitch is a multiple of 16 and at least spgk_fp8_pitch(cols).
+ *   codes : row r starts at codes + r * pitch.  16-byte aligned; pitch is a multiple of 16 and at least spgk_fp8_pitch(cols)
+ *           (large products read rows faster whose pitch is a multiple of 128).
  *   scales: 32-bit words of four blocks, a block's byte the higher the later it comes; the word of a row stands beside those of its neighbours, and the
  *           next four blocks' of all rows behind these: the scale of block b of row r is byte spgk_fp8_scale_index(rows, r, b). 16-byte aligned,
  *           spgk_fp8_scales_bytes(rows, cols) bytes.  Any run of rows can be taken out of a matrix this way, from any row on.

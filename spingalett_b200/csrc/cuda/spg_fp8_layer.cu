@@ -12,6 +12,10 @@
 // The grid has no more CTAs than the GPU has SMs; each walks the tiles of all groups, copies running ahead over a tile's end.  Where there are few tiles, up to eight CTAs of
 // a cluster share one, each with its part of the k-blocks, and send one another their sums, which are added in rank order.
 //
+// What bounds it: one row x 8192 x 16384 24.2 us (5.6 TB/s; HBM at 6.6 TB/s between a launch's first and last block, and start and end of a launch), 64 rows in 32 groups x 4096 x 8192 140 us (6.6 TB/s),
+// 1 x 8192 x 1024 5.9 us and 1 x 784 x 512 4.4 us (a launch, latency), 16384 x 8192 x 8192 750 us (2930 TFLOP/s, the tensor pipe; 879 us in a long run, under the power limit), 20011 rows in 12 groups x 4104 x 8001
+// 650 us (2020 TFLOP/s, L2: rows 4112 bytes apart lie on two lines for every 128 bytes; 520 us for 4096 inputs).
+//
 // Every wait on an mbarrier is bounded.  A role whose wait gave up records a code in `status`, raises a flag that ends all other waits, and is not told of what follows; outputs are
 // put out only of sums that are said to be complete.  Copies and products under way end, again waited for with a limit, before the memory that they write to is given back.
 #include "spg_fp8.cuh"
@@ -610,6 +614,7 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
 }
 
 // ---- pairs of CTAs, many rows -------------------------------------------------------------------------------------------------
+// (bands of tiles of units, us of 16384 x 8192 x 8192 in a long run: 4 954, 8 918, 12 903, 16 899, 24 934, 32 1018: wider ones share fewer of the rows' tiles, narrower ones fewer of the weights')
 // 256 units x up to 256 rows of a group a tile on a cluster of two (cta_group::2): each CTA holds 128 units' weights and half of the rows, so a k-block costs it 32 KB
 // for 512 cycles of products; a CTA alone would need 48. The last tile of a group multiplies no more rows than it has (in steps of 32).
 // The sixteen epilogue warps take all columns of sums to registers at once (64 a thread), so the next tile's products wait for that alone (there
