@@ -12,6 +12,7 @@
 // What bounds it: latency, of three ways from memory to memory, and 470 instructions a row of 256 logits (us, bf16: 16384 rows to 8 of 256 experts 22.9, 12 of them the choice; 16384 to 2 of 64 13.1,
 // the pairs in one cluster 14.5; 2000 to 8 of 256 14.3 in parts, 11.1 in one cluster; 32 to 2 of 8 4.6 in one block, 6.1 in two launches; one row 3.8).
 #include "spg_fp8.cuh"
+#include <type_traits>
 
 namespace {
 
@@ -84,18 +85,39 @@ __device__ __forceinline__ int32_t choose(const Logits<T, V> &logits, uint32_t t
 {
     constexpr bool SHORT = sizeof(T) == 2;
     float l[V];
-#pragma unroll
-    for (uint32_t i = 0; i < V; i++) l[i] = fmaxf(to_f32(logits.t[i]), closed()) + 0.0f;          // (the larger of a NaN and another is the other; -0 is 0)
     uint32_t key[V], at[V];
+    if constexpr (SHORT && V > 1) {
+        // two at a time: the larger of a NaN and -infinity is -infinity, -0 and 0 are 0, and the order of numbers becomes that of their bits
 #pragma unroll
-    for (uint32_t i = 0; i < V; i++) {
-        const uint32_t e = lane * V + i;
-        at[i] = e;
-        if constexpr (SHORT) {
-            const T t = from_f32<T>(l[i]);
-            const uint32_t b = *reinterpret_cast<const uint16_t *>(&t);
-            key[i] = (b ^ (b & 0x8000u ? 0xffffu : 0x8000u)) << 16 | (0xffffu - e);
-        } else key[i] = key_of(l[i]);
+        for (uint32_t i = 0; i < V; i += 2) {
+            uint32_t w = *reinterpret_cast<const uint32_t *>(logits.t + i);
+            if constexpr (std::is_same<T, __half>::value) {
+                const __half2 v = __hadd2(__hmax2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0xfc00))), __half2half2(__ushort_as_half(0)));
+                const float2 f = __half22float2(v);
+                l[i] = f.x; l[i + 1] = f.y;
+                w = *reinterpret_cast<const uint32_t *>(&v);
+            } else {
+                const __nv_bfloat162 v = __hadd2(__hmax2(*reinterpret_cast<const __nv_bfloat162 *>(&w), __bfloat162bfloat162(__ushort_as_bfloat16(0xff80))), __bfloat162bfloat162(__ushort_as_bfloat16(0)));
+                w = *reinterpret_cast<const uint32_t *>(&v);
+                l[i] = __uint_as_float(w << 16); l[i + 1] = __uint_as_float(w & 0xffff0000u);
+            }
+            const uint32_t k = w ^ ((w >> 15 & 0x00010001u) * 0xffffu | 0x80008000u);
+            key[i] = __byte_perm(0xffffu - (lane * V + i), k, 0x5410);
+            key[i + 1] = __byte_perm(0xffffu - (lane * V + i + 1), k, 0x7610);
+            at[i] = at[i + 1] = 0;
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < V; i++) {
+            l[i] = fmaxf(to_f32(logits.t[i]), closed()) + 0.0f;                  // (as above)
+            const uint32_t e = lane * V + i;
+            at[i] = e;
+            if constexpr (SHORT) {
+                const T t = from_f32<T>(l[i]);
+                const uint32_t b = *reinterpret_cast<const uint16_t *>(&t);
+                key[i] = (b ^ (b & 0x8000u ? 0xffffu : 0x8000u)) << 16 | (0xffffu - e);
+            } else key[i] = key_of(l[i]);
+        }
     }
     const auto of = [](uint32_t k) {
         if constexpr (SHORT) {

@@ -296,6 +296,29 @@ def test_next_operand(spg, lib, n, out, k, starts):
         assert (codes[n] == 0xA5).all() and (words[-16:] == 0xFF).all() and (codes[:, -(-out // 16) * 16:] == 0xA5).all()
 
 
+def test_the_longest_sums(spg, lib):
+    """2^27 inputs, a thousand of them not zero: exact."""
+    import torch
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip("less than 8 GB free")
+    rng = np.random.default_rng(2)
+    k, out, n = 1 << 27, 5, 2
+    w, x = Packed(spg, out, k), Packed(spg, n, k)
+    for m in (w, x):
+        m.codes.zero_()
+        m.words[:-16] = 127
+    at = np.sort(rng.choice(k, 1000, replace=False))
+    at[:3], at[-1] = (0, 1, 127), k - 1
+    pick = np.flatnonzero((plain.SIZES[:127] <= 8) & (plain.SIZES[:127] * 4 % 1 == 0))
+    cw, cx = rng.choice(pick, (out, 1000)).astype(np.uint8), rng.choice(pick, (n, 1000)).astype(np.uint8)
+    places = torch.from_numpy(at).cuda()
+    w.codes[:out, places], x.codes[:n, places] = torch.from_numpy(cw).cuda(), torch.from_numpy(cx).cuda()
+    y, status = torch.zeros(n, out, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert lib.spgk_layer_fp8(w.ref, None, 6, x.ref, y.data_ptr(), 2, out, None, status.data_ptr(), None) == 0, lib.spgk_error_string()
+    assert lib.spgk_gemm_tc_status(status.data_ptr(), None) == 0
+    assert np.array_equal(y.double().cpu().numpy(), plain.SIZES[cx] @ plain.SIZES[cw].T)
+
+
 def test_blocks_of_nan(spg, lib):
     """A NaN block of an input makes its row NaN, one of the weights its unit; the next operand's block with them is NaN."""
     import torch

@@ -51,12 +51,15 @@ def _logits(rng, n, experts, kind):
         l[:] = -3.0e38
         l[:, ::3] = -np.inf
         l[:, experts // 2] = -1e30
+    if kind == "small":                                          # subnormals of 16 bits, of either sign, and both zeros
+        l = rng.integers(-3, 4, (n, experts)) * 2.0 ** -24
+        l[rng.random(l.shape) < 0.2] = -0.0
     if kind == "one":                                            # all rows to the same experts
         l[:] = -np.arange(experts)
     return l
 
 
-@pytest.mark.parametrize("kind", ["plain", "ties", "masked", "lowest", "one"])
+@pytest.mark.parametrize("kind", ["plain", "ties", "masked", "lowest", "small", "one"])
 @pytest.mark.parametrize("n,experts,top,pad,t", [(1, 1, 1, 0, 2), (1, 64, 2, 0, 2), (3, 2, 2, 0, 1), (33, 7, 3, 1, 0), (100, 32, 32, 0, 2), (257, 33, 4, 3, 1), (300, 100, 8, 0, 2), (1000, 256, 8, 8, 0), (700, 257, 5, 0, 2),
                                                  (9, 1024, 32, 0, 1), (2500, 1000, 6, 1, 2), (5000, 3, 1, 0, 2), (0, 16, 2, 0, 2)])
 def test_route(lib, kind, n, experts, top, pad, t):
@@ -100,7 +103,7 @@ def test_long_routes(lib, n, experts, top):
     assert torch.equal(r.places[:-1].long(), places)
 
 
-@pytest.mark.parametrize("n,top,width,t,to,gap", [(1, 1, 1, 2, 2, 0), (3, 3, 777, 2, 2, 0), (5, 2, 1000, 1, 2, 8), (64, 8, 128, 0, 1, 0), (200, 5, 333, 1, 0, 3), (300, 2, 4096, 1, 1, 0), (17, 32, 520, 2, 1, 4), (1000, 4, 96, 0, 0, 16)])
+@pytest.mark.parametrize("n,top,width,t,to,gap", [(3, 70, 2048, 1, 1, 0), (40, 33, 701, 0, 2, 1), (7, 65, 96, 2, 1, 8), (700, 3, 4099, 1, 2, 2), (1, 1, 1, 2, 2, 0), (3, 3, 777, 2, 2, 0), (5, 2, 1000, 1, 2, 8), (64, 8, 128, 0, 1, 0), (200, 5, 333, 1, 0, 3), (300, 2, 4096, 1, 1, 0), (17, 32, 520, 2, 1, 4), (1000, 4, 96, 0, 0, 16)])
 def test_combine(lib, n, top, width, t, to, gap):
     import torch
     rng = np.random.default_rng(n + width)
