@@ -643,8 +643,8 @@ SPGK_API int spgk_fp8_quantize(const void *x, int type, uint32_t ldx, uint32_t x
 SPGK_API int spgk_fp8_dequantize(const spgk_fp8 *src, void *y, int type, uint32_t ldy, void *stream);
 /* A dense layer whose weights W (out x in) and inputs X (N x in) are both in this form:
  *   y[n][j] = act(bias[j] + sum_k W[j][k] * X[n][k])        (bias: dev fp32 [out] or NULL)
- * with exact products and fp32 sums on the tensor cores (at most 2^27 inputs).  y: rows of ldy elements of `type`, rounded once, or NULL; next: the same values quantised
- * as by spgk_fp8_quantize from fp32 (next->rows == X->rows, next->cols == out; scales of blocks behind the last are left as they were), the operand of the layer
+ * with exact products and fp32 sums on the tensor cores (at most 2^27 inputs), whose additions, one for 32 products, cut off what does not fit: some 2 * 10^-7 of the result at 8192
+ * inputs, 6 * 10^-7 where all products have one sign.  y: rows of ldy elements of `type`, rounded once, or NULL; next: the same values quantised as by spgk_fp8_quantize from fp32 (next->rows == X->rows, next->cols == out; scales of blocks behind the last are left as they were), the operand of the layer
  * behind, or NULL; one of the two at least.  ACT_SOFTMAX is left to spgk_softmax_rows, and refused with `next`.
  * status: dev int32, zero before the first call, as for spgk_layer_gemm_tc (read with spgk_gemm_tc_status). Where it says that a wait gave up, the
  * outputs whose sums were not complete are as they were before the call.

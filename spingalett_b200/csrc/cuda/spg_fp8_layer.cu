@@ -64,11 +64,16 @@ __device__ __forceinline__ void st_cluster_if(uint32_t addr, float v, uint32_t y
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void cluster_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { __syncwarp(); asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// `id`: which of the CTA's barriers, for this many threads
-__device__ __forceinline__ void some_meet(uint32_t id, uint32_t threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+// `id`: which of the CTA's barriers, for this many threads (whole warps, whose lanes come to it together)
+__device__ __forceinline__ void some_meet(uint32_t id, uint32_t threads)
+{
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
 __device__ __forceinline__ bool some_agree(uint32_t id, uint32_t threads, bool yes)
 {
     uint32_t all;
+    __syncwarp();
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"(id), "r"(threads), "r"((uint32_t)yes) : "memory");
     return all != 0;
 }

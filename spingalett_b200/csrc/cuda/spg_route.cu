@@ -9,7 +9,7 @@
 // through a cluster.  Many pairs are cut into parts: as each part's choice is made its pairs are counted by expert, one cluster sums the counts up over the
 // parts and experts, and then each part finds its pairs' places from where its experts begin.  The counts lie in the memory of the results on the way: in that of the order,
 // which is written last, and where a part's experts begin in that of its places, which only this part reads and writes.
-// What bounds it: latency, of three ways from memory to memory, and 470 instructions a row of 256 logits (us, bf16: 16384 rows to 8 of 256 experts 22.9, 12 of them the choice; 16384 to 2 of 64 13.1,
+// What bounds it: latency, of three ways from memory to memory, and 520 instructions a row of 256 logits (us, bf16: 16384 rows to 8 of 256 experts 22.6, 12 of them the choice; 16384 to 2 of 64 13.1,
 // the pairs in one cluster 14.5; 2000 to 8 of 256 14.3 in parts, 11.1 in one cluster; 32 to 2 of 8 4.6 in one block, 6.1 in two launches; one row 3.8).
 #include "spg_fp8.cuh"
 #include <type_traits>
@@ -263,13 +263,9 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) spg_route_choose_kernel(const 
     if (count) for (uint32_t e = threadIdx.x; e < experts; e += CHOOSE_THREADS) sh[e] = 0;
     spg_grid_wait();
     __syncthreads();
-    constexpr bool EARLY = V <= 16;                              // (more would not fit the registers)
-    Logits<T, V> next;
-    if (EARLY && lo + warp < hi) load_logits(logits + (uint64_t)(lo + warp) * ld, lane * V, experts, vec, next);
     for (uint32_t n = lo + warp; n < hi; n += CHOOSE_WARPS) {
-        if constexpr (!EARLY) load_logits(logits + (uint64_t)n * ld, lane * V, experts, vec, next);
-        const Logits<T, V> l = next;
-        if (EARLY && n + CHOOSE_WARPS < hi) load_logits(logits + (uint64_t)(n + CHOOSE_WARPS) * ld, lane * V, experts, vec, next);     // (on its way while this one is worked on)
+        Logits<T, V> l;
+        load_logits(logits + (uint64_t)n * ld, lane * V, experts, vec, l);
         float gate;
         const int32_t e = choose(l, top_k, normalise, lane, gate);
         if (lane < top_k) {
