@@ -41,7 +41,6 @@ constexpr uint32_t MAX_SPLIT = 8;
 constexpr uint32_t AHEAD = 8;
 constexpr uint32_t PART = 8 * TM * 4;         // a CTA's sums of eight rows
 constexpr uint32_t HEAD = 2048;
-constexpr uint32_t ROOM = 180 * 1024;         // of shared memory for a CTA (the rest of an SM's is its cache)
 constexpr uint32_t DRAIN = 1u << 12;          // attempts of a last wait
 
 struct LayerParams {
@@ -351,6 +350,8 @@ template <uint32_t NT> struct Shape {
     static constexpr uint32_t X_WORDS = (NT + 31) / 32;
     static constexpr uint32_t EPI = NT >= 64 ? 16 : 8, THREADS = 32 * (ROLES + EPI), PARTS = EPI / 4;      // warps that put out, four of them all units of the same rows
     static constexpr uint32_t CHUNK = NT >= 128 ? 16 : 8;                     // columns that such a warp puts out at a time
+    // Shared memory of a CTA; the rest of an SM's is its cache.  (us with 120, 180 and 212 KB: one row x 8192 x 16384 27.0, 26.0 and 26.1, 200 rows x 8192 x 8192 29.1, 22.9 and 21.9)
+    static constexpr uint32_t ROOM = (NT >= 64 ? 212 : 180) * 1024;
 };
 constexpr uint32_t BAND = 16;
 
@@ -970,7 +971,7 @@ template <uint32_t NT> int launch(const spgk_fp8 *W, const spgk_fp8 *X, LayerPar
     if (tiles > 0x3fffffffu) { spgk_set_error("spgk_layer_fp8", "too many tiles"); return SPGK_E_ARG; }
     p.split = split;
     const uint32_t fixed = 1024 + HEAD + table_bytes(p.experts) + SF_SLOTS * 2 * SF_TILE + parts_bytes<NT>(p.N, p.split);
-    const uint32_t most = (ROOM - fixed) / L::STAGE;
+    const uint32_t most = (L::ROOM - fixed) / L::STAGE;
     p.stages = most < MAX_STAGES ? most : MAX_STAGES;
     const uint32_t grid = p.split > 1 ? (uint32_t)tiles * p.split : (tiles < sms ? (uint32_t)tiles : sms);
     return launch_as("spg_fp8_layer_kernel", spg_fp8_layer_kernel<NT>, grid, L::THREADS, fixed + p.stages * L::STAGE, p.split, map_w, map_x, p, stream);
