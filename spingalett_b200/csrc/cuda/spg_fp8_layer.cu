@@ -965,10 +965,8 @@ template <uint32_t NT> int launch(const spgk_fp8 *W, const spgk_fp8 *X, LayerPar
     if (rc) return rc;
     CUtensorMap map_w, map_x;
     if ((rc = codes_map(&map_w, W, TM)) || (rc = codes_map(&map_x, X, NT))) return rc;
-    p.j_tiles = (p.out + TM - 1) / TM; p.j_inverse = inverse(p.j_tiles);
     const uint32_t sms = (uint32_t)dp.sm_count;
     const uint64_t tiles = most_tiles(p, NT);
-    if (tiles > 0x3fffffffu) { spgk_set_error("spgk_layer_fp8", "too many tiles"); return SPGK_E_ARG; }
     p.split = split;
     const uint32_t fixed = 1024 + HEAD + table_bytes(p.experts) + SF_SLOTS * 2 * SF_TILE + parts_bytes<NT>(p.N, p.split);
     const uint32_t most = (L::ROOM - fixed) / L::STAGE;
@@ -987,9 +985,7 @@ int launch_pairs(const spgk_fp8 *W, const spgk_fp8 *X, LayerParams p, const SpgD
     if (rc) return rc;
     CUtensorMap map_w, map_x;
     if ((rc = codes_map(&map_w, W, TM)) || (rc = codes_map(&map_x, X, PN / 2))) return rc;
-    p.j_tiles = (p.out + 255) / 256; p.j_inverse = inverse(p.j_tiles);
     const uint64_t tiles = most_tiles(p, PN);
-    if (tiles > 0x3fffffffu) { spgk_set_error("spgk_layer_fp8", "too many tiles"); return SPGK_E_ARG; }
     const uint32_t room = (uint32_t)dp.sm_count / 2, pairs = tiles < room ? (uint32_t)tiles : room;
     return launch_as("spg_fp8_pair_kernel", spg_fp8_pair_kernel, pairs * 2, P_THREADS, pair_smem(p.experts), 2, map_w, map_x, p, stream);
 }
@@ -1028,6 +1024,9 @@ int layers(const char *who, const spgk_fp8 *W, uint32_t experts, const float *bi
     p.impatient = spg_gemm_impatient();
     cudaStream_t st = (cudaStream_t)stream;
     const Plan plan = plan_of(p, (uint32_t)dp.sm_count);
+    p.j_tiles = plan.rows == PN ? (out + 255) / 256 : (out + TM - 1) / TM;
+    p.j_inverse = inverse(p.j_tiles);
+    if (most_tiles(p, plan.rows) > 0x3fffffffu) return refuse(who, "too many tiles");
     switch (plan.rows) {
         case 16: return launch<16>(W, X, p, plan.split, dp, dev, st);
         case 32: return launch<32>(W, X, p, plan.split, dp, dev, st);
