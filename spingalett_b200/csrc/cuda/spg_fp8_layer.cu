@@ -38,7 +38,7 @@ constexpr uint32_t SF_SLOTS = 4;              // words on their way, four k-bloc
 constexpr uint32_t ROLES = 3;                 // warp 0: copies, warp 1: products, warp 2: scales; the rest: outputs
 constexpr uint32_t MAX_STAGES = 12;
 constexpr uint32_t MAX_SPLIT = 8;
-constexpr uint32_t AHEAD = 8;
+constexpr uint32_t AHEAD = 8;                 // k-blocks of weights asked for ahead (us with 0, 8 and 14: one row x 8192 x 16384 27.5, 26.1 and 26.4; one row through 2 of 16 experts with 4, 8, 16 and 32: 39.3, 39.2, 39.6 and 42.4)
 constexpr uint32_t PART = 8 * TM * 4;         // a CTA's sums of eight rows
 constexpr uint32_t HEAD = 2048;
 constexpr uint32_t DRAIN = 1u << 12;          // attempts of a last wait
