@@ -412,6 +412,34 @@ def test_starts_that_the_launch_in_front_writes(spg, lib):
             assert np.array_equal(y.double().cpu().numpy(), c.want(6)[0])
 
 
+def test_calls_at_once(spg, lib):
+    """Layers of all arrangements on three streams at a time, each with outputs and a status word of its own, some of them on few SMs, in clusters and in pairs."""
+    import torch
+    rng = np.random.default_rng(12)
+    calls = [Call(spg, lib, rng, *shape, exact=True) for shape in ((3, 300, 4096), (1, 1000, 2048), (200, 500, 1024), (700, 1500, 320), (40, 90, 3001), (64, 2100, 640))]
+    calls += [Call(spg, lib, rng, 300, 400, 512, _starts(rng, 300, 9), exact=True), Call(spg, lib, rng, 2000, 600, 256, _starts(rng, 2000, 4), exact=True)]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [[torch.zeros(c.n, c.out, device="cuda") for _ in streams] for c in calls]
+    status = [torch.zeros(1, dtype=torch.int32, device="cuda") for _ in streams]
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for i, stream in enumerate(streams):
+            for j in range(len(calls)):
+                k = (j * 3 + i * 2 + turn) % len(calls)
+                c, y, st = calls[k], outs[k][i].data_ptr(), stream.cuda_stream
+                if c.starts is None:
+                    rc = lib.spgk_layer_fp8(c.w.ref, c.bd.data_ptr(), 6, c.x.ref, y, 2, c.out, None, status[i].data_ptr(), st)
+                else:
+                    rc = lib.spgk_experts_fp8(c.w.ref, c.experts, c.bd.data_ptr(), 6, c.x.ref, c.starts.data_ptr(), y, 2, c.out, None, status[i].data_ptr(), st)
+                assert rc == 0
+    torch.cuda.synchronize()
+    assert all(s.item() == 0 for s in status)
+    for c, ys in zip(calls, outs):
+        want = c.want(6)[0]
+        for y in ys:
+            assert np.array_equal(y.double().cpu().numpy(), want)
+
+
 FIRST = """
 import ctypes, sys, torch
 sys.path.insert(0, {root!r})
