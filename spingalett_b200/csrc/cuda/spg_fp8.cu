@@ -75,6 +75,9 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS) spg_fp8_dequantize_kernel(const uint8_t *codes, uint32_t pitch, const uint32_t *words, T *y, uint32_t ldy,
                                                                     uint32_t rows, uint32_t cols, uint32_t row_blocks, uint32_t each)
 {
+    // Values whose rows do not lie on the size of four leave side by side, one a lane (us of 16384 x 4097: fp32 67, 130 by four neighbours a lane, bf16 50 and 97; codes made of such
+    // rows were slower that way, 63 and 49)
+    __shared__ alignas(16) float side[VEC ? 1 : WARPS][BLOCK];
     spg_grid_trigger();
     spg_grid_wait();
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
@@ -103,15 +106,24 @@ __global__ void __launch_bounds__(THREADS) spg_fp8_dequantize_kernel(const uint8
             const float s = scale_value(word >> 8 * b & 255u);
             float v[4];
             decode4(code[b], v);
-            alignas(16) T t[4];
+            if constexpr (VEC) {
+                alignas(16) T t[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) t[i] = from_f32<T>(v[i] * s);
-            if (VEC && c + 4u <= cols) {
-                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(row + c) = *reinterpret_cast<const uint4 *>(t);
-                else *reinterpret_cast<uint2 *>(row + c) = *reinterpret_cast<const uint2 *>(t);
+                for (int i = 0; i < 4; i++) t[i] = from_f32<T>(v[i] * s);
+                if (c + 4u <= cols) {
+                    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(row + c) = *reinterpret_cast<const uint4 *>(t);
+                    else *reinterpret_cast<uint2 *>(row + c) = *reinterpret_cast<const uint2 *>(t);
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++) if (c + i < cols) row[c + i] = t[i];
+                }
             } else {
+                __syncwarp();
+                *reinterpret_cast<float4 *>(&side[warp][lane * 4u]) = make_float4(v[0] * s, v[1] * s, v[2] * s, v[3] * s);
+                __syncwarp();
+                const uint32_t first = group * GROUP + b * BLOCK + lane;
 #pragma unroll
-                for (uint32_t i = 0; i < 4; i++) if (c + i < cols) row[c + i] = t[i];
+                for (uint32_t i = 0; i < 4; i++) if (first + i * 32u < cols) row[first + i * 32u] = from_f32<T>(side[warp][i * 32u + lane]);
             }
         }
     }
