@@ -532,6 +532,7 @@ SPGK_API int spgk_nccl_abort(void *comm);
  *   up as soon as they come to it, with copies and products under way: outputs stay as they were and the status word says so. So do
  *   layers on microscaled operands (spgk_layer_mx4): all tiles, and where pairs of CTAs have several each, the last one of each;
  *   with `on` 2 instead pairs give up the wait for tensor memory whose sums are not taken yet.
+ *   Layers on 8-bit operands (spgk_layer_fp8, spgk_experts_fp8) do so with the last tile of every CTA, cluster or pair, and with `on` 2 wherever sums are not taken yet.
  * spgk_selftest_timed_call: host only: a call that answers after answer_ms under the rendezvous timeout wrapper with a
  *   limit of timeout_ms: 0 or SPGK_E_TIMEOUT.
  * spgk_selftest_once_per_device: host only: the once-per-device bookkeeping of the launchers over `devices` fake indices and
