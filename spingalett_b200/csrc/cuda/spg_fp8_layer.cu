@@ -9,6 +9,9 @@
 // one output unit, and a tile's units are one block of the next layer's input.
 // Groups of rows begin anywhere: a tile's codes come by boxes from any row on, and its scales by a warp that reads the words of its rows and lays them out as tcgen05.cp wants
 // them.  What a box brings beyond a group's last row belongs to other columns and is not put out.
+// The tensor core's additions, one for 32 products, cut off what does not fit: one after the other they lose bits always to the same side, 1.5 * 2^-24 of the sum each (measured; 256 of them, 8192 inputs
+// of one sign, 1.9 * 10^-5 of the result; 32768, 2.6 * 10^-3).  So no more than CHAIN k-blocks follow one another: a chain's sums go to registers, where the chains are added up in fp32, rounded to
+// nearest, while the next chain's products have another place in tensor memory.
 // The grid has no more CTAs than the GPU has SMs; each walks the tiles of all groups, copies running ahead over a tile's end.  Where there are few tiles, up to eight CTAs of
 // a cluster share one, each with its part of the k-blocks, and send one another their sums, which are added in rank order.
 //
@@ -323,6 +326,29 @@ template <int C> __device__ __forceinline__ void finish(const LayerParams &p, fl
     }
 }
 
+// A chain's sums of a warp's rows from tensor memory, C at a time, `stride` columns from one C to the next, added to those of the chains before (rounded to nearest)
+template <int COLS, int C> __device__ __forceinline__ void take(float (&v)[COLS], uint32_t from, uint32_t stride, uint32_t rows)
+{
+#pragma unroll
+    for (int c = 0; c < COLS; c += C) {
+        if (c / C * stride >= rows) break;
+        float sums[C];
+        tmem_ld(from + c / C * stride, sums);
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < C; k++) v[c + k] += sums[k];
+    }
+}
+
+// the last chain's sums of a warp's next rows and those of the chains before, which move up to leave
+template <int C, int COLS> __device__ __forceinline__ void next_ones(float (&now)[C], float (&v)[COLS])
+{
+#pragma unroll
+    for (int k = 0; k < C; k++) now[k] += v[k];
+#pragma unroll
+    for (int k = C; k < COLS; k++) v[k - C] = v[k];
+}
+
 // ---- scales -----------------------------------------------------------------------------------------------------------------------
 // The words of a tile's rows for four k-blocks, R times 32 of them from row `first` on (zero from `rows` on): lane l has rows l, l + 32, ...
 template <uint32_t R> __device__ __forceinline__ void load_words(uint32_t (&v)[R], const uint32_t *words, uint32_t group, uint32_t rows, uint32_t first, uint32_t lane)
@@ -348,6 +374,9 @@ template <uint32_t NT> struct Shape {
     static constexpr uint32_t USED = SFW + 2 * SF_COLS;
     static constexpr uint32_t COLS = USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
     static constexpr uint32_t X_WORDS = (NT + 31) / 32;
+    // k-blocks of a chain, whole words of scales.  Taking sums out costs the products beside it tensor memory's time, of few rows nothing that can be measured
+    // (us with 4, 8 and one chain: 256 rows x 4096 x 4096 11.7, 11.4 and 11.1, 200 x 8192 x 8192 22.5, 22.2 and 21.8; 16 x 8192 x 8192 15.2 with any)
+    static constexpr uint32_t CHAIN = NT >= 64 ? 8 : 4;
     static constexpr uint32_t EPI = NT >= 64 ? 16 : 8, THREADS = 32 * (ROLES + EPI), PARTS = EPI / 4;      // warps that put out, four of them all units of the same rows
     static constexpr uint32_t CHUNK = NT >= 128 ? 16 : 8;                     // columns that such a warp puts out at a time
     // Shared memory of a CTA; the rest of an SM's is its cache.  (us with 120, 180 and 212 KB: one row x 8192 x 16384 27.0, 26.0 and 26.1, 200 rows x 8192 x 8192 29.1, 22.9 and 21.9)
@@ -447,11 +476,14 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
             bool ok = true;
             for (; ok && t < last; t += teams) {
                 if (p.impatient == 1 && last - t <= teams && rank == 0) { atomicCAS(p.status, 0, 2); *abort_flag = 1; break; }
-                ok = p.impatient != 2 ? mbar_wait(sums_free + 8 * a, a_phase, abort_flag, p.status, 6) : mbar_test(sums_free + 8 * a, a_phase);
-                if (!ok) { atomicCAS(p.status, 0, 6); *abort_flag = 1; break; }
-                tc_fence_after();
                 // (Written out for the four blocks of a word: 260 cycles a k-block, 330 in a loop over them one by one; 27 of them are an instruction of products, 54 a wait, 6 a commit.)
+                uint32_t first = lo;                                             // of the chain
                 for (uint32_t kb = lo; ok && kb < hi;) {
+                    if (kb == lo || kb % L::CHAIN == 0) {                        // a chain begins
+                        ok = p.impatient != 2 ? mbar_wait(sums_free + 8 * a, a_phase, abort_flag, p.status, 6) : mbar_test(sums_free + 8 * a, a_phase);
+                        if (!ok) { atomicCAS(p.status, 0, 6); *abort_flag = 1; break; }
+                        first = kb;
+                    }
                     if (!(ok = mbar_wait(sf_full + 8 * q, q_phase, abort_flag, p.status, 7))) break;
                     tc_fence_after();
                     odd ^= 1u;
@@ -468,7 +500,7 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
                         tc_fence_after();
                         const uint32_t left = p.cols - kb * KB, id = idesc | i << 4 | i << 29;
                         const uint64_t w = w0 + s * (L::STAGE >> 4), x = x0 + s * (L::STAGE >> 4);
-                        umma_fp8(d, w, x, id, sf, sf + L::SFX, kb > lo, 1);
+                        umma_fp8(d, w, x, id, sf, sf + L::SFX, kb > first, 1);
                         umma_fp8(d, w + 2, x + 2, id, sf, sf + L::SFX, 1, left > 32);
                         umma_fp8(d, w + 4, x + 4, id, sf, sf + L::SFX, 1, left > 64);
                         umma_fp8(d, w + 6, x + 6, id, sf, sf + L::SFX, 1, left > 96);
@@ -476,10 +508,11 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
                         if (++s == p.stages) { s = 0; phase ^= 1u; }
                         kb++;
                     }
+                    if (!ok) break;
+                    if (kb < hi && kb % L::CHAIN) continue;
+                    umma_commit(sums_full + 8 * a);
+                    if (++a == 2) { a = 0; a_phase ^= 1u; }
                 }
-                if (!ok) break;
-                umma_commit(sums_full + 8 * a);
-                if (++a == 2) { a = 0; a_phase ^= 1u; }
             }
         }
         __syncwarp();
@@ -523,6 +556,8 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
     } else {
         const uint32_t quad = warp % 4u, part = (warp - ROLES) / 4u;
         Four four = { most + part * 64u, 6u + part, quad, 0u };
+        constexpr uint32_t COLS = NT / L::PARTS;                               // of a tile's rows this warp's, so many at a time by turns
+        const uint32_t chains = (hi - 1u) / L::CHAIN - lo / L::CHAIN + 1u;
         uint32_t a = 0, a_phase = 0;
         // Once without a row before the launch in front has ended: the outputs' instructions come from L2, and would follow the products
 #pragma unroll 1
@@ -530,25 +565,44 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
             if (!dry) {
                 if (!(tile = find(t)).rows) break;
             } else tile = { 0, 0, 0, 0 };
-            const uint32_t j0 = tile.j * TM + quad * 32u, j = j0 + lane, lanes = tmem + a * NT + (quad * 32u << 16), rows = min(tile.rows, NT);
-            float bias = 0.0f;
+            const uint32_t j0 = tile.j * TM + quad * 32u, j = j0 + lane, rows = min(tile.rows, NT), mine = rows > part * L::CHUNK ? rows - part * L::CHUNK : 0u;
+            float bias = 0.0f, v[COLS];
             bool ok = true;
+            if (!dry && p.bias && j < p.out) bias = p.bias[(uint64_t)tile.e * p.out + j];
+            each(v, [](float) { return 0.0f; });
+            const auto lanes = [&]() { return tmem + a * NT + part * L::CHUNK + (quad * 32u << 16); };
+            const auto taken = [&]() {                                           // of this warp's rows
+                tc_fence_before();
+                __syncwarp();
+                if (!dry && lane == 0) mbar_arrive(sums_free + 8 * a);
+                if (!dry && ++a == 2) { a = 0; a_phase ^= 1u; }
+            };
+#pragma unroll 1
+            for (uint32_t i = 1; i < (dry ? 2u : chains); i++) {                 // (the last chain's are added as they are put out)
+                if (!dry && !(ok = __all_sync(0xffffffffu, mbar_wait(sums_full + 8 * a, a_phase, abort_flag, p.status, 3)))) break;
+                tc_fence_after();
+                take<COLS, L::CHUNK>(v, lanes(), L::PARTS * L::CHUNK, mine);
+                taken();
+            }
             if (!dry) {
-                if (p.bias && j < p.out) bias = p.bias[(uint64_t)tile.e * p.out + j];
                 // (all four warps of a row go one way)
-                ok = some_agree(6u + part, 128, mbar_wait(sums_full + 8 * a, a_phase, abort_flag, p.status, 3));
+                ok = some_agree(6u + part, 128, ok && mbar_wait(sums_full + 8 * a, a_phase, abort_flag, p.status, 3));
                 tc_fence_after();
                 if (p.split > 1) {
                     // This CTA's sums to those that put them out, [chunk][CTA][row][unit], sent before one barrier
                     cluster_wait();                                              // all have begun
-                    const uint32_t chunks = ok ? (rows + 7u) / 8u : 0u;
-                    for (uint32_t c = part; c < chunks; c += L::PARTS) {
-                        float v[8];
-                        tmem_ld8(lanes + 8 * c, v);
+                    const uint32_t left = ok ? mine : 0u;
+#pragma unroll 1
+                    for (uint32_t g = 0; g < COLS; g += 8) {
+                        const uint32_t at = g / L::CHUNK * L::PARTS * L::CHUNK + g % L::CHUNK, c = (part * L::CHUNK + at) / 8u;
+                        if (at >= left) break;
+                        float now[8];
+                        tmem_ld8(lanes() + at, now);
                         tmem_ld_wait();
-                        const uint32_t to = mapa(parts + (c / p.split * p.split + rank) * PART + (quad * 32u + lane) * 4u, c % p.split), left = rows - 8 * c;
+                        next_ones(now, v);
+                        const uint32_t to = mapa(parts + (c / p.split * p.split + rank) * PART + (quad * 32u + lane) * 4u, c % p.split);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) st_cluster_if(to + i * TM * 4u, v[i], (uint32_t)i < left);
+                        for (uint32_t i = 0; i < 8; i++) st_cluster_if(to + i * TM * 4u, now[i], at + i < left);
                     }
                     if (!ok && lane < p.split) st_cluster_u32(mapa(told, lane), 1);
                     tc_fence_before();
@@ -560,26 +614,26 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
                 }
             }
             if (p.split == 1 || dry) {
-                const uint32_t end = dry ? 1u : ok ? rows : 0u;
 #pragma unroll 1
-                for (uint32_t c = dry ? 0 : part * L::CHUNK; c < end; c += L::PARTS * L::CHUNK) {
-                    float v[L::CHUNK];
-                    each(v, [](float) { return 0.0f; });
-                    if (!dry) { tmem_ld(lanes + c, v); tmem_ld_wait(); }
-                    finish(p, v, tile.n0 + c, dry ? 0u : rows - c, j0, lane, bias, four);
+                for (uint32_t c = 0; c < (dry ? 1u : ok ? mine : 0u); c += L::PARTS * L::CHUNK) {
+                    float now[L::CHUNK];
+                    each(now, [](float) { return 0.0f; });
+                    if (!dry) { tmem_ld(lanes() + c, now); tmem_ld_wait(); }
+                    next_ones(now, v);
+                    finish(p, now, tile.n0 + part * L::CHUNK + c, dry ? 0u : mine - c, j0, lane, bias, four);
                 }
             } else if (ok) {
 #pragma unroll 1
                 for (uint32_t c = (part * p.split + rank) * 8u; c < rows; c += p.split * L::PARTS * 8u) {
-                    float v[8];
+                    float all[8];
                     const float *sums = reinterpret_cast<const float *>(base + (parts - head)) + (c / 8 / p.split * p.split) * (PART / 4) + quad * 32u + lane;
-                    each(v, [](float) { return 0.0f; });
+                    each(all, [](float) { return 0.0f; });
 #pragma unroll 1
                     for (uint32_t r = 0; r < p.split; r++, sums += PART / 4) {   // in rank order
 #pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] += sums[i * TM];
+                        for (int i = 0; i < 8; i++) all[i] += sums[i * TM];
                     }
-                    finish(p, v, tile.n0 + c, rows - c, j0, lane, bias, four);
+                    finish(p, all, tile.n0 + c, rows - c, j0, lane, bias, four);
                 }
             }
             if (dry) {
@@ -588,10 +642,7 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
                 continue;
             }
             if (!ok) break;
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(sums_free + 8 * a);
-            if (++a == 2) { a = 0; a_phase ^= 1u; }
+            taken();
             t += teams;
         }
     }
@@ -623,25 +674,36 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
 // (bands of tiles of units, us of 16384 x 8192 x 8192 in a long run: 4 954, 8 918, 12 903, 16 899, 24 934, 32 1018: wider ones share fewer of the rows' tiles, narrower ones fewer of the weights')
 // 256 units x up to 256 rows of a group a tile on a cluster of two (cta_group::2): each CTA holds 128 units' weights and half of the rows, so a k-block costs it 32 KB
 // for 512 cycles of products; a CTA alone would need 48. The last tile of a group multiplies no more rows than it has (in steps of 32).
-// The sixteen epilogue warps take all columns of sums to registers at once (64 a thread), so the next tile's products wait for that alone (there
-// is no room in tensor memory for a second accumulator of 256 columns beside the scales).
+// Chains of products have 16 k-blocks (us of 16384 x 8192 x 8192 with 8, 16 and one chain 877, 807 and 770, of 8192 rows in 8 groups x 4096 x 8192 246, 224 and 219), and sixteen epilogue warps take 64 columns
+// a thread to registers.  Tensor memory has no room for two chains of 256 columns beside the scales: they begin at its first column and at column 224 in turn, and have 32 columns in common, which one warp in four
+// has.  It takes these first and says so; the next chain's products wait for no more (for all 64 columns of all warps: 12 % of the time; two halves of 128 columns a product, in places of their own, read the weights
+// twice: 9 %; tiles of 224 rows, which have none in common, are 2 % quicker where there are many, and 30 % slower for 512 and 1024 rows).
 constexpr uint32_t PN = 256;                                   // rows of the batch a tile
 constexpr uint32_t P_EPI = 16, P_THREADS = 32 * (ROLES + P_EPI);
 constexpr uint32_t P_COLS = PN / (P_EPI / 4);                   // columns of an epilogue warp
+constexpr uint32_t P_CHAIN = 16;
 constexpr uint32_t P_STAGE = W_BYTES + PN / 2 * KB;
 constexpr uint32_t P_STAGES = 6;
 constexpr uint32_t P_WORDS = 3 * SF_TILE;                       // of 128 units and 256 rows
-constexpr uint32_t P_SF = PN, P_SFX = 4, P_SF_COLS = 16;        // columns of tensor memory: scales behind the sums, twice; those of the rows behind the weights'
+constexpr uint32_t P_SHIFT = 224;                               // columns of tensor memory: chains begin at the first and at this one in turn
+constexpr uint32_t P_SF = P_SHIFT + PN, P_SFX = 4, P_SF_COLS = 16;   // scales behind them, twice; those of the rows behind the weights'
 constexpr uint32_t P_BAND = 12;
 __host__ __device__ constexpr uint32_t pair_smem(uint32_t experts) { return 1024 + HEAD + table_bytes(experts) + SF_SLOTS * P_WORDS + P_STAGES * P_STAGE; }
+
+// half of a warp's sums of a chain: the first chain's as they are, those behind added to them
+__device__ __forceinline__ void take_half(float (&v)[32], uint32_t from, uint32_t rows, bool add)
+{
+    if (add) take<32, 16>(v, from, 16, rows);
+    else { tmem_ld32(from, v); tmem_ld_wait(); }
+}
 
 __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LayerParams p)
 {
     extern __shared__ uint8_t raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     const uint32_t head = smem_u32(base), table = head + HEAD, words = table + table_bytes(p.experts), ring = words + SF_SLOTS * P_WORDS;
-    const uint32_t full = head, empty = full + 8 * P_STAGES, sf_full = empty + 8 * P_STAGES, sf_empty = sf_full + 8 * SF_SLOTS, sums_full = sf_empty + 8 * SF_SLOTS, sums_free = sums_full + 8;
-    const uint32_t ended = sums_free + 8, slot = ended + 8, aborted = slot + 4, late = aborted + 4, told = late + 4;
+    const uint32_t full = head, empty = full + 8 * P_STAGES, sf_full = empty + 8 * P_STAGES, sf_empty = sf_full + 8 * SF_SLOTS, sums_full = sf_empty + 8 * SF_SLOTS, sums_free = sums_full + 16;
+    const uint32_t ended = sums_free + 16, slot = ended + 8, aborted = slot + 4, late = aborted + 4, told = late + 4;
     // (told: of each of the two CTAs, how many k-blocks' copies it began, and then whether a wait gave up in it)
     volatile int *abort_flag = reinterpret_cast<volatile int *>(base + (aborted - head));
     volatile uint32_t *told_at = reinterpret_cast<volatile uint32_t *>(base + (told - head));
@@ -653,8 +715,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < P_STAGES; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
         for (uint32_t s = 0; s < SF_SLOTS; s++) { mbar_init(sf_full + 8 * s, 2); mbar_init(sf_empty + 8 * s, 1); }
-        mbar_init(sums_full, 1);
-        mbar_init(sums_free, 2 * P_EPI);
+        for (uint32_t a = 0; a < 2; a++) { mbar_init(sums_full + 8 * a, 1); mbar_init(sums_free + 8 * a, 2 * P_EPI); }
         mbar_init(ended, 1);
         for (uint32_t i = 0; i < 6; i++) abort_flag[i] = 0;
         mbar_fence_init();
@@ -706,17 +767,21 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
-            uint32_t s = 0, phase = 0, q = 0, q_phase = 0, turn = 1, odd = 0;
+            uint32_t s = 0, phase = 0, q = 0, q_phase = 0, a = 1, a_phase = 1, odd = 0, d = tmem + P_SHIFT;
             const uint32_t last = tab.first[p.experts] * p.j_tiles;
             bool ok = true;
             for (; ok && (tile = find(t)).rows; t += pairs) {
                 if (p.impatient == 1 && last - t <= pairs) { give_up(2); break; }
                 const uint32_t idesc = idesc_fp8(256, columns(tile.rows));
-                ok = p.impatient != 2 ? mbar_wait(sums_free, turn, abort_flag, p.status, 6) : mbar_test(sums_free, turn);
-                if (!ok) { give_up(6); break; }
-                turn ^= 1u;
-                tc_fence_after();
                 for (uint32_t kb = 0; kb < p.kblocks; kb++) {
+                    if (kb % P_CHAIN == 0) {
+                        ok = p.impatient != 2 ? mbar_wait(sums_free + 8 * a, a_phase, abort_flag, p.status, 6) : mbar_test(sums_free + 8 * a, a_phase);
+                        if (!ok) { give_up(6); break; }
+                        tc_fence_after();
+                        a_phase ^= a;
+                        a ^= 1u;
+                        d = tmem + P_SHIFT - (d - tmem);
+                    }
                     if (kb % 4u == 0) {
                         if (!(ok = mbar_wait(sf_full + 8 * q, q_phase, abort_flag, p.status, 7))) break;
                         tc_fence_after();
@@ -732,15 +797,15 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
                     tc_fence_after();
                     const uint32_t at = ring + s * P_STAGE, sf = tmem + P_SF + odd * P_SF_COLS, left = p.cols - kb * KB, id = idesc | (kb % 4u) << 4 | (kb % 4u) << 29;
                     const uint64_t w = smem_desc_sw128(at), x = smem_desc_sw128(at + W_BYTES);
-                    umma_fp8_pair(tmem, w, x, id, sf, sf + P_SFX, kb > 0, 1);
-                    umma_fp8_pair(tmem, w + 2, x + 2, id, sf, sf + P_SFX, 1, left > 32);
-                    umma_fp8_pair(tmem, w + 4, x + 4, id, sf, sf + P_SFX, 1, left > 64);
-                    umma_fp8_pair(tmem, w + 6, x + 6, id, sf, sf + P_SFX, 1, left > 96);
+                    umma_fp8_pair(d, w, x, id, sf, sf + P_SFX, kb % P_CHAIN > 0, 1);
+                    umma_fp8_pair(d, w + 2, x + 2, id, sf, sf + P_SFX, 1, left > 32);
+                    umma_fp8_pair(d, w + 4, x + 4, id, sf, sf + P_SFX, 1, left > 64);
+                    umma_fp8_pair(d, w + 6, x + 6, id, sf, sf + P_SFX, 1, left > 96);
                     umma_commit_pair(empty + 8 * s);
                     if (++s == P_STAGES) { s = 0; phase ^= 1u; }
+                    if (kb % P_CHAIN == P_CHAIN - 1 || kb + 1 == p.kblocks) umma_commit_pair(sums_full + 8 * a);
                 }
                 if (!ok) { give_up(2); break; }
-                umma_commit_pair(sums_full);
             }
         }
         __syncwarp();
@@ -774,52 +839,40 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
     } else {
         const uint32_t quad = warp % 4u, part = (warp - ROLES) / 4u, free_at = mapa(sums_free, 0);
         Four four = { most + part * 64u, 2u + part, quad, 0u };
-        uint32_t turn = 0;
-        // (dry: once without a row, as above)
+        const uint32_t chains = (p.kblocks + P_CHAIN - 1) / P_CHAIN, first = part * P_COLS;     // this warp's columns
+        // Of each chain all warps say once that the next one may begin, which takes the place of the chain before and of the columns in common: where this warp has none of these, when the chain before is in its
+        // registers, else when they are too, the first of its columns where the chain begins at P_SHIFT, the last where it begins at the first column.  (A word for one chain may come before all have given
+        // theirs for the chain in front: a barrier for each of two in turn.  So for sums that are whole.)
+        const auto in_common = [&](uint32_t shifted) { return part == (shifted ? 0u : P_EPI / 4 - 1); };
+        uint32_t turn = 0, phase = 0;
+        if (lane == 0 && !in_common(0)) mbar_arrive_cluster(free_at);
+        spg_grid_wait();
+        if (p.starts) some_meet(1, P_THREADS);
+        for (; (tile = find(t)).rows; t += pairs) {
+            const uint32_t j0 = tile.j * 256u + rank * TM + quad * 32u, j = j0 + lane, n0 = tile.n0 + first;
+            const uint32_t rows = tile.rows > first ? min(tile.rows - first, P_COLS) : 0u;             // this warp's
+            float bias = 0.0f, v[P_COLS], (&v_0)[32] = *reinterpret_cast<float (*)[32]>(v), (&v_1)[32] = *reinterpret_cast<float (*)[32]>(v + 32);
+            if (p.bias && j < p.out) bias = p.bias[(uint64_t)tile.e * p.out + j];
+            bool ok = true;
 #pragma unroll 1
-        for (uint32_t dry = 1;; dry = 0) {
-            if (!dry) {
-                if (!(tile = find(t)).rows) break;
-            } else tile = { 0, 0, 0, 0 };
-            const uint32_t j0 = tile.j * 256u + rank * TM + quad * 32u, j = j0 + lane, n0 = tile.n0 + part * P_COLS;
-            const uint32_t rows = min(tile.rows, PN) > part * P_COLS ? min(tile.rows, PN) - part * P_COLS : 0u;       // this warp's columns
-            const uint32_t from = tmem + (quad * 32u << 16) + part * P_COLS;
-            const bool some = tile.j * 256u + rank * TM < p.out;                 // (the same in the four warps: some of this CTA's units there are)
-            float bias = 0.0f;
-            if (!dry) {
-                if (p.bias && j < p.out) bias = p.bias[(uint64_t)tile.e * p.out + j];
-                // (all four warps of a row go one way)
-                if (!some_agree(2u + part, 128, mbar_wait(sums_full, turn, abort_flag, p.status, 3))) break;
-                turn ^= 1u;
+            for (uint32_t i = 0; i < chains; i++) {
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait(sums_full + 8 * turn, phase, abort_flag, p.status, 3)))) break;
                 tc_fence_after();
-            }
-            const bool last = !dry && t + pairs >= tab.first[p.experts] * p.j_tiles;
-            if (dry || last) {
-                // the last: nobody waits for tensor memory, and a short loop is quicker than 64 columns written out that come from L2
+                const bool now = in_common(turn), next = in_common(turn ^ 1u), high = now && !turn;
+                const uint32_t from = tmem + first + turn * P_SHIFT + (quad * 32u << 16);
 #pragma unroll 1
-                for (uint32_t c = 0; c < (dry ? 1u : some ? min(rows, P_COLS) : 0u); c += 8) {
-                    float v[8];
-                    if (!dry) { tmem_ld8(from + c, v); tmem_ld_wait(); }
-                    else each(v, [](float) { return 0.0f; });
-                    finish(p, v, n0 + c, dry ? 0u : rows - c, j0, lane, bias, four);
+                for (uint32_t h = 0; h < 2; h++) {
+                    if (h == high) take_half(v_0, from, rows, i > 0); else take_half(v_1, from + 32, rows > 32u ? rows - 32u : 0u, i > 0);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0 && (h ? !next : now)) mbar_arrive_cluster(free_at + 8 * (h ^ turn));
                 }
-                tc_fence_before();
-                if (dry) {
-                    spg_grid_wait();
-                    if (p.starts) some_meet(1, P_THREADS);
-                    continue;
-                }
-            } else {
-                float v[P_COLS];
-#pragma unroll
-                for (int i = 0; i < (int)P_COLS; i += 32) tmem_ld32(from + i, v + i);
-                tmem_ld_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(free_at);
-                if (rows && some) finish(p, v, n0, rows, j0, lane, bias, four);
+                phase ^= turn;
+                turn ^= 1u;
             }
-            t += pairs;
+            // (all four warps of a row go one way)
+            if (!some_agree(2u + part, 128, ok)) break;
+            if (rows && j0 - quad * 32u < p.out) finish(p, v, n0, rows, j0, lane, bias, four);       // (the same in the four warps: some of this CTA's units there are)
         }
     }
     __syncwarp();
