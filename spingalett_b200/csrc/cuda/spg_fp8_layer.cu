@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
         if (p.split > 1) {
             // Given back before this CTA waits for the others: one that has none on its SM, and so cannot finish, may hold up a cluster that holds some elsewhere
             if (team < tab.first[p.experts] * p.j_tiles) some_meet(2, 32 * (EPI + 1));
-            if (*abort_flag) {
+            if (__any_sync(0xffffffffu, *abort_flag)) {
                 if (elect_one()) umma_commit(ended);
                 __syncwarp();
                 mbar_wait_uniform(ended, 0, late, p.status, 5, DRAIN);
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
             if (++g == g_end) { g = lo / 4u; t += teams; tile = find(t); more = tile.rows; }
             if (more) load();                                                    // (on their way while these wait for their place)
             mbar_wait_uniform(sf_empty + 8 * q, phase, aborted, p.status, 8);
-            if (*abort_flag) break;
+            if (__any_sync(0xffffffffu, *abort_flag)) break;
             store_words(words + q * 2 * SF_TILE, w0, lane);
             store_words(words + q * 2 * SF_TILE + SF_TILE, x0, lane);
             fence_async_smem();
