@@ -677,7 +677,7 @@ SPGK_API int spgk_route_rows(const void *logits, int type, uint32_t ld, uint32_t
                              int32_t *chosen, float *gates, int32_t *starts, int32_t *order, int32_t *places, void *stream);
 /* out[n][c] = sum over j of gates[n][j] * y[places[n][j]][c], in fp32 and in the order of j, rounded once; a place that is none of y's y_rows rows counts as a
  * row of zeros, whatever its gate.  y: rows of ldy elements of `type`; places, gates: dev [N][top_k]; out: rows of ldo elements of out_type, which overlap nothing that
- * is read. */
+ * is read.  top_k is below 2^31. */
 SPGK_API int spgk_combine_rows(const void *y, int type, uint32_t ldy, uint32_t y_rows, const int32_t *places, const float *gates, uint32_t N, uint32_t top_k,
                                uint32_t width, void *out, int out_type, uint32_t ldo, void *stream);
 

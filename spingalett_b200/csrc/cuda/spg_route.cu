@@ -650,6 +650,7 @@ int spgk_combine_rows(const void *y, int type, uint32_t ldy, uint32_t y_rows, co
     const char *who = "spgk_combine_rows";
     if (!known(type) || !known(out_type)) return refuse(who, "unknown type");
     if (top_k == 0 || width == 0) return refuse(who, "nothing to add up");
+    if (top_k > 0x7fffffffu) return refuse(who, "too many places a row");        // (they are counted through in 32 bits, up to 32 at a time)
     if (N == 0) return SPGK_OK;
     if ((!y && y_rows) || !places || !gates || !out) return refuse(who, "no rows, places, gates or output");
     if ((uintptr_t)y % size_of(type) || (uintptr_t)out % size_of(out_type) || ((uintptr_t)places | (uintptr_t)gates) % 4u) return refuse(who, "not aligned");
