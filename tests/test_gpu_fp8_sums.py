@@ -96,3 +96,39 @@ def test_long_sums_of_one_sign(spg, lib, n, out, k, starts):
     additions = -(-k // 512) + 16
     off = ((got - want).abs() / want.clamp_min(1)).max().item()
     assert off <= additions * 2.0 ** -24, off * 2.0 ** 24 / additions
+
+
+@pytest.mark.parametrize("n,out,k,starts", LONG + [(1, 16384, 8192, None), (64, 1030, 8200, None), (200, 8192, 8192, None), (1000, 2048, 8192, None), (65, 300, 70001, None), (5, 640, 30000, [0, 2, 2, 5])])
+def test_long_dense_sums_that_need_no_rounding(spg, lib, n, out, k, starts):
+    """No element is zero; whole multiples of 1/64 whose magnitudes come to less than 3.52 k, below 2^18: exact in any order and any cut.  One product left out, or taken twice, is 1 at least."""
+    experts = 1 if starts is None else len(starts) - 1
+    w, x = Matrix(spg, _codes(experts * out, k, n * 2 + k, True), _scales(experts * out, k)), Matrix(spg, _codes(n, k, n + 1, True), _scales(n, k))
+    got, want, size = _run(spg, lib, w, x, out, starts)
+    assert size.max() < 2.0 ** 18
+    assert (got == want).all()
+
+
+@pytest.mark.parametrize("n,out,k,starts", [s for s in LONG if s[2] <= 20000] + [(1, 128, 8192, None), (1, 16384, 8192, None), (1, 1000, 16384, None), (100, 2000, 8192, None), (512, 8192, 8192, None), (24, 700, 8192, [0, 3, 24])])
+@pytest.mark.parametrize("signs", [True, False])
+def test_long_sums_of_any_elements(spg, lib, signs, n, out, k, starts):
+    """Elements of all sizes, scales of 1/4 to 4.  An addition has 33 numbers, each of which may lose what lies below 2^-24 of the largest, itself no larger than the sum of all magnitudes
+    of its chain; a chain has 64 additions at most, however long the sum is; the chains (see above) are added up rounding to nearest.  A block left out is seen."""
+    import torch
+    experts = 1 if starts is None else len(starts) - 1
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n + out + k)
+
+    def matrix(rows):
+        code = torch.randint(0, 127, (rows, k), device="cuda", generator=g, dtype=torch.uint8)
+        if signs:
+            code |= torch.randint(0, 2, (rows, k), device="cuda", generator=g, dtype=torch.uint8) << 7
+        return Matrix(spg, code, torch.randint(125, 130, (rows, plain.blocks(k)), device="cuda", generator=g, dtype=torch.uint8))
+    w, x = matrix(experts * out), matrix(n)
+    got, want, size = _run(spg, lib, w, x, out, starts)
+    tol = (64 * 33 + -(-k // 512) + 16) * 2.0 ** -24 * size
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / size.clamp_min(1e-30)).max().item() * 2.0 ** 24
+    if starts is None:
+        for b in (0, plain.blocks(k) // 2, plain.blocks(k) - 1):
+            lo, hi = b * plain.BLOCK, min(k, (b + 1) * plain.BLOCK)
+            part = x.values(0, n, lo, hi) @ w.values(0, out, lo, hi).T
+            assert ((got - (want - part)).abs() > tol).any()
