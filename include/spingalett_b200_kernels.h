@@ -644,9 +644,9 @@ SPGK_API int spgk_fp8_quantize(const void *x, int type, uint32_t ldx, uint32_t x
 SPGK_API int spgk_fp8_dequantize(const spgk_fp8 *src, void *y, int type, uint32_t ldy, void *stream);
 /* A dense layer whose weights W (out x in) and inputs X (N x in) are both in this form:
  *   y[n][j] = act(bias[j] + sum_k W[j][k] * X[n][k])        (bias: dev fp32 [out] or NULL)
- * with exact products and fp32 sums (at most 2^27 inputs).  The tensor cores' additions, one for 32 products, cut off what does not fit; no more than 64 of them follow one another, 16 where there are few
- * rows, then these sums are added up rounding to nearest.  Measured, from 2048 inputs on: 1.3 * 10^-6 of the result where signs are mixed, 4.2 * 10^-6 where all products have one (up to 0.9 and 1.1 * 10^-6 for
- * few rows), towards zero.  How a call's sums are cut, and so their last bits, hangs on its rows and units.  y: rows of ldy elements of `type`, rounded once, or NULL; next: the same values quantised as by spgk_fp8_quantize from fp32 (next->rows == X->rows, next->cols == out; scales of blocks behind the last are left as they were), the operand of the layer
+ * with exact products and fp32 sums (at most 2^27 inputs).  The tensor cores' additions, one for 32 products, cut off what does not fit; no more than 96 of them follow one another, 16 where there are few
+ * rows, then these sums are added up rounding to nearest.  Measured, at any length: up to 1.9 * 10^-6 of the result where signs are mixed, 7 * 10^-6 where all products have one (0.9 and 1.1 * 10^-6 for few rows),
+ * towards zero.  How a call's sums are cut, and so their last bits, hangs on its rows and units.  y: rows of ldy elements of `type`, rounded once, or NULL; next: the same values quantised as by spgk_fp8_quantize from fp32 (next->rows == X->rows, next->cols == out; scales of blocks behind the last are left as they were), the operand of the layer
  * behind, or NULL; one of the two at least.  ACT_SOFTMAX is left to spgk_softmax_rows, and refused with `next`.
  * status: dev int32, zero before the first call, as for spgk_layer_gemm_tc (read with spgk_gemm_tc_status). Where it says that a wait gave up, the
  * outputs whose sums were not complete are as they were before the call.

@@ -43,7 +43,7 @@ constexpr uint32_t MAX_STAGES = 12;
 constexpr uint32_t MAX_SPLIT = 8;
 constexpr uint32_t AHEAD = 8;                 // k-blocks of weights asked for ahead (us with 0, 8 and 14: one row x 8192 x 16384 27.5, 26.1 and 26.4; one row through 2 of 16 experts with 4, 8, 16 and 32: 39.3, 39.2, 39.6 and 42.4)
 constexpr uint32_t PART = 8 * TM * 4;         // a CTA's sums of eight rows
-constexpr uint32_t HEAD = 2048;
+constexpr uint32_t HEAD = 3072;
 constexpr uint32_t DRAIN = 1u << 12;          // attempts of a last wait
 
 struct LayerParams {
@@ -265,44 +265,45 @@ template <typename T, int C> __device__ __forceinline__ void put_rows(const Laye
     for (int i = 0; i < C; i++, y += p.ldy) put(y, v[i], (uint32_t)i < rows && j < p.out);
 }
 
-// The four warps that have the same rows of a tile, its 128 units between them: where they leave their largest magnitudes to one another, eight rows by turns in two places
+// The four warps that have the same rows of a tile, its 128 units between them: where they leave their largest magnitudes to one another, sixteen rows by turns in two places
 struct Four {
-    uint32_t *most;                           // [2][4][8]
+    uint32_t *most;                           // [2][4][16]
     uint32_t id, quad, turn;                  // their barrier, this warp among them
 };
-// Eight rows' values of this lane's unit, the four warps' 128 units being one block of the next layer's input: scales, codes, stores.
-// Lane i makes row i's scale for all.  A lane's codes are bytes of two words, one a row; two exchanges among four lanes turn each word into four units of one row.
-__device__ __forceinline__ void put_next(const LayerParams &p, const float (&v)[8], uint32_t n0, uint32_t rows, uint32_t j0, uint32_t lane, Four &four)
+constexpr uint32_t MOST = 2 * 4 * 16;
+// Eight or sixteen rows' values of this lane's unit, the four warps' 128 units being one block of the next layer's input: scales, codes, stores.
+// Lane i makes row i's scale for all.  A lane's codes are bytes of words of four rows; two exchanges among four lanes turn each word into four units of one row.
+template <int C> __device__ __forceinline__ void put_next(const LayerParams &p, const float *v, uint32_t n0, uint32_t rows, uint32_t j0, uint32_t lane, Four &four)
 {
     uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < C; i++) {
         const uint32_t a = __reduce_max_sync(0xffffffffu, __float_as_uint(v[i]) & 0x7fffffffu);
-        if (lane % 8u == (uint32_t)i) most = a;
+        if (lane % C == (uint32_t)i) most = a;
     }
-    uint32_t *place = four.most + four.turn * 32u;
+    uint32_t *place = four.most + four.turn * (MOST / 2);
     four.turn ^= 1u;
-    if (lane < 8u) place[four.quad * 8u + lane] = most;
+    if (lane < C) place[four.quad * 16u + lane] = most;
     some_meet(four.id, 128);
 #pragma unroll
-    for (uint32_t q = 0; q < 4; q++) most = max(most, place[q * 8u + lane % 8u]);
-    const uint32_t mine = scale_byte(most);                                      // row lane % 8
+    for (uint32_t q = 0; q < 4; q++) most = max(most, place[q * 16u + lane % C]);
+    const uint32_t mine = scale_byte(most);                                      // row lane % C
     const float inv = inverse_scale(mine);
-    float q[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) q[i] = v[i] * __shfl_sync(0xffffffffu, inv, i);
     const uint32_t j = j0 + lane / 4u * 4u, block = j0 / TM;
     const bool there = j < (p.out + 15u) / 16u * 16u;
 #pragma unroll
-    for (uint32_t h = 0; h < 2; h++) {
-        uint32_t w = encode4(q[4 * h], q[4 * h + 1], q[4 * h + 2], q[4 * h + 3]);
+    for (int h = 0; h < C; h += 4) {
+        float q[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) q[i] = v[h + i] * __shfl_sync(0xffffffffu, inv, h + i);
+        uint32_t w = encode4(q[0], q[1], q[2], q[3]);
         w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 2), lane & 2u ? 0x3276 : 0x5410);
         w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 1), lane & 1u ? 0x3715 : 0x6240);
-        const uint32_t i = 4u * h + lane % 4u;                                   // this lane's row now
+        const uint32_t i = h + lane % 4u;                                        // this lane's row now
         if (__shfl_sync(0xffffffffu, mine, i) == 255u) w = 0;                    // a NaN block
         if (i < rows && there) *reinterpret_cast<uint32_t *>(p.next_codes + (uint64_t)(n0 + i) * p.next_pitch + j) = w;
     }
-    if (four.quad == 0 && lane < 8u && lane < rows) p.next_scales[((uint64_t)(block / 4u) * p.N + n0 + lane) * 4u + block % 4u] = (uint8_t)mine;
+    if (four.quad == 0 && lane < C && lane < rows) p.next_scales[((uint64_t)(block / 4u) * p.N + n0 + lane) * 4u + block % 4u] = (uint8_t)mine;
 }
 // C rows' sums of this lane's unit to outputs (rows: how many of them there are; with none it only brings its instructions to the SM)
 template <int C> __device__ __forceinline__ void finish(const LayerParams &p, float (&v)[C], uint32_t n0, uint32_t rows, uint32_t j0, uint32_t lane, float bias, Four &four)
@@ -316,13 +317,10 @@ template <int C> __device__ __forceinline__ void finish(const LayerParams &p, fl
         else put_rows<__nv_bfloat16>(p, v, n0, rows, j);
     }
     if (p.next_codes) {
+        constexpr int AT_ONCE = C < 16 ? C : 16;
+        each(v, [&](float x) { return j < p.out ? x : 0.0f; });
 #pragma unroll
-        for (int i = 0; i < C; i += 8) {
-            float q[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) q[k] = j < p.out ? v[i + k] : 0.0f;
-            put_next(p, q, n0 + i, rows > (uint32_t)i ? rows - i : 0, j0, lane, four);
-        }
+        for (int i = 0; i < C; i += AT_ONCE) put_next<AT_ONCE>(p, v + i, n0 + i, rows > (uint32_t)i ? rows - i : 0, j0, lane, four);
     }
 }
 
@@ -555,7 +553,7 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
         }
     } else {
         const uint32_t quad = warp % 4u, part = (warp - ROLES) / 4u;
-        Four four = { most + part * 64u, 6u + part, quad, 0u };
+        Four four = { most + part * MOST, 6u + part, quad, 0u };
         constexpr uint32_t COLS = NT / L::PARTS;                               // of a tile's rows this warp's, so many at a time by turns
         const uint32_t chains = (hi - 1u) / L::CHAIN - lo / L::CHAIN + 1u;
         uint32_t a = 0, a_phase = 0;
@@ -674,20 +672,22 @@ __global__ void __launch_bounds__(Shape<NT>::THREADS, 1) spg_fp8_layer_kernel(co
 // (bands of tiles of units, us of 16384 x 8192 x 8192 in a long run: 4 954, 8 918, 12 903, 16 899, 24 934, 32 1018: wider ones share fewer of the rows' tiles, narrower ones fewer of the weights')
 // 256 units x up to 256 rows of a group a tile on a cluster of two (cta_group::2): each CTA holds 128 units' weights and half of the rows, so a k-block costs it 32 KB
 // for 512 cycles of products; a CTA alone would need 48. The last tile of a group multiplies no more rows than it has (in steps of 32).
-// Chains of products have 16 k-blocks (us of 16384 x 8192 x 8192 with 8, 16 and one chain 877, 807 and 770, of 8192 rows in 8 groups x 4096 x 8192 246, 224 and 219), and sixteen epilogue warps take 64 columns
+// Chains of products have 16 k-blocks (us of 16384 x 8192 x 8192 with 8, 16 and one chain 877, 807 and 770, of 8192 rows in 8 groups x 4096 x 8192 246, 224 and 219), a tile's first one 24: the tile before is
+// put out beside it (8192 rows as above to 8-bit outputs with a first chain of 16, 24 and 32: 250, 236 and 230, one chain 230).  Sixteen epilogue warps take 64 columns
 // a thread to registers.  Tensor memory has no room for two chains of 256 columns beside the scales: they begin at its first column and at column 224 in turn, and have 32 columns in common, which one warp in four
 // has.  It takes these first and says so; the next chain's products wait for no more (for all 64 columns of all warps: 12 % of the time; two halves of 128 columns a product, in places of their own, read the weights
 // twice: 9 %; tiles of 224 rows, which have none in common, are 2 % quicker where there are many, and 30 % slower for 512 and 1024 rows).
 constexpr uint32_t PN = 256;                                   // rows of the batch a tile
 constexpr uint32_t P_EPI = 16, P_THREADS = 32 * (ROLES + P_EPI);
 constexpr uint32_t P_COLS = PN / (P_EPI / 4);                   // columns of an epilogue warp
-constexpr uint32_t P_CHAIN = 16;
+constexpr uint32_t P_FIRST = 24, P_CHAIN = 16;
 constexpr uint32_t P_STAGE = W_BYTES + PN / 2 * KB;
 constexpr uint32_t P_STAGES = 6;
 constexpr uint32_t P_WORDS = 3 * SF_TILE;                       // of 128 units and 256 rows
 constexpr uint32_t P_SHIFT = 224;                               // columns of tensor memory: chains begin at the first and at this one in turn
 constexpr uint32_t P_SF = P_SHIFT + PN, P_SFX = 4, P_SF_COLS = 16;   // scales behind them, twice; those of the rows behind the weights'
 constexpr uint32_t P_BAND = 12;
+__device__ __forceinline__ bool begins_chain(uint32_t kb) { return kb >= P_FIRST && (kb - P_FIRST) % P_CHAIN == 0; }     // (besides a tile's first)
 __host__ __device__ constexpr uint32_t pair_smem(uint32_t experts) { return 1024 + HEAD + table_bytes(experts) + SF_SLOTS * P_WORDS + P_STAGES * P_STAGE; }
 
 // half of a warp's sums of a chain: the first chain's as they are, those behind added to them
@@ -774,7 +774,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
                 if (p.impatient == 1 && last - t <= pairs) { give_up(2); break; }
                 const uint32_t idesc = idesc_fp8(256, columns(tile.rows));
                 for (uint32_t kb = 0; kb < p.kblocks; kb++) {
-                    if (kb % P_CHAIN == 0) {
+                    const bool begins = kb == 0 || begins_chain(kb);
+                    if (begins) {
                         ok = p.impatient != 2 ? mbar_wait(sums_free + 8 * a, a_phase, abort_flag, p.status, 6) : mbar_test(sums_free + 8 * a, a_phase);
                         if (!ok) { give_up(6); break; }
                         tc_fence_after();
@@ -797,13 +798,13 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
                     tc_fence_after();
                     const uint32_t at = ring + s * P_STAGE, sf = tmem + P_SF + odd * P_SF_COLS, left = p.cols - kb * KB, id = idesc | (kb % 4u) << 4 | (kb % 4u) << 29;
                     const uint64_t w = smem_desc_sw128(at), x = smem_desc_sw128(at + W_BYTES);
-                    umma_fp8_pair(d, w, x, id, sf, sf + P_SFX, kb % P_CHAIN > 0, 1);
+                    umma_fp8_pair(d, w, x, id, sf, sf + P_SFX, !begins, 1);
                     umma_fp8_pair(d, w + 2, x + 2, id, sf, sf + P_SFX, 1, left > 32);
                     umma_fp8_pair(d, w + 4, x + 4, id, sf, sf + P_SFX, 1, left > 64);
                     umma_fp8_pair(d, w + 6, x + 6, id, sf, sf + P_SFX, 1, left > 96);
                     umma_commit_pair(empty + 8 * s);
                     if (++s == P_STAGES) { s = 0; phase ^= 1u; }
-                    if (kb % P_CHAIN == P_CHAIN - 1 || kb + 1 == p.kblocks) umma_commit_pair(sums_full + 8 * a);
+                    if (kb + 1 == p.kblocks || begins_chain(kb + 1)) umma_commit_pair(sums_full + 8 * a);
                 }
                 if (!ok) { give_up(2); break; }
             }
@@ -838,8 +839,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) spg_fp8_pair_kernel(const __grid
         }
     } else {
         const uint32_t quad = warp % 4u, part = (warp - ROLES) / 4u, free_at = mapa(sums_free, 0);
-        Four four = { most + part * 64u, 2u + part, quad, 0u };
-        const uint32_t chains = (p.kblocks + P_CHAIN - 1) / P_CHAIN, first = part * P_COLS;     // this warp's columns
+        Four four = { most + part * MOST, 2u + part, quad, 0u };
+        const uint32_t chains = p.kblocks <= P_FIRST ? 1u : 1u + (p.kblocks - P_FIRST + P_CHAIN - 1) / P_CHAIN, first = part * P_COLS;     // this warp's columns
         // Of each chain all warps say once that the next one may begin, which takes the place of the chain before and of the columns in common: where this warp has none of these, when the chain before is in its
         // registers, else when they are too, the first of its columns where the chain begins at P_SHIFT, the last where it begins at the first column.  (A word for one chain may come before all have given
         // theirs for the chain in front: a barrier for each of two in turn.  So for sums that are whole.)
