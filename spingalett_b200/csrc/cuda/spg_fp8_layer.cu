@@ -15,9 +15,9 @@
 // The grid has no more CTAs than the GPU has SMs; each walks the tiles of all groups, copies running ahead over a tile's end.  Where there are few tiles, up to eight CTAs of
 // a cluster share one, each with its part of the k-blocks, and send one another their sums, which are added in rank order.
 //
-// What bounds it: one row x 8192 x 16384 24.2 us (5.6 TB/s; HBM at 6.6 TB/s between a launch's first and last block, and start and end of a launch), 64 rows in 32 groups x 4096 x 8192 140 us (6.6 TB/s),
-// 1 x 8192 x 1024 5.9 us and 1 x 784 x 512 4.4 us (a launch, latency), 16384 x 8192 x 8192 750 us (2930 TFLOP/s, the tensor pipe; 879 us in a long run, under the power limit), 20011 rows in 12 groups x 4104 x 8001
-// 650 us (2020 TFLOP/s, L2: rows 4112 bytes apart lie on two lines for every 128 bytes; 520 us for 4096 inputs).
+// What bounds it: one row x 8192 x 16384 24.3 us (5.6 TB/s; HBM at 6.6 TB/s between a launch's first and last block, and start and end of a launch), 64 rows in 32 groups x 4096 x 8192 140 us (6.6 TB/s),
+// 1 x 8192 x 1024 6.2 us and 1 x 784 x 512 4.6 us (a launch, latency), 16384 x 8192 x 8192 785 us (2800 TFLOP/s, the tensor pipe and the sums that are taken out beside it; 920 us in a long run, under the power
+// limit), 20011 rows in 12 groups x 4104 x 8001 650 us (2020 TFLOP/s, L2: rows 4112 bytes apart lie on two lines for every 128 bytes; 537 us for 4096 inputs).
 //
 // Every wait on an mbarrier is bounded.  A role whose wait gave up records a code in `status`, raises a flag that ends all other waits, and is not told of what follows; outputs are
 // put out only of sums that are said to be complete.  Copies and products under way end, again waited for with a limit, before the memory that they write to is given back.
@@ -959,9 +959,12 @@ uint64_t most_tiles(const LayerParams &p, uint32_t tile_rows)
 uint32_t at_a_time(uint32_t split, uint32_t sms) { return (split == 8 ? 15u : split == 4 ? 33u : split == 2 ? 74u : 148u) * sms / 148u; }
 
 // How a call is arranged: rows of a tile (256: pairs of CTAs), CTAs that share one.  What each takes is estimated in us on a B200 (with groups of equal sizes, for want of the real ones), fitted to 1285
-// arrangements of 205 products: 1 to 5000 rows, in up to 200 groups, 128 to 16384 inputs, 128 to 8192 units.  What it picks takes 1 % longer on average than the best of
-// them, 15 % at most.  Both ends of it, us: 64 rows x 8192 x 8192 by tiles of 64 rows, two CTAs each, 16.6, by tiles of 16 24.8, in pairs 23.1; 1 x 1024 x 8192 alone 4.6, two CTAs a tile 6.2;
-// 1 x 8192 x 1024 12.0 and, eight a tile, 5.9; 512 x 8192 x 8192 in pairs 31.1, by 128 rows 38.3; 512 x 784 x 512 9.6 and 7.2.
+// arrangements of 205 products: 1 to 5000 rows, in up to 200 groups, 128 to 16384 inputs, 128 to 8192 units, when sums were not yet taken out in chains.  Of 613 products of all such sizes, measured since in 4005
+// arrangements, what it picks takes 2.5 % longer on average than the best, 14 % in one of twenty, and 47 % at most (2000 x 128 x 4096 by 64 rows 16.9 us, in pairs 11.5: the outputs of few inputs are what it
+// knows least of).  Both ends of it, us: 64 rows x 8192 x 8192 by tiles of 64 rows, two CTAs each, 16.4, by tiles of 16 27.0, in pairs 23.4; 1 x 1024 x 8192 alone 4.9, two CTAs a tile 6.3;
+// 1 x 8192 x 1024 13.9 and, eight a tile, 6.3; 512 x 8192 x 8192 in pairs 33.0, by 128 rows 38.1; 512 x 784 x 512 by 32 rows 5.5, in pairs 9.1.
+// All that holds for groups of similar sizes.  Where they are not, tiles are made for the mean: of 512 rows x 64 x (4096 x 2048) all in one group take 28.0 us, where one layer for them takes 11.2 by its own
+// arrangement, of 4096 rows 37.5 and 30.1 (in even groups, whose weights are all read, 82.8 and 98.1).
 struct Plan { uint32_t rows, split; float us; };
 float tiles_of(const LayerParams &p, uint32_t rows)
 {
