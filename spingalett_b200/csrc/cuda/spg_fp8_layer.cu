@@ -43,7 +43,8 @@ constexpr uint32_t MAX_STAGES = 12;
 constexpr uint32_t MAX_SPLIT = 8;
 constexpr uint32_t AHEAD = 8;                 // k-blocks of weights asked for ahead (us with 0, 8 and 14: one row x 8192 x 16384 27.5, 26.1 and 26.4; one row through 2 of 16 experts with 4, 8, 16 and 32: 39.3, 39.2, 39.6 and 42.4)
 constexpr uint32_t PART = 8 * TM * 4;         // a CTA's sums of eight rows
-constexpr uint32_t HEAD = 3072;
+constexpr uint32_t MOST = 2 * 4 * 16;         // words of largest magnitudes that four warps leave to one another
+constexpr uint32_t HEAD = 1024 + 4 * MOST * 4; // barriers and flags, and four times these
 constexpr uint32_t DRAIN = 1u << 12;          // attempts of a last wait
 
 struct LayerParams {
@@ -270,7 +271,6 @@ struct Four {
     uint32_t *most;                           // [2][4][16]
     uint32_t id, quad, turn;                  // their barrier, this warp among them
 };
-constexpr uint32_t MOST = 2 * 4 * 16;
 // Eight or sixteen rows' values of this lane's unit, the four warps' 128 units being one block of the next layer's input: scales, codes, stores.
 // Lane i makes row i's scale for all.  A lane's codes are bytes of words of four rows; two exchanges among four lanes turn each word into four units of one row.
 template <int C> __device__ __forceinline__ void put_next(const LayerParams &p, const float *v, uint32_t n0, uint32_t rows, uint32_t j0, uint32_t lane, Four &four)

@@ -83,9 +83,9 @@ LONG = [(1, 9700, 16384, None), (60, 9700, 16384, None), (120, 9700, 16384, None
 
 @pytest.mark.parametrize("n,out,k,starts", LONG)
 def test_long_sums_of_one_sign(spg, lib, n, out, k, starts):
-    """Products are whole multiples of 2^-11 (those of every other block; of 2^-6 in the rest) below 4, so sums of up to 3072 of them, half of them from each kind of block, lie below 1.5 * (2^12 + 2^7) < 2^13 and
-    are exact in the 24 bits that the tensor core keeps; those of a layer are not.  3072 products at most follow one another there, and 512 at least but for the ends of a CTA's part, of which there are eight at
-    most.  Their sums are added up rounding to nearest, half of 2^-23 of the sum at most each time: no more than 2^-24 of the result for each addition."""
+    """Products are whole multiples of 2^-11 (those of every other block; of 2^-6 in the rest) below 4, so sums over up to 24 blocks, half of them of each kind, lie below 1.5 * (2^12 + 2^7) < 2^13 and are
+    exact in the 24 bits that the tensor core keeps; those of a layer are not.  24 blocks at most follow one another there, and four at least but for the ends of a CTA's part, of which there are eight at most.
+    Their sums are added up rounding to nearest, half of 2^-23 of the sum at most each time: no more than 2^-24 of the result for each addition."""
     import torch
     experts = 1 if starts is None else len(starts) - 1
     scale = _scales(experts * out, k)
